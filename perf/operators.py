@@ -176,12 +176,12 @@ def prepare(case, seed):
 # ---- plain forms ----------------------------------------------------------------------------------------------------
 def _to_4bit(x):
     """(codes, scales): of every 32 values e2m1 codes, the earlier value in the lower half of a byte, and the smallest power of two, from
-    2^-62 to 2^65 and biased by 127, that lets the largest be at most 6; 255 where one is NaN."""
+    2^-127 to 2^126 and biased by 127, that lets the largest be at most 6; 255 where one is NaN."""
     g = x.reshape(*x.shape[:-1], x.shape[-1] // 32, 32)
     top = g.abs().amax(-1, keepdim=True)
-    m, e = torch.frexp(torch.where(torch.isfinite(top) & (top > 0), top, torch.where(top > 0, 2.0 ** 100, 2.0 ** -100)))
-    e = (e - 3 + (m > 0.75).to(e.dtype)).clamp(-62, 65)
-    y = torch.ldexp(g.abs(), -e)
+    m, e = torch.frexp(torch.where(torch.isfinite(top) & (top > 0), top, torch.where(top > 0, 3e38, 1e-45)))
+    e = (e - 3 + (m > 0.75).to(e.dtype)).clamp(-127, 126)
+    y = (g.abs().double() * torch.exp2(-e.double())).float()
     code = ((y > 0.25).to(torch.uint8) + (y >= 0.75) + (y > 1.25) + (y >= 1.75) + (y > 2.5) + (y >= 3.5) + (y > 5)).to(torch.uint8)
     code = code | (g.signbit().to(torch.uint8) << 3)
     code = code.reshape(*x.shape[:-1], x.shape[-1] // 2, 2)
@@ -193,7 +193,7 @@ def _values(codes, scales):
     """float32 values of a 4-bit cache."""
     table = torch.tensor([0, 0.5, 1, 1.5, 2, 3, 4, 6, -0.0, -0.5, -1, -1.5, -2, -3, -4, -6], device=codes.device)
     x = table[torch.stack((codes & 15, codes >> 4), -1).long()].reshape(*codes.shape[:-1], codes.shape[-1] // 16, 32)
-    factor = torch.where(scales == 255, torch.nan, torch.ldexp(torch.ones((), device=codes.device), scales.int().clamp(65, 192) - 127))
+    factor = torch.where(scales == 255, torch.nan, torch.exp2(scales.double() - 127).float())
     return (x * factor[..., None]).flatten(-2)
 
 
@@ -370,7 +370,7 @@ def _exact_4bit(x):
     """The 4-bit values nearest to float64 values (ties to the even code)."""
     g = x.reshape(*x.shape[:-1], -1, 32)
     top = g.abs().amax(-1, keepdim=True)
-    unit = torch.exp2(torch.ceil(torch.log2(torch.clamp(top, min=1e-30) / 6)).clamp(-62, 65))
+    unit = torch.exp2(torch.ceil(torch.log2(torch.clamp(top, min=1e-30) / 6)).clamp(-127, 126))
     y = g / unit
     step = torch.where(y.abs() < 2, 0.5, torch.where(y.abs() < 4, 1.0, 2.0)).double()
     return ((torch.round(y / step) * step).clamp(-6, 6) * unit).reshape(x.shape)
