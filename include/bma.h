@@ -145,6 +145,77 @@ typedef struct bma_attn_args {
 
 enum { BMA_BACKEND_AUTO = 0, BMA_BACKEND_SIMT = 1, BMA_BACKEND_TCGEN05 = 2 };
 
+/* ---- heads: RMS norm and rotary positions of queries and keys; the paged cache ------------------------------------------
+ * No counterpart in the reference, whose attention takes Q, K and V as they are.  What a model does with its heads before that attention,
+ * and what it decodes from:
+ *   rotate      y = turn(position, norm(x)) of every head of q and k, and the gradients
+ *   append_kv   the same of new tokens, their keys and values going into the pages of a cache
+ *   read_kv     the cached tokens of every sequence as dense keys and values
+ *   paged_attn  attention of the newest tokens over the cache
+ * norm(x) = x / sqrt(mean(x^2) + eps) * weight, in float32; turn rotates the component pairs (i, i + dim/2) (HALF) or (2i, 2i + 1) (INTERLEAVED),
+ * i < dim/2, by the angle position * frequencies[i] and multiplies them by `magnitude`; components from `dim` on stay as they are.  One
+ * rounding, at the end. */
+enum { BMA_ROTARY_HALF = 0, BMA_ROTARY_INTERLEAVED = 1 };
+
+typedef struct bma_rotary {
+  const double* frequencies;   /* [dim / 2] radians per position                              */
+  int32_t dim;                 /* components that are rotated (even, at most d); 0: no rotation */
+  int32_t layout;              /* BMA_ROTARY_*                                                */
+  float magnitude, eps;
+  const void* q_weight;        /* [d] or null: that side has no norm                          */
+  const void* k_weight;
+  int32_t weight_dtype;        /* BMA_DTYPE_* of the weights and of their gradients           */
+  int32_t reserved_;
+} bma_rotary;
+
+typedef struct bma_rotate_args {
+  int32_t B, L, Hq, Hkv, d;         /* d <= 256; Hkv == 0: there are no keys                  */
+  int32_t position_bytes;           /* 4 or 8                                                 */
+  const void* positions;            /* null: 0 .. L-1 in every sequence                       */
+  int64_t position_stride_b, position_stride_l;   /* in elements                              */
+  bma_rotary rotary;
+  bma_tensor q, k;                  /* inputs (forward; backward of a side with a norm)       */
+  bma_tensor q_out, k_out;          /* forward: outputs, backward: cotangents of them         */
+  bma_tensor dq, dk;                /* backward: gradients of q and k                         */
+  void *dq_weight, *dk_weight;      /* backward: [d] gradients of the weights                 */
+} bma_rotate_args;
+
+/* dtype of a cache: BMA_DTYPE_F32, BMA_DTYPE_BF16 or this, every 32 components of a head as e2m1 codes (two to a byte, the earlier in the lower half)
+ * and one power of two (a byte, biased by 127; 255: NaN).  Appending takes the smallest power with which the largest of the 32 is at most 6. */
+enum { BMA_DTYPE_MXFP4 = 2 };
+
+typedef struct bma_paged_cache {
+  void *k, *v;                      /* [pages, page_size, Hkv, d] (MXFP4: d / 2 bytes), the same strides for both */
+  int64_t stride_page, stride_slot, stride_head;                    /* in elements (MXFP4: bytes) */
+  uint8_t *k_scale, *v_scale;       /* MXFP4: [pages, page_size, Hkv, d / 32]                 */
+  int64_t scale_stride_page, scale_stride_slot, scale_stride_head;
+  const int32_t* page_table;        /* [B, width]: page of positions [i * page_size, (i + 1) * page_size) of a sequence */
+  int64_t table_stride;
+  int32_t pages, page_size, Hkv, d, B, width;   /* d <= 128, a multiple of 8 (MXFP4: of 32)   */
+  int32_t dtype, reserved_;
+} bma_paged_cache;
+
+/* Of the T tokens that are given of sequence b the first new_lengths[b] (null: all T) are real; they are its newest, at positions
+ * lengths[b] - new_lengths[b] and up: `lengths` counts them.  A position that the table does not cover, and a page that is not one of the
+ * cache's, is neither read nor written; the status word (bma_device_status) says so, and the results of that call are invalid. */
+typedef struct bma_append_args {
+  int32_t T, Hq;                    /* Hq == 0: no queries                                    */
+  const int32_t *lengths, *new_lengths;
+  bma_rotary rotary;
+  bma_tensor q, k, v;               /* [B, T, Hq or Hkv, d]                                   */
+  bma_tensor q_out;                 /* rotated queries; zeros for tokens that are not real    */
+} bma_append_args;
+
+typedef struct bma_paged_attn_args {
+  int32_t T, Hq;
+  const int32_t *lengths, *new_lengths;
+  float scale;
+  int32_t window;                   /* a token sees keys from `window` positions before its own; negative: from the first */
+  bma_tensor q;                     /* [B, T, Hq, d]: float32 for a float32 cache, else bfloat16 */
+  bma_tensor o;                     /* [B, T, Hq, d]; zeros for tokens that are not real      */
+  float* lse;                       /* [B, Hq, T] or null; -inf where no key is seen          */
+} bma_paged_attn_args;
+
 /* ---- entry points -------------------------------------------------------------------- */
 
 /* Library / ABI version (major*1000 + minor). */
@@ -382,6 +453,24 @@ int bma_attn_bwd_o(const bma_attn_args* args, void* d_o_bf16, const bma_mask_spe
  * written in place into (o_a, lse_a).  o_* are float32 [B,N,Hq,d] described by args->o
  * (a) and args->d_o (b); lse_* by args->lse (a) and args->delta (b). */
 int bma_attn_merge(const bma_attn_args* args, bma_stream_t stream);
+
+/* Norm and rotation of heads (see bma_rotary), and the gradients: of q and k, and of the weights of a side that has a norm.  The sums of the
+ * latter go through the workspace (bma_rotate_bwd_workspace_bytes, 16-byte aligned; 0 without weights), in an order that is fixed by the sizes. */
+int bma_rotate(const bma_rotate_args* args, bma_stream_t stream);
+size_t bma_rotate_bwd_workspace_bytes(const bma_rotate_args* args);
+int bma_rotate_bwd(const bma_rotate_args* args, void* workspace, size_t workspace_bytes, bma_stream_t stream);
+
+/* Appends the keys and values of new tokens to a cache, and norms and rotates their queries on the way. */
+int bma_append_kv(const bma_paged_cache* cache, const bma_append_args* args, bma_stream_t stream);
+
+/* Positions [0, L) of every sequence as k, v [B, L, Hkv, d], zeros from lengths[b] on; in the cache's type, bfloat16 of an MXFP4 cache. */
+int bma_read_kv(const bma_paged_cache* cache, const int32_t* lengths, int32_t L, const bma_tensor* k, const bma_tensor* v, bma_stream_t stream);
+
+/* Attention of the newest tokens of every sequence over its cached ones, itself included: O = softmax(scale q.k) v over the keys at the token's
+ * position and before (within the window).  The walks of all (sequence, kv head) pairs are cut into even shares, whose results meet through the workspace
+ * (16-byte aligned); calls that may overlap need one each.  The order of sums depends on the sizes and lengths of the call and on the device. */
+size_t bma_paged_attn_workspace_bytes(const bma_paged_cache* cache, const bma_paged_attn_args* args);
+int bma_paged_attn(const bma_paged_cache* cache, const bma_paged_attn_args* args, void* workspace, size_t workspace_bytes, bma_stream_t stream);
 
 /* Reads and clears the device-side status word that bounded waits / bounds checks write.
  * Synchronises `stream`.  Returns BMA_OK or BMA_ERR_DEVICE_CHECK; *detail gets the code. */

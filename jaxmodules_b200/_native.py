@@ -17,7 +17,8 @@ _LIB_PATH = Path(__file__).resolve().parent / "libbma.so"
 BMA_OK = 0
 BMA_ERR_ARG, BMA_ERR_UNSUPPORTED, BMA_ERR_WORKSPACE, BMA_ERR_CUDA, BMA_ERR_LIMIT = -1, -2, -3, -4, -5
 BMA_ERR_DEVICE_CHECK = 1
-BMA_DTYPE_F32, BMA_DTYPE_BF16 = 0, 1
+BMA_DTYPE_F32, BMA_DTYPE_BF16, BMA_DTYPE_MXFP4 = 0, 1, 2
+BMA_ROTARY_HALF, BMA_ROTARY_INTERLEAVED = 0, 1
 BMA_MASK_CAUSAL, BMA_MASK_BAND, BMA_MASK_BLOCK_WINDOW, BMA_MASK_SEGMENT, BMA_MASK_BITMAP, BMA_MASK_TILES = 1, 2, 4, 8, 16, 32
 BMA_MASK_COMPILE_CONSERVATIVE = 256
 F32_TILE = 128   # BMA_F32_TILE
@@ -90,6 +91,50 @@ class AttnArgs(C.Structure):
     ]
 
 
+class Rotary(C.Structure):
+    _fields_ = [
+        ("frequencies", C.c_void_p), ("dim", C.c_int32), ("layout", C.c_int32), ("magnitude", C.c_float), ("eps", C.c_float),
+        ("q_weight", C.c_void_p), ("k_weight", C.c_void_p), ("weight_dtype", C.c_int32), ("reserved_", C.c_int32),
+    ]
+
+
+class RotateArgs(C.Structure):
+    _fields_ = [
+        ("B", C.c_int32), ("L", C.c_int32), ("Hq", C.c_int32), ("Hkv", C.c_int32), ("d", C.c_int32), ("position_bytes", C.c_int32),
+        ("positions", C.c_void_p), ("position_stride_b", C.c_int64), ("position_stride_l", C.c_int64),
+        ("rotary", Rotary),
+        ("q", Tensor), ("k", Tensor), ("q_out", Tensor), ("k_out", Tensor), ("dq", Tensor), ("dk", Tensor),
+        ("dq_weight", C.c_void_p), ("dk_weight", C.c_void_p),
+    ]
+
+
+class PagedCacheArgs(C.Structure):
+    """bma_paged_cache of include/bma.h."""
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p),
+        ("stride_page", C.c_int64), ("stride_slot", C.c_int64), ("stride_head", C.c_int64),
+        ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+        ("scale_stride_page", C.c_int64), ("scale_stride_slot", C.c_int64), ("scale_stride_head", C.c_int64),
+        ("page_table", C.c_void_p), ("table_stride", C.c_int64),
+        ("pages", C.c_int32), ("page_size", C.c_int32), ("Hkv", C.c_int32), ("d", C.c_int32), ("B", C.c_int32), ("width", C.c_int32),
+        ("dtype", C.c_int32), ("reserved_", C.c_int32),
+    ]
+
+
+class AppendArgs(C.Structure):
+    _fields_ = [
+        ("T", C.c_int32), ("Hq", C.c_int32), ("lengths", C.c_void_p), ("new_lengths", C.c_void_p), ("rotary", Rotary),
+        ("q", Tensor), ("k", Tensor), ("v", Tensor), ("q_out", Tensor),
+    ]
+
+
+class PagedAttnArgs(C.Structure):
+    _fields_ = [
+        ("T", C.c_int32), ("Hq", C.c_int32), ("lengths", C.c_void_p), ("new_lengths", C.c_void_p), ("scale", C.c_float), ("window", C.c_int32),
+        ("q", Tensor), ("o", Tensor), ("lse", C.c_void_p),
+    ]
+
+
 # name -> (restype, argtypes); the single source for the loader and for the symbol test
 SIGNATURES = {
     "bma_version": (C.c_int, []),
@@ -128,6 +173,13 @@ SIGNATURES = {
                                  C.c_void_p, C.c_void_p, C.c_void_p]),
     "bma_debug_expire_wait": (C.c_int, [C.c_uint64, C.c_int32, C.c_void_p]),
     "bma_attn_merge": (C.c_int, [C.POINTER(AttnArgs), C.c_void_p]),
+    "bma_rotate": (C.c_int, [C.POINTER(RotateArgs), C.c_void_p]),
+    "bma_rotate_bwd_workspace_bytes": (C.c_size_t, [C.POINTER(RotateArgs)]),
+    "bma_rotate_bwd": (C.c_int, [C.POINTER(RotateArgs), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "bma_append_kv": (C.c_int, [C.POINTER(PagedCacheArgs), C.POINTER(AppendArgs), C.c_void_p]),
+    "bma_read_kv": (C.c_int, [C.POINTER(PagedCacheArgs), C.c_void_p, C.c_int32, C.POINTER(Tensor), C.POINTER(Tensor), C.c_void_p]),
+    "bma_paged_attn_workspace_bytes": (C.c_size_t, [C.POINTER(PagedCacheArgs), C.POINTER(PagedAttnArgs)]),
+    "bma_paged_attn": (C.c_int, [C.POINTER(PagedCacheArgs), C.POINTER(PagedAttnArgs), C.c_void_p, C.c_size_t, C.c_void_p]),
     "bma_device_status": (C.c_int, [C.c_void_p, C.POINTER(C.c_int32)]),
 }
 

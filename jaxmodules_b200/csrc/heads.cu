@@ -1,0 +1,784 @@
+// Norm and rotation of query and key heads, and what moves whole heads into and out of the pages of a cache.
+//
+// All of these read every value once and write every result once: they are bound by memory, or for a few tokens by the launch.
+//
+// Rotation.  Component pairs are (i, i + dim/2) or (2i, 2i + 1).  A lane holds two 16-byte chunks of a head that hold both halves of its pairs
+// (chunks u and u + dim/2 of a head, or chunks 2u and 2u + 1), so that no value crosses lanes; only the sum of squares does.  A head of 128
+// bfloat16 values takes 8 lanes, a warp four heads at a time.  Cosine and sine of a lane's pairs are taken once for a token and used for all
+// of its heads.
+//
+// The angle position * frequency is kept as a fraction of a turn in 64-bit integers: frequency / 2 pi as a multiple of 2^-64, times the
+// position, modulo 2^64.  That is exact but for the rounding of the frequency (2^-53 of it in float64), however far the position; in float32 a
+// position of 10^5 would leave 0.004 of the angle open.  The upper 32 bits then go through sincospi in float32.
+#include "paged.cuh"
+
+namespace bma {
+namespace {
+
+constexpr int kHeadsThreads = 128, kHeadsWarps = kHeadsThreads / 32;
+
+template <typename T> struct Bits16;   // values of a 16-byte chunk
+template <> struct Bits16<float> { static constexpr int n = 4; };
+template <> struct Bits16<__nv_bfloat16> { static constexpr int n = 8; };
+
+// VEC values: a 16-byte chunk, or one value where the tensors allow no wider access
+template <typename T, int VEC>
+struct Chunk {
+  uint4 raw;
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (VEC == 1) raw.x = sizeof(T) == 4 ? __float_as_uint(to_float(*p)) : (uint32_t)*reinterpret_cast<const unsigned short*>(p);
+    else raw = *reinterpret_cast<const uint4*>(p);
+  }
+  __device__ __forceinline__ void zero() { raw = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void get(float (&x)[VEC]) const {
+    if constexpr (VEC == 1) x[0] = sizeof(T) == 4 ? __uint_as_float(raw.x) : __uint_as_float(raw.x << 16);
+    else if constexpr (VEC == 4) {
+      x[0] = __uint_as_float(raw.x); x[1] = __uint_as_float(raw.y); x[2] = __uint_as_float(raw.z); x[3] = __uint_as_float(raw.w);
+    } else {
+      const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+    }
+  }
+};
+template <typename T, int VEC>
+__device__ __forceinline__ void store_chunk(T* p, const float (&x)[VEC]) {
+  if constexpr (VEC == 1) *p = from_float<T>(x[0]);
+  else if constexpr (VEC == 4) *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+  else {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// cosine and sine of position * frequency, times `magnitude`
+__device__ __forceinline__ void turn_of(double frequency, long long position, float magnitude, float& c, float& s) {
+  double turns = frequency * 0.15915494309189533577;
+  turns -= floor(turns);
+  const unsigned long long step = __double2ull_rz(turns * 18446744073709551616.0);
+  const long long phase = (long long)((unsigned long long)position * step);
+  sincospif((float)(int)(phase >> 32) * 4.656612873077392578125e-10f, &s, &c);   // half turns in [-1, 1]
+  c *= magnitude;
+  s *= magnitude;
+}
+
+// How the lanes of a warp lie on heads: `tpr` lanes (a power of two) to a head, each with UPT units of two chunks.
+struct HeadMap {
+  int tpr, chunks, half_chunks, dim, layout;   // half_chunks: dim / 2 in chunks (HALF layout)
+};
+
+template <int VEC>
+__device__ __forceinline__ void unit_chunks(const HeadMap& m, int u, int& ca, int& cb) {
+  if (m.layout == BMA_ROTARY_INTERLEAVED) { ca = 2 * u; cb = 2 * u + 1; }
+  else if (u < m.half_chunks) { ca = u; cb = u + m.half_chunks; }
+  else { ca = 2 * u; cb = 2 * u + 1; }   // (what is not rotated: chunks from 2 * half_chunks on)
+}
+
+// The pairs of one unit: pair j is rotated where bit j of `live` is set.
+template <int VEC>
+struct Turns {
+  float c[VEC], s[VEC];
+  uint32_t live;
+  __device__ __forceinline__ void make(const HeadMap& m, const double* frequencies, int u, long long position, float magnitude) {
+    live = 0;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      const int i = u * VEC + j;
+      c[j] = 1.f; s[j] = 0.f;
+      if (2 * i < m.dim) {
+        live |= 1u << j;
+        turn_of(__ldg(frequencies + i), position, magnitude, c[j], s[j]);
+      }
+    }
+  }
+  // BACK: by the negative angle
+  template <bool BACK>
+  __device__ __forceinline__ void apply(int layout, float (&a)[VEC], float (&b)[VEC]) const {
+    if (VEC > 1 && layout == BMA_ROTARY_INTERLEAVED) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        float& x = 2 * j < VEC ? a[(2 * j) % VEC] : b[(2 * j) % VEC];
+        float& y = 2 * j < VEC ? a[(2 * j + 1) % VEC] : b[(2 * j + 1) % VEC];
+        one<BACK>(j, x, y);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) one<BACK>(j, a[j], b[j]);
+    }
+  }
+  template <bool BACK>
+  __device__ __forceinline__ void one(int j, float& x, float& y) const {
+    const float sn = BACK ? -s[j] : s[j];
+    const float p = x * c[j] - y * sn, q = y * c[j] + x * sn;
+    if (live >> j & 1) { x = p; y = q; }
+  }
+};
+
+__device__ __forceinline__ float group_sum(float x, int tpr) {
+  for (int o = tpr >> 1; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
+}
+
+template <int VEC>
+__device__ __forceinline__ void load_weight(const void* w, int dtype, int chunk, int chunks, float (&x)[VEC]) {
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) {
+    x[j] = 0.f;
+    if (chunk < chunks) x[j] = dtype == BMA_DTYPE_F32 ? __ldg(static_cast<const float*>(w) + chunk * VEC + j)
+                                                      : __bfloat162float(static_cast<const __nv_bfloat16*>(w)[chunk * VEC + j]);
+  }
+}
+
+// One side (q, k or v) of a launch: where its heads come from and go to.
+struct Side {
+  bma_tensor in, out;
+  const void* weight;
+  int heads;
+  int turned;
+};
+
+struct HeadsParams {
+  Side side[3];          // q, k, v
+  int B, L, d, slabs, slab_heads;
+  HeadMap map;
+  const double* frequencies;
+  float magnitude, eps;
+  int weight_dtype;
+  const void* positions;
+  int position_bytes;
+  int64_t position_stride_b, position_stride_l;
+  int back;              // rotate by the negative angle (the backward pass of a rotation alone)
+  // appending
+  bma_paged_cache cache;
+  const int32_t *lengths, *new_lengths;
+  int* status;
+};
+
+enum { kRotate = 0, kAppend = 1, kAppend4 = 2 };
+
+// e2m1 codes and powers of two of a warp's heads, whose values lie in shared memory: each lane takes 8 values, four lanes 32.
+__device__ __forceinline__ void store_4bit(const float* row, bool there, int d, int tpr, int u, uint8_t* codes, uint8_t* scales) {
+  for (int p = u; p - u < kPagedHeadDim / 8; p += tpr) {       // (every lane of the warp goes round as often)
+    float x[8];
+    float top = 0.f;
+    bool nan = false;
+    const bool in = p * 8 < d;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      x[i] = in ? row[p * 8 + i] : 0.f;
+      nan |= x[i] != x[i];
+      top = fmaxf(top, fabsf(x[i]));
+    }
+    top = nan ? __uint_as_float(0x7fffffffu) : top;
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+      const float t = __shfl_xor_sync(0xffffffffu, top, o);
+      top = top != top || t != t ? __uint_as_float(0x7fffffffu) : fmaxf(top, t);
+    }
+    // smallest e with top <= 6 * 2^e = 1.5 * 2^(e + 2): from the exponent and the mantissa of top
+    const uint32_t bits = __float_as_uint(top);
+    int e = (int)(bits >> 23) - 127 - ((bits & 0x7fffffu) <= 0x400000u ? 2 : 1);
+    e = min(max(e, -127), 126);
+    const float inv = __uint_as_float((uint32_t)(127 - e) << 23);      // 2^-e, e from -127 (2^127) to 126
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w |= to_e2m1x2(x[2 * i] * inv, x[2 * i + 1] * inv) << (8 * i);
+    if (there && in) {
+      *reinterpret_cast<uint32_t*>(codes + p * 4) = w;
+      if ((p & 3) == 0) scales[p >> 2] = top != top ? 255 : (uint8_t)(e + 127);
+    }
+  }
+}
+
+// A warp takes one token and a slab of its heads (all sides counted through), `tpr` lanes to a head, NR heads at a time.
+template <typename T, int VEC, int UPT, int NR, int KIND>
+__global__ void __launch_bounds__(kHeadsThreads) heads_kernel(const __grid_constant__ HeadsParams p) {
+  __shared__ float rows[KIND == kAppend4 ? kHeadsWarps : 1][KIND == kAppend4 ? 8 : 1][KIND == kAppend4 ? kPagedHeadDim + 4 : 1];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t item = (int64_t)blockIdx.x * kHeadsWarps + warp;
+  const int64_t token = item / p.slabs;
+  const int slab = (int)(item - token * p.slabs);
+  const int b = (int)(token / p.L), t = (int)(token - (int64_t)b * p.L);
+  if (b >= p.B) return;
+  const int tpr = p.map.tpr, group = lane / tpr, u0 = lane & (tpr - 1), groups = 32 / tpr;
+
+  long long position = t;
+  bool real = true;
+  int64_t held = 0, held_scale = 0;      // offsets of the token in the cache
+  if constexpr (KIND == kRotate) {
+    if (p.positions) {
+      const int64_t at = b * p.position_stride_b + t * p.position_stride_l;
+      position = p.position_bytes == 8 ? __ldg(static_cast<const long long*>(p.positions) + at) : (long long)__ldg(static_cast<const int*>(p.positions) + at);
+    }
+  } else {
+    const NewTokens n = new_tokens(p.lengths, p.new_lengths, b, p.L);
+    position = n.first + t;
+    real = t < n.count;
+    int slot = 0;
+    const int page = real ? page_of(p.cache, b, position, slot) : 0;
+    if (page < 0) {
+      if (lane == 0) report_device_error(p.status, kStatusAppend);
+      held = -1;
+    } else if (real) {
+      held = (int64_t)page * p.cache.stride_page + (int64_t)slot * p.cache.stride_slot;
+      held_scale = (int64_t)page * p.cache.scale_stride_page + (int64_t)slot * p.cache.scale_stride_slot;
+    }
+  }
+
+  Turns<VEC> turns[UPT];
+  int ca[UPT], cb[UPT];
+  const bool turned = p.map.dim > 0;
+#pragma unroll
+  for (int i = 0; i < UPT; ++i) {
+    unit_chunks<VEC>(p.map, u0 + i * tpr, ca[i], cb[i]);
+    if (turned) turns[i].make(p.map, p.frequencies, u0 + i * tpr, position, p.magnitude);
+  }
+  const int slab_begin = slab * p.slab_heads, slab_end = slab_begin + p.slab_heads;
+  const float inv_d = 1.f / (float)p.d;
+
+  int first = 0;      // heads of the sides before
+#pragma unroll 1
+  for (int si = 0; si < (KIND == kRotate ? 2 : 3); ++si) {
+    const Side& side = p.side[si];
+    const int lo = max(slab_begin - first, 0), hi = min(slab_end - first, side.heads);
+    first += side.heads;
+    if (lo >= hi) continue;
+    const bool cached = KIND != kRotate && si > 0;
+    if (cached && (!real || held < 0)) continue;
+    const T* in = static_cast<const T*>(side.in.ptr) + b * side.in.stride_b + t * side.in.stride_l;
+    T* out = static_cast<T*>(side.out.ptr) + b * side.out.stride_b + t * side.out.stride_l;
+    int64_t out_head = side.out.stride_h;
+    if (cached) {
+      out = static_cast<T*>(si == 1 ? p.cache.k : p.cache.v) + held;      // (a 4-bit cache is not written through this)
+      out_head = p.cache.stride_head;
+    }
+    float wa[UPT][VEC], wb[UPT][VEC];
+    const bool normed = side.weight != nullptr;
+    if (normed) {
+#pragma unroll
+      for (int i = 0; i < UPT; ++i) {
+        load_weight<VEC>(side.weight, p.weight_dtype, ca[i], p.map.chunks, wa[i]);
+        load_weight<VEC>(side.weight, p.weight_dtype, cb[i], p.map.chunks, wb[i]);
+      }
+    }
+#pragma unroll 1
+    for (int h0 = lo; h0 < hi; h0 += groups * NR) {
+      Chunk<T, VEC> a[NR][UPT], c[NR][UPT];
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        const int h = h0 + r * groups + group;
+#pragma unroll
+        for (int i = 0; i < UPT; ++i) {
+          a[r][i].zero();
+          c[r][i].zero();
+          if (h < hi && real) {
+            if (ca[i] < p.map.chunks) a[r][i].load(in + h * side.in.stride_h + ca[i] * VEC);
+            if (cb[i] < p.map.chunks) c[r][i].load(in + h * side.in.stride_h + cb[i] * VEC);
+          }
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        const int h = h0 + r * groups + group;
+        float xa[UPT][VEC], xb[UPT][VEC];
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < UPT; ++i) {
+          a[r][i].get(xa[i]);
+          c[r][i].get(xb[i]);
+        }
+        if (normed) {
+#pragma unroll
+          for (int i = 0; i < UPT; ++i)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) sum = fmaf(xa[i][j], xa[i][j], fmaf(xb[i][j], xb[i][j], sum));
+          const float inv = rsqrtf(group_sum(sum, tpr) * inv_d + p.eps);
+#pragma unroll
+          for (int i = 0; i < UPT; ++i)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) { xa[i][j] *= inv * wa[i][j]; xb[i][j] *= inv * wb[i][j]; }
+        }
+        if (turned && side.turned) {
+#pragma unroll
+          for (int i = 0; i < UPT; ++i) {
+            if (p.back) turns[i].template apply<true>(p.map.layout, xa[i], xb[i]);
+            else turns[i].template apply<false>(p.map.layout, xa[i], xb[i]);
+          }
+        }
+        if (KIND == kAppend4 && cached) {
+          float* row = rows[warp][group];
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < UPT; ++i)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+              if (ca[i] < p.map.chunks) row[ca[i] * VEC + j] = xa[i][j];
+              if (cb[i] < p.map.chunks) row[cb[i] * VEC + j] = xb[i][j];
+            }
+          __syncwarp();
+          uint8_t* codes = static_cast<uint8_t*>(si == 1 ? p.cache.k : p.cache.v) + held + h * p.cache.stride_head;
+          uint8_t* scales = (si == 1 ? p.cache.k_scale : p.cache.v_scale) + held_scale + h * p.cache.scale_stride_head;
+          store_4bit(row, h < hi, p.d, tpr, u0, codes, scales);
+        } else if (h < hi) {
+          if (!real) {
+#pragma unroll
+            for (int i = 0; i < UPT; ++i)
+#pragma unroll
+              for (int j = 0; j < VEC; ++j) xa[i][j] = xb[i][j] = 0.f;
+          }
+#pragma unroll
+          for (int i = 0; i < UPT; ++i) {
+            if (ca[i] < p.map.chunks) store_chunk<T, VEC>(out + h * out_head + ca[i] * VEC, xa[i]);
+            if (cb[i] < p.map.chunks) store_chunk<T, VEC>(out + h * out_head + cb[i] * VEC, xb[i]);
+          }
+        }
+      }
+    }
+  }
+}
+
+// Backward of norm and rotation.  With g' = the cotangent turned back, x^ = x * inv and the norm's weight w:
+//   dx = inv * (g' w - x^ mean(g' w x^)),  dw = sum over tokens and heads of g' x^.
+// The first `q_ctas` CTAs take q, the others k; each warp goes over tokens and keeps its share of dw in registers, the CTAs' shares go to
+// `partial` [CTAs, d] and are added up by weight_sum_kernel in a fixed order.
+struct BackParams {
+  Side side[2];          // in: x, out: dx
+  bma_tensor g[2];
+  int B, L, d, q_ctas;
+  HeadMap map;
+  const double* frequencies;
+  float magnitude, eps;
+  int weight_dtype;
+  const void* positions;
+  int position_bytes;
+  int64_t position_stride_b, position_stride_l;
+  float* partial;
+};
+
+template <typename T, int VEC, int UPT>
+__global__ void __launch_bounds__(kHeadsThreads, 4) rotate_back_kernel(const __grid_constant__ BackParams p) {
+  __shared__ float sums[kHeadsWarps][256];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int tpr = p.map.tpr, group = lane / tpr, u0 = lane & (tpr - 1), groups = 32 / tpr;
+  const int si = (int)blockIdx.x < p.q_ctas ? 0 : 1;
+  const int cta = si ? blockIdx.x - p.q_ctas : blockIdx.x, ctas = si ? gridDim.x - p.q_ctas : p.q_ctas;
+  const Side& side = p.side[si];
+  const bma_tensor& g = p.g[si];
+  const float inv_d = 1.f / (float)p.d;
+  int ca[UPT], cb[UPT];
+  float wa[UPT][VEC], wb[UPT][VEC], da[UPT][VEC], db[UPT][VEC];
+#pragma unroll
+  for (int i = 0; i < UPT; ++i) {
+    unit_chunks<VEC>(p.map, u0 + i * tpr, ca[i], cb[i]);
+    load_weight<VEC>(side.weight, p.weight_dtype, ca[i], p.map.chunks, wa[i]);
+    load_weight<VEC>(side.weight, p.weight_dtype, cb[i], p.map.chunks, wb[i]);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) da[i][j] = db[i][j] = 0.f;
+  }
+  const int64_t tokens = (int64_t)p.B * p.L;
+#pragma unroll 1
+  for (int64_t token = (int64_t)cta * kHeadsWarps + warp; token < tokens; token += (int64_t)ctas * kHeadsWarps) {
+    const int b = (int)(token / p.L), t = (int)(token - (int64_t)b * p.L);
+    long long position = t;
+    if (p.positions) {
+      const int64_t at = b * p.position_stride_b + t * p.position_stride_l;
+      position = p.position_bytes == 8 ? __ldg(static_cast<const long long*>(p.positions) + at) : (long long)__ldg(static_cast<const int*>(p.positions) + at);
+    }
+    Turns<VEC> turns[UPT];
+    const bool turned = p.map.dim > 0;
+    if (turned) {
+#pragma unroll
+      for (int i = 0; i < UPT; ++i) turns[i].make(p.map, p.frequencies, u0 + i * tpr, position, p.magnitude);
+    }
+    const T* in = static_cast<const T*>(side.in.ptr) + b * side.in.stride_b + t * side.in.stride_l;
+    const T* gin = static_cast<const T*>(g.ptr) + b * g.stride_b + t * g.stride_l;
+    T* out = static_cast<T*>(side.out.ptr) + b * side.out.stride_b + t * side.out.stride_l;
+#pragma unroll 1
+    for (int h0 = 0; h0 < side.heads; h0 += groups) {
+      const int h = h0 + group;
+      Chunk<T, VEC> xa[UPT], xb[UPT], ga[UPT], gb[UPT];
+#pragma unroll
+      for (int i = 0; i < UPT; ++i) {
+        xa[i].zero(); xb[i].zero(); ga[i].zero(); gb[i].zero();
+        if (h < side.heads && ca[i] < p.map.chunks) {
+          xa[i].load(in + h * side.in.stride_h + ca[i] * VEC);
+          ga[i].load(gin + h * g.stride_h + ca[i] * VEC);
+        }
+        if (h < side.heads && cb[i] < p.map.chunks) {
+          xb[i].load(in + h * side.in.stride_h + cb[i] * VEC);
+          gb[i].load(gin + h * g.stride_h + cb[i] * VEC);
+        }
+      }
+      float fa[UPT][VEC], fb[UPT][VEC], ea[UPT][VEC], eb[UPT][VEC];
+      float sum = 0.f, dot = 0.f;
+#pragma unroll
+      for (int i = 0; i < UPT; ++i) {
+        xa[i].get(fa[i]); xb[i].get(fb[i]); ga[i].get(ea[i]); gb[i].get(eb[i]);
+        if (turned) turns[i].template apply<true>(p.map.layout, ea[i], eb[i]);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          sum = fmaf(fa[i][j], fa[i][j], fmaf(fb[i][j], fb[i][j], sum));
+          dot = fmaf(ea[i][j] * wa[i][j], fa[i][j], fmaf(eb[i][j] * wb[i][j], fb[i][j], dot));
+        }
+      }
+      for (int o = tpr >> 1; o; o >>= 1) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        dot += __shfl_xor_sync(0xffffffffu, dot, o);
+      }
+      const float inv = rsqrtf(sum * inv_d + p.eps), m = dot * inv * inv_d;     // m = mean(g' w x^)
+#pragma unroll
+      for (int i = 0; i < UPT; ++i) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const float ha = fa[i][j] * inv, hb = fb[i][j] * inv;
+          if (h < side.heads) {
+            da[i][j] = fmaf(ea[i][j], ha, da[i][j]);
+            db[i][j] = fmaf(eb[i][j], hb, db[i][j]);
+          }
+          ea[i][j] = inv * (ea[i][j] * wa[i][j] - ha * m);
+          eb[i][j] = inv * (eb[i][j] * wb[i][j] - hb * m);
+        }
+        if (h < side.heads) {
+          if (ca[i] < p.map.chunks) store_chunk<T, VEC>(out + h * side.out.stride_h + ca[i] * VEC, ea[i]);
+          if (cb[i] < p.map.chunks) store_chunk<T, VEC>(out + h * side.out.stride_h + cb[i] * VEC, eb[i]);
+        }
+      }
+    }
+  }
+  // the groups of a warp, the warps of the CTA
+#pragma unroll
+  for (int i = 0; i < UPT; ++i)
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      for (int o = tpr; o < 32; o <<= 1) {
+        da[i][j] += __shfl_xor_sync(0xffffffffu, da[i][j], o);
+        db[i][j] += __shfl_xor_sync(0xffffffffu, db[i][j], o);
+      }
+      if (group == 0) {
+        if (ca[i] < p.map.chunks) sums[warp][ca[i] * VEC + j] = da[i][j];
+        if (cb[i] < p.map.chunks) sums[warp][cb[i] * VEC + j] = db[i][j];
+      }
+    }
+  __syncthreads();
+  for (int c = threadIdx.x; c < p.d; c += kHeadsThreads) {
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < kHeadsWarps; ++w) s += sums[w][c];
+    p.partial[(int64_t)blockIdx.x * p.d + c] = s;
+  }
+}
+
+// dw of q (blockIdx.y 0) and k: columns of `partial` added up, 32 columns to a CTA, 32 rows at a time.
+__global__ void __launch_bounds__(1024) weight_sum_kernel(const float* partial, int q_ctas, int k_ctas, int d, void* dq, void* dk, int dtype) {
+  __shared__ float sums[32][33];
+  const bool k = blockIdx.y;
+  const float* rows = partial + (k ? (int64_t)q_ctas * d : 0);
+  const int n = k ? k_ctas : q_ctas, c = blockIdx.x * 32 + threadIdx.x;
+  void* out = k ? dk : dq;
+  if (!n || !out) return;
+  float s = 0.f;
+  if (c < d)
+    for (int r = threadIdx.y; r < n; r += 32) s += rows[(int64_t)r * d + c];
+  sums[threadIdx.y][threadIdx.x] = s;
+  __syncthreads();
+  s = sums[threadIdx.x][threadIdx.y];       // column blockIdx.x * 32 + threadIdx.y
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  const int col = blockIdx.x * 32 + threadIdx.y;
+  if (threadIdx.x == 0 && col < d) {
+    if (dtype == BMA_DTYPE_F32) static_cast<float*>(out)[col] = s;
+    else static_cast<__nv_bfloat16*>(out)[col] = __float2bfloat16_rn(s);
+  }
+}
+
+// Pages back to dense rows: a thread moves 16 bytes of the output (8 values of a 4-bit cache) of keys and of values.
+template <int DTYPE>
+__global__ void __launch_bounds__(256) read_kv_kernel(const __grid_constant__ bma_paged_cache c, const int32_t* lengths, int L, const bma_tensor k, const bma_tensor v,
+                                                      int* status) {
+  using T = typename std::conditional<DTYPE == BMA_DTYPE_F32, float, __nv_bfloat16>::type;
+  constexpr int VEC = Bits16<T>::n;
+  const int per_head = c.d / VEC, per_token = c.Hkv * per_head;
+  const int64_t token = blockIdx.x * (int64_t)blockDim.y + threadIdx.y;
+  const int b = (int)(token / L), t = (int)(token - (int64_t)b * L);
+  if (b >= c.B) return;
+  int slot = 0, page = -1;
+  const bool there = t < __ldg(lengths + b);
+  if (there) {
+    page = page_of(c, b, t, slot);
+    if (page < 0 && threadIdx.x == 0) report_device_error(status, kStatusRead);
+  }
+  const int64_t held = page < 0 ? 0 : (int64_t)page * c.stride_page + (int64_t)slot * c.stride_slot;
+  const int64_t held_scale = page < 0 ? 0 : (int64_t)page * c.scale_stride_page + (int64_t)slot * c.scale_stride_slot;
+  for (int i = threadIdx.x; i < per_token; i += blockDim.x) {
+    const int h = i / per_head, at = (i - h * per_head) * VEC;
+    uint4 x[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+    if (page >= 0) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        if constexpr (DTYPE == BMA_DTYPE_MXFP4) {
+          const uint32_t codes = __ldg(reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(s ? c.v : c.k) + held + h * c.stride_head + at / 2));
+          const float f = e8m0_value(__ldg((s ? c.v_scale : c.k_scale) + held_scale + h * c.scale_stride_head + at / 32));
+          uint32_t pairs[4], w[4];
+          from_e2m1x8(codes, pairs);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&pairs[j]));
+            const __nv_bfloat162 r = __floats2bfloat162_rn(y.x * f, y.y * f);       // (exact: two significant bits)
+            w[j] = *reinterpret_cast<const uint32_t*>(&r);
+          }
+          x[s] = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+          x[s] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(s ? c.v : c.k) + held + h * c.stride_head + at));
+        }
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const bma_tensor& o = s ? v : k;
+      *reinterpret_cast<uint4*>(static_cast<T*>(o.ptr) + b * o.stride_b + t * o.stride_l + h * o.stride_h + at) = x[s];
+    }
+  }
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------------------
+int sms() {
+  int dev = 0, n = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  return n;
+}
+
+int validate_rotary(const bma_rotary& r, int d) {
+  BMA_REQUIRE(r.dim >= 0 && r.dim % 2 == 0 && r.dim <= d, BMA_ERR_ARG);
+  BMA_REQUIRE(r.dim == 0 || r.frequencies, BMA_ERR_ARG);
+  BMA_REQUIRE(r.layout == BMA_ROTARY_HALF || r.layout == BMA_ROTARY_INTERLEAVED, BMA_ERR_ARG);
+  BMA_REQUIRE((!r.q_weight && !r.k_weight) || r.weight_dtype == BMA_DTYPE_F32 || r.weight_dtype == BMA_DTYPE_BF16, BMA_ERR_UNSUPPORTED);
+  return BMA_OK;
+}
+
+bool wide_tensor(const bma_tensor& t, int vec) {
+  return (reinterpret_cast<uintptr_t>(t.ptr) & 15) == 0 && t.stride_b % vec == 0 && t.stride_l % vec == 0 && t.stride_h % vec == 0;
+}
+
+// 16-byte chunks where every tensor allows them and no pair of the HALF layout has its halves in the middle of chunks
+bool wide_heads(const bma_rotary& r, int d, int vec) { return d % vec == 0 && (r.layout == BMA_ROTARY_INTERLEAVED || (r.dim / 2) % vec == 0); }
+
+HeadMap head_map(const bma_rotary& r, int d, int vec, int least) {
+  HeadMap m{};
+  m.chunks = ceil_div(d, vec);
+  m.half_chunks = r.dim / 2 / vec;
+  m.dim = r.dim;
+  m.layout = r.layout;
+  m.tpr = least;
+  while (m.tpr < 32 && m.tpr < (m.chunks + 1) / 2) m.tpr *= 2;
+  return m;
+}
+
+// Warps of a launch take a token and `slab_heads` of its heads: all of them where there are tokens enough for 16 warps an SM, fewer
+// (down to one pass of the warp) where there are not.
+void cut_heads(HeadsParams& p, int64_t tokens, int heads, int pass) {
+  const int64_t want = ceil_div(sms() * 16, (int)std::min<int64_t>(tokens, 1 << 20));
+  p.slab_heads = (int)std::max<int64_t>(pass, ceil_div(heads, (int)want));
+  p.slab_heads = ceil_div(p.slab_heads, pass) * pass;
+  p.slabs = ceil_div(heads, p.slab_heads);
+}
+
+template <typename T, int KIND>
+int launch_heads(HeadsParams& p, const bma_rotary& r, bool wide, cudaStream_t st) {
+  const int vec = wide ? Bits16<T>::n : 1;
+  p.map = head_map(r, p.d, vec, KIND == kAppend4 ? 4 : 1);
+  const int64_t tokens = (int64_t)p.B * p.L;
+  const int heads = p.side[0].heads + p.side[1].heads + p.side[2].heads;
+  cut_heads(p, tokens, heads, 32 / p.map.tpr);
+  const int64_t ctas = (tokens * p.slabs + kHeadsWarps - 1) / kHeadsWarps;
+  BMA_REQUIRE(ctas < (1ll << 31), BMA_ERR_LIMIT);
+  if (wide) heads_kernel<T, Bits16<T>::n, 1, 2, KIND><<<(unsigned)ctas, kHeadsThreads, 0, st>>>(p);
+  else heads_kernel<T, 1, 4, 1, KIND><<<(unsigned)ctas, kHeadsThreads, 0, st>>>(p);
+  count_launches(1);
+  BMA_CUDA_TRY(cudaGetLastError());
+  return BMA_OK;
+}
+
+int validate_heads(const bma_tensor& t, int dtype) {
+  BMA_REQUIRE(t.ptr, BMA_ERR_ARG);
+  BMA_REQUIRE(t.dtype == BMA_DTYPE_F32 || t.dtype == BMA_DTYPE_BF16, BMA_ERR_UNSUPPORTED);
+  BMA_REQUIRE(t.dtype == dtype, BMA_ERR_UNSUPPORTED);
+  return BMA_OK;
+}
+
+int validate_rotate(const bma_rotate_args* a) {
+  BMA_REQUIRE(a, BMA_ERR_ARG);
+  BMA_REQUIRE(a->B > 0 && a->L > 0 && a->Hq > 0 && a->Hkv >= 0 && a->d > 0, BMA_ERR_ARG);
+  BMA_REQUIRE(a->d <= 256, BMA_ERR_UNSUPPORTED);
+  BMA_REQUIRE(a->Hq <= 65535 && a->Hkv <= 65535, BMA_ERR_LIMIT);
+  BMA_REQUIRE(!a->positions || a->position_bytes == 4 || a->position_bytes == 8, BMA_ERR_ARG);
+  return validate_rotary(a->rotary, a->d);
+}
+
+HeadsParams rotate_params(const bma_rotate_args& a) {
+  HeadsParams p{};
+  p.B = a.B; p.L = a.L; p.d = a.d;
+  p.frequencies = a.rotary.frequencies;
+  p.magnitude = a.rotary.magnitude; p.eps = a.rotary.eps;
+  p.weight_dtype = a.rotary.weight_dtype;
+  p.positions = a.positions; p.position_bytes = a.position_bytes;
+  p.position_stride_b = a.position_stride_b; p.position_stride_l = a.position_stride_l;
+  return p;
+}
+
+// CTAs of the backward pass with weights: (q, k), in proportion to their heads; a side without a norm goes through heads_kernel.
+// Four CTAs of four warps run on an SM.
+void back_ctas(const bma_rotate_args& a, int& q, int& k) {
+  const int hq = a.rotary.q_weight ? a.Hq : 0, hk = a.rotary.k_weight ? a.Hkv : 0;
+  const int64_t tokens = (int64_t)a.B * a.L;
+  const int64_t most = (tokens + kHeadsWarps - 1) / kHeadsWarps;
+  const int64_t all = (int64_t)sms() * 4;
+  q = hq ? (int)std::max<int64_t>(1, std::min(most, all * hq / (hq + hk))) : 0;
+  k = hk ? (int)std::max<int64_t>(1, std::min(most, all * hk / (hq + hk))) : 0;
+}
+
+}  // namespace
+
+int rotate_forward(const bma_rotate_args* a, cudaStream_t st) {
+  int rc = validate_rotate(a);
+  if (rc != BMA_OK) return rc;
+  if ((rc = validate_heads(a->q, a->q.dtype)) || (rc = validate_heads(a->q_out, a->q.dtype))) return rc;
+  if (a->Hkv && ((rc = validate_heads(a->k, a->q.dtype)) || (rc = validate_heads(a->k_out, a->q.dtype)))) return rc;
+  HeadsParams p = rotate_params(*a);
+  p.side[0] = {a->q, a->q_out, a->rotary.q_weight, a->Hq, 1};
+  p.side[1] = {a->k, a->k_out, a->rotary.k_weight, a->Hkv, 1};
+  const int vec = a->q.dtype == BMA_DTYPE_F32 ? 4 : 8;
+  const bool wide = wide_heads(a->rotary, a->d, vec) && wide_tensor(a->q, vec) && wide_tensor(a->q_out, vec) &&
+                    (!a->Hkv || (wide_tensor(a->k, vec) && wide_tensor(a->k_out, vec)));
+  return a->q.dtype == BMA_DTYPE_F32 ? launch_heads<float, kRotate>(p, a->rotary, wide, st) : launch_heads<__nv_bfloat16, kRotate>(p, a->rotary, wide, st);
+}
+
+size_t rotate_back_bytes(const bma_rotate_args* a) {
+  if (validate_rotate(a) != BMA_OK) return 0;
+  int q, k;
+  back_ctas(*a, q, k);
+  return (size_t)(q + k) * a->d * sizeof(float);
+}
+
+int rotate_backward(const bma_rotate_args* a, void* workspace, size_t bytes, cudaStream_t st) {
+  int rc = validate_rotate(a);
+  if (rc != BMA_OK) return rc;
+  const bool qn = a->rotary.q_weight, kn = a->Hkv && a->rotary.k_weight;
+  const int dtype = a->q_out.dtype;
+  if ((rc = validate_heads(a->q_out, dtype)) || (rc = validate_heads(a->dq, dtype)) || (qn && (rc = validate_heads(a->q, dtype)))) return rc;
+  if (a->Hkv && ((rc = validate_heads(a->k_out, dtype)) || (rc = validate_heads(a->dk, dtype)) || (kn && (rc = validate_heads(a->k, dtype))))) return rc;
+  BMA_REQUIRE((!qn || a->dq_weight) && (!kn || a->dk_weight), BMA_ERR_ARG);
+  const int vec = dtype == BMA_DTYPE_F32 ? 4 : 8;
+  const bool fits = wide_heads(a->rotary, a->d, vec);
+  const bool q_wide = wide_tensor(a->q_out, vec) && wide_tensor(a->dq, vec) && (!qn || wide_tensor(a->q, vec));
+  const bool k_wide = wide_tensor(a->k_out, vec) && wide_tensor(a->dk, vec) && (!kn || wide_tensor(a->k, vec));
+  if (qn || kn) {
+    BMA_REQUIRE(workspace && bytes >= rotate_back_bytes(a) && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0, BMA_ERR_WORKSPACE);
+    BackParams p{};
+    p.side[0] = {a->q, a->dq, a->rotary.q_weight, qn ? a->Hq : 0, 1};
+    p.side[1] = {a->k, a->dk, a->rotary.k_weight, kn ? a->Hkv : 0, 1};
+    p.g[0] = a->q_out; p.g[1] = a->k_out;
+    p.B = a->B; p.L = a->L; p.d = a->d;
+    p.frequencies = a->rotary.frequencies;
+    p.magnitude = a->rotary.magnitude; p.eps = a->rotary.eps;
+    p.weight_dtype = a->rotary.weight_dtype;
+    p.positions = a->positions; p.position_bytes = a->position_bytes;
+    p.position_stride_b = a->position_stride_b; p.position_stride_l = a->position_stride_l;
+    p.partial = static_cast<float*>(workspace);
+    int k_ctas;
+    back_ctas(*a, p.q_ctas, k_ctas);
+    const bool wide = fits && (!qn || q_wide) && (!kn || k_wide);
+    p.map = head_map(a->rotary, a->d, wide ? vec : 1, 1);
+    const unsigned ctas = (unsigned)(p.q_ctas + k_ctas);
+    if (dtype == BMA_DTYPE_F32) {
+      if (wide) rotate_back_kernel<float, 4, 1><<<ctas, kHeadsThreads, 0, st>>>(p);
+      else rotate_back_kernel<float, 1, 4><<<ctas, kHeadsThreads, 0, st>>>(p);
+    } else {
+      if (wide) rotate_back_kernel<__nv_bfloat16, 8, 1><<<ctas, kHeadsThreads, 0, st>>>(p);
+      else rotate_back_kernel<__nv_bfloat16, 1, 4><<<ctas, kHeadsThreads, 0, st>>>(p);
+    }
+    weight_sum_kernel<<<dim3(ceil_div(a->d, 32), 2), dim3(32, 32), 0, st>>>(p.partial, p.q_ctas, k_ctas, a->d, a->dq_weight, a->dk_weight, a->rotary.weight_dtype);
+    count_launches(2);
+    BMA_CUDA_TRY(cudaGetLastError());
+  }
+  if (!qn || (a->Hkv && !kn)) {      // sides without a norm: the rotation by the negative angle
+    HeadsParams p = rotate_params(*a);
+    p.back = 1;
+    if (!qn) p.side[0] = {a->q_out, a->dq, nullptr, a->Hq, 1};
+    if (a->Hkv && !kn) p.side[1] = {a->k_out, a->dk, nullptr, a->Hkv, 1};
+    const bool wide = fits && (qn || q_wide) && (!p.side[1].heads || k_wide);
+    return dtype == BMA_DTYPE_F32 ? launch_heads<float, kRotate>(p, a->rotary, wide, st) : launch_heads<__nv_bfloat16, kRotate>(p, a->rotary, wide, st);
+  }
+  return BMA_OK;
+}
+
+int append_kv(const bma_paged_cache* c, const bma_append_args* a, cudaStream_t st) {
+  int rc = validate_cache(c);
+  if (rc != BMA_OK) return rc;
+  BMA_REQUIRE(a && a->T > 0 && a->Hq >= 0 && a->lengths, BMA_ERR_ARG);
+  BMA_REQUIRE(a->Hq <= 65535, BMA_ERR_LIMIT);
+  if ((rc = validate_rotary(a->rotary, c->d))) return rc;
+  const int dtype = c->dtype == BMA_DTYPE_MXFP4 ? a->k.dtype : c->dtype;
+  if ((rc = validate_heads(a->k, dtype)) || (rc = validate_heads(a->v, dtype))) return rc;
+  if (a->Hq && ((rc = validate_heads(a->q, dtype)) || (rc = validate_heads(a->q_out, dtype)))) return rc;
+  HeadsParams p{};
+  p.B = c->B; p.L = a->T; p.d = c->d;
+  p.frequencies = a->rotary.frequencies;
+  p.magnitude = a->rotary.magnitude; p.eps = a->rotary.eps;
+  p.weight_dtype = a->rotary.weight_dtype;
+  p.side[0] = {a->q, a->q_out, a->rotary.q_weight, a->Hq, 1};
+  p.side[1] = {a->k, {}, a->rotary.k_weight, c->Hkv, 1};
+  p.side[2] = {a->v, {}, nullptr, c->Hkv, 0};
+  p.cache = *c;
+  p.lengths = a->lengths; p.new_lengths = a->new_lengths;
+  BMA_REQUIRE((p.status = device_status_ptr()) != nullptr, BMA_ERR_CUDA);
+  const int vec = dtype == BMA_DTYPE_F32 ? 4 : 8;
+  const bool wide = wide_heads(a->rotary, c->d, vec) && wide_tensor(a->k, vec) && wide_tensor(a->v, vec) &&
+                    (!a->Hq || (wide_tensor(a->q, vec) && wide_tensor(a->q_out, vec)));
+  if (c->dtype == BMA_DTYPE_MXFP4)
+    return dtype == BMA_DTYPE_F32 ? launch_heads<float, kAppend4>(p, a->rotary, wide, st) : launch_heads<__nv_bfloat16, kAppend4>(p, a->rotary, wide, st);
+  return dtype == BMA_DTYPE_F32 ? launch_heads<float, kAppend>(p, a->rotary, wide, st) : launch_heads<__nv_bfloat16, kAppend>(p, a->rotary, wide, st);
+}
+
+int read_kv(const bma_paged_cache* c, const int32_t* lengths, int L, const bma_tensor* k, const bma_tensor* v, cudaStream_t st) {
+  int rc = validate_cache(c);
+  if (rc != BMA_OK) return rc;
+  BMA_REQUIRE(lengths && L > 0 && k && v, BMA_ERR_ARG);
+  const int dtype = c->dtype == BMA_DTYPE_F32 ? BMA_DTYPE_F32 : BMA_DTYPE_BF16, vec = dtype == BMA_DTYPE_F32 ? 4 : 8;
+  if ((rc = validate_heads(*k, dtype)) || (rc = validate_heads(*v, dtype))) return rc;
+  BMA_REQUIRE(wide_tensor(*k, vec) && wide_tensor(*v, vec), BMA_ERR_UNSUPPORTED);
+  int* status = device_status_ptr();
+  BMA_REQUIRE(status != nullptr, BMA_ERR_CUDA);
+  const int per_token = c->Hkv * c->d / vec;
+  const int x = per_token >= 256 ? 256 : ((per_token + 31) & ~31), y = 256 / x;
+  const int64_t ctas = ((int64_t)c->B * L + y - 1) / y;
+  BMA_REQUIRE(ctas < (1ll << 31), BMA_ERR_LIMIT);
+  const dim3 block(x, y);
+  if (c->dtype == BMA_DTYPE_F32) read_kv_kernel<BMA_DTYPE_F32><<<(unsigned)ctas, block, 0, st>>>(*c, lengths, L, *k, *v, status);
+  else if (c->dtype == BMA_DTYPE_BF16) read_kv_kernel<BMA_DTYPE_BF16><<<(unsigned)ctas, block, 0, st>>>(*c, lengths, L, *k, *v, status);
+  else read_kv_kernel<BMA_DTYPE_MXFP4><<<(unsigned)ctas, block, 0, st>>>(*c, lengths, L, *k, *v, status);
+  count_launches(1);
+  BMA_CUDA_TRY(cudaGetLastError());
+  return BMA_OK;
+}
+
+}  // namespace bma
+
+using namespace bma;
+
+extern "C" {
+int bma_rotate(const bma_rotate_args* args, bma_stream_t stream) { return rotate_forward(args, static_cast<cudaStream_t>(stream)); }
+size_t bma_rotate_bwd_workspace_bytes(const bma_rotate_args* args) { return rotate_back_bytes(args); }
+int bma_rotate_bwd(const bma_rotate_args* args, void* workspace, size_t workspace_bytes, bma_stream_t stream) {
+  return rotate_backward(args, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+int bma_append_kv(const bma_paged_cache* cache, const bma_append_args* args, bma_stream_t stream) {
+  return append_kv(cache, args, static_cast<cudaStream_t>(stream));
+}
+int bma_read_kv(const bma_paged_cache* cache, const int32_t* lengths, int32_t L, const bma_tensor* k, const bma_tensor* v, bma_stream_t stream) {
+  return read_kv(cache, lengths, L, k, v, static_cast<cudaStream_t>(stream));
+}
+}

@@ -27,7 +27,8 @@ using OptTensor = std::optional<Tensor>;
 #define BMA_FUNCTIONS(X)                                                                                                      \
   X(bma_mask_compile_workspace_bytes) X(bma_mask_compile) X(bma_attn_plan) X(bma_attn_bwd_plan) X(bma_attn_fwd_implies_lists) X(bma_attn_fwd_workspace_bytes) \
   X(bma_attn_fwd_uses_workspace) X(bma_attn_fwd_ws) X(bma_attn_f32_workspace_bytes) X(bma_attn_fwd_f32) X(bma_attn_bwd_f32) X(bma_attn_bwd_f32_o) X(bma_attn_bwd_preprocess)       \
-  X(bma_attn_bwd_workspace_bytes) X(bma_attn_bwd_scratch_bytes) X(bma_attn_bwd_scratch_min_bytes) X(bma_attn_bwd) X(bma_attn_bwd_o)
+  X(bma_attn_bwd_workspace_bytes) X(bma_attn_bwd_scratch_bytes) X(bma_attn_bwd_scratch_min_bytes) X(bma_attn_bwd) X(bma_attn_bwd_o) \
+  X(bma_rotate) X(bma_rotate_bwd_workspace_bytes) X(bma_rotate_bwd) X(bma_append_kv) X(bma_read_kv) X(bma_paged_attn_workspace_bytes) X(bma_paged_attn)
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;
   BMA_FUNCTIONS(X)
@@ -262,6 +263,313 @@ std::tuple<Tensor, Tensor, Tensor> backward(const Tensor& q, const Tensor& k, co
   return {dq, dk, dv};
 }
 
+// ---- heads and the paged cache ------------------------------------------------------------------------------------
+// These check their arguments here: a small call takes as long on the host as on the device.
+int dtype_of(const Tensor& t, const char* name) {
+  TORCH_CHECK_TYPE(t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16, name, " must be float32 or bfloat16, not ", t.scalar_type());
+  return t.scalar_type() == at::kFloat ? BMA_DTYPE_F32 : BMA_DTYPE_BF16;
+}
+
+// The tensors of a call, which have to lie on the device of the first: looked at when everything else has been.
+struct Devices {
+  const Tensor* at[16];
+  const char* names[16];
+  int n = 0;
+  void add(const Tensor& t, const char* name) {
+    at[n] = &t;
+    names[n++] = name;
+  }
+  void check() const {
+    for (int i = 0; i < n; ++i) {
+      TORCH_CHECK(at[i]->is_cuda(), names[i], " must be a CUDA tensor; there is no CPU path");
+      TORCH_CHECK_VALUE(at[i]->device() == at[0]->device(), names[i], " is on ", at[i]->device().str(), ", not on ", at[0]->device().str());
+    }
+  }
+};
+
+// [B, L, H, d] heads; copied only where the components of a head do not lie side by side
+Tensor heads_of(const Tensor& t, const char* name) {
+  TORCH_CHECK_VALUE(t.dim() == 4, name, " must be [batch, length, heads, components]");
+  TORCH_CHECK_VALUE(t.size(0) > 0 && t.size(1) > 0 && t.size(2) > 0 && t.size(3) > 0, name, " is empty");
+  TORCH_CHECK_VALUE(t.size(0) <= INT32_MAX && t.size(1) <= INT32_MAX && t.size(2) <= 65535, name, " is too large");
+  return t.stride(3) == 1 || t.size(3) == 1 ? t : t.contiguous();
+}
+
+bma_rotary rotary_of(Devices& on, int64_t d, const OptTensor& frequencies, int layout, double magnitude, const OptTensor& q_weight, const OptTensor& k_weight,
+                     double eps) {
+  bma_rotary r{};
+  r.layout = layout;
+  r.magnitude = (float)magnitude;
+  r.eps = (float)eps;
+  if (frequencies) {
+    TORCH_CHECK_TYPE(frequencies->scalar_type() == at::kDouble, "frequencies must be float64");
+    TORCH_CHECK_VALUE(frequencies->dim() == 1 && frequencies->is_contiguous(), "frequencies must be a contiguous vector");
+    TORCH_CHECK_VALUE(frequencies->numel() > 0 && 2 * frequencies->numel() <= d, "frequencies must have between 1 and " + std::to_string(d / 2) + " values");
+    on.add(*frequencies, "frequencies");
+    r.frequencies = frequencies->data_ptr<double>();
+    r.dim = (int32_t)(2 * frequencies->numel());
+  }
+  const Tensor* first = nullptr;
+  auto weight = [&](const OptTensor& w, const char* name) -> const void* {
+    if (!w) return nullptr;
+    r.weight_dtype = dtype_of(*w, name);
+    TORCH_CHECK_VALUE(w->dim() == 1 && w->numel() == d && w->is_contiguous(), name, " must be a contiguous vector of " + std::to_string(d) + " values");
+    TORCH_CHECK_TYPE(!first || first->scalar_type() == w->scalar_type(), "q_weight and k_weight must share a dtype");
+    on.add(*w, name);
+    first = &*w;
+    return w->data_ptr();
+  };
+  r.q_weight = weight(q_weight, "q_weight");
+  r.k_weight = weight(k_weight, "k_weight");
+  TORCH_CHECK_VALUE(!first || eps >= 0, "eps must not be negative");
+  return r;
+}
+
+bma_rotate_args rotate_args(Devices& on, const Tensor& q, const OptTensor& k, const OptTensor& positions, const OptTensor& frequencies, int layout, double magnitude,
+                            const OptTensor& q_weight, const OptTensor& k_weight, double eps) {
+  bma_rotate_args a{};
+  a.B = (int32_t)q.size(0); a.L = (int32_t)q.size(1); a.Hq = (int32_t)q.size(2); a.d = (int32_t)q.size(3);
+  dtype_of(q, "q");
+  TORCH_CHECK_VALUE(a.d <= 256, "heads of at most 256 components");
+  if (k) {
+    TORCH_CHECK_VALUE(k->size(0) == a.B && k->size(1) == a.L && k->size(3) == a.d, "k must have the batch, length and components of q");
+    TORCH_CHECK_TYPE(k->scalar_type() == q.scalar_type(), "q and k must share a dtype");
+    a.Hkv = (int32_t)k->size(2);
+  }
+  TORCH_CHECK_VALUE(k || !k_weight, "k_weight without k");
+  TORCH_CHECK_VALUE(frequencies || q_weight || k_weight, "neither frequencies nor weights: there is nothing to do");
+  on.add(q, "q");
+  if (k) on.add(*k, "k");
+  a.rotary = rotary_of(on, a.d, frequencies, layout, magnitude, q_weight, k_weight, eps);
+  if (positions) {
+    const Tensor& p = *positions;
+    TORCH_CHECK_TYPE(p.scalar_type() == at::kInt || p.scalar_type() == at::kLong, "positions must be int32 or int64");
+    TORCH_CHECK_VALUE((p.dim() == 1 && p.size(0) == a.L) || (p.dim() == 2 && p.size(0) == a.B && p.size(1) == a.L), "positions must be [length] or [batch, length]");
+    on.add(p, "positions");
+    a.positions = p.data_ptr();
+    a.position_bytes = p.scalar_type() == at::kInt ? 4 : 8;
+    a.position_stride_b = p.dim() == 2 ? p.stride(0) : 0;
+    a.position_stride_l = p.stride(p.dim() - 1);
+  }
+  return a;
+}
+
+std::tuple<Tensor, OptTensor> rotate(const Tensor& q_in, const OptTensor& k_in, const OptTensor& positions, const OptTensor& frequencies, int layout, double magnitude,
+                                     const OptTensor& q_weight, const OptTensor& k_weight, double eps, uintptr_t stream) {
+  const Tensor q = heads_of(q_in, "q");
+  OptTensor k, k_out;
+  if (k_in) k = heads_of(*k_in, "k");
+  Devices on;
+  bma_rotate_args a = rotate_args(on, q, k, positions, frequencies, layout, magnitude, q_weight, k_weight, eps);
+  on.check();
+  const at::TensorOptions like = q.options().requires_grad(false);
+  Tensor q_out = at::empty(q.sizes(), like);
+  a.q = describe(q); a.q_out = describe(q_out);
+  if (k) {
+    k_out = at::empty(k->sizes(), like);
+    a.k = describe(*k); a.k_out = describe(*k_out);
+  }
+  int rc;
+  {
+    Group group("bma.rotate");
+    rc = lib.bma_rotate(&a, reinterpret_cast<bma_stream_t>(stream));
+  }
+  check(rc, "bma_rotate");
+  return {q_out, k_out};
+}
+
+// Gradients of (q, k, q_weight, k_weight), as far as they are there.
+std::tuple<Tensor, OptTensor, OptTensor, OptTensor> rotate_backward(const Tensor& q_in, const OptTensor& k_in, const OptTensor& positions, const OptTensor& frequencies,
+                                                                    int layout, double magnitude, const OptTensor& q_weight, const OptTensor& k_weight, double eps,
+                                                                    const Tensor& g_q_in, const OptTensor& g_k_in, uintptr_t stream) {
+  const Tensor q = heads_of(q_in, "q"), g_q = heads_of(g_q_in, "the cotangent of q");
+  OptTensor k, g_k, dk, dqw, dkw;
+  if (k_in) {
+    k = heads_of(*k_in, "k");
+    g_k = heads_of(*g_k_in, "the cotangent of k");
+  }
+  Devices on;
+  bma_rotate_args a = rotate_args(on, q, k, positions, frequencies, layout, magnitude, q_weight, k_weight, eps);
+  TORCH_CHECK_VALUE(g_q.sizes() == q.sizes() && (!k || g_k->sizes() == k->sizes()), "the cotangents must have the shapes of the results");
+  TORCH_CHECK_TYPE(g_q.scalar_type() == q.scalar_type() && (!k || g_k->scalar_type() == q.scalar_type()), "the cotangents must have the dtype of the results");
+  on.add(g_q, "the cotangent of q");
+  if (k) on.add(*g_k, "the cotangent of k");
+  on.check();
+  const at::TensorOptions like = q.options().requires_grad(false);
+  Tensor dq = at::empty(q.sizes(), like);
+  a.q = describe(q); a.q_out = describe(g_q); a.dq = describe(dq);
+  if (k) {
+    dk = at::empty(k->sizes(), like);
+    a.k = describe(*k); a.k_out = describe(*g_k); a.dk = describe(*dk);
+  }
+  if (q_weight) a.dq_weight = (dqw = at::empty(q_weight->sizes(), q_weight->options().requires_grad(false)))->data_ptr();
+  if (k_weight) a.dk_weight = (dkw = at::empty(k_weight->sizes(), k_weight->options().requires_grad(false)))->data_ptr();
+  const size_t ws_bytes = lib.bma_rotate_bwd_workspace_bytes(&a);
+  Tensor ws;
+  if (ws_bytes) ws = bytes_on(q, ws_bytes);
+  int rc;
+  {
+    Group group("bma.rotate_bwd");
+    rc = lib.bma_rotate_bwd(&a, ws_bytes ? ws.data_ptr() : nullptr, ws_bytes, reinterpret_cast<bma_stream_t>(stream));
+  }
+  check(rc, "bma_rotate_bwd");
+  return {dq, dk, dqw, dkw};
+}
+
+bma_paged_cache cache_of(Devices& on, const Tensor& k, const Tensor& v, const Tensor& table, const OptTensor& k_scale, const OptTensor& v_scale) {
+  bma_paged_cache c{};
+  on.add(k, "the pages of keys");
+  on.add(v, "the pages of values");
+  on.add(table, "the page table");
+  TORCH_CHECK_VALUE(k.dim() == 4 && v.dim() == 4, "the pages must be [pages, page_size, heads, components]");
+  TORCH_CHECK_VALUE(k.sizes() == v.sizes() && k.strides() == v.strides(), "the pages of keys and of values must have the same shape and strides");
+  TORCH_CHECK_TYPE(k.scalar_type() == v.scalar_type(), "the pages of keys and of values must share a dtype");
+  TORCH_CHECK_VALUE(k.numel() > 0, "the pages are empty");
+  TORCH_CHECK_VALUE(k.stride(3) == 1, "the components of a head must lie side by side in a page");
+  TORCH_CHECK_VALUE(k.size(0) <= INT32_MAX && k.size(1) <= INT32_MAX && k.size(2) <= 65535, "too many pages, slots or heads");
+  c.pages = (int32_t)k.size(0); c.page_size = (int32_t)k.size(1); c.Hkv = (int32_t)k.size(2); c.d = (int32_t)std::min<int64_t>(k.size(3), 1 << 20);
+  c.stride_page = k.stride(0); c.stride_slot = k.stride(1); c.stride_head = k.stride(2);
+  int64_t unit = 16;                     // values of 16 bytes
+  if (k.scalar_type() == at::kByte) {
+    c.dtype = BMA_DTYPE_MXFP4;
+    c.d *= 2;
+    TORCH_CHECK_VALUE(k_scale && v_scale, "a 4-bit cache has k_scale and v_scale");
+    TORCH_CHECK_VALUE(c.d % 32 == 0 && c.d <= 128, "a 4-bit cache has heads of 32, 64, 96 or 128 components");
+    for (const OptTensor* s : {&k_scale, &v_scale}) {
+      const Tensor& t = **s;
+      TORCH_CHECK_TYPE(t.scalar_type() == at::kByte, "the scales must be uint8");
+      TORCH_CHECK_VALUE(t.dim() == 4 && t.size(0) == k.size(0) && t.size(1) == k.size(1) && t.size(2) == k.size(2) && t.size(3) * 32 == c.d,
+                        "the scales must be [pages, page_size, heads, components / 32]");
+      TORCH_CHECK_VALUE(t.stride(3) == 1 || t.size(3) == 1, "the scales of a head must lie side by side");
+      TORCH_CHECK_VALUE(t.strides() == k_scale->strides(), "the scales of keys and of values must have the same strides");
+      on.add(t, "the scales");
+    }
+    c.k_scale = k_scale->data_ptr<uint8_t>(); c.v_scale = v_scale->data_ptr<uint8_t>();
+    c.scale_stride_page = k_scale->stride(0); c.scale_stride_slot = k_scale->stride(1); c.scale_stride_head = k_scale->stride(2);
+  } else {
+    c.dtype = dtype_of(k, "pages (of other than 4-bit caches)");
+    unit = c.dtype == BMA_DTYPE_F32 ? 4 : 8;
+    TORCH_CHECK_VALUE(!k_scale && !v_scale, "only a 4-bit cache (uint8 pages) has scales");
+    TORCH_CHECK_VALUE(c.d % 8 == 0 && c.d <= 128, "a cache has heads of a multiple of 8 components, at most 128");
+  }
+  TORCH_CHECK_VALUE((reinterpret_cast<uintptr_t>(k.data_ptr()) | reinterpret_cast<uintptr_t>(v.data_ptr())) % 16 == 0 && c.stride_page % unit == 0 &&
+                        c.stride_slot % unit == 0 && c.stride_head % unit == 0,
+                    "every head of every slot must start on 16 bytes");
+  c.k = k.data_ptr(); c.v = v.data_ptr();
+  TORCH_CHECK_TYPE(table.scalar_type() == at::kInt, "the page table must be int32");
+  TORCH_CHECK_VALUE(table.dim() == 2 && table.numel() > 0 && (table.stride(1) == 1 || table.size(1) == 1), "the page table must be [batch, width], its rows contiguous");
+  TORCH_CHECK_VALUE(table.size(0) <= 65535, "a batch of at most 65535 sequences");
+  TORCH_CHECK_VALUE(table.size(1) * (int64_t)c.page_size < (1ll << 31) - 4096, "the page table covers too many positions");
+  c.page_table = table.data_ptr<int32_t>();
+  c.table_stride = table.stride(0);
+  c.B = (int32_t)table.size(0); c.width = (int32_t)table.size(1);
+  return c;
+}
+
+const int32_t* counts_of(Devices& on, const Tensor& t, const bma_paged_cache& c, const char* name) {
+  TORCH_CHECK_TYPE(t.scalar_type() == at::kInt, name, " must be int32");
+  TORCH_CHECK_VALUE(t.dim() == 1 && t.size(0) == c.B && t.is_contiguous(), name, " must be a contiguous vector with a value for each row of the page table");
+  on.add(t, name);
+  return t.data_ptr<int32_t>();
+}
+
+void fits_cache(Devices& on, const Tensor& t, const bma_paged_cache& c, int64_t heads, const char* name) {
+  TORCH_CHECK_VALUE(t.size(0) == c.B && t.size(3) == c.d && (heads < 0 || t.size(2) == heads), name, " does not fit the cache");
+  const int dtype = dtype_of(t, name);
+  TORCH_CHECK_TYPE(c.dtype == BMA_DTYPE_MXFP4 || dtype == c.dtype, name, " must have the dtype of the cache");
+  on.add(t, name);
+}
+
+OptTensor append(const Tensor& pages_k, const Tensor& pages_v, const Tensor& table, const OptTensor& k_scale, const OptTensor& v_scale, const Tensor& k_in,
+                 const Tensor& v_in, const Tensor& lengths, const OptTensor& new_lengths, const OptTensor& q_in, const OptTensor& frequencies, int layout, double magnitude,
+                 const OptTensor& q_weight, const OptTensor& k_weight, double eps, uintptr_t stream) {
+  Devices on;
+  const bma_paged_cache c = cache_of(on, pages_k, pages_v, table, k_scale, v_scale);
+  const Tensor k = heads_of(k_in, "k"), v = heads_of(v_in, "v");
+  OptTensor q, q_out;
+  if (q_in) q = heads_of(*q_in, "q");
+  bma_append_args a{};
+  a.T = (int32_t)k.size(1);
+  fits_cache(on, k, c, c.Hkv, "k");
+  fits_cache(on, v, c, c.Hkv, "v");
+  TORCH_CHECK_VALUE(v.size(1) == a.T && (!q || q->size(1) == a.T), "q, k and v must have the same number of tokens");
+  TORCH_CHECK_TYPE(v.scalar_type() == k.scalar_type() && (!q || q->scalar_type() == k.scalar_type()), "q, k and v must share a dtype");
+  TORCH_CHECK_VALUE(q || !q_weight, "q_weight without q");
+  TORCH_CHECK_VALUE(!q || frequencies || q_weight, "neither frequencies nor q_weight: there is nothing to do with q");
+  a.lengths = counts_of(on, lengths, c, "lengths");
+  if (new_lengths) a.new_lengths = counts_of(on, *new_lengths, c, "new_lengths");
+  a.rotary = rotary_of(on, c.d, frequencies, layout, magnitude, q_weight, k_weight, eps);
+  if (q) fits_cache(on, *q, c, -1, "q");
+  on.check();
+  a.k = describe(k); a.v = describe(v);
+  if (q) {
+    q_out = at::empty(q->sizes(), q->options().requires_grad(false));
+    a.Hq = (int32_t)q->size(2);
+    a.q = describe(*q); a.q_out = describe(*q_out);
+  }
+  int rc;
+  {
+    Group group("bma.append_kv");
+    rc = lib.bma_append_kv(&c, &a, reinterpret_cast<bma_stream_t>(stream));
+  }
+  check(rc, "bma_append_kv");
+  return q_out;
+}
+
+std::tuple<Tensor, Tensor> read_pages(const Tensor& pages_k, const Tensor& pages_v, const Tensor& table, const OptTensor& k_scale, const OptTensor& v_scale,
+                                const Tensor& lengths, int64_t L, uintptr_t stream) {
+  Devices on;
+  const bma_paged_cache c = cache_of(on, pages_k, pages_v, table, k_scale, v_scale);
+  TORCH_CHECK_VALUE(L > 0 && L <= INT32_MAX, "max_length must be positive");
+  const int32_t* at_lengths = counts_of(on, lengths, c, "lengths");
+  on.check();
+  const at::TensorOptions like = pages_k.options().dtype(c.dtype == BMA_DTYPE_F32 ? at::kFloat : at::kBFloat16).requires_grad(false);
+  Tensor k = at::empty({c.B, L, c.Hkv, c.d}, like), v = at::empty({c.B, L, c.Hkv, c.d}, like);
+  const bma_tensor dk = describe(k), dv = describe(v);
+  int rc;
+  {
+    Group group("bma.read_kv");
+    rc = lib.bma_read_kv(&c, at_lengths, (int32_t)L, &dk, &dv, reinterpret_cast<bma_stream_t>(stream));
+  }
+  check(rc, "bma_read_kv");
+  return {k, v};
+}
+
+std::tuple<Tensor, OptTensor> paged(const Tensor& pages_k, const Tensor& pages_v, const Tensor& table, const OptTensor& k_scale, const OptTensor& v_scale,
+                                    const Tensor& q_in, const Tensor& lengths, const OptTensor& new_lengths, std::optional<double> scale,
+                                    std::optional<int64_t> window, bool bf16_out, bool with_lse, uintptr_t stream) {
+  Devices on;
+  const bma_paged_cache c = cache_of(on, pages_k, pages_v, table, k_scale, v_scale);
+  const Tensor q = heads_of(q_in, "q");
+  fits_cache(on, q, c, -1, "q");
+  TORCH_CHECK_TYPE(c.dtype != BMA_DTYPE_MXFP4 || q.scalar_type() == at::kBFloat16, "q must be bfloat16 for a 4-bit cache");
+  TORCH_CHECK_VALUE(q.size(2) % c.Hkv == 0, "the heads of the cache must divide those of q");
+  TORCH_CHECK_VALUE(!window || (*window >= 0 && *window <= INT32_MAX), "window must not be negative");
+  bma_paged_attn_args a{};
+  a.T = (int32_t)q.size(1); a.Hq = (int32_t)q.size(2);
+  a.lengths = counts_of(on, lengths, c, "lengths");
+  if (new_lengths) a.new_lengths = counts_of(on, *new_lengths, c, "new_lengths");
+  a.scale = (float)(scale ? *scale : 1.0 / std::sqrt((double)c.d));
+  a.window = window ? (int32_t)*window : -1;
+  on.check();
+  const at::TensorOptions f32 = q.options().dtype(at::kFloat).requires_grad(false);
+  Tensor o = at::empty(q.sizes(), bf16_out ? f32.dtype(at::kBFloat16) : f32);
+  OptTensor lse;
+  if (with_lse) lse = at::empty({c.B, a.Hq, a.T}, f32);
+  a.q = describe(q); a.o = describe(o);
+  a.lse = lse ? lse->data_ptr<float>() : nullptr;
+  const size_t ws_bytes = lib.bma_paged_attn_workspace_bytes(&c, &a);
+  Tensor ws;
+  if (ws_bytes) ws = bytes_on(q, ws_bytes);
+  int rc;
+  {
+    Group group("bma.paged_attn");
+    rc = lib.bma_paged_attn(&c, &a, ws_bytes ? ws.data_ptr() : nullptr, ws_bytes, reinterpret_cast<bma_stream_t>(stream));
+  }
+  check(rc, "bma_paged_attn");
+  return {o, lse};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_host, m) {
@@ -274,4 +582,9 @@ PYBIND11_MODULE(_host, m) {
   m.def("preprocess", torch::wrap_pybind_function(preprocess));
   m.def("backward_bytes", torch::wrap_pybind_function(backward_bytes));
   m.def("backward", torch::wrap_pybind_function(backward));
+  m.def("rotate", torch::wrap_pybind_function(rotate));
+  m.def("rotate_backward", torch::wrap_pybind_function(rotate_backward));
+  m.def("append", torch::wrap_pybind_function(append));
+  m.def("read", torch::wrap_pybind_function(read_pages));
+  m.def("paged", torch::wrap_pybind_function(paged));
 }
