@@ -211,8 +211,8 @@ typedef struct bma_paged_attn_args {
   const int32_t *lengths, *new_lengths;
   float scale;
   int32_t window;                   /* a token sees keys from `window` positions before its own; negative: from the first */
-  bma_tensor q;                     /* [B, T, Hq, d]: float32 for a float32 cache, else bfloat16 */
-  bma_tensor o;                     /* [B, T, Hq, d]; zeros for tokens that are not real      */
+  bma_tensor q;                     /* [B, T, Hq, d]: float32 for a float32 cache, else bfloat16; heads on 16 bytes */
+  bma_tensor o;                     /* [B, T, Hq, d], heads on 16 bytes; zeros for tokens that are not real */
   float* lse;                       /* [B, Hq, T] or null; -inf where no key is seen          */
 } bma_paged_attn_args;
 

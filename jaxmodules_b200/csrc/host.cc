@@ -540,7 +540,9 @@ std::tuple<Tensor, OptTensor> paged(const Tensor& pages_k, const Tensor& pages_v
                                     std::optional<int64_t> window, bool bf16_out, bool with_lse, uintptr_t stream) {
   Devices on;
   const bma_paged_cache c = cache_of(on, pages_k, pages_v, table, k_scale, v_scale);
-  const Tensor q = heads_of(q_in, "q");
+  Tensor q = heads_of(q_in, "q");
+  const int64_t bytes = q.element_size();
+  if (reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 || q.stride(0) * bytes % 16 || q.stride(1) * bytes % 16 || q.stride(2) * bytes % 16) q = q.clone(at::MemoryFormat::Contiguous);
   fits_cache(on, q, c, -1, "q");
   TORCH_CHECK_TYPE(c.dtype != BMA_DTYPE_MXFP4 || q.scalar_type() == at::kBFloat16, "q must be bfloat16 for a 4-bit cache");
   TORCH_CHECK_VALUE(q.size(2) % c.Hkv == 0, "the heads of the cache must divide those of q");

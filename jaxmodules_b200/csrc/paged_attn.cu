@@ -1,115 +1,1145 @@
 // Attention of the newest tokens of every sequence over a paged cache.
+//
+// Every key and value in reach is read once and meets the few rows (tokens x query heads of its kv head) of one sequence: the kernels are bound
+// by memory.  What they have to do is to keep enough loads in flight, and to give every SM the same share of bytes whatever the
+// lengths are, which only the device knows.
+//
+// Work.  The walk over the keys of one (sequence, tile of rows, kv head) is an item, cut into units of kUnit keys.  All units of all items lie in
+// one sequence, which is cut into as many even runs as CTAs fit on the chip; a run ends in the middle of an item as a rule.  Each CTA finds its
+// run from the lengths.  An item that lies within one run is finished there; the parts of others go to the workspace, at most two from a
+// CTA, and paged_join_kernel puts them together in the order of the keys.
+//
+// Within a CTA the four warps take tiles of a unit in turn, each with its own ring of stages in shared memory that it fills by cp.async: no warp
+// waits for another before the end of an item, and the ring runs on into the next item.  Pages are looked up for every key (any page
+// size), a tile ahead of the copy.
+//
+// Keys outside [lo, hi), which no row of the tile sees, are not read: zeros stand there.  Where the rows of a tile see different keys of a tile of
+// keys (several new tokens), each token's rows are multiplied by values that are zero where the token does not see them, so that an infinity or
+// a NaN reaches only the rows that see it.
 #include "paged.cuh"
 
 namespace bma {
 namespace {
 
-constexpr int kRows = 16, kKeys = 32;
+constexpr int kWarps = 4, kThreads = kWarps * 32;
+constexpr float kLn2 = 0.6931471805599453f;
 
-__device__ __forceinline__ float held_value(const bma_paged_cache& c, bool v, int64_t at, int64_t scale_at, int h, int i) {
-  const void* p = v ? c.v : c.k;
-  if (c.dtype == BMA_DTYPE_F32) return static_cast<const float*>(p)[at + h * c.stride_head + i];
-  if (c.dtype == BMA_DTYPE_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[at + h * c.stride_head + i]);
-  const uint8_t code = static_cast<const uint8_t*>(p)[at + h * c.stride_head + i / 2] >> (i & 1 ? 4 : 0);
-  uint32_t pairs[4];
-  from_e2m1x8(code & 15, pairs);
-  return __low2float(*reinterpret_cast<const __half2*>(&pairs[0])) * e8m0_value((v ? c.v_scale : c.k_scale)[scale_at + h * c.scale_stride_head + i / 32]);
+struct PagedParams {
+  bma_paged_cache c;
+  bma_paged_attn_args a;
+  int G, rows, row_tiles, entries;     // query heads to a kv head, rows to a kv head, tiles of them, (sequence, tile) pairs
+  int positions;                       // what the page table covers
+  float scale_log2;
+  int* status;
+  float* part_o;                       // [2 * CTAs][rows of a tile][DP]
+  float2* part_ml;                     // [2 * CTAs][rows of a tile]
+  int4* meta;                          // [CTAs]: item whose first part the CTA has (-1: none), slot of that part, CTA with the last part
+};
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool there) {     // 16 bytes, or zeros
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_committed() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_awaited() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void matrices(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void matrices_turned(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Where a CTA puts the parts of its warps together: eight rows of a warp at a time, lines of DP + 8 floats (the rows of a quarter warp in different banks); the last
+// 8 floats of a line hold maximum and sum of four rows, r, r + 8, r + 16 and r + 24.
+template <int DP>
+struct Buffer {
+  static constexpr int kLine = DP + 8, kFloats = kWarps * 8 * kLine;
+  float* at;
+  __device__ __forceinline__ float* line(int warp, int r) const { return at + (warp * 8 + r) * kLine; }
+  __device__ __forceinline__ float2& stat(int warp, int row) const { return *reinterpret_cast<float2*>(line(warp, row & 7) + DP + (row >> 3) * 2); }
+};
+__device__ __forceinline__ uint32_t smem_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+// The keys that a tile of rows sees, and who its rows are.
+struct Entry {
+  int b, row0;             // sequence, first row
+  int first, count;        // position of the first new token, number of real ones
+  int lo, hi, base;        // keys [lo, hi); the walk starts at `base`
+  int units;               // at least 1: an item without keys is written, too
+};
+template <int ROWS, int TILE>
+__device__ __forceinline__ Entry entry_of(const PagedParams& p, int e) {
+  Entry x;
+  x.b = e / p.row_tiles;
+  x.row0 = (e - x.b * p.row_tiles) * ROWS;
+  const NewTokens n = new_tokens(p.a.lengths, p.a.new_lengths, x.b, p.a.T);
+  x.count = n.count;
+  x.first = (int)max(n.first, (int64_t)-(1 << 30));
+  const int t0 = x.row0 / p.G, t1 = min((min(x.row0 + ROWS, p.rows) - 1) / p.G, x.count - 1);
+  x.lo = x.hi = 0;
+  if (t0 <= t1) {
+    const int64_t end = n.first + t1 + 1;
+    x.hi = (int)min(max(end, (int64_t)0), (int64_t)p.positions);
+    if (end > p.positions) report_device_error(p.status, kStatusPaged);
+    x.lo = p.a.window < 0 ? 0 : (int)min(max(n.first + t0 - p.a.window, (int64_t)0), (int64_t)x.hi);
+  }
+  x.base = x.lo & ~(TILE - 1);
+  x.units = max(1, (x.hi - x.base + kWarps * TILE - 1) / (kWarps * TILE));
+  return x;
 }
 
-// One CTA: a sequence, a kv head, and up to 16 of the rows (token, query head of the group), one pass over the keys.
-__global__ void __launch_bounds__(128) paged_rows_kernel(const __grid_constant__ bma_paged_cache c, const __grid_constant__ bma_paged_attn_args a, int* status) {
-  __shared__ float q[kRows][kPagedHeadDim], kv[kKeys][kPagedHeadDim + 1], p[kRows][kKeys + 1], shift[kRows];
-  const int G = a.Hq / c.Hkv, rows = a.T * G;
-  const int h = blockIdx.y, b = blockIdx.z, r0 = blockIdx.x * kRows, n = min(kRows, rows - r0);
-  const NewTokens news = new_tokens(a.lengths, a.new_lengths, b, a.T);
-  auto position = [&](int r) -> int64_t { const int t = (r0 + r) / G; return t < news.count ? news.first + t : -1; };
-  auto value = [&](const bma_tensor& t, int r, int i) { return (int64_t)b * t.stride_b + ((r0 + r) / G) * t.stride_l + (h * G + (r0 + r) % G) * t.stride_h + i; };
-  for (int i = threadIdx.x; i < n * c.d; i += 128) {
-    const int r = i / c.d;
-    const int64_t at = value(a.q, r, i % c.d);
-    q[r][i % c.d] = a.q.dtype == BMA_DTYPE_F32 ? static_cast<const float*>(a.q.ptr)[at] : __bfloat162float(static_cast<const __nv_bfloat16*>(a.q.ptr)[at]);
+// A place in the sequence of units.
+template <int ROWS, int TILE>
+struct Cursor {
+  Entry x;
+  int e, h, unit;
+  __device__ __forceinline__ void next(const PagedParams& p) {
+    if (++unit < x.units) return;
+    unit = 0;
+    if (++h < p.c.Hkv) return;
+    h = 0;
+    if (++e < p.entries) x = entry_of<ROWS, TILE>(p, e);
   }
-  int64_t lo = 0, hi = 0;
-  for (int r = 0; r < n; ++r) {
-    const int64_t at = position(r);
-    if (at >= 0) hi = at + 1;
-    if (r == 0 && a.window >= 0 && at > a.window) lo = at - a.window;
+  __device__ __forceinline__ int tile(int warp) const { return x.base + (unit * kWarps + warp) * TILE; }
+};
+
+// [begin, end) of CTA `cta`'s run
+__device__ __forceinline__ int64_t run_begin(int64_t total, int cta, int ctas) { return total * cta / ctas; }
+
+// Where in the cache a key's heads lie, in units of 16 bytes (the host has checked that this fits); none: kNowhere.
+constexpr uint32_t kNowhere = 0xffffffffu;
+struct Place {
+  int page, slot;
+  __device__ __forceinline__ void look_up(const PagedParams& p, const Entry& x, int key) {
+    page = -1;
+    slot = 0;
+    if (key >= x.lo && key < x.hi) {
+      const int i = key / p.c.page_size;
+      slot = key - i * p.c.page_size;
+      page = __ldg(p.c.page_table + (int64_t)x.b * p.c.table_stride + i);
+      if (page < 0) page = -2;       // (told from a key that is not looked up)
+    }
   }
-  float m = -INFINITY, l = 0.f, o[kRows];     // statistics: threads r < n; the sums of column threadIdx.x: all rows
-  for (int r = 0; r < kRows; ++r) o[r] = 0.f;
-  for (int64_t k0 = lo; k0 < hi; k0 += kKeys) {
-    const int keys = (int)min((int64_t)kKeys, hi - k0);
-    for (int side = 0; side < 2; ++side) {
-      __syncthreads();
-      for (int j = threadIdx.x / 32; j < keys; j += 4) {
-        int slot = 0;
-        const int page = page_of(c, b, k0 + j, slot);
-        if (page < 0 && threadIdx.x % 32 == 0) report_device_error(status, kStatusPaged);
-        const int64_t at = (int64_t)page * c.stride_page + (int64_t)slot * c.stride_slot, sat = (int64_t)page * c.scale_stride_page + (int64_t)slot * c.scale_stride_slot;
-        for (int i = threadIdx.x % 32; i < c.d; i += 32) kv[j][i] = page < 0 ? 0.f : held_value(c, side, at, sat, h, i);
+  __device__ __forceinline__ bool there(const PagedParams& p) const {
+    if (page >= 0 && page < p.c.pages) return true;
+    if (page != -1) report_device_error(p.status, kStatusPaged);
+    return false;
+  }
+  template <int BYTES>      // of a unit of the strides
+  __device__ __forceinline__ uint32_t at(const PagedParams& p, int h) const {
+    return there(p) ? (uint32_t)(((int64_t)page * p.c.stride_page + (int64_t)slot * p.c.stride_slot + (int64_t)h * p.c.stride_head) * BYTES / 16) : kNowhere;
+  }
+};
+
+__device__ __forceinline__ const __nv_bfloat16* query_row(const PagedParams& p, const Entry& x, int h, int row) {
+  return static_cast<const __nv_bfloat16*>(p.a.q.ptr) + x.b * p.a.q.stride_b + (row / p.G) * p.a.q.stride_l + (h * p.G + row % p.G) * p.a.q.stride_h;
+}
+
+// Statistics and masks of the rows of a warp's matrix tiles: this lane's are rows g and g + 8 of each of MT tiles of 16.
+template <int MT>
+struct Rows {
+  float m[MT][2], l[MT][2];    // maximum so far (log2 units), this lane's share of the sum
+  int at[MT][2];               // position of the row's token; below every key where it is not real
+  __device__ __forceinline__ void start(const PagedParams& p, const Entry& x, int g) {
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const int row = x.row0 + i * 16 + s * 8 + g, t = row / p.G;
+        at[i][s] = row < p.rows && t < x.count ? x.first + t : -1;
+        m[i][s] = -INFINITY;
+        l[i][s] = 0.f;
       }
-      __syncthreads();
-      if (side == 0) {
-        for (int i = threadIdx.x; i < n * kKeys; i += 128) {
-          const int r = i / kKeys, j = i % kKeys;
-          const int64_t at = position(r), key = k0 + j;
-          float s = 0.f;
-          if (j < keys)
-            for (int x = 0; x < c.d; ++x) s = fmaf(q[r][x], kv[j][x], s);
-          p[r][j] = j < keys && key <= at && (a.window < 0 || key >= at - a.window) ? s * a.scale : -INFINITY;
-        }
-        __syncthreads();
-        if (threadIdx.x < n) {
-          const int r = threadIdx.x;
-          float top = m;
-          for (int j = 0; j < kKeys; ++j) top = fmaxf(top, p[r][j]);
-          const float base = top == -INFINITY ? 0.f : top;
-          shift[r] = expf(m - base);
-          float sum = 0.f;          // (a tile's sums first: short chains)
-          for (int j = 0; j < kKeys; ++j) {
-            const bool seen = p[r][j] != -INFINITY;
-            p[r][j] = seen ? expf(p[r][j] - base) : -1.f;      // (a key that is not seen adds nothing, whatever its value)
-            if (seen) sum += p[r][j];
+  }
+  template <int DP>
+  __device__ __forceinline__ void stats(const Buffer<DP>& buffer, int warp, int lane, int down = 0) const {
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        float x = l[i][s];
+        x += __shfl_xor_sync(0xffffffffu, x, 1);
+        x += __shfl_xor_sync(0xffffffffu, x, 2);
+        if ((lane & 3) == 0) buffer.stat(warp, i * 16 + s * 8 + (lane >> 2)) = make_float2(m[i][s] - down, x);
+      }
+  }
+  __device__ __forceinline__ bool sees(const PagedParams& p, int i, int s, int key) const {
+    return key <= at[i][s] && (p.a.window < 0 || key >= at[i][s] - p.a.window);
+  }
+};
+// Whether rows of the tile of rows see different parts of the keys [k0, k0 + n), or no row sees some of them.
+template <int ROWS>
+__device__ __forceinline__ bool is_cut(const PagedParams& p, const Entry& x, int k0, int n) {
+  const int t0 = x.row0 / p.G, t1 = min((min(x.row0 + ROWS, p.rows) - 1) / p.G, x.count - 1);
+  return k0 < x.lo || k0 + n - 1 > x.first + t0 || (p.a.window >= 0 && k0 < x.first + t1 - p.a.window);
+}
+
+// ---- bfloat16: matrix instructions fed by ldmatrix ------------------------------------------------------------------
+// Rows (tokens x heads) are the M of mma.m16n8k16, keys its N for the scores and its K for the sums.  tcgen05 would want 128 rows or a
+// transposed softmax; there are 1 to 32 rows here, and mma.sync needs a fifth of the time that the bytes take.
+template <int DP, int MT>
+struct CoreBf16 {
+  static constexpr int kDP = DP, kRows = MT * 16, kTile = 16, kStages = DP == 128 ? 3 : 4, kMinCtas = 2;
+  static constexpr int kRowBytes = DP * 2, kSide = kTile * kRowBytes, kStageBytes = 2 * kSide, kExtra = 0;
+  using Cur = Cursor<kRows, kTile>;
+
+  uint32_t q[MT][DP / 16][4];
+  float o[MT][DP / 8][4];
+  Rows<MT> rows;
+  Place place;
+
+  __device__ __forceinline__ void prepare(uint8_t*) {}
+  __device__ __forceinline__ void look_up(const PagedParams& p, const Cur& c, int warp, int lane) { place.look_up(p, c.x, c.tile(warp) + (lane & 15)); }
+  __device__ __forceinline__ void settle(uint8_t*) {}
+  __device__ __forceinline__ void issue(const PagedParams& p, const Cur& c, uint8_t* stage, int lane) {
+    constexpr int kChunks = DP / 8, kAtOnce = 32 / kChunks;     // 16-byte chunks of a row, rows copied by one instruction
+    const uint32_t mine = place.at<2>(p, c.h);
+    const int chunk = lane % kChunks;
+    const uint32_t to = smem_at(stage);
+    const char* k = static_cast<const char*>(p.c.k);
+    const char* v = static_cast<const char*>(p.c.v);
+#pragma unroll
+    for (int i = 0; i < kTile / kAtOnce; ++i) {
+      const int r = i * kAtOnce + lane / kChunks;
+      const uint32_t at = __shfl_sync(0xffffffffu, mine, r);
+      const bool there = at != kNowhere && chunk * 8 < p.c.d;
+      const int64_t from = there ? (int64_t)at * 16 + chunk * 16 : 0;
+      const uint32_t dst = to + r * kRowBytes + ((chunk ^ (r & 7)) << 4);
+      copy16(dst, k + from, there);
+      copy16(dst + kSide, v + from, there);
+    }
+  }
+  __device__ __forceinline__ void begin(const PagedParams& p, const Cur& c, uint8_t*, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+    rows.start(p, c.x, g);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const int row = c.x.row0 + i * 16 + s * 8 + g;
+        const __nv_bfloat16* from = query_row(p, c.x, c.h, min(row, p.rows - 1));
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int d = k * 16 + u * 8 + 2 * t;
+            q[i][k][u * 2 + s] = row < p.rows && d < p.c.d ? __ldg(reinterpret_cast<const uint32_t*>(from + d)) : 0u;
           }
-          l = fmaf(l, shift[r], sum);
-          m = top;
-        }
-      } else if (threadIdx.x < c.d) {
-        for (int r = 0; r < n; ++r) {
-          float sum = 0.f;
-          for (int j = 0; j < keys; ++j)
-            if (!(p[r][j] < 0.f)) sum = fmaf(p[r][j], kv[j][threadIdx.x], sum);
-          o[r] = fmaf(o[r], shift[r], sum);
+      }
+#pragma unroll
+      for (int j = 0; j < DP / 8; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][j][e] = 0.f;
+    }
+  }
+  __device__ __forceinline__ void take(const PagedParams& p, const Cur& c, const uint8_t* stage, int k0, int lane) {
+    const int t = lane & 3;
+    const uint32_t ks = smem_at(stage), vs = ks + kSide;
+    float s[MT][2][4];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[i][n][e] = 0.f;
+    {
+      const int r = ((lane >> 4) << 3) + (lane & 7), half = (lane >> 3) & 1;
+#pragma unroll
+      for (int k = 0; k < DP / 16; ++k) {
+        uint32_t b[4];
+        matrices(b, ks + r * kRowBytes + (((2 * k + half) ^ (r & 7)) << 4));
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          mma_bf16(s[i][0], q[i][k], b[0], b[1]);
+          mma_bf16(s[i][1], q[i][k], b[2], b[3]);
         }
       }
     }
-  }
-  __syncthreads();
-  if (threadIdx.x < n) {
-    shift[threadIdx.x] = l > 0.f || l != l ? 1.f / l : 0.f;
-    const int t = (r0 + threadIdx.x) / G, head = h * G + (r0 + threadIdx.x) % G;
-    if (a.lse) a.lse[((int64_t)b * a.Hq + head) * a.T + t] = l > 0.f || l != l ? m + logf(l) : -INFINITY;
-  }
-  __syncthreads();
-  if (threadIdx.x < c.d)
-    for (int r = 0; r < n; ++r) {
-      const int64_t at = value(a.o, r, threadIdx.x);
-      const float x = o[r] * shift[r];
-      if (a.o.dtype == BMA_DTYPE_F32) static_cast<float*>(a.o.ptr)[at] = x;
-      else static_cast<__nv_bfloat16*>(a.o.ptr)[at] = __float2bfloat16_rn(x);
+    const bool cut = is_cut<kRows>(p, c.x, k0, kTile);
+    uint32_t w[MT][4];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      float top[2] = {rows.m[i][0], rows.m[i][1]};
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float x = s[i][n][e] * p.scale_log2;
+          if (cut && !rows.sees(p, i, e >> 1, k0 + n * 8 + 2 * t + (e & 1))) x = -INFINITY;
+          s[i][n][e] = x;
+          top[e >> 1] = fmaxf(top[e >> 1], x);
+        }
+      rescale<DP / 8>(i, top, o[i]);
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[i][n][e] = exp2_approx(s[i][n][e] - top[e >> 1]);
+          rows.l[i][e >> 1] += s[i][n][e];
+        }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(s[i][u >> 1][(u & 1) * 2], s[i][u >> 1][(u & 1) * 2 + 1]);
+        w[i][u] = *reinterpret_cast<const uint32_t*>(&h);
+      }
     }
+    const int r = (((lane >> 3) & 1) << 3) + (lane & 7), second = lane >> 4;
+    const int t0 = c.x.row0 / p.G, t1 = (min(c.x.row0 + kRows, p.rows) - 1) / p.G;
+    if (!cut || t0 == t1) {
+#pragma unroll
+      for (int j = 0; j < DP / 16; ++j) {
+        uint32_t b[4];
+        matrices_turned(b, vs + r * kRowBytes + (((2 * j + second) ^ (r & 7)) << 4));
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          mma_bf16(o[i][2 * j], w[i], b[0], b[1]);
+          mma_bf16(o[i][2 * j + 1], w[i], b[2], b[3]);
+        }
+      }
+      return;
+    }
+    for (int tok = t0; tok <= min(t1, c.x.count - 1); ++tok) {
+      const int at = c.x.first + tok;
+      uint32_t seen[2] = {0, 0};      // of this lane's keys 2t, 2t + 1 and 2t + 8, 2t + 9
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int key = k0 + (u >> 1) * 8 + 2 * t + (u & 1);
+        if (key <= at && (p.a.window < 0 || key >= at - p.a.window)) seen[u >> 1] |= u & 1 ? 0xffff0000u : 0xffffu;
+      }
+#pragma unroll
+      for (int j = 0; j < DP / 16; ++j) {
+        uint32_t b[4];
+        matrices_turned(b, vs + r * kRowBytes + (((2 * j + second) ^ (r & 7)) << 4));
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            float x[4] = {0.f, 0.f, 0.f, 0.f};
+            mma_bf16(x, w[i], b[2 * n] & seen[0], b[2 * n + 1] & seen[1]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (rows.at[i][e >> 1] == at) o[i][2 * j + n][e] += x[e];
+          }
+      }
+    }
+  }
+  // Takes the lane's maxima to those of the rows, and what has been added up to the new ones; `top` becomes what exponents are taken against.
+  template <int N>
+  __device__ __forceinline__ void rescale(int i, float (&top)[2], float (&acc)[N][4]) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      top[s] = fmaxf(top[s], __shfl_xor_sync(0xffffffffu, top[s], 1));
+      top[s] = fmaxf(top[s], __shfl_xor_sync(0xffffffffu, top[s], 2));
+    }
+    const bool moved = top[0] != rows.m[i][0] || top[1] != rows.m[i][1];
+    if (__any_sync(0xffffffffu, moved)) {
+      float f[2];
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        f[s] = top[s] == -INFINITY ? 1.f : exp2_approx(rows.m[i][s] - top[s]);
+        rows.l[i][s] *= f[s];
+        rows.m[i][s] = top[s];
+      }
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[j][e] *= f[e >> 1];
+    }
+#pragma unroll
+    for (int s = 0; s < 2; ++s) top[s] = top[s] == -INFINITY ? 0.f : top[s];
+  }
+  __device__ __forceinline__ void stats(const Buffer<DP>& buffer, int warp, int lane) const { rows.stats(buffer, warp, lane); }
+  // Rows [8 pass, 8 pass + 8), times factor[row], into out[row - 8 pass][DP + 8]
+  __device__ __forceinline__ void put(int pass, float factor, float* out, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        if (pass == i * 2 + s) {
+#pragma unroll
+          for (int j = 0; j < DP / 8; ++j)
+            *reinterpret_cast<float2*>(out + g * (DP + 8) + j * 8 + 2 * t) = make_float2(o[i][j][2 * s] * factor, o[i][j][2 * s + 1] * factor);
+        }
+  }
+};
+
+// ---- 4 bits: the same products in float16 -----------------------------------------------------------------------------
+// A key's or value's 32 components share a power of two; the largest of a head's, 2^E, is taken out of it, and codes times what remains, 2^(e - E) <= 1,
+// are float16.  2^E of a key multiplies its scores in float32.  2^E of a value joins the exponent of its weight: the running maximum is over score + E, so
+// that the weights that go through float16 are at most 1, and the sum of weights takes 2^-E back out.  Rows of Q are brought to at most 2 by a power of two
+// as well.  Codes are held times 2^13 and weights times 2^15, as large as float16 allows: codes are exact down to 2^-36 of the head's largest, weights
+// good to 2^-12 of themselves down to 2^-29 of the row's largest, and to 2^-40 of that below.  (E counts as at least -65.)
+//
+// One lane holds keys' components in the order that the codes have in memory, and the rows of Q in the same: the sum over d may run in any order.
+// For the sums, codes of two keys are put side by side in a byte, which the conversion then takes to a pair of float16.
+template <int DP, int MT>
+struct Core4bit {
+  static constexpr int kDP = DP, kRows = MT * 16, kTile = 32, kStages = 4, kMinCtas = 2;
+  static constexpr int kRowBytes = DP / 2, kSide = kTile * kRowBytes, kGroups = DP / 32;
+  // after keys and values: powers of two of codes, keys' [32][4] and values' [4][32], and three floats of every key (settle)
+  static constexpr int kKeyPowers = 2 * kSide, kValuePowers = kKeyPowers + 256, kKeyTop = kValuePowers + 256, kStageBytes = kKeyTop + 384, kExtra = 0;
+  using Cur = Cursor<kRows, kTile>;
+  static constexpr int kWords = DP / 32;       // of 8 codes: a lane's of one key (a quarter of the head)
+  static constexpr int kCodeUp = 13, kWeightUp = 15;
+
+  uint32_t q[MT][DP / 16][4];
+  float o[MT][DP / 8][4];
+  float scale[MT][2];
+  Rows<MT> rows;
+  Place place;
+  uint32_t k_bytes, v_bytes;    // the powers of two of this lane's key of the last tile issued
+  uint8_t* pending;             // and its stage
+
+  // Places of keys in the matrix tiles: column n of 8 is key (n >> 1 & 1) | (n & 1) << 1 | (n >> 2) << 2 of 8.  (The lanes of a quarter warp then
+  // read values from different banks.)
+  static __device__ __forceinline__ int key_of(int n) { return (n >> 1 & 1) | (n & 1) << 1 | (n & 4); }
+
+  __device__ __forceinline__ void prepare(uint8_t*) { pending = nullptr; }
+  __device__ __forceinline__ void look_up(const PagedParams& p, const Cur& c, int warp, int lane) { place.look_up(p, c.x, c.tile(warp) + lane); }
+  // 16-byte chunks of a row are permuted so that neither keys nor values meet in banks
+  static __device__ __forceinline__ int chunk_at(int r, int chunk) { return DP == 128 ? chunk ^ (r >> 1 & 3) : chunk ^ (r >> 2 & 1); }
+
+  __device__ __forceinline__ void issue(const PagedParams& p, const Cur& c, uint8_t* stage, int lane) {
+    constexpr int kChunks = DP / 32, kAtOnce = 32 / kChunks;
+    const uint32_t mine = place.at<1>(p, c.h);
+    const int chunk = lane % kChunks;
+    const uint32_t to = smem_at(stage);
+    const char* k = static_cast<const char*>(p.c.k);
+    const char* v = static_cast<const char*>(p.c.v);
+#pragma unroll
+    for (int i = 0; i < kTile / kAtOnce; ++i) {
+      const int r = i * kAtOnce + lane / kChunks;
+      const uint32_t at = __shfl_sync(0xffffffffu, mine, r);
+      const bool there = at != kNowhere && chunk * 32 < p.c.d;
+      const int64_t from = there ? (int64_t)at * 16 + chunk * 16 : 0;
+      const uint32_t dst = to + r * kRowBytes + (chunk_at(r, chunk) << 4);
+      copy16(dst, k + from, there);
+      copy16(dst + kSide, v + from, there);
+    }
+    settle(nullptr, lane);
+    k_bytes = v_bytes = 0;
+    if (mine != kNowhere) {
+      const int64_t at = (int64_t)place.page * p.c.scale_stride_page + (int64_t)place.slot * p.c.scale_stride_slot + (int64_t)c.h * p.c.scale_stride_head;
+      const int n = p.c.d / 32;
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i)
+        if (i < n) {
+          k_bytes |= (uint32_t)__ldg(p.c.k_scale + at + i) << (8 * i);
+          v_bytes |= (uint32_t)__ldg(p.c.v_scale + at + i) << (8 * i);
+        }
+    }
+    pending = stage;
+  }
+  __device__ __forceinline__ void settle(uint8_t*) { settle(nullptr, threadIdx.x & 31); }
+  static __device__ __forceinline__ int largest(uint32_t bytes) {     // E + 127 of a head
+    int top = 127 - 65;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int b = bytes >> (8 * i) & 255;
+      if (b != 255) top = max(top, b);
+    }
+    return top;
+  }
+  static __device__ __forceinline__ uint16_t power(uint32_t bytes, int i, int top) {   // 2^(e - E + kCodeUp) as float16, 2^-24 being its smallest
+    const int b = bytes >> (8 * i) & 255, x = b - top + kCodeUp;
+    if (b == 255) return 0x7fff;
+    return x >= -14 ? (uint16_t)((x + 15) << 10) : x >= -24 ? (uint16_t)(1 << (x + 24)) : (uint16_t)0;
+  }
+  // The powers of two that were asked for with the last tile, into its stage.
+  __device__ __forceinline__ void settle(uint8_t*, int lane) {
+    if (!pending) return;
+    const int kt = largest(k_bytes), vt = largest(v_bytes);
+    uint16_t* kp = reinterpret_cast<uint16_t*>(pending + kKeyPowers);
+    uint16_t* vp = reinterpret_cast<uint16_t*>(pending + kValuePowers);
+    float* top = reinterpret_cast<float*>(pending + kKeyTop);
+    const int r = lane & 7, n = (r & 1) << 1 | (r >> 1 & 1) | (r & 4), place_of = (lane & 24) + n;       // (key_of is its own inverse)
+    *reinterpret_cast<uint2*>(kp + lane * 4) = make_uint2(power(k_bytes, 0, kt) | (uint32_t)power(k_bytes, 1, kt) << 16, power(k_bytes, 2, kt) | (uint32_t)power(k_bytes, 3, kt) << 16);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) vp[i * 32 + place_of] = power(v_bytes, i, vt);
+    top[place_of] = __uint_as_float((uint32_t)(kt - kCodeUp) << 23);               // what a score is to be multiplied by,
+    top[32 + place_of] = (float)(vt - 127);                                          // what its exponent gets,
+    top[64 + place_of] = __uint_as_float((uint32_t)(254 + kCodeUp - vt) << 23);      // and a weight's part of their sum
+    pending = nullptr;
+  }
+  __device__ __forceinline__ void begin(const PagedParams& p, const Cur& c, uint8_t*, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+    rows.start(p, c.x, g);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const int row = c.x.row0 + i * 16 + s * 8 + g;
+        const __nv_bfloat16* from = query_row(p, c.x, c.h, min(row, p.rows - 1));
+        // components (DP / 4) t and up
+        float x[DP / 4];
+        float top = 0.f;
+#pragma unroll
+        for (int k = 0; k < DP / 4; k += 8) {
+          const int d = DP / 4 * t + k;
+          const uint4 v = row < p.rows && d < p.c.d ? __ldg(reinterpret_cast<const uint4*>(from + d)) : make_uint4(0, 0, 0, 0);
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int z = 0; z < 8; ++z) {
+            x[k + z] = __uint_as_float(z & 1 ? w[z / 2] & 0xffff0000u : w[z / 2] << 16);
+            top = fmaxf(top, fabsf(x[k + z]));
+          }
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int e = min(max((int)(__float_as_uint(top) >> 23), 1), 253);      // top < 2^(e - 126)
+        const float down = __uint_as_float((uint32_t)(254 - e) << 23);
+        scale[i][s] = p.scale_log2 * __uint_as_float((uint32_t)e << 23);
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const __half2 h = __floats2half2_rn(x[4 * k + 2 * u] * down, x[4 * k + 2 * u + 1] * down);
+            q[i][k][u * 2 + s] = *reinterpret_cast<const uint32_t*>(&h);
+          }
+      }
+#pragma unroll
+      for (int j = 0; j < DP / 8; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][j][e] = 0.f;
+    }
+  }
+  static __device__ __forceinline__ uint32_t times(uint32_t a, uint32_t b) {
+    const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+  __device__ __forceinline__ void take(const PagedParams& p, const Cur& c, const uint8_t* stage, int k0, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+    const bool cut = is_cut<kRows>(p, c.x, k0, kTile);
+    const float* tops = reinterpret_cast<const float*>(stage + kKeyTop);
+    float s[MT][4][4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[i][n][e] = 0.f;
+      const int r = n * 8 + key_of(g);
+      uint32_t codes[kWords];
+      if constexpr (DP == 128) {
+        const uint4 x = *reinterpret_cast<const uint4*>(stage + r * kRowBytes + (chunk_at(r, t) << 4));
+        codes[0] = x.x; codes[1] = x.y; codes[2] = x.z; codes[3] = x.w;
+      } else {
+        const uint2 x = *reinterpret_cast<const uint2*>(stage + r * kRowBytes + (chunk_at(r, t >> 1) << 4) + (t & 1) * 8);
+        codes[0] = x.x; codes[1] = x.y;
+      }
+      const uint32_t f = *reinterpret_cast<const uint16_t*>(stage + kKeyPowers + r * 8 + (DP == 128 ? t : t >> 1) * 2) * 0x10001u;
+#pragma unroll
+      for (int w = 0; w < kWords; ++w) {
+        uint32_t b[4];
+        from_e2m1x8(codes[w], b);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) b[u] = times(b[u], f);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          mma_f16(s[i][n], q[i][2 * w], b[0], b[1]);
+          mma_f16(s[i][n], q[i][2 * w + 1], b[2], b[3]);
+        }
+      }
+    }
+    uint32_t w[MT][2][4];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      float top[2] = {rows.m[i][0], rows.m[i][1]};
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const float2 ek = *reinterpret_cast<const float2*>(tops + n * 8 + 2 * t), ev = *reinterpret_cast<const float2*>(tops + 32 + n * 8 + 2 * t);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float x = fmaf(s[i][n][e] * (e & 1 ? ek.y : ek.x), scale[i][e >> 1], e & 1 ? ev.y : ev.x);
+          if (cut && !rows.sees(p, i, e >> 1, k0 + n * 8 + key_of(2 * t + (e & 1)))) x = -INFINITY;
+          s[i][n][e] = x;
+          top[e >> 1] = fmaxf(top[e >> 1], x);
+        }
+      }
+      rescale(i, top);
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const float2 em = *reinterpret_cast<const float2*>(tops + 64 + n * 8 + 2 * t);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = exp2_approx(s[i][n][e] - top[e >> 1]);
+          rows.l[i][e >> 1] = fmaf(x, e & 1 ? em.y : em.x, rows.l[i][e >> 1]);
+          s[i][n][e] = x;
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const __half2 x = __floats2half2_rn(s[i][2 * h + (u >> 1)][(u & 1) * 2], s[i][2 * h + (u >> 1)][(u & 1) * 2 + 1]);
+          w[i][h][u] = *reinterpret_cast<const uint32_t*>(&x);
+        }
+    }
+    const int t0 = c.x.row0 / p.G, t1 = (min(c.x.row0 + kRows, p.rows) - 1) / p.G;
+    if (!cut || t0 == t1) values<false>(p, stage, k0, lane, w, 0);
+    else
+      for (int tok = t0; tok <= min(t1, c.x.count - 1); ++tok) values<true>(p, stage, k0, lane, w, c.x.first + tok);
+  }
+  // o += w V.  ONE: only the rows of the token at `at`, of the keys that it sees.
+  template <bool ONE>
+  __device__ __forceinline__ void values(const PagedParams& p, const uint8_t* stage, int k0, int lane, const uint32_t (&w)[MT][2][4], int at) {
+    const int g = lane >> 2, t = lane & 3;
+    constexpr int kN = DP / 8 / 8;      // words of 8 codes that a lane holds of a key: the head's DP / 8 columns of g
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t b[2][DP / 8];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int n = 2 * h + u, ra = n * 8 + key_of(2 * t), rb = n * 8 + key_of(2 * t + 1);
+        uint32_t f = *reinterpret_cast<const uint32_t*>(stage + kValuePowers + ((DP == 128 ? g >> 1 : g >> 2) * 32 + n * 8 + 2 * t) * 2);
+        uint32_t seen = 0xffffffffu;
+        if (ONE) {
+          seen = 0;
+          if (k0 + ra <= at && (p.a.window < 0 || k0 + ra >= at - p.a.window)) seen |= 0xffffu;
+          if (k0 + rb <= at && (p.a.window < 0 || k0 + rb >= at - p.a.window)) seen |= 0xffff0000u;
+        }
+        uint32_t ca[kN], cb[kN];
+        const uint8_t* v = stage + kSide;
+        if constexpr (DP == 128) {
+          const uint2 xa = *reinterpret_cast<const uint2*>(v + ra * kRowBytes + (chunk_at(ra, g >> 1) << 4) + (g & 1) * 8);
+          const uint2 xb = *reinterpret_cast<const uint2*>(v + rb * kRowBytes + (chunk_at(rb, g >> 1) << 4) + (g & 1) * 8);
+          ca[0] = xa.x; ca[1] = xa.y; cb[0] = xb.x; cb[1] = xb.y;
+        } else {
+          ca[0] = *reinterpret_cast<const uint32_t*>(v + ra * kRowBytes + (chunk_at(ra, g >> 2) << 4) + (g & 3) * 4);
+          cb[0] = *reinterpret_cast<const uint32_t*>(v + rb * kRowBytes + (chunk_at(rb, g >> 2) << 4) + (g & 3) * 4);
+        }
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+          const uint32_t even = (ca[i] & 0x0f0f0f0fu) | (cb[i] & 0x0f0f0f0fu) << 4, odd = (ca[i] >> 4 & 0x0f0f0f0fu) | (cb[i] & 0xf0f0f0f0u);
+          uint32_t x[4], y[4];
+          from_e2m1x8(even, x);
+          from_e2m1x8(odd, y);
+#pragma unroll
+          for (int z = 0; z < 4; ++z) {
+            b[u][i * 8 + 2 * z] = times(x[z], f) & seen;
+            b[u][i * 8 + 2 * z + 1] = times(y[z], f) & seen;
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < DP / 8; ++j)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          if (!ONE) mma_f16(o[i][j], w[i][h], b[0][j], b[1][j]);
+          else {
+            float x[4] = {0.f, 0.f, 0.f, 0.f};
+            mma_f16(x, w[i][h], b[0][j], b[1][j]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (rows.at[i][e >> 1] == at) o[i][j][e] += x[e];
+          }
+        }
+    }
+  }
+  __device__ __forceinline__ void rescale(int i, float (&top)[2]) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      top[s] = fmaxf(top[s], __shfl_xor_sync(0xffffffffu, top[s], 1));
+      top[s] = fmaxf(top[s], __shfl_xor_sync(0xffffffffu, top[s], 2));
+    }
+    const bool moved = top[0] != rows.m[i][0] || top[1] != rows.m[i][1];
+    if (__any_sync(0xffffffffu, moved)) {
+      float f[2];
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        f[s] = top[s] == -INFINITY ? 1.f : exp2_approx(rows.m[i][s] - top[s]);
+        rows.l[i][s] *= f[s];
+        rows.m[i][s] = top[s];
+      }
+#pragma unroll
+      for (int j = 0; j < DP / 8; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][j][e] *= f[e >> 1];
+    }
+#pragma unroll
+    for (int s = 0; s < 2; ++s) top[s] = top[s] == -INFINITY ? 0.f : top[s] - kWeightUp;
+  }
+  // (sums of weights are too large by 2^(kWeightUp + kCodeUp), those of values as well)
+  __device__ __forceinline__ void stats(const Buffer<DP>& buffer, int warp, int lane) const { rows.stats(buffer, warp, lane, kWeightUp + kCodeUp); }
+  __device__ __forceinline__ void put(int pass, float factor, float* out, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        if (pass == i * 2 + s) {
+#pragma unroll
+          for (int j = 0; j < DP / 8; ++j)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) out[g * (DP + 8) + (2 * t + u) * (DP / 8) + j] = o[i][j][2 * s + u] * factor;
+        }
+  }
+};
+
+// ---- float32: FMA arithmetic ----------------------------------------------------------------------------------------------
+// For the scores two lanes share a key, for the sums a lane has DP / 32 columns; the rows of Q are read from shared memory, by all lanes at once.
+template <int DP, int ROWS>
+struct CoreF32 {
+  static constexpr int kDP = DP, kRows = ROWS, kTile = 16, kStages = 2, kMinCtas = 1;
+  static constexpr int kRowBytes = DP * 4, kSide = kTile * kRowBytes, kStageBytes = 2 * kSide;
+  static constexpr int kQRow = DP + 4;         // floats: the second half of a row lies 4 further on, in other banks than the first
+  static constexpr int kExtra = ROWS * kQRow * 4 + kWarps * kTile * ROWS * 4;
+  static constexpr int kCols = DP / 32;
+  using Cur = Cursor<kRows, kTile>;
+
+  float o[ROWS][kCols];
+  float m[ROWS], l[ROWS];      // of all rows; l: this lane's key's share
+  Place place;
+  float *qs, *ps;
+
+  __device__ __forceinline__ void prepare(uint8_t* extra) {
+    qs = reinterpret_cast<float*>(extra);
+    ps = qs + ROWS * kQRow + (threadIdx.x >> 5) * kTile * ROWS;
+  }
+  __device__ __forceinline__ void look_up(const PagedParams& p, const Cur& c, int warp, int lane) { place.look_up(p, c.x, c.tile(warp) + (lane & 15)); }
+  __device__ __forceinline__ void settle(uint8_t*) {}
+  __device__ __forceinline__ void issue(const PagedParams& p, const Cur& c, uint8_t* stage, int lane) {
+    constexpr int kChunks = DP / 4, kAtOnce = 32 / kChunks;
+    const uint32_t mine = place.at<4>(p, c.h);
+    const int chunk = lane % kChunks;
+    const uint32_t to = smem_at(stage);
+    const char* k = static_cast<const char*>(p.c.k);
+    const char* v = static_cast<const char*>(p.c.v);
+#pragma unroll
+    for (int i = 0; i < kTile / kAtOnce; ++i) {
+      const int r = i * kAtOnce + lane / kChunks;
+      const uint32_t at = __shfl_sync(0xffffffffu, mine, r);
+      const bool there = at != kNowhere && chunk * 4 < p.c.d;
+      const int64_t from = there ? (int64_t)at * 16 + chunk * 16 : 0;
+      const uint32_t dst = to + r * kRowBytes + ((chunk ^ (r & 7)) << 4);
+      copy16(dst, k + from, there);
+      copy16(dst + kSide, v + from, there);
+    }
+  }
+  __device__ __forceinline__ void begin(const PagedParams& p, const Cur& c, uint8_t*, int lane) {
+    const int n = min(ROWS, p.rows - c.x.row0);
+    __syncthreads();             // (the last item's rows have been read)
+    for (int i = threadIdx.x; i < ROWS * DP; i += kThreads) {
+      const int r = i / DP, d = i % DP, row = c.x.row0 + r;
+      float x = 0.f;
+      if (r < n && d < p.c.d)
+        x = __ldg(static_cast<const float*>(p.a.q.ptr) + c.x.b * p.a.q.stride_b + (row / p.G) * p.a.q.stride_l + (c.h * p.G + row % p.G) * p.a.q.stride_h + d);
+      qs[r * kQRow + d + (d >= DP / 2 ? 4 : 0)] = x;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      m[r] = -INFINITY;
+      l[r] = 0.f;
+#pragma unroll
+      for (int j = 0; j < kCols; ++j) o[r][j] = 0.f;
+    }
+  }
+  __device__ __forceinline__ void take(const PagedParams& p, const Cur& c, const uint8_t* stage, int k0, int lane) {
+    const int key = lane & 15, half = lane >> 4;
+    float s[ROWS];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) s[r] = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < DP / 8; ++i) {
+      const int chunk = half * (DP / 8) + i;
+      const float4 k = *reinterpret_cast<const float4*>(stage + key * kRowBytes + ((chunk ^ (key & 7)) << 4));
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+        const float4 x = *reinterpret_cast<const float4*>(qs + r * kQRow + chunk * 4 + half * 4);
+        s[r] = fmaf(x.x, k.x, fmaf(x.y, k.y, fmaf(x.z, k.z, fmaf(x.w, k.w, s[r]))));
+      }
+    }
+    const bool cut = is_cut<kRows>(p, c.x, k0, kTile);
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      float x = (s[r] + __shfl_xor_sync(0xffffffffu, s[r], 16)) * p.scale_log2;
+      bool seen = true;
+      if (cut) {
+        const int row = c.x.row0 + r, t = row / p.G, at = row < p.rows && t < c.x.count ? c.x.first + t : -1, k = k0 + key;
+        seen = k <= at && (p.a.window < 0 || k >= at - p.a.window);
+        if (!seen) x = -INFINITY;
+      }
+      float top = fmaxf(m[r], x);
+#pragma unroll
+      for (int b = 1; b < 16; b <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, b));
+      const float base = top == -INFINITY ? 0.f : top;
+      if (top != m[r]) {
+        const float f = exp2_approx(m[r] - base);
+        l[r] *= f;
+#pragma unroll
+        for (int j = 0; j < kCols; ++j) o[r][j] *= f;
+        m[r] = top;
+      }
+      x = exp2f(x - base);
+      l[r] += x;
+      s[r] = seen ? x : -1.f;
+    }
+    const bool strict = cut && p.a.T > 1;      // some row sees what another does not
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+      if (half == 0) ps[key * ROWS + r] = s[r] == -1.f && !strict ? 0.f : s[r];
+    __syncwarp();
+#pragma unroll 4
+    for (int k = 0; k < kTile; ++k) {
+      float v[kCols];
+      const uint8_t* row = stage + kSide + k * kRowBytes;
+      if constexpr (kCols == 4) {
+        const float4 x = *reinterpret_cast<const float4*>(row + ((lane ^ (k & 7)) << 4));
+        v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+      } else {
+        const float2 x = *reinterpret_cast<const float2*>(row + (((lane >> 1) ^ (k & 7)) << 4) + (lane & 1) * 8);
+        v[0] = x.x; v[1] = x.y;
+      }
+#pragma unroll
+      for (int r4 = 0; r4 < ROWS; r4 += 4) {
+        const float4 w4 = *reinterpret_cast<const float4*>(ps + k * ROWS + r4);
+        const float w[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int j = 0; j < kCols; ++j) {
+            if (strict && w[r] == -1.f) continue;
+            o[r4 + r][j] = fmaf(w[r], v[j], o[r4 + r][j]);
+          }
+      }
+    }
+    __syncwarp();
+  }
+  __device__ __forceinline__ void stats(const Buffer<DP>& buffer, int warp, int lane) const {
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      float x = l[r];
+#pragma unroll
+      for (int b = 1; b < 16; b <<= 1) x += __shfl_xor_sync(0xffffffffu, x, b);
+      if (lane == 0) buffer.stat(warp, r) = make_float2(m[r], x);
+    }
+  }
+  __device__ __forceinline__ void put_rows(int pass, const float* factors, float* out, int lane) {
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+      if (r >> 3 == pass)
+#pragma unroll
+        for (int j = 0; j < kCols; ++j) out[(r & 7) * (DP + 8) + lane * kCols + j] = o[r][j] * factors[r & 7];
+  }
+};
+
+// ---- the walk ---------------------------------------------------------------------------------------------------------------
+template <class Core>
+constexpr int paged_smem() {
+  return kWarps * Core::kStages * Core::kStageBytes + Buffer<Core::kDP>::kFloats * 4 + Core::kExtra;
+}
+template <class Core> struct IsSimt { static constexpr bool value = false; };
+template <int DP, int ROWS> struct IsSimt<CoreF32<DP, ROWS>> { static constexpr bool value = true; };
+
+// A finished row's value: four components and (at the first) the log-sum-exp; zeros for a token that is not real.
+__device__ __forceinline__ void write_result(const PagedParams& p, int b, int h, int row, bool real, int col, float4 x, float top, float sum) {
+  const bool any = real && (sum > 0.f || sum != sum);
+  const float f = any ? 1.f / sum : 0.f;
+  x = any ? make_float4(x.x * f, x.y * f, x.z * f, x.w * f) : make_float4(0.f, 0.f, 0.f, 0.f);
+  const int t = row / p.G, head = h * p.G + row % p.G;
+  const int64_t at = b * p.a.o.stride_b + t * p.a.o.stride_l + head * p.a.o.stride_h + col;
+  if (col < p.c.d) {
+    if (p.a.o.dtype == BMA_DTYPE_F32) *reinterpret_cast<float4*>(static_cast<float*>(p.a.o.ptr) + at) = x;
+    else {
+      const __nv_bfloat162 lo = __floats2bfloat162_rn(x.x, x.y), hi = __floats2bfloat162_rn(x.z, x.w);
+      *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.a.o.ptr) + at) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+    }
+  }
+  if (col == 0 && p.a.lse) p.a.lse[((int64_t)b * p.a.Hq + head) * p.a.T + t] = any ? fmaf(top, kLn2, logf(sum)) : -INFINITY;
 }
 
+// The warps' parts of an item put together: written as the result where the CTA has all of it, else as a part.
+template <class Core>
+__device__ __forceinline__ void finish(const PagedParams& p, Core& core, const typename Core::Cur& c, bool whole, int slot, const Buffer<Core::kDP>& buffer, int warp, int lane) {
+  constexpr int DP = Core::kDP;
+  core.stats(buffer, warp, lane);
+  __syncthreads();
+  const int n = min(Core::kRows, p.rows - c.x.row0);
+  auto joined = [&](int row, float& top, float& sum) {      // over the warps; what their exponents are taken against
+    top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, buffer.stat(w, row).x);
+    const float base = top == -INFINITY ? 0.f : top;
+    sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float2 x = buffer.stat(w, row);
+      sum = fmaf(x.y, exp2_approx(x.x - base), sum);
+    }
+    return base;
+  };
+  for (int pass = 0; pass * 8 < n; ++pass) {
+    if constexpr (IsSimt<Core>::value) {
+      float f[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        float top, sum;
+        const int row = min(pass * 8 + r, Core::kRows - 1);
+        const float base = joined(row, top, sum);
+        f[r] = exp2_approx(buffer.stat(warp, row).x - base);
+      }
+      core.put_rows(pass, f, buffer.line(warp, 0), lane);
+    } else {
+      float top, sum;
+      const int row = pass * 8 + (lane >> 2);
+      const float base = joined(row, top, sum);
+      core.put(pass, exp2_approx(buffer.stat(warp, row).x - base), buffer.line(warp, 0), lane);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 8 * (DP / 4); i += kThreads) {
+      const int r = i / (DP / 4), col = i % (DP / 4) * 4, row = pass * 8 + r;
+      if (row >= n) break;
+      float4 x = *reinterpret_cast<const float4*>(buffer.line(0, r) + col);
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w) {
+        const float4 y = *reinterpret_cast<const float4*>(buffer.line(w, r) + col);
+        x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+      }
+      float top, sum;
+      joined(row, top, sum);
+      if (!whole) {
+        const int64_t at = (int64_t)slot * Core::kRows + row;
+        *reinterpret_cast<float4*>(p.part_o + at * DP + col) = x;
+        if (col == 0) p.part_ml[at] = make_float2(top, sum);
+      } else write_result(p, c.x.b, c.h, c.x.row0 + row, (c.x.row0 + row) / p.G < c.x.count, col, x, top, sum);
+    }
+    __syncthreads();
+  }
+}
+
+template <class Core>
+__global__ void __launch_bounds__(kThreads, Core::kMinCtas) paged_kernel(const __grid_constant__ PagedParams p) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  using Cur = typename Core::Cur;
+  constexpr int NS = Core::kStages;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  uint8_t* ring = smem + warp * NS * Core::kStageBytes;
+  const Buffer<Core::kDP> buffer{reinterpret_cast<float*>(smem + kWarps * NS * Core::kStageBytes)};
+  asm volatile("griddepcontrol.launch_dependents;");
+
+  // The run of this CTA: prefix sums of the entries' units, kThreads at a time.
+  int64_t* scan = reinterpret_cast<int64_t*>(buffer.at);      // sums of the warps, then the entry that the run begins in, and where
+  auto block_scan = [&](int x, int64_t& before, int64_t& all) {
+    int64_t y = x;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t z = __shfl_up_sync(0xffffffffu, y, o);
+      if (lane >= o) y += z;
+    }
+    if (lane == 31) scan[warp] = y;
+    __syncthreads();
+    before = y - x;
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) before += scan[w];
+      all += scan[w];
+    }
+    __syncthreads();
+  };
+  auto units_of = [&](int e) { return e < p.entries ? entry_of<Core::kRows, Core::kTile>(p, e).units : 0; };
+  int64_t total = 0, before = 0, all = 0;
+  int own = 0;
+  for (int e0 = 0; e0 < p.entries; e0 += kThreads) {
+    own = units_of(e0 + threadIdx.x);
+    block_scan(own, before, all);
+    total += all;
+  }
+  total *= p.c.Hkv;
+  if (threadIdx.x == 0) p.meta[blockIdx.x] = make_int4(-1, 0, 0, 0);
+  const int ctas = (int)min((int64_t)gridDim.x, total);       // (no run is empty)
+  if (blockIdx.x >= ctas) return;
+  const int64_t begin = run_begin(total, blockIdx.x, ctas), end = run_begin(total, blockIdx.x + 1, ctas);
+  int64_t gone = 0;
+  for (int e0 = 0; e0 < p.entries; e0 += kThreads) {
+    if (p.entries > kThreads) {
+      own = units_of(e0 + threadIdx.x);
+      block_scan(own, before, all);
+    }
+    const int64_t from = (gone + before) * p.c.Hkv;
+    if (begin >= from && begin < from + (int64_t)own * p.c.Hkv) {
+      scan[kWarps + 1] = e0 + threadIdx.x;
+      scan[kWarps + 2] = begin - from;
+    }
+    gone += all;
+  }
+  __syncthreads();
+  Cur next;
+  next.e = (int)scan[kWarps + 1];
+  const int64_t within = scan[kWarps + 2];
+  next.x = entry_of<Core::kRows, Core::kTile>(p, next.e);
+  next.h = (int)(within / next.x.units);
+  next.unit = (int)(within - (int64_t)next.h * next.x.units);
+  __syncthreads();              // (the buffer is used again)
+
+  Core core;
+  core.prepare(reinterpret_cast<uint8_t*>(buffer.at + Buffer<Core::kDP>::kFloats));
+  Cur here = next;
+  const int n = (int)(end - begin);
+  core.look_up(p, next, warp, lane);
+  auto issue = [&](int i) {
+    if (i < n) {
+      core.issue(p, next, ring + i % NS * Core::kStageBytes, lane);
+      if (i + 1 < n) {
+        next.next(p);
+        core.look_up(p, next, warp, lane);
+      }
+    }
+    copies_committed();
+  };
+  for (int i = 0; i < NS - 1; ++i) issue(i);
+  bool fresh = true;           // the first unit of an item in this run
+  int first_unit = here.unit;
+  bool first_item = true;
+  for (int i = 0; i < n; ++i) {
+    core.settle(nullptr);
+    issue(i + NS - 1);
+    copies_awaited<NS - 1>();
+    __syncwarp();
+    if (fresh) {
+      core.begin(p, here, nullptr, lane);
+      first_unit = here.unit;
+      fresh = false;
+    }
+    const int k0 = here.tile(warp);
+    if (k0 < here.x.hi) core.take(p, here, ring + i % NS * Core::kStageBytes, k0, lane);
+    __syncwarp();
+    const bool last = here.unit + 1 == here.x.units;
+    if (last || i + 1 == n) {
+      const bool whole = last && first_unit == 0;
+      const int slot = 2 * blockIdx.x + (first_item ? 0 : 1);
+      if (!whole && !last && first_unit == 0 && threadIdx.x == 0) {      // the first part of an item that goes on in other CTAs
+        const int64_t item_end = end + (here.x.units - here.unit - 1);   // (this run ends with unit here.unit of it)
+        int cta = (int)((item_end - 1) * ctas / total);             // the CTA whose run holds its last unit
+        while (run_begin(total, cta + 1, ctas) < item_end) ++cta;
+        while (run_begin(total, cta, ctas) >= item_end) --cta;
+        p.meta[blockIdx.x] = make_int4(here.e, here.h, slot, cta);
+      }
+      finish<Core>(p, core, here, whole, slot, buffer, warp, lane);
+      fresh = true;
+      first_item = false;
+    }
+    here.next(p);
+  }
+  copies_awaited<0>();
+}
+
+// One warp: a row of an item that several CTAs had parts of.
+template <int DP, int ROWS>
+__global__ void __launch_bounds__(kThreads) paged_join_kernel(const __grid_constant__ PagedParams p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int4 m = p.meta[blockIdx.x];
+  if (m.x < 0) return;
+  const int lane = threadIdx.x & 31, row = blockIdx.y * kWarps + (threadIdx.x >> 5);
+  const int b = m.x / p.row_tiles, row0 = (m.x - b * p.row_tiles) * ROWS;
+  if (row >= min(ROWS, p.rows - row0)) return;
+  const int parts = m.w - blockIdx.x + 1;
+  auto slot = [&](int i) { return ((int64_t)(i == 0 ? m.z : 2 * (blockIdx.x + i))) * ROWS + row; };
+  float top = -INFINITY;
+  for (int i = lane; i < parts; i += 32) top = fmaxf(top, p.part_ml[slot(i)].x);
+  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float base = top == -INFINITY ? 0.f : top;
+  float x[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
+  if (lane * 4 >= DP) return;
+#pragma unroll 4
+  for (int i = 0; i < parts; ++i) {
+    const int64_t at = slot(i);
+    const float2 ml = p.part_ml[at];
+    const float f = exp2_approx(ml.x - base);
+    sum = fmaf(ml.y, f, sum);
+    const float4 y = *reinterpret_cast<const float4*>(p.part_o + at * DP + lane * 4);
+    x[0] = fmaf(y.x, f, x[0]); x[1] = fmaf(y.y, f, x[1]); x[2] = fmaf(y.z, f, x[2]); x[3] = fmaf(y.w, f, x[3]);
+  }
+  const bool real = (row0 + row) / p.G < new_tokens(p.a.lengths, p.a.new_lengths, b, p.a.T).count;
+  write_result(p, b, m.y, row0 + row, real, lane * 4, make_float4(x[0], x[1], x[2], x[3]), top, sum);
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------------------
 int validate_paged(const bma_paged_cache* c, const bma_paged_attn_args* a) {
   int rc = validate_cache(c);
   if (rc != BMA_OK) return rc;
   BMA_REQUIRE(a && a->T > 0 && a->Hq > 0 && a->lengths, BMA_ERR_ARG);
   BMA_REQUIRE(a->Hq % c->Hkv == 0, BMA_ERR_ARG);
   BMA_REQUIRE(a->Hq <= 65535 && (int64_t)a->T * a->Hq < (1ll << 30), BMA_ERR_LIMIT);
-  BMA_REQUIRE(a->q.ptr && a->o.ptr, BMA_ERR_ARG);
   BMA_REQUIRE(a->q.dtype == (c->dtype == BMA_DTYPE_F32 ? BMA_DTYPE_F32 : BMA_DTYPE_BF16), BMA_ERR_UNSUPPORTED);
   BMA_REQUIRE(a->o.dtype == BMA_DTYPE_F32 || a->o.dtype == BMA_DTYPE_BF16, BMA_ERR_UNSUPPORTED);
+  // the kernels count in 16 bytes
+  const int64_t bytes = c->dtype == BMA_DTYPE_F32 ? 4 : c->dtype == BMA_DTYPE_BF16 ? 2 : 1;
+  const int64_t last = ((int64_t)(c->pages - 1) * c->stride_page + (int64_t)(c->page_size - 1) * c->stride_slot + (int64_t)(c->Hkv - 1) * c->stride_head) * bytes / 16;
+  BMA_REQUIRE(c->stride_page >= 0 && c->stride_slot >= 0 && c->stride_head >= 0 && last < (int64_t)kNowhere, BMA_ERR_LIMIT);
   return BMA_OK;
+}
+
+struct PagedLaunch {
+  int rows_of_tile, dp, tile, ctas_per_sm;
+  int ctas, entries, row_tiles;
+  size_t bytes() const { return (size_t)ctas * (2 * (size_t)rows_of_tile * (dp * 4 + 8) + 16); }
+};
+
+// The instance for a call: heads of up to 64 or 128 components; tiles of as many rows as the call has, up to 32 on the tensor core (more would not
+// leave room for the sums in registers) and 16 in FMA arithmetic.  As many CTAs as run at once, or as there can be units.
+bool plan_paged(const bma_paged_cache& c, const bma_paged_attn_args& a, PagedLaunch& l) {
+  const int rows = a.T * (a.Hq / c.Hkv);
+  l.dp = c.d <= 64 ? 64 : 128;
+  l.tile = c.dtype == BMA_DTYPE_MXFP4 ? 32 : 16;
+  l.rows_of_tile = c.dtype == BMA_DTYPE_F32 ? (rows <= 4 ? 4 : rows <= 8 ? 8 : 16) : rows <= 16 ? 16 : 32;
+  l.ctas_per_sm = c.dtype == BMA_DTYPE_F32 && l.dp == 128 ? 1 : 2;
+  l.row_tiles = ceil_div(rows, l.rows_of_tile);
+  const int64_t entries = (int64_t)c.B * l.row_tiles;
+  if (entries >= (1 << 30)) return false;
+  l.entries = (int)entries;
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const int64_t units = entries * c.Hkv * (((int64_t)c.width * c.page_size + kWarps * l.tile - 1) / (kWarps * l.tile) + 1);
+  l.ctas = (int)std::min<int64_t>((int64_t)sms * l.ctas_per_sm, units);
+  return true;
+}
+
+template <class Core>
+int launch_paged(const PagedParams& p, const PagedLaunch& l, cudaStream_t st) {
+  constexpr int smem = paged_smem<Core>();
+  BMA_CUDA_TRY(cudaFuncSetAttribute(paged_kernel<Core>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  paged_kernel<Core><<<l.ctas, kThreads, smem, st>>>(p);
+  BMA_CUDA_TRY(cudaGetLastError());
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(l.ctas, ceil_div(std::min(Core::kRows, p.rows), kWarps));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;      // (its CTAs come up while the last parts are written)
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  BMA_CUDA_TRY(cudaLaunchKernelEx(&cfg, paged_join_kernel<Core::kDP, Core::kRows>, p));
+  count_launches(2);
+  return BMA_OK;
+}
+
+template <int DP>
+int dispatch_paged(const PagedParams& p, const PagedLaunch& l, cudaStream_t st) {
+  switch (p.c.dtype) {
+    case BMA_DTYPE_F32:
+      if (l.rows_of_tile == 4) return launch_paged<CoreF32<DP, 4>>(p, l, st);
+      if (l.rows_of_tile == 8) return launch_paged<CoreF32<DP, 8>>(p, l, st);
+      return launch_paged<CoreF32<DP, 16>>(p, l, st);
+    case BMA_DTYPE_BF16:
+      return l.rows_of_tile == 16 ? launch_paged<CoreBf16<DP, 1>>(p, l, st) : launch_paged<CoreBf16<DP, 2>>(p, l, st);
+    default:
+      return l.rows_of_tile == 16 ? launch_paged<Core4bit<DP, 1>>(p, l, st) : launch_paged<Core4bit<DP, 2>>(p, l, st);
+  }
 }
 
 }  // namespace
@@ -119,18 +1149,37 @@ using namespace bma;
 
 extern "C" {
 
-size_t bma_paged_attn_workspace_bytes(const bma_paged_cache* cache, const bma_paged_attn_args* args) { return 0; }
+size_t bma_paged_attn_workspace_bytes(const bma_paged_cache* cache, const bma_paged_attn_args* args) {
+  PagedLaunch l;
+  return validate_paged(cache, args) == BMA_OK && plan_paged(*cache, *args, l) ? l.bytes() : 0;
+}
 
 int bma_paged_attn(const bma_paged_cache* cache, const bma_paged_attn_args* args, void* workspace, size_t workspace_bytes, bma_stream_t stream) {
   int rc = validate_paged(cache, args);
   if (rc != BMA_OK) return rc;
-  int* status = device_status_ptr();
-  BMA_REQUIRE(status != nullptr, BMA_ERR_CUDA);
-  const dim3 grid(ceil_div(args->T * (args->Hq / cache->Hkv), kRows), cache->Hkv, cache->B);
-  paged_rows_kernel<<<grid, 128, 0, static_cast<cudaStream_t>(stream)>>>(*cache, *args, status);
-  count_launches(1);
-  BMA_CUDA_TRY(cudaGetLastError());
-  return BMA_OK;
+  BMA_REQUIRE(args->q.ptr && args->o.ptr, BMA_ERR_ARG);
+  for (const bma_tensor* t : {&args->q, &args->o}) {            // rows start on 16 bytes
+    const int vec = t->dtype == BMA_DTYPE_F32 ? 4 : 8;
+    BMA_REQUIRE((reinterpret_cast<uintptr_t>(t->ptr) & 15) == 0 && t->stride_b % vec == 0 && t->stride_l % vec == 0 && t->stride_h % vec == 0, BMA_ERR_UNSUPPORTED);
+  }
+  PagedLaunch l;
+  BMA_REQUIRE(plan_paged(*cache, *args, l), BMA_ERR_LIMIT);
+  BMA_REQUIRE(workspace && workspace_bytes >= l.bytes() && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0, BMA_ERR_WORKSPACE);
+  PagedParams p{};
+  p.c = *cache;
+  p.a = *args;
+  p.G = args->Hq / cache->Hkv;
+  p.rows = args->T * p.G;
+  p.row_tiles = l.row_tiles;
+  p.entries = l.entries;
+  p.positions = cache->width * cache->page_size;
+  p.scale_log2 = args->scale * kLog2e;
+  BMA_REQUIRE((p.status = device_status_ptr()) != nullptr, BMA_ERR_CUDA);
+  p.part_o = static_cast<float*>(workspace);
+  p.part_ml = reinterpret_cast<float2*>(p.part_o + (size_t)2 * l.ctas * l.rows_of_tile * l.dp);
+  p.meta = reinterpret_cast<int4*>(p.part_ml + (size_t)2 * l.ctas * l.rows_of_tile);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return l.dp == 64 ? dispatch_paged<64>(p, l, st) : dispatch_paged<128>(p, l, st);
 }
 
 }
