@@ -29,6 +29,8 @@ struct PagedParams {
   bma_paged_attn_args a;
   int G, rows, row_tiles, entries;     // query heads to a kv head, rows to a kv head, tiles of them, (sequence, tile) pairs
   int positions;                       // what the page table covers
+  int page_shift;                      // log2 of the page size, -1 where that is no power of two
+  int scale_words;                     // 4 bits: a head's four powers of two can be read at once
   float scale_log2;
   int* status;
   float* part_o;                       // [2 * CTAs][rows of a tile][DP]
@@ -126,7 +128,7 @@ struct Place {
     page = -1;
     slot = 0;
     if (key >= x.lo && key < x.hi) {
-      const int i = key / p.c.page_size;
+      const int i = p.page_shift < 0 ? key / p.c.page_size : key >> p.page_shift;
       slot = key - i * p.c.page_size;
       page = __ldg(p.c.page_table + (int64_t)x.b * p.c.table_stride + i);
       if (page < 0) page = -2;       // (told from a key that is not looked up)
@@ -147,36 +149,60 @@ __device__ __forceinline__ const __nv_bfloat16* query_row(const PagedParams& p, 
   return static_cast<const __nv_bfloat16*>(p.a.q.ptr) + x.b * p.a.q.stride_b + (row / p.G) * p.a.q.stride_l + (h * p.G + row % p.G) * p.a.q.stride_h;
 }
 
-// Statistics and masks of the rows of a warp's matrix tiles: this lane's are rows g and g + 8 of each of MT tiles of 16.
-template <int MT>
+// Statistics and masks of a warp's rows: scores lie in the accumulators as [keys, rows], and this lane's rows are 2t and 2t + 1 of each of NT tiles of 8.
+template <int NT>
 struct Rows {
-  float m[MT][2], l[MT][2];    // maximum so far (log2 units), this lane's share of the sum
-  int at[MT][2];               // position of the row's token; below every key where it is not real
-  __device__ __forceinline__ void start(const PagedParams& p, const Entry& x, int g) {
+  float m[NT][2], l[NT][2];    // maximum so far (log2 units), this lane's share of the sum
+  int at[NT][2];               // position of the row's token; below every key where it is not real
+  __device__ __forceinline__ void start(const PagedParams& p, const Entry& x, int lane) {
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int i = 0; i < NT; ++i)
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        const int row = x.row0 + i * 16 + s * 8 + g, t = row / p.G;
+        const int row = x.row0 + i * 8 + (lane & 3) * 2 + s, t = row / p.G;
         at[i][s] = row < p.rows && t < x.count ? x.first + t : -1;
         m[i][s] = -INFINITY;
         l[i][s] = 0.f;
       }
   }
-  template <int DP>
-  __device__ __forceinline__ void stats(const Buffer<DP>& buffer, int warp, int lane, int down = 0) const {
+  __device__ __forceinline__ bool sees(const PagedParams& p, int i, int s, int key) const {
+    return key <= at[i][s] && (p.a.window < 0 || key >= at[i][s] - p.a.window);
+  }
+  // Takes this lane's maxima to those of the rows, and what has been added up (o, a column for each row) to the new ones; `top` becomes what exponents
+  // are taken against, 2^up below the maximum.
+  template <int N>
+  __device__ __forceinline__ void rescale(int i, float (&top)[2], float (&o)[N][4], float up = 0.f) {
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int b = 4; b < 32; b <<= 1) top[s] = fmaxf(top[s], __shfl_xor_sync(0xffffffffu, top[s], b));
+    if (__any_sync(0xffffffffu, top[0] != m[i][0] || top[1] != m[i][1])) {
+      float f[2];
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        f[s] = top[s] == -INFINITY ? 1.f : exp2_approx(m[i][s] - top[s]);
+        l[i][s] *= f[s];
+        m[i][s] = top[s];
+      }
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[j][e] *= f[e & 1];
+    }
+#pragma unroll
+    for (int s = 0; s < 2; ++s) top[s] = top[s] == -INFINITY ? 0.f : top[s] - up;
+  }
+  template <int DP>
+  __device__ __forceinline__ void stats(const Buffer<DP>& buffer, int warp, int lane, float up = 0.f) const {
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         float x = l[i][s];
-        x += __shfl_xor_sync(0xffffffffu, x, 1);
-        x += __shfl_xor_sync(0xffffffffu, x, 2);
-        if ((lane & 3) == 0) buffer.stat(warp, i * 16 + s * 8 + (lane >> 2)) = make_float2(m[i][s] - down, x);
+#pragma unroll
+        for (int b = 4; b < 32; b <<= 1) x += __shfl_xor_sync(0xffffffffu, x, b);
+        if (lane < 4) buffer.stat(warp, i * 8 + lane * 2 + s) = make_float2(m[i][s] - up, x);
       }
-  }
-  __device__ __forceinline__ bool sees(const PagedParams& p, int i, int s, int key) const {
-    return key <= at[i][s] && (p.a.window < 0 || key >= at[i][s] - p.a.window);
   }
 };
 // Whether rows of the tile of rows see different parts of the keys [k0, k0 + n), or no row sees some of them.
@@ -185,333 +211,296 @@ __device__ __forceinline__ bool is_cut(const PagedParams& p, const Entry& x, int
   const int t0 = x.row0 / p.G, t1 = min((min(x.row0 + ROWS, p.rows) - 1) / p.G, x.count - 1);
   return k0 < x.lo || k0 + n - 1 > x.first + t0 || (p.a.window >= 0 && k0 < x.first + t1 - p.a.window);
 }
+// Halves of a pair of keys that the token at `at` sees, as a mask of 16-bit values
+__device__ __forceinline__ uint32_t seen_pair(const PagedParams& p, int at, int key) {
+  uint32_t m = 0;
+  if (key <= at && (p.a.window < 0 || key >= at - p.a.window)) m |= 0xffffu;
+  if (key + 1 <= at && (p.a.window < 0 || key + 1 >= at - p.a.window)) m |= 0xffff0000u;
+  return m;
+}
+// An 8 x 8 matrix of 16-bit values, [keys, rows], turned
+__device__ __forceinline__ uint32_t turned(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// Copies of a tile's rows of BYTES bytes (16 * CHUNKS), keys to `to`, values SIDE further on; `mine` is the place of this lane's key (lane % TILE), SLOT(r, chunk) where
+// chunk `chunk` of row r goes.
+template <int TILE, int CHUNKS, int SIDE, typename F>
+__device__ __forceinline__ void copy_rows(const PagedParams& p, uint32_t mine, int chunks, uint32_t to, int lane, F slot) {
+  constexpr int kAtOnce = 32 / CHUNKS;       // rows copied by one instruction
+  const int chunk = lane % CHUNKS;
+  const char* k = static_cast<const char*>(p.c.k) + chunk * 16;
+  const char* v = static_cast<const char*>(p.c.v) + chunk * 16;
+  if (__all_sync(0xffffffffu, mine != kNowhere) && chunks == CHUNKS) {
+#pragma unroll
+    for (int i = 0; i < TILE / kAtOnce; ++i) {
+      const int r = i * kAtOnce + lane / CHUNKS;
+      const int64_t from = (int64_t)__shfl_sync(0xffffffffu, mine, r) * 16;
+      const uint32_t dst = to + slot(r, chunk);
+      copy16(dst, k + from, true);
+      copy16(dst + SIDE, v + from, true);
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < TILE / kAtOnce; ++i) {
+    const int r = i * kAtOnce + lane / CHUNKS;
+    const uint32_t at = __shfl_sync(0xffffffffu, mine, r);
+    const bool there = at != kNowhere && chunk < chunks;
+    const int64_t from = there ? (int64_t)at * 16 : -(int64_t)chunk * 16;
+    const uint32_t dst = to + slot(r, chunk);
+    copy16(dst, k + from, there);
+    copy16(dst + SIDE, v + from, there);
+  }
+}
 
 // ---- bfloat16: matrix instructions fed by ldmatrix ------------------------------------------------------------------
-// Rows (tokens x heads) are the M of mma.m16n8k16, keys its N for the scores and its K for the sums.  tcgen05 would want 128 rows or a
-// transposed softmax; there are 1 to 32 rows here, and mma.sync needs a fifth of the time that the bytes take.
-template <int DP, int MT>
+// Keys are the M of mma.m16n8k16 and rows (tokens x heads) its N for the scores; components are the M and rows the N for the sums: 8 rows are a
+// tile, where rows as M would make 16 of one.  The weights go from the accumulators of the one to the operand of the other by movmatrix.
+template <int DP, int NT>
 struct CoreBf16 {
-  static constexpr int kDP = DP, kRows = MT * 16, kTile = 16, kStages = DP == 128 ? 3 : 4, kMinCtas = 2;
+  static constexpr int kDP = DP, kRows = NT * 8, kTile = 16, kStages = DP == 128 ? 3 : 4, kMinCtas = 2;
   static constexpr int kRowBytes = DP * 2, kSide = kTile * kRowBytes, kStageBytes = 2 * kSide, kExtra = 0;
   using Cur = Cursor<kRows, kTile>;
 
-  uint32_t q[MT][DP / 16][4];
-  float o[MT][DP / 8][4];
-  Rows<MT> rows;
+  uint32_t q[NT][DP / 16][2];
+  float o[NT][DP / 16][4];
+  Rows<NT> rows;
   Place place;
 
   __device__ __forceinline__ void prepare(uint8_t*) {}
   __device__ __forceinline__ void look_up(const PagedParams& p, const Cur& c, int warp, int lane) { place.look_up(p, c.x, c.tile(warp) + (lane & 15)); }
-  __device__ __forceinline__ void settle(uint8_t*) {}
+  __device__ __forceinline__ void settle() {}
   __device__ __forceinline__ void issue(const PagedParams& p, const Cur& c, uint8_t* stage, int lane) {
-    constexpr int kChunks = DP / 8, kAtOnce = 32 / kChunks;     // 16-byte chunks of a row, rows copied by one instruction
-    const uint32_t mine = place.at<2>(p, c.h);
-    const int chunk = lane % kChunks;
-    const uint32_t to = smem_at(stage);
-    const char* k = static_cast<const char*>(p.c.k);
-    const char* v = static_cast<const char*>(p.c.v);
-#pragma unroll
-    for (int i = 0; i < kTile / kAtOnce; ++i) {
-      const int r = i * kAtOnce + lane / kChunks;
-      const uint32_t at = __shfl_sync(0xffffffffu, mine, r);
-      const bool there = at != kNowhere && chunk * 8 < p.c.d;
-      const int64_t from = there ? (int64_t)at * 16 + chunk * 16 : 0;
-      const uint32_t dst = to + r * kRowBytes + ((chunk ^ (r & 7)) << 4);
-      copy16(dst, k + from, there);
-      copy16(dst + kSide, v + from, there);
-    }
+    copy_rows<kTile, DP / 8, kSide>(p, place.at<2>(p, c.h), p.c.d / 8, smem_at(stage), lane, [](int r, int chunk) { return r * kRowBytes + ((chunk ^ (r & 7)) << 4); });
   }
-  __device__ __forceinline__ void begin(const PagedParams& p, const Cur& c, uint8_t*, int lane) {
+  __device__ __forceinline__ void begin(const PagedParams& p, const Cur& c, int lane) {
     const int g = lane >> 2, t = lane & 3;
-    rows.start(p, c.x, g);
+    rows.start(p, c.x, lane);
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
+    for (int i = 0; i < NT; ++i) {
+      const int row = c.x.row0 + i * 8 + g;
+      const __nv_bfloat16* from = query_row(p, c.x, c.h, min(row, p.rows - 1));
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const int row = c.x.row0 + i * 16 + s * 8 + g;
-        const __nv_bfloat16* from = query_row(p, c.x, c.h, min(row, p.rows - 1));
+      for (int k = 0; k < DP / 16; ++k)
 #pragma unroll
-        for (int k = 0; k < DP / 16; ++k)
+        for (int u = 0; u < 2; ++u) {
+          const int d = k * 16 + u * 8 + 2 * t;
+          q[i][k][u] = row < p.rows && d < p.c.d ? __ldg(reinterpret_cast<const uint32_t*>(from + d)) : 0u;
+        }
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const int d = k * 16 + u * 8 + 2 * t;
-            q[i][k][u * 2 + s] = row < p.rows && d < p.c.d ? __ldg(reinterpret_cast<const uint32_t*>(from + d)) : 0u;
-          }
-      }
-#pragma unroll
-      for (int j = 0; j < DP / 8; ++j)
+      for (int j = 0; j < DP / 16; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[i][j][e] = 0.f;
     }
   }
   __device__ __forceinline__ void take(const PagedParams& p, const Cur& c, const uint8_t* stage, int k0, int lane) {
-    const int t = lane & 3;
+    const int g = lane >> 2, t = lane & 3;
     const uint32_t ks = smem_at(stage), vs = ks + kSide;
-    float s[MT][2][4];
+    float s[NT][4];
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int i = 0; i < NT; ++i)
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[i][n][e] = 0.f;
+      for (int e = 0; e < 4; ++e) s[i][e] = 0.f;
     {
-      const int r = ((lane >> 4) << 3) + (lane & 7), half = (lane >> 3) & 1;
+      const int r = lane & 15, half = lane >> 4;
 #pragma unroll
       for (int k = 0; k < DP / 16; ++k) {
-        uint32_t b[4];
-        matrices(b, ks + r * kRowBytes + (((2 * k + half) ^ (r & 7)) << 4));
+        uint32_t a[4];
+        matrices(a, ks + r * kRowBytes + (((2 * k + half) ^ (r & 7)) << 4));
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          mma_bf16(s[i][0], q[i][k], b[0], b[1]);
-          mma_bf16(s[i][1], q[i][k], b[2], b[3]);
-        }
+        for (int i = 0; i < NT; ++i) mma_bf16(s[i], a, q[i][k][0], q[i][k][1]);
       }
     }
     const bool cut = is_cut<kRows>(p, c.x, k0, kTile);
-    uint32_t w[MT][4];
+    uint32_t w[NT][2];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
+    for (int i = 0; i < NT; ++i) {
       float top[2] = {rows.m[i][0], rows.m[i][1]};
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int e = 0; e < 4; ++e) {
+        float x = s[i][e] * p.scale_log2;
+        if (cut && !rows.sees(p, i, e & 1, k0 + (e >> 1) * 8 + g)) x = -INFINITY;
+        s[i][e] = x;
+        top[e & 1] = fmaxf(top[e & 1], x);
+      }
+      rows.rescale(i, top, o[i]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float x = s[i][n][e] * p.scale_log2;
-          if (cut && !rows.sees(p, i, e >> 1, k0 + n * 8 + 2 * t + (e & 1))) x = -INFINITY;
-          s[i][n][e] = x;
-          top[e >> 1] = fmaxf(top[e >> 1], x);
-        }
-      rescale<DP / 8>(i, top, o[i]);
+      for (int e = 0; e < 4; ++e) {
+        s[i][e] = exp2_approx(s[i][e] - top[e & 1]);
+        rows.l[i][e & 1] += s[i][e];
+      }
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[i][n][e] = exp2_approx(s[i][n][e] - top[e >> 1]);
-          rows.l[i][e >> 1] += s[i][n][e];
-        }
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(s[i][u >> 1][(u & 1) * 2], s[i][u >> 1][(u & 1) * 2 + 1]);
-        w[i][u] = *reinterpret_cast<const uint32_t*>(&h);
+      for (int u = 0; u < 2; ++u) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(s[i][2 * u], s[i][2 * u + 1]);
+        w[i][u] = turned(*reinterpret_cast<const uint32_t*>(&h));
       }
     }
-    const int r = (((lane >> 3) & 1) << 3) + (lane & 7), second = lane >> 4;
+    const int r = ((lane >> 4) << 3) + (lane & 7), second = (lane >> 3) & 1;
     const int t0 = c.x.row0 / p.G, t1 = (min(c.x.row0 + kRows, p.rows) - 1) / p.G;
     if (!cut || t0 == t1) {
 #pragma unroll
       for (int j = 0; j < DP / 16; ++j) {
-        uint32_t b[4];
-        matrices_turned(b, vs + r * kRowBytes + (((2 * j + second) ^ (r & 7)) << 4));
+        uint32_t a[4];
+        matrices_turned(a, vs + r * kRowBytes + (((2 * j + second) ^ (r & 7)) << 4));
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          mma_bf16(o[i][2 * j], w[i], b[0], b[1]);
-          mma_bf16(o[i][2 * j + 1], w[i], b[2], b[3]);
-        }
+        for (int i = 0; i < NT; ++i) mma_bf16(o[i][j], a, w[i][0], w[i][1]);
       }
       return;
     }
     for (int tok = t0; tok <= min(t1, c.x.count - 1); ++tok) {
       const int at = c.x.first + tok;
-      uint32_t seen[2] = {0, 0};      // of this lane's keys 2t, 2t + 1 and 2t + 8, 2t + 9
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int key = k0 + (u >> 1) * 8 + 2 * t + (u & 1);
-        if (key <= at && (p.a.window < 0 || key >= at - p.a.window)) seen[u >> 1] |= u & 1 ? 0xffff0000u : 0xffffu;
-      }
+      const uint32_t seen[2] = {seen_pair(p, at, k0 + 2 * t), seen_pair(p, at, k0 + 8 + 2 * t)};
 #pragma unroll
       for (int j = 0; j < DP / 16; ++j) {
-        uint32_t b[4];
-        matrices_turned(b, vs + r * kRowBytes + (((2 * j + second) ^ (r & 7)) << 4));
+        uint32_t a[4];
+        matrices_turned(a, vs + r * kRowBytes + (((2 * j + second) ^ (r & 7)) << 4));
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
+        for (int e = 0; e < 4; ++e) a[e] &= seen[e >> 1];
 #pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            float x[4] = {0.f, 0.f, 0.f, 0.f};
-            mma_bf16(x, w[i], b[2 * n] & seen[0], b[2 * n + 1] & seen[1]);
+        for (int i = 0; i < NT; ++i) {
+          float x[4] = {0.f, 0.f, 0.f, 0.f};
+          mma_bf16(x, a, w[i][0], w[i][1]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (rows.at[i][e >> 1] == at) o[i][2 * j + n][e] += x[e];
-          }
+          for (int e = 0; e < 4; ++e)
+            if (rows.at[i][e & 1] == at) o[i][j][e] += x[e];
+        }
       }
     }
-  }
-  // Takes the lane's maxima to those of the rows, and what has been added up to the new ones; `top` becomes what exponents are taken against.
-  template <int N>
-  __device__ __forceinline__ void rescale(int i, float (&top)[2], float (&acc)[N][4]) {
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      top[s] = fmaxf(top[s], __shfl_xor_sync(0xffffffffu, top[s], 1));
-      top[s] = fmaxf(top[s], __shfl_xor_sync(0xffffffffu, top[s], 2));
-    }
-    const bool moved = top[0] != rows.m[i][0] || top[1] != rows.m[i][1];
-    if (__any_sync(0xffffffffu, moved)) {
-      float f[2];
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        f[s] = top[s] == -INFINITY ? 1.f : exp2_approx(rows.m[i][s] - top[s]);
-        rows.l[i][s] *= f[s];
-        rows.m[i][s] = top[s];
-      }
-#pragma unroll
-      for (int j = 0; j < N; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[j][e] *= f[e >> 1];
-    }
-#pragma unroll
-    for (int s = 0; s < 2; ++s) top[s] = top[s] == -INFINITY ? 0.f : top[s];
   }
   __device__ __forceinline__ void stats(const Buffer<DP>& buffer, int warp, int lane) const { rows.stats(buffer, warp, lane); }
-  // Rows [8 pass, 8 pass + 8), times factor[row], into out[row - 8 pass][DP + 8]
-  __device__ __forceinline__ void put(int pass, float factor, float* out, int lane) {
+  // Rows [8 pass, 8 pass + 8) times factor(row) into lines
+  template <typename F>
+  __device__ __forceinline__ void put(int pass, F factor, float* out, int lane) const {
     const int g = lane >> 2, t = lane & 3;
+    const float f[2] = {factor(pass * 8 + 2 * t), factor(pass * 8 + 2 * t + 1)};
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int i = 0; i < NT; ++i)
+      if (pass == i) {
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
-        if (pass == i * 2 + s) {
+        for (int j = 0; j < DP / 16; ++j)
 #pragma unroll
-          for (int j = 0; j < DP / 8; ++j)
-            *reinterpret_cast<float2*>(out + g * (DP + 8) + j * 8 + 2 * t) = make_float2(o[i][j][2 * s] * factor, o[i][j][2 * s + 1] * factor);
-        }
+          for (int e = 0; e < 4; ++e) out[(2 * t + (e & 1)) * Buffer<DP>::kLine + j * 16 + (e >> 1) * 8 + g] = o[i][j][e] * f[e & 1];
+      }
   }
 };
 
 // ---- 4 bits: the same products in float16 -----------------------------------------------------------------------------
-// A key's or value's 32 components share a power of two; the largest of a head's, 2^E, is taken out of it, and codes times what remains, 2^(e - E) <= 1,
-// are float16.  2^E of a key multiplies its scores in float32.  2^E of a value joins the exponent of its weight: the running maximum is over score + E, so
-// that the weights that go through float16 are at most 1, and the sum of weights takes 2^-E back out.  Rows of Q are brought to at most 2 by a power of two
-// as well.  Codes are held times 2^13 and weights times 2^15, as large as float16 allows: codes are exact down to 2^-36 of the head's largest, weights
-// good to 2^-12 of themselves down to 2^-29 of the row's largest, and to 2^-40 of that below.  (E counts as at least -65.)
+// Codes become float16 as they are, and products of codes are exact; the powers of two join elsewhere.  Keys: a k-step of the instruction lies within 32
+// components, whose sum is multiplied by their power in float32.  Values: of a head's powers the largest, 2^E, is taken out and joins the exponent of the weight;
+// what remains, 2^(e - E) <= 1, multiplies the weights of each 32 components.  The running maximum is over score + E, so that the weights that go through
+// float16 are at most 1, and the sum of weights takes 2^-E back out.  Rows of Q are brought to at most 2 by a power of two.  Weights are held times
+// 2^15, as large as float16 allows: they are good to 2^-12 of themselves down to 2^-29 of the row's largest, and to 2^-40 of that below.  (E
+// counts as at least -65, so that no sum of weights overflows.)
 //
-// One lane holds keys' components in the order that the codes have in memory, and the rows of Q in the same: the sum over d may run in any order.
-// For the sums, codes of two keys are put side by side in a byte, which the conversion then takes to a pair of float16.
-template <int DP, int MT>
+// Where components lie among those of a k-step, or of a tile of the sums, is free as long as both operands agree: ldmatrix hands each lane four codes of 32 components
+// (turned: of two keys), and they are taken in the order in which they come.
+template <int DP, int NT>
 struct Core4bit {
-  static constexpr int kDP = DP, kRows = MT * 16, kTile = 32, kStages = 4, kMinCtas = 2;
+  static constexpr int kDP = DP, kRows = NT * 8, kTile = 32, kStages = 4, kMinCtas = 2;
   static constexpr int kRowBytes = DP / 2, kSide = kTile * kRowBytes, kGroups = DP / 32;
-  // after keys and values: powers of two of codes, keys' [32][4] and values' [4][32], and three floats of every key (settle)
-  static constexpr int kKeyPowers = 2 * kSide, kValuePowers = kKeyPowers + 256, kKeyTop = kValuePowers + 256, kStageBytes = kKeyTop + 384, kExtra = 0;
+  // after keys and values: powers of keys [32][4] (float32), of values [4][32] (float16), E and 2^-E of values [32][2]
+  static constexpr int kKeyPowers = 2 * kSide, kValuePowers = kKeyPowers + 512, kTops = kValuePowers + 256, kStageBytes = kTops + 256, kExtra = 0;
+  static constexpr float kWeightUp = 15.f;
   using Cur = Cursor<kRows, kTile>;
-  static constexpr int kWords = DP / 32;       // of 8 codes: a lane's of one key (a quarter of the head)
-  static constexpr int kCodeUp = 13, kWeightUp = 15;
 
-  uint32_t q[MT][DP / 16][4];
-  float o[MT][DP / 8][4];
-  float scale[MT][2];
-  Rows<MT> rows;
+  uint32_t q[NT][DP / 16][2];
+  float o[NT][DP / 16][4];
+  float scale[NT][2];
+  Rows<NT> rows;
   Place place;
   uint32_t k_bytes, v_bytes;    // the powers of two of this lane's key of the last tile issued
   uint8_t* pending;             // and its stage
 
-  // Places of keys in the matrix tiles: column n of 8 is key (n >> 1 & 1) | (n & 1) << 1 | (n >> 2) << 2 of 8.  (The lanes of a quarter warp then
-  // read values from different banks.)
-  static __device__ __forceinline__ int key_of(int n) { return (n >> 1 & 1) | (n & 1) << 1 | (n & 4); }
-
   __device__ __forceinline__ void prepare(uint8_t*) { pending = nullptr; }
   __device__ __forceinline__ void look_up(const PagedParams& p, const Cur& c, int warp, int lane) { place.look_up(p, c.x, c.tile(warp) + lane); }
-  // 16-byte chunks of a row are permuted so that neither keys nor values meet in banks
-  static __device__ __forceinline__ int chunk_at(int r, int chunk) { return DP == 128 ? chunk ^ (r >> 1 & 3) : chunk ^ (r >> 2 & 1); }
+  // 16-byte chunks of a row are permuted so that 8 rows of a chunk lie in different banks
+  static __device__ __forceinline__ int chunk_at(int r, int chunk) { return r * kRowBytes + ((DP == 128 ? chunk ^ (r >> 1 & 3) : chunk ^ (r >> 2 & 1)) << 4); }
 
   __device__ __forceinline__ void issue(const PagedParams& p, const Cur& c, uint8_t* stage, int lane) {
-    constexpr int kChunks = DP / 32, kAtOnce = 32 / kChunks;
+    settle();
     const uint32_t mine = place.at<1>(p, c.h);
-    const int chunk = lane % kChunks;
-    const uint32_t to = smem_at(stage);
-    const char* k = static_cast<const char*>(p.c.k);
-    const char* v = static_cast<const char*>(p.c.v);
-#pragma unroll
-    for (int i = 0; i < kTile / kAtOnce; ++i) {
-      const int r = i * kAtOnce + lane / kChunks;
-      const uint32_t at = __shfl_sync(0xffffffffu, mine, r);
-      const bool there = at != kNowhere && chunk * 32 < p.c.d;
-      const int64_t from = there ? (int64_t)at * 16 + chunk * 16 : 0;
-      const uint32_t dst = to + r * kRowBytes + (chunk_at(r, chunk) << 4);
-      copy16(dst, k + from, there);
-      copy16(dst + kSide, v + from, there);
-    }
-    settle(nullptr, lane);
     k_bytes = v_bytes = 0;
     if (mine != kNowhere) {
       const int64_t at = (int64_t)place.page * p.c.scale_stride_page + (int64_t)place.slot * p.c.scale_stride_slot + (int64_t)c.h * p.c.scale_stride_head;
-      const int n = p.c.d / 32;
+      if (p.scale_words) {
+        k_bytes = __ldg(reinterpret_cast<const uint32_t*>(p.c.k_scale + at));
+        v_bytes = __ldg(reinterpret_cast<const uint32_t*>(p.c.v_scale + at));
+      } else {
+        const int n = p.c.d / 32;
 #pragma unroll
-      for (int i = 0; i < kGroups; ++i)
-        if (i < n) {
-          k_bytes |= (uint32_t)__ldg(p.c.k_scale + at + i) << (8 * i);
-          v_bytes |= (uint32_t)__ldg(p.c.v_scale + at + i) << (8 * i);
-        }
-    }
-    pending = stage;
-  }
-  __device__ __forceinline__ void settle(uint8_t*) { settle(nullptr, threadIdx.x & 31); }
-  static __device__ __forceinline__ int largest(uint32_t bytes) {     // E + 127 of a head
-    int top = 127 - 65;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int b = bytes >> (8 * i) & 255;
-      if (b != 255) top = max(top, b);
-    }
-    return top;
-  }
-  static __device__ __forceinline__ uint16_t power(uint32_t bytes, int i, int top) {   // 2^(e - E + kCodeUp) as float16, 2^-24 being its smallest
-    const int b = bytes >> (8 * i) & 255, x = b - top + kCodeUp;
-    if (b == 255) return 0x7fff;
-    return x >= -14 ? (uint16_t)((x + 15) << 10) : x >= -24 ? (uint16_t)(1 << (x + 24)) : (uint16_t)0;
-  }
-  // The powers of two that were asked for with the last tile, into its stage.
-  __device__ __forceinline__ void settle(uint8_t*, int lane) {
-    if (!pending) return;
-    const int kt = largest(k_bytes), vt = largest(v_bytes);
-    uint16_t* kp = reinterpret_cast<uint16_t*>(pending + kKeyPowers);
-    uint16_t* vp = reinterpret_cast<uint16_t*>(pending + kValuePowers);
-    float* top = reinterpret_cast<float*>(pending + kKeyTop);
-    const int r = lane & 7, n = (r & 1) << 1 | (r >> 1 & 1) | (r & 4), place_of = (lane & 24) + n;       // (key_of is its own inverse)
-    *reinterpret_cast<uint2*>(kp + lane * 4) = make_uint2(power(k_bytes, 0, kt) | (uint32_t)power(k_bytes, 1, kt) << 16, power(k_bytes, 2, kt) | (uint32_t)power(k_bytes, 3, kt) << 16);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) vp[i * 32 + place_of] = power(v_bytes, i, vt);
-    top[place_of] = __uint_as_float((uint32_t)(kt - kCodeUp) << 23);               // what a score is to be multiplied by,
-    top[32 + place_of] = (float)(vt - 127);                                          // what its exponent gets,
-    top[64 + place_of] = __uint_as_float((uint32_t)(254 + kCodeUp - vt) << 23);      // and a weight's part of their sum
-    pending = nullptr;
-  }
-  __device__ __forceinline__ void begin(const PagedParams& p, const Cur& c, uint8_t*, int lane) {
-    const int g = lane >> 2, t = lane & 3;
-    rows.start(p, c.x, g);
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const int row = c.x.row0 + i * 16 + s * 8 + g;
-        const __nv_bfloat16* from = query_row(p, c.x, c.h, min(row, p.rows - 1));
-        // components (DP / 4) t and up
-        float x[DP / 4];
-        float top = 0.f;
-#pragma unroll
-        for (int k = 0; k < DP / 4; k += 8) {
-          const int d = DP / 4 * t + k;
-          const uint4 v = row < p.rows && d < p.c.d ? __ldg(reinterpret_cast<const uint4*>(from + d)) : make_uint4(0, 0, 0, 0);
-          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-          for (int z = 0; z < 8; ++z) {
-            x[k + z] = __uint_as_float(z & 1 ? w[z / 2] & 0xffff0000u : w[z / 2] << 16);
-            top = fmaxf(top, fabsf(x[k + z]));
-          }
-        }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const int e = min(max((int)(__float_as_uint(top) >> 23), 1), 253);      // top < 2^(e - 126)
-        const float down = __uint_as_float((uint32_t)(254 - e) << 23);
-        scale[i][s] = p.scale_log2 * __uint_as_float((uint32_t)e << 23);
-#pragma unroll
-        for (int k = 0; k < DP / 16; ++k)
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const __half2 h = __floats2half2_rn(x[4 * k + 2 * u] * down, x[4 * k + 2 * u + 1] * down);
-            q[i][k][u * 2 + s] = *reinterpret_cast<const uint32_t*>(&h);
+        for (int i = 0; i < kGroups; ++i)
+          if (i < n) {
+            k_bytes |= (uint32_t)__ldg(p.c.k_scale + at + i) << (8 * i);
+            v_bytes |= (uint32_t)__ldg(p.c.v_scale + at + i) << (8 * i);
           }
       }
+    }
+    pending = stage;
+    copy_rows<kTile, DP / 32, kSide>(p, mine, p.c.d / 32, smem_at(stage), lane, [](int r, int chunk) { return chunk_at(r, chunk); });
+  }
+  // The powers of two that were asked for with the last tile, into its stage.
+  __device__ __forceinline__ void settle() {
+    if (!pending) return;
+    const int lane = threadIdx.x & 31;
+    float kp[4];
+    uint16_t* vp = reinterpret_cast<uint16_t*>(pending + kValuePowers);
+    int top = 127 - 65;
 #pragma unroll
-      for (int j = 0; j < DP / 8; ++j)
+    for (int i = 0; i < kGroups; ++i) {
+      const int b = v_bytes >> (8 * i) & 255;
+      top = b == 255 ? top : max(top, b);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      kp[i] = i < kGroups ? e8m0_value(k_bytes >> (8 * i) & 255) : 0.f;
+      if (i < kGroups) {
+        const int b = v_bytes >> (8 * i) & 255, x = b - top + 15;       // 2^(x - 15) in float16, subnormal where x is not positive
+        vp[i * 32 + lane] = b == 255 ? 0x7fff : x > 0 ? x << 10 : 0x400 >> min(1 - x, 31);
+      }
+    }
+    *reinterpret_cast<float4*>(pending + kKeyPowers + lane * 16) = make_float4(kp[0], kp[1], kp[2], kp[3]);
+    *reinterpret_cast<float2*>(pending + kTops + lane * 8) = make_float2((float)(top - 127), top == 254 ? __uint_as_float(0x00400000u) : __uint_as_float((uint32_t)(254 - top) << 23));
+    pending = nullptr;
+  }
+  __device__ __forceinline__ void begin(const PagedParams& p, const Cur& c, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+    rows.start(p, c.x, lane);
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      const int row = c.x.row0 + i * 8 + g;
+      const __nv_bfloat16* from = query_row(p, c.x, c.h, min(row, p.rows - 1));
+      float x[kGroups][8];       // components 8t and up of each 32
+      float top = 0.f;
+#pragma unroll
+      for (int k = 0; k < kGroups; ++k) {
+        const int d = k * 32 + t * 8;
+        const uint4 v = row < p.rows && d < p.c.d ? __ldg(reinterpret_cast<const uint4*>(from + d)) : make_uint4(0, 0, 0, 0);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int z = 0; z < 8; ++z) {
+          x[k][z] = __uint_as_float(z & 1 ? w[z / 2] & 0xffff0000u : w[z / 2] << 16);
+          top = fmaxf(top, fabsf(x[k][z]));
+        }
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const int e = min(max((int)(__float_as_uint(top) >> 23), 1), 253);      // top < 2^(e - 126)
+      const float down = __uint_as_float((uint32_t)(254 - e) << 23), up = p.scale_log2 * __uint_as_float((uint32_t)e << 23);
+      scale[i][0] = __shfl_sync(0xffffffffu, up, t * 8);                      // (row 2t is that of lanes 8t to 8t + 3)
+      scale[i][1] = __shfl_sync(0xffffffffu, up, t * 8 + 4);
+#pragma unroll
+      for (int k = 0; k < DP / 16; ++k)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int z = (k & 1) * 4 + u * 2;
+          const __half2 h = __floats2half2_rn(x[k / 2][z] * down, x[k / 2][z + 1] * down);
+          q[i][k][u] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+#pragma unroll
+      for (int j = 0; j < DP / 16; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[i][j][e] = 0.f;
     }
@@ -520,172 +509,148 @@ struct Core4bit {
     const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
     return *reinterpret_cast<const uint32_t*>(&r);
   }
-  __device__ __forceinline__ void take(const PagedParams& p, const Cur& c, const uint8_t* stage, int k0, int lane) {
-    const int g = lane >> 2, t = lane & 3;
-    const bool cut = is_cut<kRows>(p, c.x, k0, kTile);
-    const float* tops = reinterpret_cast<const float*>(stage + kKeyTop);
-    float s[MT][4][4];
+  // Scores of keys 16 h and up: s[i][e] for key (e >> 1) * 8 + g, row 2t + (e & 1)
+  __device__ __forceinline__ void scores(const uint8_t* stage, int h, int lane, float (&s)[NT][4]) const {
+    const int g = lane >> 2;
+    uint32_t w[2][kGroups];      // codes of keys g and g + 8
+    if constexpr (DP == 128) {
 #pragma unroll
-    for (int n = 0; n < 4; ++n) {
+      for (int u = 0; u < 2; ++u) matrices(w[u], smem_at(stage) + chunk_at(h * 16 + u * 8 + (lane & 7), lane >> 3));
+    } else {
+      uint32_t x[4];
+      matrices(x, smem_at(stage) + chunk_at(h * 16 + (lane >> 4) * 8 + (lane & 7), lane >> 3 & 1));
+      w[0][0] = x[0]; w[0][1] = x[1]; w[1][0] = x[2]; w[1][1] = x[3];
+    }
+    float f[2][4];
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
+    for (int u = 0; u < 2; ++u) {
+      const float4 x = *reinterpret_cast<const float4*>(stage + kKeyPowers + (h * 16 + u * 8 + g) * 16);
+      f[u][0] = x.x; f[u][1] = x.y; f[u][2] = x.z; f[u][3] = x.w;
+    }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[i][n][e] = 0.f;
-      const int r = n * 8 + key_of(g);
-      uint32_t codes[kWords];
-      if constexpr (DP == 128) {
-        const uint4 x = *reinterpret_cast<const uint4*>(stage + r * kRowBytes + (chunk_at(r, t) << 4));
-        codes[0] = x.x; codes[1] = x.y; codes[2] = x.z; codes[3] = x.w;
-      } else {
-        const uint2 x = *reinterpret_cast<const uint2*>(stage + r * kRowBytes + (chunk_at(r, t >> 1) << 4) + (t & 1) * 8);
-        codes[0] = x.x; codes[1] = x.y;
-      }
-      const uint32_t f = *reinterpret_cast<const uint16_t*>(stage + kKeyPowers + r * 8 + (DP == 128 ? t : t >> 1) * 2) * 0x10001u;
+    for (int k = 0; k < kGroups; ++k) {
+      uint32_t x[4], y[4];
+      from_e2m1x8(w[0][k], x);
+      from_e2m1x8(w[1][k], y);
+      const uint32_t a[2][4] = {{x[0], y[0], x[1], y[1]}, {x[2], y[2], x[3], y[3]}};
 #pragma unroll
-      for (int w = 0; w < kWords; ++w) {
-        uint32_t b[4];
-        from_e2m1x8(codes[w], b);
+      for (int i = 0; i < NT; ++i) {
+        float z[4] = {0.f, 0.f, 0.f, 0.f};
+        mma_f16(z, a[0], q[i][2 * k][0], q[i][2 * k][1]);
+        mma_f16(z, a[1], q[i][2 * k + 1][0], q[i][2 * k + 1][1]);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) b[u] = times(b[u], f);
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          mma_f16(s[i][n], q[i][2 * w], b[0], b[1]);
-          mma_f16(s[i][n], q[i][2 * w + 1], b[2], b[3]);
-        }
+        for (int e = 0; e < 4; ++e) s[i][e] = k ? fmaf(z[e], f[e >> 1][k], s[i][e]) : z[e] * f[e >> 1][k];
       }
     }
-    uint32_t w[MT][2][4];
+  }
+  __device__ __forceinline__ void take(const PagedParams& p, const Cur& c, const uint8_t* stage, int k0, int lane) {
+    const int g = lane >> 2;
+    const bool cut = is_cut<kRows>(p, c.x, k0, kTile);
+    float s[2][NT][4];
+    scores(stage, 0, lane, s[0]);
+    scores(stage, 1, lane, s[1]);
+    float2 tops[2][2];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) tops[h][u] = *reinterpret_cast<const float2*>(stage + kTops + (h * 16 + u * 8 + g) * 8);
+    uint32_t w[2][NT][2];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
       float top[2] = {rows.m[i][0], rows.m[i][1]};
-#pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        const float2 ek = *reinterpret_cast<const float2*>(tops + n * 8 + 2 * t), ev = *reinterpret_cast<const float2*>(tops + 32 + n * 8 + 2 * t);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float x = fmaf(s[i][n][e] * (e & 1 ? ek.y : ek.x), scale[i][e >> 1], e & 1 ? ev.y : ev.x);
-          if (cut && !rows.sees(p, i, e >> 1, k0 + n * 8 + key_of(2 * t + (e & 1)))) x = -INFINITY;
-          s[i][n][e] = x;
-          top[e >> 1] = fmaxf(top[e >> 1], x);
-        }
-      }
-      rescale(i, top);
-#pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        const float2 em = *reinterpret_cast<const float2*>(tops + 64 + n * 8 + 2 * t);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float x = exp2_approx(s[i][n][e] - top[e >> 1]);
-          rows.l[i][e >> 1] = fmaf(x, e & 1 ? em.y : em.x, rows.l[i][e >> 1]);
-          s[i][n][e] = x;
-        }
-      }
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const __half2 x = __floats2half2_rn(s[i][2 * h + (u >> 1)][(u & 1) * 2], s[i][2 * h + (u >> 1)][(u & 1) * 2 + 1]);
-          w[i][h][u] = *reinterpret_cast<const uint32_t*>(&x);
+        for (int e = 0; e < 4; ++e) {
+          float x = fmaf(s[h][i][e], scale[i][e & 1], tops[h][e >> 1].x);
+          if (cut && !rows.sees(p, i, e & 1, k0 + h * 16 + (e >> 1) * 8 + g)) x = -INFINITY;
+          s[h][i][e] = x;
+          top[e & 1] = fmaxf(top[e & 1], x);
         }
+      rows.rescale(i, top, o[i], kWeightUp);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[h][i][e] = exp2_approx(s[h][i][e] - top[e & 1]);
+          rows.l[i][e & 1] = fmaf(s[h][i][e], tops[h][e >> 1].y, rows.l[i][e & 1]);
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const __half2 x = __floats2half2_rn(s[h][i][2 * u], s[h][i][2 * u + 1]);
+          w[h][i][u] = turned(*reinterpret_cast<const uint32_t*>(&x));
+        }
+      }
     }
     const int t0 = c.x.row0 / p.G, t1 = (min(c.x.row0 + kRows, p.rows) - 1) / p.G;
-    if (!cut || t0 == t1) values<false>(p, stage, k0, lane, w, 0);
-    else
-      for (int tok = t0; tok <= min(t1, c.x.count - 1); ++tok) values<true>(p, stage, k0, lane, w, c.x.first + tok);
-  }
-  // o += w V.  ONE: only the rows of the token at `at`, of the keys that it sees.
-  template <bool ONE>
-  __device__ __forceinline__ void values(const PagedParams& p, const uint8_t* stage, int k0, int lane, const uint32_t (&w)[MT][2][4], int at) {
-    const int g = lane >> 2, t = lane & 3;
-    constexpr int kN = DP / 8 / 8;      // words of 8 codes that a lane holds of a key: the head's DP / 8 columns of g
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      uint32_t b[2][DP / 8];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int n = 2 * h + u, ra = n * 8 + key_of(2 * t), rb = n * 8 + key_of(2 * t + 1);
-        uint32_t f = *reinterpret_cast<const uint32_t*>(stage + kValuePowers + ((DP == 128 ? g >> 1 : g >> 2) * 32 + n * 8 + 2 * t) * 2);
-        uint32_t seen = 0xffffffffu;
-        if (ONE) {
-          seen = 0;
-          if (k0 + ra <= at && (p.a.window < 0 || k0 + ra >= at - p.a.window)) seen |= 0xffffu;
-          if (k0 + rb <= at && (p.a.window < 0 || k0 + rb >= at - p.a.window)) seen |= 0xffff0000u;
-        }
-        uint32_t ca[kN], cb[kN];
-        const uint8_t* v = stage + kSide;
-        if constexpr (DP == 128) {
-          const uint2 xa = *reinterpret_cast<const uint2*>(v + ra * kRowBytes + (chunk_at(ra, g >> 1) << 4) + (g & 1) * 8);
-          const uint2 xb = *reinterpret_cast<const uint2*>(v + rb * kRowBytes + (chunk_at(rb, g >> 1) << 4) + (g & 1) * 8);
-          ca[0] = xa.x; ca[1] = xa.y; cb[0] = xb.x; cb[1] = xb.y;
-        } else {
-          ca[0] = *reinterpret_cast<const uint32_t*>(v + ra * kRowBytes + (chunk_at(ra, g >> 2) << 4) + (g & 3) * 4);
-          cb[0] = *reinterpret_cast<const uint32_t*>(v + rb * kRowBytes + (chunk_at(rb, g >> 2) << 4) + (g & 3) * 4);
-        }
-#pragma unroll
-        for (int i = 0; i < kN; ++i) {
-          const uint32_t even = (ca[i] & 0x0f0f0f0fu) | (cb[i] & 0x0f0f0f0fu) << 4, odd = (ca[i] >> 4 & 0x0f0f0f0fu) | (cb[i] & 0xf0f0f0f0u);
-          uint32_t x[4], y[4];
-          from_e2m1x8(even, x);
-          from_e2m1x8(odd, y);
-#pragma unroll
-          for (int z = 0; z < 4; ++z) {
-            b[u][i * 8 + 2 * z] = times(x[z], f) & seen;
-            b[u][i * 8 + 2 * z + 1] = times(y[z], f) & seen;
-          }
-        }
+    if (!cut || t0 == t1) {
+      values<false>(p, stage, k0, 0, lane, w[0], 0);
+      values<false>(p, stage, k0, 1, lane, w[1], 0);
+    } else
+      for (int tok = t0; tok <= min(t1, c.x.count - 1); ++tok) {
+        values<true>(p, stage, k0, 0, lane, w[0], c.x.first + tok);
+        values<true>(p, stage, k0, 1, lane, w[1], c.x.first + tok);
       }
+  }
+  // o += V^T w over keys 16 h and up.  ONE: only the rows of the token at `at`, of the keys that it sees.
+  template <bool ONE>
+  __device__ __forceinline__ void values(const PagedParams& p, const uint8_t* stage, int k0, int h, int lane, const uint32_t (&w)[NT][2], int at) {
+    const int t = lane & 3;
+    uint32_t x[kGroups][2];      // four codes of keys 2t (lower half) and 2t + 1, and of keys 8 further on
 #pragma unroll
-      for (int j = 0; j < DP / 8; ++j)
+    for (int k = 0; k < kGroups; k += 2) {
+      uint32_t y[4];
+      matrices_turned(y, smem_at(stage) + kSide + chunk_at(h * 16 + (lane >> 3 & 1) * 8 + (lane & 7), k + (lane >> 4)));
+      x[k][0] = y[0]; x[k][1] = y[1]; x[k + 1][0] = y[2]; x[k + 1][1] = y[3];
+    }
+    uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
+    if (ONE) {
+      seen[0] = seen_pair(p, at, k0 + h * 16 + 2 * t);
+      seen[1] = seen_pair(p, at, k0 + h * 16 + 8 + 2 * t);
+    }
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          if (!ONE) mma_f16(o[i][j], w[i][h], b[0][j], b[1][j]);
+    for (int k = 0; k < kGroups; ++k) {
+      const uint32_t f0 = *reinterpret_cast<const uint32_t*>(stage + kValuePowers + (k * 32 + h * 16 + 2 * t) * 2);
+      const uint32_t f1 = *reinterpret_cast<const uint32_t*>(stage + kValuePowers + (k * 32 + h * 16 + 8 + 2 * t) * 2);
+      // a byte for each pair of keys and component
+      const uint32_t one = __byte_perm(x[k][0], x[k][1], 0x5410), two = __byte_perm(x[k][0], x[k][1], 0x7632);
+      uint32_t even[4], odd[4];
+      from_e2m1x8((one & 0x0f0f0f0fu) | ((two << 4) & 0xf0f0f0f0u), even);      // components 0 and 2 of four, of keys 2t; of keys 8 + 2t
+      from_e2m1x8(((one >> 4) & 0x0f0f0f0fu) | (two & 0xf0f0f0f0u), odd);
+      const uint32_t a[2][4] = {{even[0], odd[0], even[2], odd[2]}, {even[1], odd[1], even[3], odd[3]}};
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        uint32_t b0 = times(w[i][0], f0), b1 = times(w[i][1], f1);
+        if (ONE) { b0 &= seen[0]; b1 &= seen[1]; }          // (weight and power: a value that is not seen may be NaN by its power alone)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          if (!ONE) mma_f16(o[i][2 * k + j], a[j], b0, b1);
           else {
-            float x[4] = {0.f, 0.f, 0.f, 0.f};
-            mma_f16(x, w[i][h], b[0][j], b[1][j]);
+            float z[4] = {0.f, 0.f, 0.f, 0.f};
+            mma_f16(z, a[j], b0, b1);
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              if (rows.at[i][e >> 1] == at) o[i][j][e] += x[e];
+              if (rows.at[i][e & 1] == at) o[i][2 * k + j][e] += z[e];
           }
         }
-    }
-  }
-  __device__ __forceinline__ void rescale(int i, float (&top)[2]) {
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      top[s] = fmaxf(top[s], __shfl_xor_sync(0xffffffffu, top[s], 1));
-      top[s] = fmaxf(top[s], __shfl_xor_sync(0xffffffffu, top[s], 2));
-    }
-    const bool moved = top[0] != rows.m[i][0] || top[1] != rows.m[i][1];
-    if (__any_sync(0xffffffffu, moved)) {
-      float f[2];
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        f[s] = top[s] == -INFINITY ? 1.f : exp2_approx(rows.m[i][s] - top[s]);
-        rows.l[i][s] *= f[s];
-        rows.m[i][s] = top[s];
       }
-#pragma unroll
-      for (int j = 0; j < DP / 8; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[i][j][e] *= f[e >> 1];
     }
-#pragma unroll
-    for (int s = 0; s < 2; ++s) top[s] = top[s] == -INFINITY ? 0.f : top[s] - kWeightUp;
   }
-  // (sums of weights are too large by 2^(kWeightUp + kCodeUp), those of values as well)
-  __device__ __forceinline__ void stats(const Buffer<DP>& buffer, int warp, int lane) const { rows.stats(buffer, warp, lane, kWeightUp + kCodeUp); }
-  __device__ __forceinline__ void put(int pass, float factor, float* out, int lane) {
+  __device__ __forceinline__ void stats(const Buffer<DP>& buffer, int warp, int lane) const { rows.stats(buffer, warp, lane, kWeightUp); }
+  template <typename F>
+  __device__ __forceinline__ void put(int pass, F factor, float* out, int lane) const {
     const int g = lane >> 2, t = lane & 3;
+    const float f[2] = {factor(pass * 8 + 2 * t), factor(pass * 8 + 2 * t + 1)};
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int i = 0; i < NT; ++i)
+      if (pass == i) {
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
-        if (pass == i * 2 + s) {
+        for (int k = 0; k < kGroups; ++k)
 #pragma unroll
-          for (int j = 0; j < DP / 8; ++j)
-#pragma unroll
-            for (int u = 0; u < 2; ++u) out[g * (DP + 8) + (2 * t + u) * (DP / 8) + j] = o[i][j][2 * s + u] * factor;
-        }
+          for (int s = 0; s < 2; ++s)
+            *reinterpret_cast<float4*>(out + (2 * t + s) * Buffer<DP>::kLine + k * 32 + g * 4) =
+                make_float4(o[i][2 * k][s] * f[s], o[i][2 * k][2 + s] * f[s], o[i][2 * k + 1][s] * f[s], o[i][2 * k + 1][2 + s] * f[s]);
+      }
   }
 };
 
@@ -710,26 +675,11 @@ struct CoreF32 {
     ps = qs + ROWS * kQRow + (threadIdx.x >> 5) * kTile * ROWS;
   }
   __device__ __forceinline__ void look_up(const PagedParams& p, const Cur& c, int warp, int lane) { place.look_up(p, c.x, c.tile(warp) + (lane & 15)); }
-  __device__ __forceinline__ void settle(uint8_t*) {}
+  __device__ __forceinline__ void settle() {}
   __device__ __forceinline__ void issue(const PagedParams& p, const Cur& c, uint8_t* stage, int lane) {
-    constexpr int kChunks = DP / 4, kAtOnce = 32 / kChunks;
-    const uint32_t mine = place.at<4>(p, c.h);
-    const int chunk = lane % kChunks;
-    const uint32_t to = smem_at(stage);
-    const char* k = static_cast<const char*>(p.c.k);
-    const char* v = static_cast<const char*>(p.c.v);
-#pragma unroll
-    for (int i = 0; i < kTile / kAtOnce; ++i) {
-      const int r = i * kAtOnce + lane / kChunks;
-      const uint32_t at = __shfl_sync(0xffffffffu, mine, r);
-      const bool there = at != kNowhere && chunk * 4 < p.c.d;
-      const int64_t from = there ? (int64_t)at * 16 + chunk * 16 : 0;
-      const uint32_t dst = to + r * kRowBytes + ((chunk ^ (r & 7)) << 4);
-      copy16(dst, k + from, there);
-      copy16(dst + kSide, v + from, there);
-    }
+    copy_rows<kTile, DP / 4, kSide>(p, place.at<4>(p, c.h), p.c.d / 4, smem_at(stage), lane, [](int r, int chunk) { return r * kRowBytes + ((chunk ^ (r & 7)) << 4); });
   }
-  __device__ __forceinline__ void begin(const PagedParams& p, const Cur& c, uint8_t*, int lane) {
+  __device__ __forceinline__ void begin(const PagedParams& p, const Cur& c, int lane) {
     const int n = min(ROWS, p.rows - c.x.row0);
     __syncthreads();             // (the last item's rows have been read)
     for (int i = threadIdx.x; i < ROWS * DP; i += kThreads) {
@@ -828,12 +778,15 @@ struct CoreF32 {
       if (lane == 0) buffer.stat(warp, r) = make_float2(m[r], x);
     }
   }
-  __device__ __forceinline__ void put_rows(int pass, const float* factors, float* out, int lane) {
+  template <typename F>
+  __device__ __forceinline__ void put(int pass, F factor, float* out, int lane) const {
 #pragma unroll
     for (int r = 0; r < ROWS; ++r)
-      if (r >> 3 == pass)
+      if (r >> 3 == pass) {
+        const float f = factor(r);
 #pragma unroll
-        for (int j = 0; j < kCols; ++j) out[(r & 7) * (DP + 8) + lane * kCols + j] = o[r][j] * factors[r & 7];
+        for (int j = 0; j < kCols; ++j) out[(r & 7) * Buffer<DP>::kLine + lane * kCols + j] = o[r][j] * f;
+      }
   }
 };
 
@@ -842,8 +795,6 @@ template <class Core>
 constexpr int paged_smem() {
   return kWarps * Core::kStages * Core::kStageBytes + Buffer<Core::kDP>::kFloats * 4 + Core::kExtra;
 }
-template <class Core> struct IsSimt { static constexpr bool value = false; };
-template <int DP, int ROWS> struct IsSimt<CoreF32<DP, ROWS>> { static constexpr bool value = true; };
 
 // A finished row's value: four components and (at the first) the log-sum-exp; zeros for a token that is not real.
 __device__ __forceinline__ void write_result(const PagedParams& p, int b, int h, int row, bool real, int col, float4 x, float top, float sum) {
@@ -883,22 +834,11 @@ __device__ __forceinline__ void finish(const PagedParams& p, Core& core, const t
     return base;
   };
   for (int pass = 0; pass * 8 < n; ++pass) {
-    if constexpr (IsSimt<Core>::value) {
-      float f[8];
-#pragma unroll
-      for (int r = 0; r < 8; ++r) {
-        float top, sum;
-        const int row = min(pass * 8 + r, Core::kRows - 1);
-        const float base = joined(row, top, sum);
-        f[r] = exp2_approx(buffer.stat(warp, row).x - base);
-      }
-      core.put_rows(pass, f, buffer.line(warp, 0), lane);
-    } else {
+    core.put(pass, [&](int row) {
       float top, sum;
-      const int row = pass * 8 + (lane >> 2);
       const float base = joined(row, top, sum);
-      core.put(pass, exp2_approx(buffer.stat(warp, row).x - base), buffer.line(warp, 0), lane);
-    }
+      return exp2_approx(buffer.stat(warp, row).x - base);
+    }, buffer.line(warp, 0), lane);
     __syncthreads();
     for (int i = threadIdx.x; i < 8 * (DP / 4); i += kThreads) {
       const int r = i / (DP / 4), col = i % (DP / 4) * 4, row = pass * 8 + r;
@@ -1005,12 +945,12 @@ __global__ void __launch_bounds__(kThreads, Core::kMinCtas) paged_kernel(const _
   int first_unit = here.unit;
   bool first_item = true;
   for (int i = 0; i < n; ++i) {
-    core.settle(nullptr);
+    core.settle();
     issue(i + NS - 1);
     copies_awaited<NS - 1>();
     __syncwarp();
     if (fresh) {
-      core.begin(p, here, nullptr, lane);
+      core.begin(p, here, lane);
       first_unit = here.unit;
       fresh = false;
     }
@@ -1095,7 +1035,7 @@ bool plan_paged(const bma_paged_cache& c, const bma_paged_attn_args& a, PagedLau
   const int rows = a.T * (a.Hq / c.Hkv);
   l.dp = c.d <= 64 ? 64 : 128;
   l.tile = c.dtype == BMA_DTYPE_MXFP4 ? 32 : 16;
-  l.rows_of_tile = c.dtype == BMA_DTYPE_F32 ? (rows <= 4 ? 4 : rows <= 8 ? 8 : 16) : rows <= 16 ? 16 : 32;
+  l.rows_of_tile = c.dtype == BMA_DTYPE_F32 && rows <= 4 ? 4 : rows <= 8 ? 8 : c.dtype == BMA_DTYPE_F32 || rows <= 16 ? 16 : 32;
   l.ctas_per_sm = c.dtype == BMA_DTYPE_F32 && l.dp == 128 ? 1 : 2;
   l.row_tiles = ceil_div(rows, l.rows_of_tile);
   const int64_t entries = (int64_t)c.B * l.row_tiles;
@@ -1136,9 +1076,11 @@ int dispatch_paged(const PagedParams& p, const PagedLaunch& l, cudaStream_t st) 
       if (l.rows_of_tile == 8) return launch_paged<CoreF32<DP, 8>>(p, l, st);
       return launch_paged<CoreF32<DP, 16>>(p, l, st);
     case BMA_DTYPE_BF16:
-      return l.rows_of_tile == 16 ? launch_paged<CoreBf16<DP, 1>>(p, l, st) : launch_paged<CoreBf16<DP, 2>>(p, l, st);
+      if (l.rows_of_tile == 8) return launch_paged<CoreBf16<DP, 1>>(p, l, st);
+      return l.rows_of_tile == 16 ? launch_paged<CoreBf16<DP, 2>>(p, l, st) : launch_paged<CoreBf16<DP, 4>>(p, l, st);
     default:
-      return l.rows_of_tile == 16 ? launch_paged<Core4bit<DP, 1>>(p, l, st) : launch_paged<Core4bit<DP, 2>>(p, l, st);
+      if (l.rows_of_tile == 8) return launch_paged<Core4bit<DP, 1>>(p, l, st);
+      return l.rows_of_tile == 16 ? launch_paged<Core4bit<DP, 2>>(p, l, st) : launch_paged<Core4bit<DP, 4>>(p, l, st);
   }
 }
 
@@ -1173,6 +1115,12 @@ int bma_paged_attn(const bma_paged_cache* cache, const bma_paged_attn_args* args
   p.row_tiles = l.row_tiles;
   p.entries = l.entries;
   p.positions = cache->width * cache->page_size;
+  p.page_shift = -1;
+  for (int i = 0; i < 31; ++i)
+    if (cache->page_size == 1 << i) p.page_shift = i;
+  p.scale_words = cache->dtype == BMA_DTYPE_MXFP4 && cache->d == 128 &&
+                  ((reinterpret_cast<uintptr_t>(cache->k_scale) | reinterpret_cast<uintptr_t>(cache->v_scale) | (uintptr_t)cache->scale_stride_page |
+                    (uintptr_t)cache->scale_stride_slot | (uintptr_t)cache->scale_stride_head) & 3) == 0;
   p.scale_log2 = args->scale * kLog2e;
   BMA_REQUIRE((p.status = device_status_ptr()) != nullptr, BMA_ERR_CUDA);
   p.part_o = static_cast<float*>(workspace);
