@@ -30,6 +30,7 @@ struct PagedParams {
   int G, rows, row_tiles, entries;     // query heads to a kv head, rows to a kv head, tiles of them, (sequence, tile) pairs
   int positions;                       // what the page table covers
   int page_shift;                      // log2 of the page size, -1 where that is no power of two
+  uint32_t page_units, slot_units, head_units;      // strides of the cache, in 16 bytes
   int scale_words;                     // 4 bits: a head's four powers of two can be read at once
   float scale_log2;
   int* status;
@@ -59,17 +60,22 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], 
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_f16_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {      // nothing to add to
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+               : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// Where a CTA puts the parts of its warps together: eight rows of a warp at a time, lines of DP + 8 floats (the rows of a quarter warp in different banks); the last
+// Where a CTA puts the parts of its warps together, in the stages that they have just read: eight rows of a warp at a time, lines of DP + 8 floats; the last
 // 8 floats of a line hold maximum and sum of four rows, r, r + 8, r + 16 and r + 24.
 template <int DP>
 struct Buffer {
-  static constexpr int kLine = DP + 8, kFloats = kWarps * 8 * kLine;
-  float* at;
-  __device__ __forceinline__ float* line(int warp, int r) const { return at + (warp * 8 + r) * kLine; }
+  static constexpr int kLine = DP + 8, kBytes = 8 * kLine * 4;
+  uint8_t* at;          // of warp 0
+  int stride;           // bytes to the next warp's
+  __device__ __forceinline__ float* line(int warp, int r) const { return reinterpret_cast<float*>(at + warp * stride) + r * kLine; }
   __device__ __forceinline__ float2& stat(int warp, int row) const { return *reinterpret_cast<float2*>(line(warp, row & 7) + DP + (row >> 3) * 2); }
 };
 __device__ __forceinline__ uint32_t smem_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -80,6 +86,10 @@ struct Entry {
   int first, count;        // position of the first new token, number of real ones
   int lo, hi, base;        // keys [lo, hi); the walk starts at `base`
   int units;               // at least 1: an item without keys is written, too
+  int t0, t1;              // tokens of the rows, real ones
+  int all_from, all_to;    // every row sees keys [all_from, all_to]
+  bool one;                // the rows are of one token
+  __device__ __forceinline__ bool cut(int k0, int n) const { return k0 < all_from || k0 + n - 1 > all_to; }
 };
 template <int ROWS, int TILE>
 __device__ __forceinline__ Entry entry_of(const PagedParams& p, int e) {
@@ -89,14 +99,19 @@ __device__ __forceinline__ Entry entry_of(const PagedParams& p, int e) {
   const NewTokens n = new_tokens(p.a.lengths, p.a.new_lengths, x.b, p.a.T);
   x.count = n.count;
   x.first = (int)max(n.first, (int64_t)-(1 << 30));
-  const int t0 = x.row0 / p.G, t1 = min((min(x.row0 + ROWS, p.rows) - 1) / p.G, x.count - 1);
+  x.t0 = x.row0 / p.G;
+  const int last = (min(x.row0 + ROWS, p.rows) - 1) / p.G;
+  x.one = x.t0 == last;
+  x.t1 = min(last, x.count - 1);
   x.lo = x.hi = 0;
-  if (t0 <= t1) {
-    const int64_t end = n.first + t1 + 1;
+  if (x.t0 <= x.t1) {
+    const int64_t end = n.first + x.t1 + 1;
     x.hi = (int)min(max(end, (int64_t)0), (int64_t)p.positions);
     if (end > p.positions) report_device_error(p.status, kStatusPaged);
-    x.lo = p.a.window < 0 ? 0 : (int)min(max(n.first + t0 - p.a.window, (int64_t)0), (int64_t)x.hi);
+    x.lo = p.a.window < 0 ? 0 : (int)min(max(n.first + x.t0 - p.a.window, (int64_t)0), (int64_t)x.hi);
   }
+  x.all_to = x.first + x.t0;
+  x.all_from = p.a.window < 0 ? x.lo : max(x.lo, (int)max((int64_t)x.first + x.t1 - p.a.window, (int64_t)0));
   x.base = x.lo & ~(TILE - 1);
   x.units = max(1, (x.hi - x.base + kWarps * TILE - 1) / (kWarps * TILE));
   return x;
@@ -139,9 +154,8 @@ struct Place {
     if (page != -1) report_device_error(p.status, kStatusPaged);
     return false;
   }
-  template <int BYTES>      // of a unit of the strides
   __device__ __forceinline__ uint32_t at(const PagedParams& p, int h) const {
-    return there(p) ? (uint32_t)(((int64_t)page * p.c.stride_page + (int64_t)slot * p.c.stride_slot + (int64_t)h * p.c.stride_head) * BYTES / 16) : kNowhere;
+    return there(p) ? page * p.page_units + slot * p.slot_units + h * p.head_units : kNowhere;
   }
 };
 
@@ -205,12 +219,6 @@ struct Rows {
       }
   }
 };
-// Whether rows of the tile of rows see different parts of the keys [k0, k0 + n), or no row sees some of them.
-template <int ROWS>
-__device__ __forceinline__ bool is_cut(const PagedParams& p, const Entry& x, int k0, int n) {
-  const int t0 = x.row0 / p.G, t1 = min((min(x.row0 + ROWS, p.rows) - 1) / p.G, x.count - 1);
-  return k0 < x.lo || k0 + n - 1 > x.first + t0 || (p.a.window >= 0 && k0 < x.first + t1 - p.a.window);
-}
 // Halves of a pair of keys that the token at `at` sees, as a mask of 16-bit values
 __device__ __forceinline__ uint32_t seen_pair(const PagedParams& p, int at, int key) {
   uint32_t m = 0;
@@ -261,7 +269,7 @@ __device__ __forceinline__ void copy_rows(const PagedParams& p, uint32_t mine, i
 // tile, where rows as M would make 16 of one.  The weights go from the accumulators of the one to the operand of the other by movmatrix.
 template <int DP, int NT>
 struct CoreBf16 {
-  static constexpr int kDP = DP, kRows = NT * 8, kTile = 16, kStages = DP == 128 ? 3 : 4, kMinCtas = 2;
+  static constexpr int kDP = DP, kRows = NT * 8, kTile = 16, kStages = DP == 128 ? (NT == 1 ? 2 : 3) : 4, kMinCtas = NT == 1 ? 3 : 2;
   static constexpr int kRowBytes = DP * 2, kSide = kTile * kRowBytes, kStageBytes = 2 * kSide, kExtra = 0;
   using Cur = Cursor<kRows, kTile>;
 
@@ -274,7 +282,7 @@ struct CoreBf16 {
   __device__ __forceinline__ void look_up(const PagedParams& p, const Cur& c, int warp, int lane) { place.look_up(p, c.x, c.tile(warp) + (lane & 15)); }
   __device__ __forceinline__ void settle() {}
   __device__ __forceinline__ void issue(const PagedParams& p, const Cur& c, uint8_t* stage, int lane) {
-    copy_rows<kTile, DP / 8, kSide>(p, place.at<2>(p, c.h), p.c.d / 8, smem_at(stage), lane, [](int r, int chunk) { return r * kRowBytes + ((chunk ^ (r & 7)) << 4); });
+    copy_rows<kTile, DP / 8, kSide>(p, place.at(p, c.h), p.c.d / 8, smem_at(stage), lane, [](int r, int chunk) { return r * kRowBytes + ((chunk ^ (r & 7)) << 4); });
   }
   __device__ __forceinline__ void begin(const PagedParams& p, const Cur& c, int lane) {
     const int g = lane >> 2, t = lane & 3;
@@ -314,7 +322,7 @@ struct CoreBf16 {
         for (int i = 0; i < NT; ++i) mma_bf16(s[i], a, q[i][k][0], q[i][k][1]);
       }
     }
-    const bool cut = is_cut<kRows>(p, c.x, k0, kTile);
+    const bool cut = c.x.cut(k0, kTile);
     uint32_t w[NT][2];
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
@@ -339,8 +347,7 @@ struct CoreBf16 {
       }
     }
     const int r = ((lane >> 4) << 3) + (lane & 7), second = (lane >> 3) & 1;
-    const int t0 = c.x.row0 / p.G, t1 = (min(c.x.row0 + kRows, p.rows) - 1) / p.G;
-    if (!cut || t0 == t1) {
+    if (!cut || c.x.one) {
 #pragma unroll
       for (int j = 0; j < DP / 16; ++j) {
         uint32_t a[4];
@@ -350,7 +357,7 @@ struct CoreBf16 {
       }
       return;
     }
-    for (int tok = t0; tok <= min(t1, c.x.count - 1); ++tok) {
+    for (int tok = c.x.t0; tok <= c.x.t1; ++tok) {
       const int at = c.x.first + tok;
       const uint32_t seen[2] = {seen_pair(p, at, k0 + 2 * t), seen_pair(p, at, k0 + 8 + 2 * t)};
 #pragma unroll
@@ -399,9 +406,9 @@ struct CoreBf16 {
 // (turned: of two keys), and they are taken in the order in which they come.
 template <int DP, int NT>
 struct Core4bit {
-  static constexpr int kDP = DP, kRows = NT * 8, kTile = 32, kStages = 4, kMinCtas = 2;
+  static constexpr int kDP = DP, kRows = NT * 8, kTile = 32, kStages = 3, kMinCtas = NT == 1 ? 3 : 2;
   static constexpr int kRowBytes = DP / 2, kSide = kTile * kRowBytes, kGroups = DP / 32;
-  // after keys and values: powers of keys [32][4] (float32), of values [4][32] (float16), E and 2^-E of values [32][2]
+  // after keys and values: powers of keys [32][4] (float32), of values [4][32] (float16, by key_of's rows), E and 2^-E of values [32][2]
   static constexpr int kKeyPowers = 2 * kSide, kValuePowers = kKeyPowers + 512, kTops = kValuePowers + 256, kStageBytes = kTops + 256, kExtra = 0;
   static constexpr float kWeightUp = 15.f;
   using Cur = Cursor<kRows, kTile>;
@@ -421,7 +428,7 @@ struct Core4bit {
 
   __device__ __forceinline__ void issue(const PagedParams& p, const Cur& c, uint8_t* stage, int lane) {
     settle();
-    const uint32_t mine = place.at<1>(p, c.h);
+    const uint32_t mine = place.at(p, c.h);
     k_bytes = v_bytes = 0;
     if (mine != kNowhere) {
       const int64_t at = (int64_t)place.page * p.c.scale_stride_page + (int64_t)place.slot * p.c.scale_stride_slot + (int64_t)c.h * p.c.scale_stride_head;
@@ -435,7 +442,7 @@ struct Core4bit {
           if (i < n) {
             k_bytes |= (uint32_t)__ldg(p.c.k_scale + at + i) << (8 * i);
             v_bytes |= (uint32_t)__ldg(p.c.v_scale + at + i) << (8 * i);
-          }
+          } else v_bytes |= (v_bytes & 255) << (8 * i);      // (no components there)
       }
     }
     pending = stage;
@@ -445,21 +452,42 @@ struct Core4bit {
   __device__ __forceinline__ void settle() {
     if (!pending) return;
     const int lane = threadIdx.x & 31;
+    // pairs of bytes, 0 and 2, 1 and 3
+    const uint32_t v02 = v_bytes & 0x00ff00ffu, v13 = v_bytes >> 8 & 0x00ff00ffu;
+    const uint32_t tops = __vmaxu2(v02, v13);
+    int top = max(max((int)(tops & 0xffffu), (int)(tops >> 16)), 127 - 65);
+    const uint32_t down = (uint32_t)(15 - top) & 0xffffu;
+    // 2^(e - E) is float16 of exponent x = e - E + 15 where that is positive
+    uint32_t x02 = __viaddmax_s16x2_relu(v02, down | down << 16, 0u), x13 = __viaddmax_s16x2_relu(v13, down | down << 16, 0u);
+    const bool nan = (v_bytes & (v_bytes & 0x7f7f7f7fu) + 0x01010101u | k_bytes & (k_bytes & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+    const bool small = ((x02 - 0x00010001u) & ~x02 | (x13 - 0x00010001u) & ~x13) & (kGroups == 4 ? 0x80008000u : 0x8000u);
     float kp[4];
-    uint16_t* vp = reinterpret_cast<uint16_t*>(pending + kValuePowers);
-    int top = 127 - 65;
 #pragma unroll
-    for (int i = 0; i < kGroups; ++i) {
-      const int b = v_bytes >> (8 * i) & 255;
-      top = b == 255 ? top : max(top, b);
-    }
+    for (int i = 0; i < 4; ++i) kp[i] = __uint_as_float((i == 0 ? k_bytes << 23 : i == 1 ? k_bytes << 15 : i == 2 ? k_bytes << 7 : k_bytes >> 1) & 0x7f800000u);      // (2^-127 counts as 0 here)
+    x02 <<= 10;
+    x13 <<= 10;
+    if (__any_sync(0xffffffffu, nan || small)) {        // bytes of 255, powers under 2^-14 of the head's largest
+      top = 127 - 65;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      kp[i] = i < kGroups ? e8m0_value(k_bytes >> (8 * i) & 255) : 0.f;
-      if (i < kGroups) {
-        const int b = v_bytes >> (8 * i) & 255, x = b - top + 15;       // 2^(x - 15) in float16, subnormal where x is not positive
-        vp[i * 32 + lane] = b == 255 ? 0x7fff : x > 0 ? x << 10 : 0x400 >> min(1 - x, 31);
+      for (int i = 0; i < 4; ++i) {
+        const int b = v_bytes >> (8 * i) & 255;
+        top = b == 255 ? top : max(top, b);
       }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int b = v_bytes >> (8 * i) & 255, x = b - top + 15;
+        const uint32_t f = b == 255 ? 0x7fff : x > 0 ? x << 10 : 0x400 >> min(1 - x, 31);
+        uint32_t& w = i & 1 ? x13 : x02;
+        w = i & 2 ? (w & 0xffffu) | f << 16 : (w & 0xffff0000u) | f;
+        if ((k_bytes >> (8 * i) & 255) == 255) kp[i] = __uint_as_float(0x7fffffffu);
+      }
+    }
+    uint16_t* vp = reinterpret_cast<uint16_t*>(pending + kValuePowers) + (lane & 16) + (lane & 6) + (lane >> 3 & 1) + (lane & 1) * 8;      // the row m of the key
+    vp[0] = (uint16_t)x02;
+    vp[32] = (uint16_t)x13;
+    if (kGroups == 4) {
+      vp[64] = (uint16_t)(x02 >> 16);
+      vp[96] = (uint16_t)(x13 >> 16);
     }
     *reinterpret_cast<float4*>(pending + kKeyPowers + lane * 16) = make_float4(kp[0], kp[1], kp[2], kp[3]);
     *reinterpret_cast<float2*>(pending + kTops + lane * 8) = make_float2((float)(top - 127), top == 254 ? __uint_as_float(0x00400000u) : __uint_as_float((uint32_t)(254 - top) << 23));
@@ -509,22 +537,24 @@ struct Core4bit {
     const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
     return *reinterpret_cast<const uint32_t*>(&r);
   }
-  // Scores of keys 16 h and up: s[i][e] for key (e >> 1) * 8 + g, row 2t + (e & 1)
+  // The key of row m of a tile of 16: so that the values' codes of keys m = 2t and 2t + 8, which the sums want in one register, lie in neighbouring keys.
+  static __device__ __forceinline__ int key_of(int m) { return (m & 1) * 8 + (m & 6) + (m >> 3); }
+  // Scores of keys 16 h and up: s[i][e] for key key_of((e >> 1) * 8 + g), row 2t + (e & 1)
   __device__ __forceinline__ void scores(const uint8_t* stage, int h, int lane, float (&s)[NT][4]) const {
     const int g = lane >> 2;
     uint32_t w[2][kGroups];      // codes of keys g and g + 8
     if constexpr (DP == 128) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) matrices(w[u], smem_at(stage) + chunk_at(h * 16 + u * 8 + (lane & 7), lane >> 3));
+      for (int u = 0; u < 2; ++u) matrices(w[u], smem_at(stage) + chunk_at(h * 16 + key_of(u * 8 + (lane & 7)), lane >> 3));
     } else {
       uint32_t x[4];
-      matrices(x, smem_at(stage) + chunk_at(h * 16 + (lane >> 4) * 8 + (lane & 7), lane >> 3 & 1));
+      matrices(x, smem_at(stage) + chunk_at(h * 16 + key_of((lane >> 4) * 8 + (lane & 7)), lane >> 3 & 1));
       w[0][0] = x[0]; w[0][1] = x[1]; w[1][0] = x[2]; w[1][1] = x[3];
     }
     float f[2][4];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const float4 x = *reinterpret_cast<const float4*>(stage + kKeyPowers + (h * 16 + u * 8 + g) * 16);
+      const float4 x = *reinterpret_cast<const float4*>(stage + kKeyPowers + (h * 16 + key_of(u * 8 + g)) * 16);
       f[u][0] = x.x; f[u][1] = x.y; f[u][2] = x.z; f[u][3] = x.w;
     }
 #pragma unroll
@@ -535,8 +565,8 @@ struct Core4bit {
       const uint32_t a[2][4] = {{x[0], y[0], x[1], y[1]}, {x[2], y[2], x[3], y[3]}};
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
-        float z[4] = {0.f, 0.f, 0.f, 0.f};
-        mma_f16(z, a[0], q[i][2 * k][0], q[i][2 * k][1]);
+        float z[4];
+        mma_f16_first(z, a[0], q[i][2 * k][0], q[i][2 * k][1]);
         mma_f16(z, a[1], q[i][2 * k + 1][0], q[i][2 * k + 1][1]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[i][e] = k ? fmaf(z[e], f[e >> 1][k], s[i][e]) : z[e] * f[e >> 1][k];
@@ -545,7 +575,7 @@ struct Core4bit {
   }
   __device__ __forceinline__ void take(const PagedParams& p, const Cur& c, const uint8_t* stage, int k0, int lane) {
     const int g = lane >> 2;
-    const bool cut = is_cut<kRows>(p, c.x, k0, kTile);
+    const bool cut = c.x.cut(k0, kTile);
     float s[2][NT][4];
     scores(stage, 0, lane, s[0]);
     scores(stage, 1, lane, s[1]);
@@ -553,7 +583,7 @@ struct Core4bit {
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int u = 0; u < 2; ++u) tops[h][u] = *reinterpret_cast<const float2*>(stage + kTops + (h * 16 + u * 8 + g) * 8);
+      for (int u = 0; u < 2; ++u) tops[h][u] = *reinterpret_cast<const float2*>(stage + kTops + (h * 16 + key_of(u * 8 + g)) * 8);
     uint32_t w[2][NT][2];
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
@@ -563,7 +593,7 @@ struct Core4bit {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           float x = fmaf(s[h][i][e], scale[i][e & 1], tops[h][e >> 1].x);
-          if (cut && !rows.sees(p, i, e & 1, k0 + h * 16 + (e >> 1) * 8 + g)) x = -INFINITY;
+          if (cut && !rows.sees(p, i, e & 1, k0 + h * 16 + key_of((e >> 1) * 8 + g))) x = -INFINITY;
           s[h][i][e] = x;
           top[e & 1] = fmaxf(top[e & 1], x);
         }
@@ -582,12 +612,11 @@ struct Core4bit {
         }
       }
     }
-    const int t0 = c.x.row0 / p.G, t1 = (min(c.x.row0 + kRows, p.rows) - 1) / p.G;
-    if (!cut || t0 == t1) {
+    if (!cut || c.x.one) {
       values<false>(p, stage, k0, 0, lane, w[0], 0);
       values<false>(p, stage, k0, 1, lane, w[1], 0);
     } else
-      for (int tok = t0; tok <= min(t1, c.x.count - 1); ++tok) {
+      for (int tok = c.x.t0; tok <= c.x.t1; ++tok) {
         values<true>(p, stage, k0, 0, lane, w[0], c.x.first + tok);
         values<true>(p, stage, k0, 1, lane, w[1], c.x.first + tok);
       }
@@ -596,7 +625,8 @@ struct Core4bit {
   template <bool ONE>
   __device__ __forceinline__ void values(const PagedParams& p, const uint8_t* stage, int k0, int h, int lane, const uint32_t (&w)[NT][2], int at) {
     const int t = lane & 3;
-    uint32_t x[kGroups][2];      // four codes of keys 2t (lower half) and 2t + 1, and of keys 8 further on
+    // four codes of keys 2t and 2t + 1 (rows m = 2t and 2t + 8 of the tile), and of keys 8 further on (m = 2t + 1 and 2t + 9)
+    uint32_t x[kGroups][2];
 #pragma unroll
     for (int k = 0; k < kGroups; k += 2) {
       uint32_t y[4];
@@ -605,18 +635,18 @@ struct Core4bit {
     }
     uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
     if (ONE) {
-      seen[0] = seen_pair(p, at, k0 + h * 16 + 2 * t);
-      seen[1] = seen_pair(p, at, k0 + h * 16 + 8 + 2 * t);
+      const uint32_t a = seen_pair(p, at, k0 + h * 16 + 2 * t), b = seen_pair(p, at, k0 + h * 16 + 8 + 2 * t);
+      seen[0] = __byte_perm(a, b, 0x5410);
+      seen[1] = __byte_perm(a, b, 0x7632);
     }
 #pragma unroll
     for (int k = 0; k < kGroups; ++k) {
       const uint32_t f0 = *reinterpret_cast<const uint32_t*>(stage + kValuePowers + (k * 32 + h * 16 + 2 * t) * 2);
       const uint32_t f1 = *reinterpret_cast<const uint32_t*>(stage + kValuePowers + (k * 32 + h * 16 + 8 + 2 * t) * 2);
       // a byte for each pair of keys and component
-      const uint32_t one = __byte_perm(x[k][0], x[k][1], 0x5410), two = __byte_perm(x[k][0], x[k][1], 0x7632);
       uint32_t even[4], odd[4];
-      from_e2m1x8((one & 0x0f0f0f0fu) | ((two << 4) & 0xf0f0f0f0u), even);      // components 0 and 2 of four, of keys 2t; of keys 8 + 2t
-      from_e2m1x8(((one >> 4) & 0x0f0f0f0fu) | (two & 0xf0f0f0f0u), odd);
+      from_e2m1x8((x[k][0] & 0x0f0f0f0fu) | ((x[k][1] * 16u) & 0xf0f0f0f0u), even);                      // components 0 and 2 of four, of rows m = 2t; of 2t + 8
+      from_e2m1x8((__umulhi(x[k][0], 1u << 28) & 0x0f0f0f0fu) | (x[k][1] & 0xf0f0f0f0u), odd);           // (a shift by the multiplier, which has time)
       const uint32_t a[2][4] = {{even[0], odd[0], even[2], odd[2]}, {even[1], odd[1], even[3], odd[3]}};
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
@@ -626,8 +656,8 @@ struct Core4bit {
         for (int j = 0; j < 2; ++j) {
           if (!ONE) mma_f16(o[i][2 * k + j], a[j], b0, b1);
           else {
-            float z[4] = {0.f, 0.f, 0.f, 0.f};
-            mma_f16(z, a[j], b0, b1);
+            float z[4];
+            mma_f16_first(z, a[j], b0, b1);
 #pragma unroll
             for (int e = 0; e < 4; ++e)
               if (rows.at[i][e & 1] == at) o[i][2 * k + j][e] += z[e];
@@ -677,7 +707,7 @@ struct CoreF32 {
   __device__ __forceinline__ void look_up(const PagedParams& p, const Cur& c, int warp, int lane) { place.look_up(p, c.x, c.tile(warp) + (lane & 15)); }
   __device__ __forceinline__ void settle() {}
   __device__ __forceinline__ void issue(const PagedParams& p, const Cur& c, uint8_t* stage, int lane) {
-    copy_rows<kTile, DP / 4, kSide>(p, place.at<4>(p, c.h), p.c.d / 4, smem_at(stage), lane, [](int r, int chunk) { return r * kRowBytes + ((chunk ^ (r & 7)) << 4); });
+    copy_rows<kTile, DP / 4, kSide>(p, place.at(p, c.h), p.c.d / 4, smem_at(stage), lane, [](int r, int chunk) { return r * kRowBytes + ((chunk ^ (r & 7)) << 4); });
   }
   __device__ __forceinline__ void begin(const PagedParams& p, const Cur& c, int lane) {
     const int n = min(ROWS, p.rows - c.x.row0);
@@ -713,7 +743,7 @@ struct CoreF32 {
         s[r] = fmaf(x.x, k.x, fmaf(x.y, k.y, fmaf(x.z, k.z, fmaf(x.w, k.w, s[r]))));
       }
     }
-    const bool cut = is_cut<kRows>(p, c.x, k0, kTile);
+    const bool cut = c.x.cut(k0, kTile);
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
       float x = (s[r] + __shfl_xor_sync(0xffffffffu, s[r], 16)) * p.scale_log2;
@@ -793,7 +823,8 @@ struct CoreF32 {
 // ---- the walk ---------------------------------------------------------------------------------------------------------------
 template <class Core>
 constexpr int paged_smem() {
-  return kWarps * Core::kStages * Core::kStageBytes + Buffer<Core::kDP>::kFloats * 4 + Core::kExtra;
+  static_assert(Core::kStageBytes >= Buffer<Core::kDP>::kBytes && Core::kStageBytes % 16 == 0, "a warp's rows fit into a stage");
+  return kWarps * Core::kStages * Core::kStageBytes + Core::kExtra;
 }
 
 // A finished row's value: four components and (at the first) the log-sum-exp; zeros for a token that is not real.
@@ -868,11 +899,10 @@ __global__ void __launch_bounds__(kThreads, Core::kMinCtas) paged_kernel(const _
   constexpr int NS = Core::kStages;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   uint8_t* ring = smem + warp * NS * Core::kStageBytes;
-  const Buffer<Core::kDP> buffer{reinterpret_cast<float*>(smem + kWarps * NS * Core::kStageBytes)};
   asm volatile("griddepcontrol.launch_dependents;");
 
   // The run of this CTA: prefix sums of the entries' units, kThreads at a time.
-  int64_t* scan = reinterpret_cast<int64_t*>(buffer.at);      // sums of the warps, then the entry that the run begins in, and where
+  int64_t* scan = reinterpret_cast<int64_t*>(smem);      // sums of the warps, then the entry that the run begins in, and where
   auto block_scan = [&](int x, int64_t& before, int64_t& all) {
     int64_t y = x;
     for (int o = 1; o < 32; o <<= 1) {
@@ -923,16 +953,18 @@ __global__ void __launch_bounds__(kThreads, Core::kMinCtas) paged_kernel(const _
   next.x = entry_of<Core::kRows, Core::kTile>(p, next.e);
   next.h = (int)(within / next.x.units);
   next.unit = (int)(within - (int64_t)next.h * next.x.units);
-  __syncthreads();              // (the buffer is used again)
+  __syncthreads();              // (copies go there next)
 
   Core core;
-  core.prepare(reinterpret_cast<uint8_t*>(buffer.at + Buffer<Core::kDP>::kFloats));
+  core.prepare(smem + kWarps * NS * Core::kStageBytes);
   Cur here = next;
   const int n = (int)(end - begin);
   core.look_up(p, next, warp, lane);
+  int to = 0, from = 0;        // stages to fill and to read next
   auto issue = [&](int i) {
     if (i < n) {
-      core.issue(p, next, ring + i % NS * Core::kStageBytes, lane);
+      core.issue(p, next, ring + to * Core::kStageBytes, lane);
+      to = to == NS - 1 ? 0 : to + 1;
       if (i + 1 < n) {
         next.next(p);
         core.look_up(p, next, warp, lane);
@@ -955,7 +987,7 @@ __global__ void __launch_bounds__(kThreads, Core::kMinCtas) paged_kernel(const _
       fresh = false;
     }
     const int k0 = here.tile(warp);
-    if (k0 < here.x.hi) core.take(p, here, ring + i % NS * Core::kStageBytes, k0, lane);
+    if (k0 < here.x.hi) core.take(p, here, ring + from * Core::kStageBytes, k0, lane);
     __syncwarp();
     const bool last = here.unit + 1 == here.x.units;
     if (last || i + 1 == n) {
@@ -968,11 +1000,13 @@ __global__ void __launch_bounds__(kThreads, Core::kMinCtas) paged_kernel(const _
         while (run_begin(total, cta, ctas) >= item_end) --cta;
         p.meta[blockIdx.x] = make_int4(here.e, here.h, slot, cta);
       }
+      const Buffer<Core::kDP> buffer{smem + from * Core::kStageBytes, NS * Core::kStageBytes};
       finish<Core>(p, core, here, whole, slot, buffer, warp, lane);
       fresh = true;
       first_item = false;
     }
     here.next(p);
+    from = from == NS - 1 ? 0 : from + 1;
   }
   copies_awaited<0>();
 }
@@ -1036,7 +1070,7 @@ bool plan_paged(const bma_paged_cache& c, const bma_paged_attn_args& a, PagedLau
   l.dp = c.d <= 64 ? 64 : 128;
   l.tile = c.dtype == BMA_DTYPE_MXFP4 ? 32 : 16;
   l.rows_of_tile = c.dtype == BMA_DTYPE_F32 && rows <= 4 ? 4 : rows <= 8 ? 8 : c.dtype == BMA_DTYPE_F32 || rows <= 16 ? 16 : 32;
-  l.ctas_per_sm = c.dtype == BMA_DTYPE_F32 && l.dp == 128 ? 1 : 2;
+  l.ctas_per_sm = c.dtype == BMA_DTYPE_F32 ? (l.dp == 128 ? 1 : 2) : l.rows_of_tile == 8 ? 3 : 2;
   l.row_tiles = ceil_div(rows, l.rows_of_tile);
   const int64_t entries = (int64_t)c.B * l.row_tiles;
   if (entries >= (1 << 30)) return false;
@@ -1115,6 +1149,10 @@ int bma_paged_attn(const bma_paged_cache* cache, const bma_paged_attn_args* args
   p.row_tiles = l.row_tiles;
   p.entries = l.entries;
   p.positions = cache->width * cache->page_size;
+  const int64_t bytes = cache->dtype == BMA_DTYPE_F32 ? 4 : cache->dtype == BMA_DTYPE_BF16 ? 2 : 1;      // (their products fit 32 bits: validate_paged)
+  p.page_units = (uint32_t)(cache->stride_page * bytes / 16);
+  p.slot_units = (uint32_t)(cache->stride_slot * bytes / 16);
+  p.head_units = (uint32_t)(cache->stride_head * bytes / 16);
   p.page_shift = -1;
   for (int i = 0; i < 31; ++i)
     if (cache->page_size == 1 << i) p.page_shift = i;
