@@ -452,43 +452,33 @@ struct Core4bit {
   __device__ __forceinline__ void settle() {
     if (!pending) return;
     const int lane = threadIdx.x & 31;
-    // pairs of bytes, 0 and 2, 1 and 3
-    const uint32_t v02 = v_bytes & 0x00ff00ffu, v13 = v_bytes >> 8 & 0x00ff00ffu;
-    const uint32_t tops = __vmaxu2(v02, v13);
-    int top = max(max((int)(tops & 0xffffu), (int)(tops >> 16)), 127 - 65);
-    const uint32_t down = (uint32_t)(15 - top) & 0xffffu;
-    // 2^(e - E) is float16 of exponent x = e - E + 15 where that is positive
-    uint32_t x02 = __viaddmax_s16x2_relu(v02, down | down << 16, 0u), x13 = __viaddmax_s16x2_relu(v13, down | down << 16, 0u);
-    const bool nan = (v_bytes & (v_bytes & 0x7f7f7f7fu) + 0x01010101u | k_bytes & (k_bytes & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-    const bool small = ((x02 - 0x00010001u) & ~x02 | (x13 - 0x00010001u) & ~x13) & (kGroups == 4 ? 0x80008000u : 0x8000u);
+    int b[4] = {(int)(v_bytes & 255), (int)(v_bytes >> 8 & 255), (int)(v_bytes >> 16 & 255), (int)(v_bytes >> 24)};
+    if (kGroups == 2) b[2] = b[3] = b[0];
+    int top = max(max(b[0], b[1]), max(b[2], b[3]));
+    const int least = min(min(b[0], b[1]), min(b[2], b[3]));
+    const bool rare = top == 255 || least < top - 14 || (k_bytes & ((k_bytes & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u);
+    top = max(top, 127 - 65);
+    uint32_t f[4];      // 2^(e - E) as float16
     float kp[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) kp[i] = __uint_as_float((i == 0 ? k_bytes << 23 : i == 1 ? k_bytes << 15 : i == 2 ? k_bytes << 7 : k_bytes >> 1) & 0x7f800000u);      // (2^-127 counts as 0 here)
-    x02 <<= 10;
-    x13 <<= 10;
-    if (__any_sync(0xffffffffu, nan || small)) {        // bytes of 255, powers under 2^-14 of the head's largest
+    for (int i = 0; i < 4; ++i) {
+      f[i] = b[i] * 1024 + (15 - top) * 1024;
+      kp[i] = __uint_as_float((i == 0 ? k_bytes << 23 : i == 1 ? k_bytes << 15 : i == 2 ? k_bytes << 7 : k_bytes >> 1) & 0x7f800000u);      // (2^-127 counts as 0)
+    }
+    if (__any_sync(0xffffffffu, rare || least < 127 - 65 - 14)) {        // bytes of 255, powers under 2^-14 of the head's largest
       top = 127 - 65;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int b = v_bytes >> (8 * i) & 255;
-        top = b == 255 ? top : max(top, b);
-      }
+      for (int i = 0; i < 4; ++i) top = b[i] == 255 ? top : max(top, b[i]);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int b = v_bytes >> (8 * i) & 255, x = b - top + 15;
-        const uint32_t f = b == 255 ? 0x7fff : x > 0 ? x << 10 : 0x400 >> min(1 - x, 31);
-        uint32_t& w = i & 1 ? x13 : x02;
-        w = i & 2 ? (w & 0xffffu) | f << 16 : (w & 0xffff0000u) | f;
+        const int x = b[i] - top + 15;
+        f[i] = b[i] == 255 ? 0x7fff : x > 0 ? x << 10 : 0x400 >> min(1 - x, 31);
         if ((k_bytes >> (8 * i) & 255) == 255) kp[i] = __uint_as_float(0x7fffffffu);
       }
     }
     uint16_t* vp = reinterpret_cast<uint16_t*>(pending + kValuePowers) + (lane & 16) + (lane & 6) + (lane >> 3 & 1) + (lane & 1) * 8;      // the row m of the key
-    vp[0] = (uint16_t)x02;
-    vp[32] = (uint16_t)x13;
-    if (kGroups == 4) {
-      vp[64] = (uint16_t)(x02 >> 16);
-      vp[96] = (uint16_t)(x13 >> 16);
-    }
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i) vp[i * 32] = (uint16_t)f[i];
     *reinterpret_cast<float4*>(pending + kKeyPowers + lane * 16) = make_float4(kp[0], kp[1], kp[2], kp[3]);
     *reinterpret_cast<float2*>(pending + kTops + lane * 8) = make_float2((float)(top - 127), top == 254 ? __uint_as_float(0x00400000u) : __uint_as_float((uint32_t)(254 - top) << 23));
     pending = nullptr;
