@@ -4,24 +4,29 @@
 //
 // Rotation.  Component pairs are (i, i + dim/2) or (2i, 2i + 1).  A lane holds two 16-byte chunks of a head that hold both halves of its pairs
 // (chunks u and u + dim/2 of a head, or chunks 2u and 2u + 1), so that no value crosses lanes; only the sum of squares does.  A head of 128
-// bfloat16 values takes 8 lanes, a warp four heads at a time.  Cosine and sine of a lane's pairs are taken once for a token and used for all
-// of its heads.
+// bfloat16 values takes 8 lanes, a warp four heads at a time.  Cosine and sine of a token are taken once by the warp, through shared memory, and
+// with the weights of a side make four factors of a pair, which serve all heads of that side: out = x * F + y * G, two values to an instruction.
+// (Taken by every lane for itself, with weights applied first, forward and backward of 4 x 4096 tokens of 64 heads of 128 took 144 and 208 us,
+// bound by instructions, three times as many.)
 //
 // The angle position * frequency is kept as a fraction of a turn in 64-bit integers: frequency / 2 pi as a multiple of 2^-64, times the
 // position, modulo 2^64.  That is exact but for the rounding of the frequency (2^-53 of it in float64), however far the position; in float32 a
 // position of 10^5 would leave 0.004 of the angle open.  The upper 32 bits then go through sincospi in float32.
+//
+// Tensors whose rows no 16-byte access fits, and heads whose halves begin in the middle of a chunk, go through the kernels' narrow form, a value at a time.
 #include "paged.cuh"
 
 namespace bma {
 namespace {
 
 constexpr int kHeadsThreads = 128, kHeadsWarps = kHeadsThreads / 32;
+constexpr int kHeadsCtas = 20;      // at most so many CTAs to an SM, each over its share of the tokens (four waves)
 
 template <typename T> struct Bits16;   // values of a 16-byte chunk
 template <> struct Bits16<float> { static constexpr int n = 4; };
 template <> struct Bits16<__nv_bfloat16> { static constexpr int n = 8; };
 
-// VEC values: a 16-byte chunk, or one value where the tensors allow no wider access
+// VEC values: one, where the tensors allow no wider access
 template <typename T, int VEC>
 struct Chunk {
   uint4 raw;
@@ -56,11 +61,14 @@ __device__ __forceinline__ void store_chunk(T* p, const float (&x)[VEC]) {
   }
 }
 
-// cosine and sine of position * frequency, times `magnitude`
-__device__ __forceinline__ void turn_of(double frequency, long long position, float magnitude, float& c, float& s) {
+// frequency / 2 pi as a multiple of 2^-64, modulo 1
+__device__ __forceinline__ unsigned long long step_of(double frequency) {
   double turns = frequency * 0.15915494309189533577;
   turns -= floor(turns);
-  const unsigned long long step = __double2ull_rz(turns * 18446744073709551616.0);
+  return __double2ull_rz(turns * 18446744073709551616.0);
+}
+// cosine and sine of position * frequency, times `magnitude`
+__device__ __forceinline__ void turn_of(unsigned long long step, long long position, float magnitude, float& c, float& s) {
   const long long phase = (long long)((unsigned long long)position * step);
   sincospif((float)(int)(phase >> 32) * 4.656612873077392578125e-10f, &s, &c);   // half turns in [-1, 1]
   c *= magnitude;
@@ -92,7 +100,7 @@ struct Turns {
       c[j] = 1.f; s[j] = 0.f;
       if (2 * i < m.dim) {
         live |= 1u << j;
-        turn_of(__ldg(frequencies + i), position, magnitude, c[j], s[j]);
+        turn_of(step_of(__ldg(frequencies + i)), position, magnitude, c[j], s[j]);
       }
     }
   }
@@ -161,6 +169,29 @@ struct HeadsParams {
 
 enum { kRotate = 0, kAppend = 1, kAppend4 = 2 };
 
+template <typename P>
+__device__ __forceinline__ long long position_of(const P& p, int b, int t) {
+  if (!p.positions) return t;
+  const int64_t at = b * p.position_stride_b + t * p.position_stride_l;
+  return p.position_bytes == 8 ? __ldg(static_cast<const long long*>(p.positions) + at) : (long long)__ldg(static_cast<const int*>(p.positions) + at);
+}
+// Whether token t of those given of sequence b is real; its position, and its offsets in the cache (negative where there is no place for it)
+__device__ __forceinline__ bool token_place(const HeadsParams& p, int b, int t, int lane, long long& position, int64_t& held, int64_t& held_scale) {
+  const NewTokens n = new_tokens(p.lengths, p.new_lengths, b, p.L);
+  position = n.first + t;
+  if (t >= n.count) return false;
+  int slot = 0;
+  const int page = page_of(p.cache, b, position, slot);
+  if (page < 0) {
+    if (lane == 0) report_device_error(p.status, kStatusAppend);
+    held = -1;
+  } else {
+    held = (int64_t)page * p.cache.stride_page + (int64_t)slot * p.cache.stride_slot;
+    held_scale = (int64_t)page * p.cache.scale_stride_page + (int64_t)slot * p.cache.scale_stride_slot;
+  }
+  return true;
+}
+
 // e2m1 codes and powers of two of a warp's heads, whose values lie in shared memory: each lane takes 8 values, four lanes 32.
 __device__ __forceinline__ void store_4bit(const float* row, bool there, int d, int tpr, int u, uint8_t* codes, uint8_t* scales) {
   for (int p = u; p - u < kPagedHeadDim / 8; p += tpr) {       // (every lane of the warp goes round as often)
@@ -210,25 +241,8 @@ __global__ void __launch_bounds__(kHeadsThreads) heads_kernel(const __grid_const
   long long position = t;
   bool real = true;
   int64_t held = 0, held_scale = 0;      // offsets of the token in the cache
-  if constexpr (KIND == kRotate) {
-    if (p.positions) {
-      const int64_t at = b * p.position_stride_b + t * p.position_stride_l;
-      position = p.position_bytes == 8 ? __ldg(static_cast<const long long*>(p.positions) + at) : (long long)__ldg(static_cast<const int*>(p.positions) + at);
-    }
-  } else {
-    const NewTokens n = new_tokens(p.lengths, p.new_lengths, b, p.L);
-    position = n.first + t;
-    real = t < n.count;
-    int slot = 0;
-    const int page = real ? page_of(p.cache, b, position, slot) : 0;
-    if (page < 0) {
-      if (lane == 0) report_device_error(p.status, kStatusAppend);
-      held = -1;
-    } else if (real) {
-      held = (int64_t)page * p.cache.stride_page + (int64_t)slot * p.cache.stride_slot;
-      held_scale = (int64_t)page * p.cache.scale_stride_page + (int64_t)slot * p.cache.scale_stride_slot;
-    }
-  }
+  if constexpr (KIND == kRotate) position = position_of(p, b, t);
+  else real = token_place(p, b, t, lane, position, held, held_scale);
 
   Turns<VEC> turns[UPT];
   int ca[UPT], cb[UPT];
@@ -384,11 +398,7 @@ __global__ void __launch_bounds__(kHeadsThreads, 4) rotate_back_kernel(const __g
 #pragma unroll 1
   for (int64_t token = (int64_t)cta * kHeadsWarps + warp; token < tokens; token += (int64_t)ctas * kHeadsWarps) {
     const int b = (int)(token / p.L), t = (int)(token - (int64_t)b * p.L);
-    long long position = t;
-    if (p.positions) {
-      const int64_t at = b * p.position_stride_b + t * p.position_stride_l;
-      position = p.position_bytes == 8 ? __ldg(static_cast<const long long*>(p.positions) + at) : (long long)__ldg(static_cast<const int*>(p.positions) + at);
-    }
+    const long long position = position_of(p, b, t);
     Turns<VEC> turns[UPT];
     const bool turned = p.map.dim > 0;
     if (turned) {
@@ -470,6 +480,342 @@ __global__ void __launch_bounds__(kHeadsThreads, 4) rotate_back_kernel(const __g
 #pragma unroll
     for (int w = 0; w < kHeadsWarps; ++w) s += sums[w][c];
     p.partial[(int64_t)blockIdx.x * p.d + c] = s;
+  }
+}
+
+// ---- 16-byte chunks -----------------------------------------------------------------------------------------------------
+// A lane's unit of a head: VEC pairs of neighbouring values (as float2), those of chunk `ca`, then those of chunk `cb`.
+template <typename T>
+struct Unit {
+  static constexpr int VEC = Bits16<T>::n;
+  uint4 a, b;
+  __device__ __forceinline__ void load(const T* p, int ca, int cb, int chunks) {
+    a = b = make_uint4(0, 0, 0, 0);
+    if (ca < chunks) a = *reinterpret_cast<const uint4*>(p + ca * VEC);
+    if (cb < chunks) b = *reinterpret_cast<const uint4*>(p + cb * VEC);
+  }
+  __device__ __forceinline__ void zero() { a = b = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void get(float2 (&v)[VEC]) const {
+    const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      if constexpr (VEC == 8) v[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+      else v[i] = make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+    }
+  }
+  __device__ __forceinline__ void set(const float2 (&v)[VEC]) {
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      if constexpr (VEC == 8) {
+        const __nv_bfloat162 h = __float22bfloat162_rn(v[i]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      } else {
+        w[2 * i] = __float_as_uint(v[i].x);
+        w[2 * i + 1] = __float_as_uint(v[i].y);
+      }
+    }
+    a = make_uint4(w[0], w[1], w[2], w[3]);
+    b = make_uint4(w[4], w[5], w[6], w[7]);
+  }
+  __device__ __forceinline__ void store(T* p, int ca, int cb, int chunks) const {
+    if (ca < chunks) *reinterpret_cast<uint4*>(p + ca * VEC) = a;
+    if (cb < chunks) *reinterpret_cast<uint4*>(p + cb * VEC) = b;
+  }
+};
+__device__ __forceinline__ float2 swapped(float2 v) { return make_float2(v.y, v.x); }
+__device__ __forceinline__ float2 twice(float x) { return make_float2(x, x); }
+
+// 64-bit steps of the pairs (a CTA makes them once), and a warp's cosines and sines of a token.
+constexpr int kPairs = 128;
+__device__ __forceinline__ void make_steps(unsigned long long* steps, const double* frequencies, int pairs) {
+  for (int i = threadIdx.x; i < pairs; i += blockDim.x) steps[i] = step_of(__ldg(frequencies + i));
+  __syncthreads();
+}
+__device__ __forceinline__ void make_turns(float2* turns, const unsigned long long* steps, int pairs, long long position, float magnitude, int lane) {
+  __syncwarp();            // (those of the last token have been read)
+  for (int i = lane; i < pairs; i += 32) {
+    float c, s;
+    turn_of(steps[i], position, magnitude, c, s);
+    turns[i] = make_float2(c, s);
+  }
+  __syncwarp();
+}
+
+// Bits of the unit's pairs of components that are rotated: component pairs u * VEC and up are (value j of chunk a, value j of chunk b) in the HALF layout,
+// else neighbours.
+template <int VEC>
+__device__ __forceinline__ uint32_t live_pairs(int u, int pairs) {
+  const int n = min(max(pairs - u * VEC, 0), VEC);
+  return (1u << n) - 1u;
+}
+
+// The same work as heads_kernel's.  FULL: every component is rotated.
+template <typename T, int LAYOUT, bool FULL, int KIND>
+__global__ void __launch_bounds__(kHeadsThreads) heads_wide_kernel(const __grid_constant__ HeadsParams p) {
+  constexpr int VEC = Bits16<T>::n, NR = 2;
+  constexpr bool HALF = LAYOUT == BMA_ROTARY_HALF;
+  __shared__ unsigned long long steps[kPairs];
+  __shared__ float2 turns[kHeadsWarps][kPairs];
+  __shared__ float rows[KIND == kAppend4 ? kHeadsWarps : 1][KIND == kAppend4 ? 8 : 1][KIND == kAppend4 ? kPagedHeadDim + 4 : 1];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int tpr = p.map.tpr, group = lane / tpr, u = lane & (tpr - 1), groups = 32 / tpr, chunks = p.map.chunks;
+  const int pairs = p.map.dim / 2;
+  make_steps(steps, p.frequencies, pairs);
+  int ca, cb;
+  unit_chunks<VEC>(p.map, u, ca, cb);
+  const uint32_t live = live_pairs<VEC>(u, pairs);
+  const float inv_d = 1.f / (float)p.d;
+  const int64_t items = (int64_t)p.B * p.L * p.slabs;
+#pragma unroll 1
+  for (int64_t item = (int64_t)blockIdx.x * kHeadsWarps + warp; item < items; item += (int64_t)gridDim.x * kHeadsWarps) {
+    const int64_t token = item / p.slabs;
+    const int slab = (int)(item - token * p.slabs);
+    const int b = (int)(token / p.L), t = (int)(token - (int64_t)b * p.L);
+    long long position = t;
+    bool real = true;
+    int64_t held = 0, held_scale = 0;      // offsets of the token in the cache
+    if constexpr (KIND == kRotate) position = position_of(p, b, t);
+    else real = token_place(p, b, t, lane, position, held, held_scale);
+    if (pairs && real) make_turns(turns[warp], steps, pairs, position, p.back ? -p.magnitude : p.magnitude, lane);
+    const int slab_begin = slab * p.slab_heads, slab_end = slab_begin + p.slab_heads;
+    int first = 0;      // heads of the sides before
+#pragma unroll 1
+    for (int si = 0; si < (KIND == kRotate ? 2 : 3); ++si) {
+      const Side& side = p.side[si];
+      const int lo = max(slab_begin - first, 0), hi = min(slab_end - first, side.heads);
+      first += side.heads;
+      if (lo >= hi) continue;
+      const bool cached = KIND != kRotate && si > 0;
+      if (cached && (!real || held < 0)) continue;
+      const T* in = static_cast<const T*>(side.in.ptr) + b * side.in.stride_b + t * side.in.stride_l;
+      T* out = static_cast<T*>(side.out.ptr) + b * side.out.stride_b + t * side.out.stride_l;
+      int64_t out_head = side.out.stride_h;
+      if (cached) {
+        out = static_cast<T*>(si == 1 ? p.cache.k : p.cache.v) + held;      // (a 4-bit cache is not written through this)
+        out_head = p.cache.stride_head;
+      }
+      const bool normed = side.weight != nullptr, plain = !normed && !side.turned;
+      // out = v * F + (the other half of the pair) * G
+      float2 F[VEC], G[VEC];
+      if (!plain) {
+        float2 w[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) w[i] = make_float2(1.f, 1.f);
+        if (normed) {
+          float wa[VEC], wb[VEC];
+          load_weight<VEC>(side.weight, p.weight_dtype, ca, chunks, wa);
+          load_weight<VEC>(side.weight, p.weight_dtype, cb, chunks, wb);
+#pragma unroll
+          for (int i = 0; i < VEC / 2; ++i) {
+            w[i] = make_float2(wa[2 * i], wa[2 * i + 1]);
+            w[VEC / 2 + i] = make_float2(wb[2 * i], wb[2 * i + 1]);
+          }
+        }
+        float2 cs[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          cs[j] = make_float2(1.f, 0.f);
+          if (side.turned && (FULL || live >> j & 1) && real && u * VEC + j < pairs) cs[j] = turns[warp][u * VEC + j];
+          if (p.back) cs[j].x = (FULL || live >> j & 1) ? -cs[j].x : cs[j].x;      // (-magnitude gave -cos and -sin)
+        }
+        if constexpr (HALF) {
+#pragma unroll
+          for (int i = 0; i < VEC / 2; ++i) {
+            const float2 c = make_float2(cs[2 * i].x, cs[2 * i + 1].x), s = make_float2(cs[2 * i].y, cs[2 * i + 1].y);
+            F[i] = __fmul2_rn(c, w[i]);
+            F[VEC / 2 + i] = __fmul2_rn(c, w[VEC / 2 + i]);
+            G[i] = __fmul2_rn(make_float2(-s.x, -s.y), w[VEC / 2 + i]);
+            G[VEC / 2 + i] = __fmul2_rn(s, w[i]);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) {
+            F[j] = __fmul2_rn(twice(cs[j].x), w[j]);
+            G[j] = __fmul2_rn(make_float2(-cs[j].y, cs[j].y), swapped(w[j]));
+          }
+        }
+      }
+#pragma unroll 1
+      for (int h0 = lo; h0 < hi; h0 += groups * NR) {
+        Unit<T> x[NR];
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+          const int h = h0 + r * groups + group;
+          if (h < hi && real) x[r].load(in + h * side.in.stride_h, ca, cb, chunks);
+          else x[r].zero();
+        }
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+          const int h = h0 + r * groups + group;
+          float2 v[VEC];
+          if (!plain || KIND == kAppend4) x[r].get(v);
+          if (!plain) {
+            float2 o[VEC];
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+              float2 other = HALF ? v[(i + VEC / 2) % VEC] : swapped(v[i]);
+              // what is not rotated takes nothing of its neighbour, not even a zero times infinity
+              if (!FULL && !(HALF ? live != 0 : live >> i & 1)) other = make_float2(0.f, 0.f);
+              o[i] = __ffma2_rn(v[i], F[i], __fmul2_rn(other, G[i]));
+            }
+            if (normed) {
+              float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+              for (int i = 0; i < VEC; ++i) sum = __ffma2_rn(v[i], v[i], sum);
+              const float2 inv = twice(rsqrtf(group_sum(sum.x + sum.y, tpr) * inv_d + p.eps));
+#pragma unroll
+              for (int i = 0; i < VEC; ++i) o[i] = __fmul2_rn(o[i], inv);
+            }
+            if (KIND == kAppend4 && cached) {
+#pragma unroll
+              for (int i = 0; i < VEC; ++i) v[i] = o[i];
+            } else x[r].set(o);
+          }
+          if (KIND == kAppend4 && cached) {
+            float* row = rows[warp][group];
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < VEC / 2; ++i) {
+              if (ca < chunks) *reinterpret_cast<float2*>(row + ca * VEC + 2 * i) = v[i];
+              if (cb < chunks) *reinterpret_cast<float2*>(row + cb * VEC + 2 * i) = v[VEC / 2 + i];
+            }
+            __syncwarp();
+            uint8_t* codes = static_cast<uint8_t*>(si == 1 ? p.cache.k : p.cache.v) + held + h * p.cache.stride_head;
+            uint8_t* scales = (si == 1 ? p.cache.k_scale : p.cache.v_scale) + held_scale + h * p.cache.scale_stride_head;
+            store_4bit(row, h < hi, p.d, tpr, u, codes, scales);
+          } else if (h < hi) {
+            if (!real) x[r].zero();
+            x[r].store(out + h * out_head, ca, cb, chunks);
+          }
+        }
+      }
+    }
+  }
+}
+
+// The same work as rotate_back_kernel's.
+template <typename T, int LAYOUT, bool FULL>
+__global__ void __launch_bounds__(kHeadsThreads, 4) rotate_back_wide_kernel(const __grid_constant__ BackParams p) {
+  constexpr int VEC = Bits16<T>::n;
+  constexpr bool HALF = LAYOUT == BMA_ROTARY_HALF;
+  constexpr int CS = HALF ? VEC / 2 : VEC;
+  __shared__ unsigned long long steps[kPairs];
+  __shared__ float2 turns[kHeadsWarps][kPairs];
+  __shared__ float sums[kHeadsWarps][256];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int tpr = p.map.tpr, group = lane / tpr, u = lane & (tpr - 1), groups = 32 / tpr, chunks = p.map.chunks;
+  const int si = (int)blockIdx.x < p.q_ctas ? 0 : 1;
+  const int cta = si ? blockIdx.x - p.q_ctas : blockIdx.x, ctas = si ? gridDim.x - p.q_ctas : p.q_ctas;
+  const Side& side = p.side[si];
+  const bma_tensor& g = p.g[si];
+  const float inv_d = 1.f / (float)p.d;
+  const int pairs = p.map.dim / 2;
+  make_steps(steps, p.frequencies, pairs);
+  int ca, cb;
+  unit_chunks<VEC>(p.map, u, ca, cb);
+  const uint32_t live = live_pairs<VEC>(u, pairs);
+  float2 w[VEC], dw[VEC];
+  {
+    float wa[VEC], wb[VEC];
+    load_weight<VEC>(side.weight, p.weight_dtype, ca, chunks, wa);
+    load_weight<VEC>(side.weight, p.weight_dtype, cb, chunks, wb);
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) {
+      w[i] = make_float2(wa[2 * i], wa[2 * i + 1]);
+      w[VEC / 2 + i] = make_float2(wb[2 * i], wb[2 * i + 1]);
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) dw[i] = make_float2(0.f, 0.f);
+  }
+  const int64_t tokens = (int64_t)p.B * p.L;
+#pragma unroll 1
+  for (int64_t token = (int64_t)cta * kHeadsWarps + warp; token < tokens; token += (int64_t)ctas * kHeadsWarps) {
+    const int b = (int)(token / p.L), t = (int)(token - (int64_t)b * p.L);
+    // cosines and sines of the unit's values: HALF, of pairs 2i and 2i + 1; else of both values of pair i, the sine with its sign
+    float2 c[CS], s[CS];
+    if (pairs) make_turns(turns[warp], steps, pairs, position_of(p, b, t), p.magnitude, lane);
+#pragma unroll
+    for (int i = 0; i < CS; ++i) {
+      const auto at = [&](int j) { return (FULL || live >> j & 1) && u * VEC + j < pairs ? turns[warp][u * VEC + j] : make_float2(1.f, 0.f); };
+      if constexpr (HALF) {
+        const float2 x = at(2 * i), y = at(2 * i + 1);
+        c[i] = make_float2(x.x, y.x);
+        s[i] = make_float2(x.y, y.y);
+      } else {
+        const float2 x = at(i);
+        c[i] = twice(x.x);
+        s[i] = make_float2(x.y, -x.y);
+      }
+    }
+    const T* in = static_cast<const T*>(side.in.ptr) + b * side.in.stride_b + t * side.in.stride_l;
+    const T* gin = static_cast<const T*>(g.ptr) + b * g.stride_b + t * g.stride_l;
+    T* out = static_cast<T*>(side.out.ptr) + b * side.out.stride_b + t * side.out.stride_l;
+#pragma unroll 1
+    for (int h0 = 0; h0 < side.heads; h0 += groups) {
+      const int h = h0 + group;
+      const bool there = h < side.heads;
+      Unit<T> x, y;
+      if (there) {
+        x.load(in + h * side.in.stride_h, ca, cb, chunks);
+        y.load(gin + h * g.stride_h, ca, cb, chunks);
+      } else {
+        x.zero();
+        y.zero();
+      }
+      float2 v[VEC], e[VEC], f[VEC];
+      x.get(v);
+      y.get(e);
+      float2 sum = make_float2(0.f, 0.f), dot = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        float2 other = HALF ? e[(i + VEC / 2) % VEC] : swapped(e[i]);
+        if (!FULL && !(HALF ? live != 0 : live >> i & 1)) other = make_float2(0.f, 0.f);
+        if constexpr (HALF) {
+          const int k = i % (VEC / 2);
+          f[i] = __ffma2_rn(e[i], c[k], __fmul2_rn(other, i < VEC / 2 ? s[k] : make_float2(-s[k].x, -s[k].y)));
+        } else f[i] = __ffma2_rn(e[i], c[i], __fmul2_rn(other, s[i]));
+      }
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        e[i] = __fmul2_rn(f[i], v[i]);                 // g' x
+        sum = __ffma2_rn(v[i], v[i], sum);
+        dot = __ffma2_rn(e[i], w[i], dot);
+      }
+      float sum1 = sum.x + sum.y, dot1 = dot.x + dot.y;
+      for (int o = tpr >> 1; o; o >>= 1) {
+        sum1 += __shfl_xor_sync(0xffffffffu, sum1, o);
+        dot1 += __shfl_xor_sync(0xffffffffu, dot1, o);
+      }
+      const float inv = rsqrtf(sum1 * inv_d + p.eps);
+      const float2 inv2 = twice(inv), m = twice(-(dot1 * inv * inv_d) * inv * inv);    // -inv^2 mean(g' w x^)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        if (there) dw[i] = __ffma2_rn(e[i], inv2, dw[i]);
+        f[i] = __ffma2_rn(v[i], m, __fmul2_rn(__fmul2_rn(f[i], w[i]), inv2));
+      }
+      if (there) {
+        y.set(f);
+        y.store(out + h * side.out.stride_h, ca, cb, chunks);
+      }
+    }
+  }
+  // the groups of a warp, the warps of the CTA
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) {
+    for (int o = tpr; o < 32; o <<= 1) {
+      dw[i].x += __shfl_xor_sync(0xffffffffu, dw[i].x, o);
+      dw[i].y += __shfl_xor_sync(0xffffffffu, dw[i].y, o);
+    }
+    const int chunk = i < VEC / 2 ? ca : cb;
+    if (group == 0 && chunk < chunks) *reinterpret_cast<float2*>(&sums[warp][chunk * VEC + 2 * (i % (VEC / 2))]) = dw[i];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < p.d; i += kHeadsThreads) {
+    float x = 0.f;
+#pragma unroll
+    for (int k = 0; k < kHeadsWarps; ++k) x += sums[k][i];
+    p.partial[(int64_t)blockIdx.x * p.d + i] = x;
   }
 }
 
@@ -593,10 +939,16 @@ int launch_heads(HeadsParams& p, const bma_rotary& r, bool wide, cudaStream_t st
   const int64_t tokens = (int64_t)p.B * p.L;
   const int heads = p.side[0].heads + p.side[1].heads + p.side[2].heads;
   cut_heads(p, tokens, heads, 32 / p.map.tpr);
-  const int64_t ctas = (tokens * p.slabs + kHeadsWarps - 1) / kHeadsWarps;
+  int64_t ctas = (tokens * p.slabs + kHeadsWarps - 1) / kHeadsWarps;
   BMA_REQUIRE(ctas < (1ll << 31), BMA_ERR_LIMIT);
-  if (wide) heads_kernel<T, Bits16<T>::n, 1, 2, KIND><<<(unsigned)ctas, kHeadsThreads, 0, st>>>(p);
-  else heads_kernel<T, 1, 4, 1, KIND><<<(unsigned)ctas, kHeadsThreads, 0, st>>>(p);
+  if (wide) {
+    ctas = std::min<int64_t>(ctas, (int64_t)sms() * kHeadsCtas);
+    const bool full = r.dim == p.d;
+#define BMA_WIDE(LAYOUT, FULL) heads_wide_kernel<T, LAYOUT, FULL, KIND><<<(unsigned)ctas, kHeadsThreads, 0, st>>>(p)
+    if (r.layout == BMA_ROTARY_HALF) { if (full) BMA_WIDE(BMA_ROTARY_HALF, true); else BMA_WIDE(BMA_ROTARY_HALF, false); }
+    else { if (full) BMA_WIDE(BMA_ROTARY_INTERLEAVED, true); else BMA_WIDE(BMA_ROTARY_INTERLEAVED, false); }
+#undef BMA_WIDE
+  } else heads_kernel<T, 1, 4, 1, KIND><<<(unsigned)ctas, kHeadsThreads, 0, st>>>(p);
   count_launches(1);
   BMA_CUDA_TRY(cudaGetLastError());
   return BMA_OK;
@@ -693,13 +1045,18 @@ int rotate_backward(const bma_rotate_args* a, void* workspace, size_t bytes, cud
     const bool wide = fits && (!qn || q_wide) && (!kn || k_wide);
     p.map = head_map(a->rotary, a->d, wide ? vec : 1, 1);
     const unsigned ctas = (unsigned)(p.q_ctas + k_ctas);
-    if (dtype == BMA_DTYPE_F32) {
-      if (wide) rotate_back_kernel<float, 4, 1><<<ctas, kHeadsThreads, 0, st>>>(p);
-      else rotate_back_kernel<float, 1, 4><<<ctas, kHeadsThreads, 0, st>>>(p);
-    } else {
-      if (wide) rotate_back_kernel<__nv_bfloat16, 8, 1><<<ctas, kHeadsThreads, 0, st>>>(p);
-      else rotate_back_kernel<__nv_bfloat16, 1, 4><<<ctas, kHeadsThreads, 0, st>>>(p);
-    }
+    const bool full = a->rotary.dim == a->d, half = a->rotary.layout == BMA_ROTARY_HALF;
+#define BMA_BACK(T)                                                                                                       \
+  do {                                                                                                                    \
+    if (!wide) rotate_back_kernel<T, 1, 4><<<ctas, kHeadsThreads, 0, st>>>(p);                                            \
+    else if (half && full) rotate_back_wide_kernel<T, BMA_ROTARY_HALF, true><<<ctas, kHeadsThreads, 0, st>>>(p);          \
+    else if (half) rotate_back_wide_kernel<T, BMA_ROTARY_HALF, false><<<ctas, kHeadsThreads, 0, st>>>(p);                 \
+    else if (full) rotate_back_wide_kernel<T, BMA_ROTARY_INTERLEAVED, true><<<ctas, kHeadsThreads, 0, st>>>(p);           \
+    else rotate_back_wide_kernel<T, BMA_ROTARY_INTERLEAVED, false><<<ctas, kHeadsThreads, 0, st>>>(p);                    \
+  } while (0)
+    if (dtype == BMA_DTYPE_F32) BMA_BACK(float);
+    else BMA_BACK(__nv_bfloat16);
+#undef BMA_BACK
     weight_sum_kernel<<<dim3(ceil_div(a->d, 32), 2), dim3(32, 32), 0, st>>>(p.partial, p.q_ctas, k_ctas, a->d, a->dq_weight, a->dk_weight, a->rotary.weight_dtype);
     count_launches(2);
     BMA_CUDA_TRY(cudaGetLastError());
