@@ -20,7 +20,7 @@ namespace bma {
 namespace {
 
 constexpr int kHeadsThreads = 128, kHeadsWarps = kHeadsThreads / 32;
-constexpr int kHeadsCtas = 20;      // at most so many CTAs to an SM, each over its share of the tokens (four waves)
+constexpr int kHeadsCtas = 8;       // at most so many CTAs to an SM, each over its share of the tokens (two waves)
 
 template <typename T> struct Bits16;   // values of a 16-byte chunk
 template <> struct Bits16<float> { static constexpr int n = 4; };
@@ -148,6 +148,7 @@ struct Side {
   const void* weight;
   int heads;
   int turned;
+  int before;            // heads of the sides before
 };
 
 struct HeadsParams {
@@ -550,50 +551,132 @@ __device__ __forceinline__ uint32_t live_pairs(int u, int pairs) {
   return (1u << n) - 1u;
 }
 
+// The rows ahead of a warp: the heads of a token that it takes at once, item by item and side by side as it will come to them.  Each lane copies its own
+// 32 bytes of them into its own place in shared memory, where it alone reads them: kAhead rows are on their way without a register or a barrier.
+constexpr int kAhead = 4;      // (a power of two)
+template <typename T, int KIND>
+struct RowsAhead {
+  static constexpr int kSides = KIND == kRotate ? 2 : 3;
+  int item, items, stride;           // items of this warp: item, item + stride, ...
+  int b, t, begin;                   // its token, first head
+  int si, h, hi;                     // next rows: heads h + group below hi of side si
+  const T* at;                       // this lane's head of them
+  int64_t step;                      // to the next rows
+  int to;
+  bool real;
+
+  __device__ __forceinline__ void start(const HeadsParams& p, int first, int all, int by, int group, int groups) {
+    item = first;
+    items = all;
+    stride = by;
+    to = 0;
+    h = hi = 0;
+    if (open(p)) next(p, group, groups);
+  }
+  __device__ __forceinline__ bool open(const HeadsParams& p) {
+    if (item >= items) return false;
+    const int token = p.slabs == 1 ? item : item / p.slabs;
+    begin = (item - token * p.slabs) * p.slab_heads;
+    b = token / p.L;
+    t = token - b * p.L;
+    real = KIND == kRotate || t < new_tokens(p.lengths, p.new_lengths, b, p.L).count;
+    si = -1;
+    return true;
+  }
+  // To the next side that has rows; item >= items: there is none.
+  __device__ __forceinline__ void next(const HeadsParams& p, int group, int groups) {
+    do {
+      while (real && ++si < kSides) {
+        const Side& side = p.side[si];
+        h = max(begin - side.before, 0);
+        hi = min(begin + p.slab_heads - side.before, side.heads);
+        if (h >= hi) continue;
+        at = static_cast<const T*>(side.in.ptr) + b * side.in.stride_b + t * side.in.stride_l + (h + group) * side.in.stride_h;
+        step = groups * side.in.stride_h;
+        return;
+      }
+      item += stride;
+    } while (open(p));
+  }
+  // Asks for the next rows, if there are any.  `ring`: the shared address of this lane's place, 2 * kAhead chunks, 512 bytes apart; A, B: it has chunks a and b.
+  __device__ __forceinline__ void fetch(const HeadsParams& p, uint32_t ring, int group, int groups, int ca, int cb, bool A, bool B) {
+    constexpr int VEC = Bits16<T>::n;
+    if (item < items) {
+      const bool there = h + group < hi;
+      const uint32_t dst = ring + to * 1024;
+      if (there && A) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(at + ca * VEC) : "memory");
+      if (there && B) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + 512), "l"(at + cb * VEC) : "memory");
+      to = (to + 1) & (kAhead - 1);
+      at += step;
+      h += groups;
+      if (h >= hi) next(p, group, groups);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+};
+
 // The same work as heads_kernel's.  FULL: every component is rotated.
 template <typename T, int LAYOUT, bool FULL, int KIND>
-__global__ void __launch_bounds__(kHeadsThreads) heads_wide_kernel(const __grid_constant__ HeadsParams p) {
-  constexpr int VEC = Bits16<T>::n, NR = 2;
+__global__ void __launch_bounds__(kHeadsThreads, 4) heads_wide_kernel(const __grid_constant__ HeadsParams p) {
+  constexpr int VEC = Bits16<T>::n;
   constexpr bool HALF = LAYOUT == BMA_ROTARY_HALF;
   __shared__ unsigned long long steps[kPairs];
   __shared__ float2 turns[kHeadsWarps][kPairs];
+  __shared__ uint4 rings[kHeadsWarps][kAhead][2][32];
+  __shared__ __align__(16) float weights[2][2 * kPairs];
   __shared__ float rows[KIND == kAppend4 ? kHeadsWarps : 1][KIND == kAppend4 ? 8 : 1][KIND == kAppend4 ? kPagedHeadDim + 4 : 1];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int tpr = p.map.tpr, group = lane / tpr, u = lane & (tpr - 1), groups = 32 / tpr, chunks = p.map.chunks;
   const int pairs = p.map.dim / 2;
-  make_steps(steps, p.frequencies, pairs);
   int ca, cb;
   unit_chunks<VEC>(p.map, u, ca, cb);
   const uint32_t live = live_pairs<VEC>(u, pairs);
   const float inv_d = 1.f / (float)p.d;
-  const int64_t items = (int64_t)p.B * p.L * p.slabs;
+  const bool A = ca < chunks, B = cb < chunks;
+  const int items = p.B * p.L * p.slabs, first_item = blockIdx.x * kHeadsWarps + warp, stride = gridDim.x * kHeadsWarps;      // (below 2^31: launch_heads)
+  uint4* ring = &rings[warp][0][0][lane];
+  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+  RowsAhead<T, KIND> ahead;
+  ahead.start(p, first_item, items, stride, group, groups);
+#pragma unroll
+  for (int i = 0; i < kAhead - 1; ++i) ahead.fetch(p, ring_at, group, groups, ca, cb, A, B);
+  for (int i = threadIdx.x; i < 2 * p.d; i += kHeadsThreads) {
+    const int si = i >= p.d, k = i - si * p.d;
+    const void* w = p.side[si].weight;
+    weights[si][k] = !w ? 1.f : p.weight_dtype == BMA_DTYPE_F32 ? __ldg(static_cast<const float*>(w) + k) : __bfloat162float(static_cast<const __nv_bfloat16*>(w)[k]);
+  }
+  make_steps(steps, p.frequencies, pairs);
+  int from = 0;
 #pragma unroll 1
-  for (int64_t item = (int64_t)blockIdx.x * kHeadsWarps + warp; item < items; item += (int64_t)gridDim.x * kHeadsWarps) {
-    const int64_t token = item / p.slabs;
-    const int slab = (int)(item - token * p.slabs);
-    const int b = (int)(token / p.L), t = (int)(token - (int64_t)b * p.L);
+  for (int item = first_item; item < items; item += stride) {
+    const int token = p.slabs == 1 ? item : item / p.slabs;
+    const int slab_begin = (item - token * p.slabs) * p.slab_heads, slab_end = slab_begin + p.slab_heads;
+    const int b = token / p.L, t = token - b * p.L;
     long long position = t;
     bool real = true;
     int64_t held = 0, held_scale = 0;      // offsets of the token in the cache
     if constexpr (KIND == kRotate) position = position_of(p, b, t);
     else real = token_place(p, b, t, lane, position, held, held_scale);
     if (pairs && real) make_turns(turns[warp], steps, pairs, position, p.back ? -p.magnitude : p.magnitude, lane);
-    const int slab_begin = slab * p.slab_heads, slab_end = slab_begin + p.slab_heads;
-    int first = 0;      // heads of the sides before
 #pragma unroll 1
     for (int si = 0; si < (KIND == kRotate ? 2 : 3); ++si) {
       const Side& side = p.side[si];
-      const int lo = max(slab_begin - first, 0), hi = min(slab_end - first, side.heads);
-      first += side.heads;
+      const int lo = max(slab_begin - side.before, 0), hi = min(slab_end - side.before, side.heads);
       if (lo >= hi) continue;
       const bool cached = KIND != kRotate && si > 0;
-      if (cached && (!real || held < 0)) continue;
-      const T* in = static_cast<const T*>(side.in.ptr) + b * side.in.stride_b + t * side.in.stride_l;
       T* out = static_cast<T*>(side.out.ptr) + b * side.out.stride_b + t * side.out.stride_l;
       int64_t out_head = side.out.stride_h;
       if (cached) {
         out = static_cast<T*>(si == 1 ? p.cache.k : p.cache.v) + held;      // (a 4-bit cache is not written through this)
         out_head = p.cache.stride_head;
+      }
+      out += (lo + group) * out_head;
+      if (KIND != kRotate && !real) {       // zeros for queries of tokens that are not real
+        Unit<T> zero;
+        zero.zero();
+        if (!cached)
+          for (int h = lo + group; h < hi; h += groups, out += groups * out_head) zero.store(out, ca, cb, chunks);
+        continue;
       }
       const bool normed = side.weight != nullptr, plain = !normed && !side.turned;
       // out = v * F + (the other half of the pair) * G
@@ -603,20 +686,17 @@ __global__ void __launch_bounds__(kHeadsThreads) heads_wide_kernel(const __grid_
 #pragma unroll
         for (int i = 0; i < VEC; ++i) w[i] = make_float2(1.f, 1.f);
         if (normed) {
-          float wa[VEC], wb[VEC];
-          load_weight<VEC>(side.weight, p.weight_dtype, ca, chunks, wa);
-          load_weight<VEC>(side.weight, p.weight_dtype, cb, chunks, wb);
 #pragma unroll
           for (int i = 0; i < VEC / 2; ++i) {
-            w[i] = make_float2(wa[2 * i], wa[2 * i + 1]);
-            w[VEC / 2 + i] = make_float2(wb[2 * i], wb[2 * i + 1]);
+            if (A) w[i] = *reinterpret_cast<const float2*>(&weights[si][ca * VEC + 2 * i]);
+            if (B) w[VEC / 2 + i] = *reinterpret_cast<const float2*>(&weights[si][cb * VEC + 2 * i]);
           }
         }
         float2 cs[VEC];
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
           cs[j] = make_float2(1.f, 0.f);
-          if (side.turned && (FULL || live >> j & 1) && real && u * VEC + j < pairs) cs[j] = turns[warp][u * VEC + j];
+          if (side.turned && (FULL || live >> j & 1) && u * VEC + j < pairs) cs[j] = turns[warp][u * VEC + j];
           if (p.back) cs[j].x = (FULL || live >> j & 1) ? -cs[j].x : cs[j].x;      // (-magnitude gave -cos and -sin)
         }
         if constexpr (HALF) {
@@ -636,62 +716,58 @@ __global__ void __launch_bounds__(kHeadsThreads) heads_wide_kernel(const __grid_
           }
         }
       }
+      const int64_t out_step = groups * out_head;
 #pragma unroll 1
-      for (int h0 = lo; h0 < hi; h0 += groups * NR) {
-        Unit<T> x[NR];
+      for (int h = lo + group; h - group < hi; h += groups, out += out_step) {
+        ahead.fetch(p, ring_at, group, groups, ca, cb, A, B);
+        asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+        Unit<T> x;
+        x.zero();
+        if (h < hi && A) x.a = ring[from * 64];
+        if (h < hi && B) x.b = ring[from * 64 + 32];
+        from = (from + 1) & (kAhead - 1);
+        float2 v[VEC];
+        if (!plain || KIND == kAppend4) x.get(v);
+        if (!plain) {
+          float2 o[VEC];
 #pragma unroll
-        for (int r = 0; r < NR; ++r) {
-          const int h = h0 + r * groups + group;
-          if (h < hi && real) x[r].load(in + h * side.in.stride_h, ca, cb, chunks);
-          else x[r].zero();
-        }
+          for (int i = 0; i < VEC; ++i) {
+            float2 other = HALF ? v[(i + VEC / 2) % VEC] : swapped(v[i]);
+            // what is not rotated takes nothing of its neighbour, not even a zero times infinity
+            if (!FULL && !(HALF ? live != 0 : live >> i & 1)) other = make_float2(0.f, 0.f);
+            o[i] = __ffma2_rn(v[i], F[i], __fmul2_rn(other, G[i]));
+          }
+          if (normed) {
+            float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int r = 0; r < NR; ++r) {
-          const int h = h0 + r * groups + group;
-          float2 v[VEC];
-          if (!plain || KIND == kAppend4) x[r].get(v);
-          if (!plain) {
-            float2 o[VEC];
+            for (int i = 0; i < VEC; ++i) sum = __ffma2_rn(v[i], v[i], sum);
+            const float2 inv = twice(rsqrtf(group_sum(sum.x + sum.y, tpr) * inv_d + p.eps));
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-              float2 other = HALF ? v[(i + VEC / 2) % VEC] : swapped(v[i]);
-              // what is not rotated takes nothing of its neighbour, not even a zero times infinity
-              if (!FULL && !(HALF ? live != 0 : live >> i & 1)) other = make_float2(0.f, 0.f);
-              o[i] = __ffma2_rn(v[i], F[i], __fmul2_rn(other, G[i]));
-            }
-            if (normed) {
-              float2 sum = make_float2(0.f, 0.f);
-#pragma unroll
-              for (int i = 0; i < VEC; ++i) sum = __ffma2_rn(v[i], v[i], sum);
-              const float2 inv = twice(rsqrtf(group_sum(sum.x + sum.y, tpr) * inv_d + p.eps));
-#pragma unroll
-              for (int i = 0; i < VEC; ++i) o[i] = __fmul2_rn(o[i], inv);
-            }
-            if (KIND == kAppend4 && cached) {
-#pragma unroll
-              for (int i = 0; i < VEC; ++i) v[i] = o[i];
-            } else x[r].set(o);
+            for (int i = 0; i < VEC; ++i) o[i] = __fmul2_rn(o[i], inv);
           }
           if (KIND == kAppend4 && cached) {
-            float* row = rows[warp][group];
-            __syncwarp();
 #pragma unroll
-            for (int i = 0; i < VEC / 2; ++i) {
-              if (ca < chunks) *reinterpret_cast<float2*>(row + ca * VEC + 2 * i) = v[i];
-              if (cb < chunks) *reinterpret_cast<float2*>(row + cb * VEC + 2 * i) = v[VEC / 2 + i];
-            }
-            __syncwarp();
-            uint8_t* codes = static_cast<uint8_t*>(si == 1 ? p.cache.k : p.cache.v) + held + h * p.cache.stride_head;
-            uint8_t* scales = (si == 1 ? p.cache.k_scale : p.cache.v_scale) + held_scale + h * p.cache.scale_stride_head;
-            store_4bit(row, h < hi, p.d, tpr, u, codes, scales);
-          } else if (h < hi) {
-            if (!real) x[r].zero();
-            x[r].store(out + h * out_head, ca, cb, chunks);
-          }
+            for (int i = 0; i < VEC; ++i) v[i] = o[i];
+          } else x.set(o);
         }
+        if (KIND != kRotate && cached && held < 0) continue;
+        if (KIND == kAppend4 && cached) {
+          float* row = rows[warp][group];
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < VEC / 2; ++i) {
+            if (ca < chunks) *reinterpret_cast<float2*>(row + ca * VEC + 2 * i) = v[i];
+            if (cb < chunks) *reinterpret_cast<float2*>(row + cb * VEC + 2 * i) = v[VEC / 2 + i];
+          }
+          __syncwarp();
+          uint8_t* codes = static_cast<uint8_t*>(si == 1 ? p.cache.k : p.cache.v) + held + h * p.cache.stride_head;
+          uint8_t* scales = (si == 1 ? p.cache.k_scale : p.cache.v_scale) + held_scale + h * p.cache.scale_stride_head;
+          store_4bit(row, h < hi, p.d, tpr, u, codes, scales);
+        } else if (h < hi) x.store(out, ca, cb, chunks);
       }
     }
   }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 // The same work as rotate_back_kernel's.
@@ -728,10 +804,10 @@ __global__ void __launch_bounds__(kHeadsThreads, 4) rotate_back_wide_kernel(cons
 #pragma unroll
     for (int i = 0; i < VEC; ++i) dw[i] = make_float2(0.f, 0.f);
   }
-  const int64_t tokens = (int64_t)p.B * p.L;
+  const int tokens = p.B * p.L;
 #pragma unroll 1
-  for (int64_t token = (int64_t)cta * kHeadsWarps + warp; token < tokens; token += (int64_t)ctas * kHeadsWarps) {
-    const int b = (int)(token / p.L), t = (int)(token - (int64_t)b * p.L);
+  for (int token = cta * kHeadsWarps + warp; token < tokens; token += ctas * kHeadsWarps) {
+    const int b = token / p.L, t = token - b * p.L;
     // cosines and sines of the unit's values: HALF, of pairs 2i and 2i + 1; else of both values of pair i, the sine with its sign
     float2 c[CS], s[CS];
     if (pairs) make_turns(turns[warp], steps, pairs, position_of(p, b, t), p.magnitude, lane);
@@ -939,8 +1015,10 @@ int launch_heads(HeadsParams& p, const bma_rotary& r, bool wide, cudaStream_t st
   const int64_t tokens = (int64_t)p.B * p.L;
   const int heads = p.side[0].heads + p.side[1].heads + p.side[2].heads;
   cut_heads(p, tokens, heads, 32 / p.map.tpr);
+  p.side[1].before = p.side[0].heads;
+  p.side[2].before = p.side[0].heads + p.side[1].heads;
+  BMA_REQUIRE(tokens * p.slabs < (1ll << 30), BMA_ERR_LIMIT);
   int64_t ctas = (tokens * p.slabs + kHeadsWarps - 1) / kHeadsWarps;
-  BMA_REQUIRE(ctas < (1ll << 31), BMA_ERR_LIMIT);
   if (wide) {
     ctas = std::min<int64_t>(ctas, (int64_t)sms() * kHeadsCtas);
     const bool full = r.dim == p.d;
@@ -1000,7 +1078,7 @@ int rotate_forward(const bma_rotate_args* a, cudaStream_t st) {
   if ((rc = validate_heads(a->q, a->q.dtype)) || (rc = validate_heads(a->q_out, a->q.dtype))) return rc;
   if (a->Hkv && ((rc = validate_heads(a->k, a->q.dtype)) || (rc = validate_heads(a->k_out, a->q.dtype)))) return rc;
   HeadsParams p = rotate_params(*a);
-  p.side[0] = {a->q, a->q_out, a->rotary.q_weight, a->Hq, 1};
+  p.side[0] = {a->q, a->q_out, a->rotary.q_weight, a->Hq, 1, 0};
   p.side[1] = {a->k, a->k_out, a->rotary.k_weight, a->Hkv, 1};
   const int vec = a->q.dtype == BMA_DTYPE_F32 ? 4 : 8;
   const bool wide = wide_heads(a->rotary, a->d, vec) && wide_tensor(a->q, vec) && wide_tensor(a->q_out, vec) &&
@@ -1042,6 +1120,7 @@ int rotate_backward(const bma_rotate_args* a, void* workspace, size_t bytes, cud
     p.partial = static_cast<float*>(workspace);
     int k_ctas;
     back_ctas(*a, p.q_ctas, k_ctas);
+    BMA_REQUIRE((int64_t)a->B * a->L < (1ll << 30), BMA_ERR_LIMIT);
     const bool wide = fits && (!qn || q_wide) && (!kn || k_wide);
     p.map = head_map(a->rotary, a->d, wide ? vec : 1, 1);
     const unsigned ctas = (unsigned)(p.q_ctas + k_ctas);
@@ -1086,7 +1165,7 @@ int append_kv(const bma_paged_cache* c, const bma_append_args* a, cudaStream_t s
   p.frequencies = a->rotary.frequencies;
   p.magnitude = a->rotary.magnitude; p.eps = a->rotary.eps;
   p.weight_dtype = a->rotary.weight_dtype;
-  p.side[0] = {a->q, a->q_out, a->rotary.q_weight, a->Hq, 1};
+  p.side[0] = {a->q, a->q_out, a->rotary.q_weight, a->Hq, 1, 0};
   p.side[1] = {a->k, {}, a->rotary.k_weight, c->Hkv, 1};
   p.side[2] = {a->v, {}, nullptr, c->Hkv, 0};
   p.cache = *c;
