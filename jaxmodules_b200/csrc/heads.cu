@@ -778,7 +778,7 @@ __global__ void __launch_bounds__(kHeadsThreads, 4) rotate_back_wide_kernel(cons
   constexpr int CS = HALF ? VEC / 2 : VEC;
   __shared__ unsigned long long steps[kPairs];
   __shared__ float2 turns[kHeadsWarps][kPairs];
-  __shared__ float sums[kHeadsWarps][256];
+  __shared__ uint4 rings[kHeadsWarps][kAhead][4][32];       // (the sums of the warps lie there at the end)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int tpr = p.map.tpr, group = lane / tpr, u = lane & (tpr - 1), groups = 32 / tpr, chunks = p.map.chunks;
   const int si = (int)blockIdx.x < p.q_ctas ? 0 : 1;
@@ -786,11 +786,55 @@ __global__ void __launch_bounds__(kHeadsThreads, 4) rotate_back_wide_kernel(cons
   const Side& side = p.side[si];
   const bma_tensor& g = p.g[si];
   const float inv_d = 1.f / (float)p.d;
-  const int pairs = p.map.dim / 2;
-  make_steps(steps, p.frequencies, pairs);
+  const int pairs = p.map.dim / 2, heads = side.heads;
   int ca, cb;
   unit_chunks<VEC>(p.map, u, ca, cb);
+  const bool A = ca < chunks, B = cb < chunks;
   const uint32_t live = live_pairs<VEC>(u, pairs);
+  const int tokens = p.B * p.L, stride = ctas * kHeadsWarps;       // (below 2^30: rotate_backward)
+
+  // rows on their way, as in RowsAhead: four chunks, of x and of the cotangent
+  uint4* ring = &rings[warp][0][0][lane];
+  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+  const int64_t x_step = groups * side.in.stride_h, g_step = groups * g.stride_h;
+  const T *ax = nullptr, *ag = nullptr;
+  int next_token = cta * kHeadsWarps + warp, next_head = 0, to = 0;
+  auto open = [&] {
+    if (next_token >= tokens) return;
+    const int b = next_token / p.L, t = next_token - b * p.L;
+    ax = static_cast<const T*>(side.in.ptr) + b * side.in.stride_b + t * side.in.stride_l + group * side.in.stride_h;
+    ag = static_cast<const T*>(g.ptr) + b * g.stride_b + t * g.stride_l + group * g.stride_h;
+  };
+  auto fetch = [&] {
+    if (next_token < tokens) {
+      const uint32_t dst = ring_at + to * 2048;
+      if (next_head + group < heads) {
+        if (A) {
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(ax + ca * VEC) : "memory");
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + 1024), "l"(ag + ca * VEC) : "memory");
+        }
+        if (B) {
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + 512), "l"(ax + cb * VEC) : "memory");
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + 1536), "l"(ag + cb * VEC) : "memory");
+        }
+      }
+      to = (to + 1) & (kAhead - 1);
+      ax += x_step;
+      ag += g_step;
+      next_head += groups;
+      if (next_head >= heads) {
+        next_head = 0;
+        next_token += stride;
+        open();
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  open();
+#pragma unroll
+  for (int i = 0; i < kAhead - 1; ++i) fetch();
+  make_steps(steps, p.frequencies, pairs);
+
   float2 w[VEC], dw[VEC];
   {
     float wa[VEC], wb[VEC];
@@ -804,12 +848,13 @@ __global__ void __launch_bounds__(kHeadsThreads, 4) rotate_back_wide_kernel(cons
 #pragma unroll
     for (int i = 0; i < VEC; ++i) dw[i] = make_float2(0.f, 0.f);
   }
-  const int tokens = p.B * p.L;
+  int from = 0;
 #pragma unroll 1
-  for (int token = cta * kHeadsWarps + warp; token < tokens; token += ctas * kHeadsWarps) {
+  for (int token = cta * kHeadsWarps + warp; token < tokens; token += stride) {
     const int b = token / p.L, t = token - b * p.L;
-    // cosines and sines of the unit's values: HALF, of pairs 2i and 2i + 1; else of both values of pair i, the sine with its sign
-    float2 c[CS], s[CS];
+    // cosines and sines of the unit's values: HALF, of pairs 2i and 2i + 1 and the sines with the other sign, too; else of both values of pair i, the sine
+    // with its sign
+    float2 c[CS], s[CS], ns[CS];
     if (pairs) make_turns(turns[warp], steps, pairs, position_of(p, b, t), p.magnitude, lane);
 #pragma unroll
     for (int i = 0; i < CS; ++i) {
@@ -818,27 +863,26 @@ __global__ void __launch_bounds__(kHeadsThreads, 4) rotate_back_wide_kernel(cons
         const float2 x = at(2 * i), y = at(2 * i + 1);
         c[i] = make_float2(x.x, y.x);
         s[i] = make_float2(x.y, y.y);
+        ns[i] = make_float2(-x.y, -y.y);
       } else {
         const float2 x = at(i);
         c[i] = twice(x.x);
         s[i] = make_float2(x.y, -x.y);
       }
     }
-    const T* in = static_cast<const T*>(side.in.ptr) + b * side.in.stride_b + t * side.in.stride_l;
-    const T* gin = static_cast<const T*>(g.ptr) + b * g.stride_b + t * g.stride_l;
-    T* out = static_cast<T*>(side.out.ptr) + b * side.out.stride_b + t * side.out.stride_l;
+    T* out = static_cast<T*>(side.out.ptr) + b * side.out.stride_b + t * side.out.stride_l + group * side.out.stride_h;
+    const int64_t out_step = groups * side.out.stride_h;
 #pragma unroll 1
-    for (int h0 = 0; h0 < side.heads; h0 += groups) {
-      const int h = h0 + group;
-      const bool there = h < side.heads;
+    for (int h = group; h - group < heads; h += groups, out += out_step) {
+      fetch();
+      asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+      const bool there = h < heads;
       Unit<T> x, y;
-      if (there) {
-        x.load(in + h * side.in.stride_h, ca, cb, chunks);
-        y.load(gin + h * g.stride_h, ca, cb, chunks);
-      } else {
-        x.zero();
-        y.zero();
-      }
+      x.zero();
+      y.zero();
+      if (there && A) { x.a = ring[from * 128]; y.a = ring[from * 128 + 64]; }
+      if (there && B) { x.b = ring[from * 128 + 32]; y.b = ring[from * 128 + 96]; }
+      from = (from + 1) & (kAhead - 1);
       float2 v[VEC], e[VEC], f[VEC];
       x.get(v);
       y.get(e);
@@ -849,12 +893,13 @@ __global__ void __launch_bounds__(kHeadsThreads, 4) rotate_back_wide_kernel(cons
         if (!FULL && !(HALF ? live != 0 : live >> i & 1)) other = make_float2(0.f, 0.f);
         if constexpr (HALF) {
           const int k = i % (VEC / 2);
-          f[i] = __ffma2_rn(e[i], c[k], __fmul2_rn(other, i < VEC / 2 ? s[k] : make_float2(-s[k].x, -s[k].y)));
+          f[i] = __ffma2_rn(e[i], c[k], __fmul2_rn(other, i < VEC / 2 ? s[k] : ns[k]));
         } else f[i] = __ffma2_rn(e[i], c[i], __fmul2_rn(other, s[i]));
       }
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
         e[i] = __fmul2_rn(f[i], v[i]);                 // g' x
+        f[i] = __fmul2_rn(f[i], w[i]);
         sum = __ffma2_rn(v[i], v[i], sum);
         dot = __ffma2_rn(e[i], w[i], dot);
       }
@@ -863,19 +908,22 @@ __global__ void __launch_bounds__(kHeadsThreads, 4) rotate_back_wide_kernel(cons
         sum1 += __shfl_xor_sync(0xffffffffu, sum1, o);
         dot1 += __shfl_xor_sync(0xffffffffu, dot1, o);
       }
-      const float inv = rsqrtf(sum1 * inv_d + p.eps);
+      const float inv = there ? rsqrtf(sum1 * inv_d + p.eps) : 0.f;
       const float2 inv2 = twice(inv), m = twice(-(dot1 * inv * inv_d) * inv * inv);    // -inv^2 mean(g' w x^)
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        if (there) dw[i] = __ffma2_rn(e[i], inv2, dw[i]);
-        f[i] = __ffma2_rn(v[i], m, __fmul2_rn(__fmul2_rn(f[i], w[i]), inv2));
+        dw[i] = __ffma2_rn(e[i], inv2, dw[i]);
+        f[i] = __ffma2_rn(v[i], m, __fmul2_rn(f[i], inv2));
       }
       if (there) {
         y.set(f);
-        y.store(out + h * side.out.stride_h, ca, cb, chunks);
+        y.store(out, ca, cb, chunks);
       }
     }
   }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();
+  float (*sums)[256] = reinterpret_cast<float (*)[256]>(&rings[0][0][0][0]);
   // the groups of a warp, the warps of the CTA
 #pragma unroll
   for (int i = 0; i < VEC; ++i) {

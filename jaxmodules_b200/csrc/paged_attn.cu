@@ -1001,34 +1001,54 @@ __global__ void __launch_bounds__(kThreads, Core::kMinCtas) paged_kernel(const _
   copies_awaited<0>();
 }
 
-// One warp: a row of an item that several CTAs had parts of.
+// One CTA: a row of an item that several CTAs had parts of, its warps taking parts in turn.
 template <int DP, int ROWS>
 __global__ void __launch_bounds__(kThreads) paged_join_kernel(const __grid_constant__ PagedParams p) {
+  __shared__ float4 sums[kWarps][DP / 4];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int4 m = p.meta[blockIdx.x];
   if (m.x < 0) return;
-  const int lane = threadIdx.x & 31, row = blockIdx.y * kWarps + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.y;
   const int b = m.x / p.row_tiles, row0 = (m.x - b * p.row_tiles) * ROWS;
   if (row >= min(ROWS, p.rows - row0)) return;
   const int parts = m.w - blockIdx.x + 1;
-  auto slot = [&](int i) { return ((int64_t)(i == 0 ? m.z : 2 * (blockIdx.x + i))) * ROWS + row; };
+  auto slot = [&](int i) { return (int64_t)(i == 0 ? m.z : 2 * (blockIdx.x + i)) * ROWS + row; };
   float top = -INFINITY;
   for (int i = lane; i < parts; i += 32) top = fmaxf(top, p.part_ml[slot(i)].x);
+#pragma unroll
   for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   const float base = top == -INFINITY ? 0.f : top;
-  float x[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
-  if (lane * 4 >= DP) return;
-#pragma unroll 4
-  for (int i = 0; i < parts; ++i) {
-    const int64_t at = slot(i);
-    const float2 ml = p.part_ml[at];
-    const float f = exp2_approx(ml.x - base);
-    sum = fmaf(ml.y, f, sum);
-    const float4 y = *reinterpret_cast<const float4*>(p.part_o + at * DP + lane * 4);
-    x[0] = fmaf(y.x, f, x[0]); x[1] = fmaf(y.y, f, x[1]); x[2] = fmaf(y.z, f, x[2]); x[3] = fmaf(y.w, f, x[3]);
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+  float sum = 0.f;
+  for (int i0 = 0; i0 < parts; i0 += 32) {
+    float f = 0.f;                       // of part i0 + lane
+    if (i0 + lane < parts) {
+      const float2 ml = p.part_ml[slot(i0 + lane)];
+      f = exp2_approx(ml.x - base);
+      sum = fmaf(ml.y, f, sum);
+    }
+#pragma unroll
+    for (int k = 0; k < 32; k += kWarps) {
+      const int i = i0 + k + warp;
+      const float fi = __shfl_sync(0xffffffffu, f, k + warp);
+      if (i < parts && lane * 4 < DP) {
+        const float4 y = *reinterpret_cast<const float4*>(p.part_o + slot(i) * DP + lane * 4);
+        x.x = fmaf(y.x, fi, x.x); x.y = fmaf(y.y, fi, x.y); x.z = fmaf(y.z, fi, x.z); x.w = fmaf(y.w, fi, x.w);
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane * 4 < DP) sums[warp][lane] = x;
+  __syncthreads();
+  if (warp || lane * 4 >= DP) return;
+#pragma unroll
+  for (int w = 1; w < kWarps; ++w) {
+    const float4 y = sums[w][lane];
+    x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
   }
   const bool real = (row0 + row) / p.G < new_tokens(p.a.lengths, p.a.new_lengths, b, p.a.T).count;
-  write_result(p, b, m.y, row0 + row, real, lane * 4, make_float4(x[0], x[1], x[2], x[3]), top, sum);
+  write_result(p, b, m.y, row0 + row, real, lane * 4, x, top, sum);
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------
@@ -1079,7 +1099,7 @@ int launch_paged(const PagedParams& p, const PagedLaunch& l, cudaStream_t st) {
   paged_kernel<Core><<<l.ctas, kThreads, smem, st>>>(p);
   BMA_CUDA_TRY(cudaGetLastError());
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(l.ctas, ceil_div(std::min(Core::kRows, p.rows), kWarps));
+  cfg.gridDim = dim3(l.ctas, std::min(Core::kRows, p.rows));
   cfg.blockDim = dim3(kThreads);
   cfg.stream = st;
   cudaLaunchAttribute attr{};
