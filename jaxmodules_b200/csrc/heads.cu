@@ -1015,12 +1015,6 @@ __global__ void __launch_bounds__(256) read_kv_kernel(const __grid_constant__ bm
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------
-int sms() {
-  int dev = 0, n = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-  return n;
-}
-
 int validate_rotary(const bma_rotary& r, int d) {
   BMA_REQUIRE(r.dim >= 0 && r.dim % 2 == 0 && r.dim <= d, BMA_ERR_ARG);
   BMA_REQUIRE(r.dim == 0 || r.frequencies, BMA_ERR_ARG);
@@ -1050,7 +1044,7 @@ HeadMap head_map(const bma_rotary& r, int d, int vec, int least) {
 // Warps of a launch take a token and `slab_heads` of its heads: all of them where there are tokens enough for 16 warps an SM, fewer
 // (down to one pass of the warp) where there are not.
 void cut_heads(HeadsParams& p, int64_t tokens, int heads, int pass) {
-  const int64_t want = ceil_div(sms() * 16, (int)std::min<int64_t>(tokens, 1 << 20));
+  const int64_t want = ceil_div(device_sms(current_device()) * 16, (int)std::min<int64_t>(tokens, 1 << 20));
   p.slab_heads = (int)std::max<int64_t>(pass, ceil_div(heads, (int)want));
   p.slab_heads = ceil_div(p.slab_heads, pass) * pass;
   p.slabs = ceil_div(heads, p.slab_heads);
@@ -1068,7 +1062,7 @@ int launch_heads(HeadsParams& p, const bma_rotary& r, bool wide, cudaStream_t st
   BMA_REQUIRE(tokens * p.slabs < (1ll << 30), BMA_ERR_LIMIT);
   int64_t ctas = (tokens * p.slabs + kHeadsWarps - 1) / kHeadsWarps;
   if (wide) {
-    ctas = std::min<int64_t>(ctas, (int64_t)sms() * kHeadsCtas);
+    ctas = std::min<int64_t>(ctas, (int64_t)device_sms(current_device()) * kHeadsCtas);
     const bool full = r.dim == p.d;
 #define BMA_WIDE(LAYOUT, FULL) heads_wide_kernel<T, LAYOUT, FULL, KIND><<<(unsigned)ctas, kHeadsThreads, 0, st>>>(p)
     if (r.layout == BMA_ROTARY_HALF) { if (full) BMA_WIDE(BMA_ROTARY_HALF, true); else BMA_WIDE(BMA_ROTARY_HALF, false); }
@@ -1113,7 +1107,7 @@ void back_ctas(const bma_rotate_args& a, int& q, int& k) {
   const int hq = a.rotary.q_weight ? a.Hq : 0, hk = a.rotary.k_weight ? a.Hkv : 0;
   const int64_t tokens = (int64_t)a.B * a.L;
   const int64_t most = (tokens + kHeadsWarps - 1) / kHeadsWarps;
-  const int64_t all = (int64_t)sms() * 4;
+  const int64_t all = (int64_t)device_sms(current_device()) * 4;
   q = hq ? (int)std::max<int64_t>(1, std::min(most, all * hq / (hq + hk))) : 0;
   k = hk ? (int)std::max<int64_t>(1, std::min(most, all * hk / (hq + hk))) : 0;
 }

@@ -8,7 +8,10 @@
 #include <nvtx3/nvToolsExt.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/utils/pybind.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
 
 #include <algorithm>
 #include <cmath>
@@ -28,7 +31,7 @@ using OptTensor = std::optional<Tensor>;
   X(bma_mask_compile_workspace_bytes) X(bma_mask_compile) X(bma_attn_plan) X(bma_attn_bwd_plan) X(bma_attn_fwd_implies_lists) X(bma_attn_fwd_workspace_bytes) \
   X(bma_attn_fwd_uses_workspace) X(bma_attn_fwd_ws) X(bma_attn_f32_workspace_bytes) X(bma_attn_fwd_f32) X(bma_attn_bwd_f32) X(bma_attn_bwd_f32_o) X(bma_attn_bwd_preprocess)       \
   X(bma_attn_bwd_workspace_bytes) X(bma_attn_bwd_scratch_bytes) X(bma_attn_bwd_scratch_min_bytes) X(bma_attn_bwd) X(bma_attn_bwd_o) \
-  X(bma_rotate) X(bma_rotate_bwd_workspace_bytes) X(bma_rotate_bwd) X(bma_append_kv) X(bma_read_kv) X(bma_paged_attn_workspace_bytes) X(bma_paged_attn)
+  X(bma_error_string) X(bma_rotate) X(bma_rotate_bwd_workspace_bytes) X(bma_rotate_bwd) X(bma_append_kv) X(bma_read_kv) X(bma_paged_attn_workspace_bytes) X(bma_paged_attn)
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;
   BMA_FUNCTIONS(X)
@@ -264,7 +267,7 @@ std::tuple<Tensor, Tensor, Tensor> backward(const Tensor& q, const Tensor& k, co
 }
 
 // ---- heads and the paged cache ------------------------------------------------------------------------------------
-// These check their arguments here: a small call takes as long on the host as on the device.
+// These check their arguments and find their stream here: a small call takes as long on the host as on the device.
 int dtype_of(const Tensor& t, const char* name) {
   TORCH_CHECK_TYPE(t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16, name, " must be float32 or bfloat16, not ", t.scalar_type());
   return t.scalar_type() == at::kFloat ? BMA_DTYPE_F32 : BMA_DTYPE_BF16;
@@ -286,6 +289,21 @@ struct Devices {
     }
   }
 };
+
+// The device of a call, made current, and its stream there.
+struct Place {
+  c10::DeviceGuard guard;
+  bma_stream_t stream;
+  explicit Place(const Tensor& t) : guard(t.device()), stream(c10::impl::VirtualGuardImpl(at::kCUDA).getStream(t.device()).native_handle()) {}
+};
+
+bool wants_gradient(std::initializer_list<const Tensor*> tensors) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor* t : tensors)
+    if (t && t->requires_grad()) return true;
+  return false;
+}
+const Tensor* pointer(const OptTensor& t) { return t ? &*t : nullptr; }
 
 // [B, L, H, d] heads; copied only where the components of a head do not lie side by side
 Tensor heads_of(const Tensor& t, const char* name) {
@@ -354,14 +372,22 @@ bma_rotate_args rotate_args(Devices& on, const Tensor& q, const OptTensor& k, co
   return a;
 }
 
-std::tuple<Tensor, OptTensor> rotate(const Tensor& q_in, const OptTensor& k_in, const OptTensor& positions, const OptTensor& frequencies, int layout, double magnitude,
-                                     const OptTensor& q_weight, const OptTensor& k_weight, double eps, uintptr_t stream) {
+struct Rotation {
+  OptTensor positions, frequencies;
+  int layout;
+  double magnitude;
+  OptTensor q_weight, k_weight;
+  double eps;
+};
+
+std::tuple<Tensor, OptTensor> rotate_forward(const Tensor& q_in, const OptTensor& k_in, const Rotation& r, bool from_python) {
   const Tensor q = heads_of(q_in, "q");
   OptTensor k, k_out;
   if (k_in) k = heads_of(*k_in, "k");
   Devices on;
-  bma_rotate_args a = rotate_args(on, q, k, positions, frequencies, layout, magnitude, q_weight, k_weight, eps);
+  bma_rotate_args a = rotate_args(on, q, k, r.positions, r.frequencies, r.layout, r.magnitude, r.q_weight, r.k_weight, r.eps);
   on.check();
+  const Place place(q);
   const at::TensorOptions like = q.options().requires_grad(false);
   Tensor q_out = at::empty(q.sizes(), like);
   a.q = describe(q); a.q_out = describe(q_out);
@@ -370,18 +396,16 @@ std::tuple<Tensor, OptTensor> rotate(const Tensor& q_in, const OptTensor& k_in, 
     a.k = describe(*k); a.k_out = describe(*k_out);
   }
   int rc;
-  {
+  if (from_python) {
     Group group("bma.rotate");
-    rc = lib.bma_rotate(&a, reinterpret_cast<bma_stream_t>(stream));
-  }
-  check(rc, "bma_rotate");
+    rc = lib.bma_rotate(&a, place.stream);
+  } else rc = lib.bma_rotate(&a, place.stream);
+  TORCH_CHECK(rc == BMA_OK, "bma_rotate: status ", std::to_string(rc), ": ", lib.bma_error_string(rc));
   return {q_out, k_out};
 }
 
-// Gradients of (q, k, q_weight, k_weight), as far as they are there.
-std::tuple<Tensor, OptTensor, OptTensor, OptTensor> rotate_backward(const Tensor& q_in, const OptTensor& k_in, const OptTensor& positions, const OptTensor& frequencies,
-                                                                    int layout, double magnitude, const OptTensor& q_weight, const OptTensor& k_weight, double eps,
-                                                                    const Tensor& g_q_in, const OptTensor& g_k_in, uintptr_t stream) {
+// Gradients of (q, k, q_weight, k_weight), as far as they are there.  Runs on a thread of the autograd engine, without Python.
+std::tuple<Tensor, OptTensor, OptTensor, OptTensor> rotate_backward(const Tensor& q_in, const OptTensor& k_in, const Rotation& r, const Tensor& g_q_in, const OptTensor& g_k_in) {
   const Tensor q = heads_of(q_in, "q"), g_q = heads_of(g_q_in, "the cotangent of q");
   OptTensor k, g_k, dk, dqw, dkw;
   if (k_in) {
@@ -389,12 +413,13 @@ std::tuple<Tensor, OptTensor, OptTensor, OptTensor> rotate_backward(const Tensor
     g_k = heads_of(*g_k_in, "the cotangent of k");
   }
   Devices on;
-  bma_rotate_args a = rotate_args(on, q, k, positions, frequencies, layout, magnitude, q_weight, k_weight, eps);
+  bma_rotate_args a = rotate_args(on, q, k, r.positions, r.frequencies, r.layout, r.magnitude, r.q_weight, r.k_weight, r.eps);
   TORCH_CHECK_VALUE(g_q.sizes() == q.sizes() && (!k || g_k->sizes() == k->sizes()), "the cotangents must have the shapes of the results");
   TORCH_CHECK_TYPE(g_q.scalar_type() == q.scalar_type() && (!k || g_k->scalar_type() == q.scalar_type()), "the cotangents must have the dtype of the results");
   on.add(g_q, "the cotangent of q");
   if (k) on.add(*g_k, "the cotangent of k");
   on.check();
+  const Place place(q);
   const at::TensorOptions like = q.options().requires_grad(false);
   Tensor dq = at::empty(q.sizes(), like);
   a.q = describe(q); a.q_out = describe(g_q); a.dq = describe(dq);
@@ -402,18 +427,61 @@ std::tuple<Tensor, OptTensor, OptTensor, OptTensor> rotate_backward(const Tensor
     dk = at::empty(k->sizes(), like);
     a.k = describe(*k); a.k_out = describe(*g_k); a.dk = describe(*dk);
   }
-  if (q_weight) a.dq_weight = (dqw = at::empty(q_weight->sizes(), q_weight->options().requires_grad(false)))->data_ptr();
-  if (k_weight) a.dk_weight = (dkw = at::empty(k_weight->sizes(), k_weight->options().requires_grad(false)))->data_ptr();
+  if (r.q_weight) a.dq_weight = (dqw = at::empty(r.q_weight->sizes(), r.q_weight->options().requires_grad(false)))->data_ptr();
+  if (r.k_weight) a.dk_weight = (dkw = at::empty(r.k_weight->sizes(), r.k_weight->options().requires_grad(false)))->data_ptr();
   const size_t ws_bytes = lib.bma_rotate_bwd_workspace_bytes(&a);
   Tensor ws;
   if (ws_bytes) ws = bytes_on(q, ws_bytes);
-  int rc;
-  {
-    Group group("bma.rotate_bwd");
-    rc = lib.bma_rotate_bwd(&a, ws_bytes ? ws.data_ptr() : nullptr, ws_bytes, reinterpret_cast<bma_stream_t>(stream));
-  }
-  check(rc, "bma_rotate_bwd");
+  nvtxRangePushA("bma.rotate_bwd");
+  const int rc = lib.bma_rotate_bwd(&a, ws_bytes ? ws.data_ptr() : nullptr, ws_bytes, place.stream);
+  nvtxRangePop();
+  TORCH_CHECK(rc == BMA_OK, "bma_rotate_bwd: status ", std::to_string(rc), ": ", lib.bma_error_string(rc));
   return {dq, dk, dqw, dkw};
+}
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+struct RotateNode : torch::autograd::Function<RotateNode> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const OptTensor& k, const OptTensor& positions, const OptTensor& frequencies, int64_t layout,
+                               double magnitude, const OptTensor& q_weight, const OptTensor& k_weight, double eps) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const auto or_none = [](const OptTensor& t) { return t ? *t : Tensor(); };
+    auto [q_out, k_out] = rotate_forward(q, k, {positions, frequencies, (int)layout, magnitude, q_weight, k_weight, eps}, true);
+    // a rotation alone is undone without its input: only the shape, the dtype and the device are kept
+    ctx->save_for_backward({q_weight ? q : Tensor(), k && k_weight ? *k : Tensor(), or_none(positions), or_none(frequencies), or_none(q_weight), or_none(k_weight)});
+    ctx->saved_data["layout"] = layout;
+    ctx->saved_data["magnitude"] = magnitude;
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["q"] = at::empty({0}, q.options().requires_grad(false));
+    ctx->saved_data["q_sizes"] = q.sizes().vec();
+    if (k) ctx->saved_data["k_sizes"] = k->sizes().vec();
+    ctx->set_materialize_grads(false);
+    variable_list out{q_out};
+    if (k_out) out.push_back(*k_out);
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    const auto optional = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
+    const Rotation r{optional(saved[2]), optional(saved[3]), (int)ctx->saved_data["layout"].toInt(), ctx->saved_data["magnitude"].toDouble(), optional(saved[4]),
+                     optional(saved[5]), ctx->saved_data["eps"].toDouble()};
+    const bool keys = grads.size() > 1;
+    const Tensor like = ctx->saved_data["q"].toTensor();
+    // an undefined cotangent stands for zeros
+    const Tensor g_q = grads[0].defined() ? grads[0] : at::zeros(ctx->saved_data["q_sizes"].toIntVector(), like.options());
+    OptTensor g_k;
+    if (keys) g_k = grads[1].defined() ? grads[1] : at::zeros(ctx->saved_data["k_sizes"].toIntVector(), like.options());
+    const auto [dq, dk, dqw, dkw] = rotate_backward(saved[0].defined() ? saved[0] : g_q, keys ? (saved[1].defined() ? OptTensor(saved[1]) : g_k) : OptTensor(), r, g_q, g_k);
+    const auto or_none = [](const OptTensor& t) { return t ? *t : Tensor(); };
+    return {dq, or_none(dk), Tensor(), Tensor(), Tensor(), Tensor(), or_none(dqw), or_none(dkw), Tensor()};
+  }
+};
+
+std::tuple<Tensor, OptTensor> rotate(const Tensor& q, const OptTensor& k, const OptTensor& positions, const OptTensor& frequencies, int layout, double magnitude,
+                                     const OptTensor& q_weight, const OptTensor& k_weight, double eps) {
+  if (!wants_gradient({&q, pointer(k), pointer(q_weight), pointer(k_weight)})) return rotate_forward(q, k, {positions, frequencies, layout, magnitude, q_weight, k_weight, eps}, true);
+  const variable_list out = RotateNode::apply(q, k, positions, frequencies, (int64_t)layout, magnitude, q_weight, k_weight, eps);
+  return {out[0], out.size() > 1 ? OptTensor(out[1]) : OptTensor()};
 }
 
 bma_paged_cache cache_of(Devices& on, const Tensor& k, const Tensor& v, const Tensor& table, const OptTensor& k_scale, const OptTensor& v_scale) {
@@ -482,7 +550,9 @@ void fits_cache(Devices& on, const Tensor& t, const bma_paged_cache& c, int64_t 
 
 OptTensor append(const Tensor& pages_k, const Tensor& pages_v, const Tensor& table, const OptTensor& k_scale, const OptTensor& v_scale, const Tensor& k_in,
                  const Tensor& v_in, const Tensor& lengths, const OptTensor& new_lengths, const OptTensor& q_in, const OptTensor& frequencies, int layout, double magnitude,
-                 const OptTensor& q_weight, const OptTensor& k_weight, double eps, uintptr_t stream) {
+                 const OptTensor& q_weight, const OptTensor& k_weight, double eps) {
+  TORCH_CHECK_VALUE(!wants_gradient({&k_in, &v_in, pointer(q_in), pointer(q_weight), pointer(k_weight), &pages_k, &pages_v}),
+                    "append_kv is not differentiable: call it under torch.no_grad()");
   Devices on;
   const bma_paged_cache c = cache_of(on, pages_k, pages_v, table, k_scale, v_scale);
   const Tensor k = heads_of(k_in, "k"), v = heads_of(v_in, "v");
@@ -501,6 +571,7 @@ OptTensor append(const Tensor& pages_k, const Tensor& pages_v, const Tensor& tab
   a.rotary = rotary_of(on, c.d, frequencies, layout, magnitude, q_weight, k_weight, eps);
   if (q) fits_cache(on, *q, c, -1, "q");
   on.check();
+  const Place place(pages_k);
   a.k = describe(k); a.v = describe(v);
   if (q) {
     q_out = at::empty(q->sizes(), q->options().requires_grad(false));
@@ -510,26 +581,28 @@ OptTensor append(const Tensor& pages_k, const Tensor& pages_v, const Tensor& tab
   int rc;
   {
     Group group("bma.append_kv");
-    rc = lib.bma_append_kv(&c, &a, reinterpret_cast<bma_stream_t>(stream));
+    rc = lib.bma_append_kv(&c, &a, place.stream);
   }
   check(rc, "bma_append_kv");
   return q_out;
 }
 
 std::tuple<Tensor, Tensor> read_pages(const Tensor& pages_k, const Tensor& pages_v, const Tensor& table, const OptTensor& k_scale, const OptTensor& v_scale,
-                                const Tensor& lengths, int64_t L, uintptr_t stream) {
+                                const Tensor& lengths, int64_t L) {
   Devices on;
   const bma_paged_cache c = cache_of(on, pages_k, pages_v, table, k_scale, v_scale);
+  TORCH_CHECK_VALUE(!wants_gradient({&pages_k, &pages_v}), "read_kv is not differentiable: call it under torch.no_grad()");
   TORCH_CHECK_VALUE(L > 0 && L <= INT32_MAX, "max_length must be positive");
   const int32_t* at_lengths = counts_of(on, lengths, c, "lengths");
   on.check();
+  const Place place(pages_k);
   const at::TensorOptions like = pages_k.options().dtype(c.dtype == BMA_DTYPE_F32 ? at::kFloat : at::kBFloat16).requires_grad(false);
   Tensor k = at::empty({c.B, L, c.Hkv, c.d}, like), v = at::empty({c.B, L, c.Hkv, c.d}, like);
   const bma_tensor dk = describe(k), dv = describe(v);
   int rc;
   {
     Group group("bma.read_kv");
-    rc = lib.bma_read_kv(&c, at_lengths, (int32_t)L, &dk, &dv, reinterpret_cast<bma_stream_t>(stream));
+    rc = lib.bma_read_kv(&c, at_lengths, (int32_t)L, &dk, &dv, place.stream);
   }
   check(rc, "bma_read_kv");
   return {k, v};
@@ -537,7 +610,8 @@ std::tuple<Tensor, Tensor> read_pages(const Tensor& pages_k, const Tensor& pages
 
 std::tuple<Tensor, OptTensor> paged(const Tensor& pages_k, const Tensor& pages_v, const Tensor& table, const OptTensor& k_scale, const OptTensor& v_scale,
                                     const Tensor& q_in, const Tensor& lengths, const OptTensor& new_lengths, std::optional<double> scale,
-                                    std::optional<int64_t> window, bool bf16_out, bool with_lse, uintptr_t stream) {
+                                    std::optional<int64_t> window, bool bf16_out, bool with_lse) {
+  TORCH_CHECK_VALUE(!wants_gradient({&q_in, &pages_k, &pages_v}), "paged_attention is not differentiable: call it under torch.no_grad()");
   Devices on;
   const bma_paged_cache c = cache_of(on, pages_k, pages_v, table, k_scale, v_scale);
   Tensor q = heads_of(q_in, "q");
@@ -554,6 +628,7 @@ std::tuple<Tensor, OptTensor> paged(const Tensor& pages_k, const Tensor& pages_v
   a.scale = (float)(scale ? *scale : 1.0 / std::sqrt((double)c.d));
   a.window = window ? (int32_t)*window : -1;
   on.check();
+  const Place place(pages_k);
   const at::TensorOptions f32 = q.options().dtype(at::kFloat).requires_grad(false);
   Tensor o = at::empty(q.sizes(), bf16_out ? f32.dtype(at::kBFloat16) : f32);
   OptTensor lse;
@@ -566,7 +641,7 @@ std::tuple<Tensor, OptTensor> paged(const Tensor& pages_k, const Tensor& pages_v
   int rc;
   {
     Group group("bma.paged_attn");
-    rc = lib.bma_paged_attn(&c, &a, ws_bytes ? ws.data_ptr() : nullptr, ws_bytes, reinterpret_cast<bma_stream_t>(stream));
+    rc = lib.bma_paged_attn(&c, &a, ws_bytes ? ws.data_ptr() : nullptr, ws_bytes, place.stream);
   }
   check(rc, "bma_paged_attn");
   return {o, lse};
@@ -585,7 +660,6 @@ PYBIND11_MODULE(_host, m) {
   m.def("backward_bytes", torch::wrap_pybind_function(backward_bytes));
   m.def("backward", torch::wrap_pybind_function(backward));
   m.def("rotate", torch::wrap_pybind_function(rotate));
-  m.def("rotate_backward", torch::wrap_pybind_function(rotate_backward));
   m.def("append", torch::wrap_pybind_function(append));
   m.def("read", torch::wrap_pybind_function(read_pages));
   m.def("paged", torch::wrap_pybind_function(paged));

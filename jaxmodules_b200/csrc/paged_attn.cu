@@ -1085,17 +1085,20 @@ bool plan_paged(const bma_paged_cache& c, const bma_paged_attn_args& a, PagedLau
   const int64_t entries = (int64_t)c.B * l.row_tiles;
   if (entries >= (1 << 30)) return false;
   l.entries = (int)entries;
-  int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   const int64_t units = entries * c.Hkv * (((int64_t)c.width * c.page_size + kWarps * l.tile - 1) / (kWarps * l.tile) + 1);
-  l.ctas = (int)std::min<int64_t>((int64_t)sms * l.ctas_per_sm, units);
+  l.ctas = (int)std::min<int64_t>((int64_t)device_sms(current_device()) * l.ctas_per_sm, units);
   return true;
 }
 
 template <class Core>
 int launch_paged(const PagedParams& p, const PagedLaunch& l, cudaStream_t st) {
   constexpr int smem = paged_smem<Core>();
-  BMA_CUDA_TRY(cudaFuncSetAttribute(paged_kernel<Core>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  static std::atomic<bool> allowed[kMaxDevices] = {};        // of this instance, by device
+  std::atomic<bool>& set = allowed[current_device()];
+  if (!set.load(std::memory_order_relaxed)) {
+    BMA_CUDA_TRY(cudaFuncSetAttribute(paged_kernel<Core>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    set.store(true, std::memory_order_relaxed);
+  }
   paged_kernel<Core><<<l.ctas, kThreads, smem, st>>>(p);
   BMA_CUDA_TRY(cudaGetLastError());
   cudaLaunchConfig_t cfg{};

@@ -52,30 +52,6 @@ def layout_of(layout: str) -> int:
     return _LAYOUTS[layout]
 
 
-class _RotateHeads(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, positions, frequencies, layout, magnitude, q_weight, k_weight, eps):
-        ctx.how = (layout, magnitude, eps)
-        ctx.like = [None if t is None else t.new_empty(0) for t in (q, k)]      # dtype and device
-        ctx.shapes = [None if t is None else t.shape for t in (q, k)]
-        # a rotation alone is undone without its input
-        ctx.save_for_backward(None if q_weight is None else q, None if k_weight is None else k, positions, frequencies, q_weight, k_weight)
-        ctx.set_materialize_grads(False)
-        with nat.device_guard(q.device):
-            return nat.host().rotate(q, k, positions, frequencies, layout, magnitude, q_weight, k_weight, eps, nat.stream(q.device))
-
-    @staticmethod
-    def backward(ctx, *grads):
-        q, k, positions, frequencies, q_weight, k_weight = ctx.saved_tensors
-        layout, magnitude, eps = ctx.how
-        # an undefined cotangent stands for zeros
-        g_q, g_k = (like.new_zeros(shape) if g is None and like is not None else g for g, like, shape in zip(grads, ctx.like, ctx.shapes))
-        with nat.device_guard(g_q.device):
-            dq, dk, dqw, dkw = nat.host().rotate_backward(g_q if q is None else q, g_k if k is None else k, positions, frequencies, layout, magnitude, q_weight,
-                                                          k_weight, eps, g_q, g_k, nat.stream(g_q.device))
-        return dq, dk, None, None, None, None, dqw, dkw, None
-
-
 def rotate_heads(q: torch.Tensor, k: Optional[torch.Tensor], positions: Optional[torch.Tensor] = None, frequencies: Optional[torch.Tensor] = None, *,
                  layout: str = "half", magnitude: float = 1.0, q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
                  eps: float = 1e-6) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
@@ -93,10 +69,4 @@ def rotate_heads(q: torch.Tensor, k: Optional[torch.Tensor], positions: Optional
     Repeated calls give the same bits, gradients included.  The gradients of the weights are sums over all tokens and heads in an order that
     the sizes of the call fix.
     """
-    args = (q, k, positions, frequencies, layout_of(layout), float(magnitude), q_weight, k_weight, float(eps))
-    if not q.is_cuda:
-        raise RuntimeError("rotate_heads needs CUDA tensors; there is no CPU path")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
-        return _RotateHeads.apply(*args)
-    with nat.device_guard(q.device):
-        return nat.host().rotate(*args, nat.stream(q.device))
+    return nat.host().rotate(q, k, positions, frequencies, layout_of(layout), magnitude, q_weight, k_weight, eps)

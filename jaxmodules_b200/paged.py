@@ -49,18 +49,6 @@ class PagedCache:
         return cls(*zeros(d, dtype), page_table)
 
 
-def _pages(cache: PagedCache):
-    return cache.k, cache.v, cache.page_table, cache.k_scale, cache.v_scale
-
-
-def _device(cache: PagedCache, where: str, *inputs):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (*inputs, cache.k, cache.v)):
-        raise ValueError(f"{where} is not differentiable: call it under torch.no_grad()")
-    if not cache.k.is_cuda:
-        raise RuntimeError(f"{where} needs CUDA tensors; there is no CPU path")
-    return cache.k.device
-
-
 def append_kv(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor, *, new_lengths: Optional[torch.Tensor] = None,
               q: Optional[torch.Tensor] = None, frequencies: Optional[torch.Tensor] = None, layout: str = "half", magnitude: float = 1.0,
               q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6) -> Optional[torch.Tensor]:
@@ -77,19 +65,15 @@ def append_kv(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, lengths: torc
     Tokens at positions that the page table does not cover, or whose page is not in the cache, are not written, and
     ``attention.device_status`` reports it.  Two real tokens must not lie in one slot of one page.  Not differentiable.
     """
-    dev = _device(cache, "append_kv", k, v, q, q_weight, k_weight)
-    with nat.device_guard(dev):
-        return nat.host().append(*_pages(cache), k, v, lengths, new_lengths, q, frequencies, layout_of(layout), float(magnitude), q_weight, k_weight, float(eps),
-                                 nat.stream(dev))
+    return nat.host().append(cache.k, cache.v, cache.page_table, cache.k_scale, cache.v_scale, k, v, lengths, new_lengths, q, frequencies, layout_of(layout),
+                             magnitude, q_weight, k_weight, eps)
 
 
 def read_kv(cache: PagedCache, lengths: torch.Tensor, max_length: int) -> Tuple[torch.Tensor, torch.Tensor]:
     """The cached tokens as dense keys and values ``[B, max_length, Hkv, d]`` in position order, zeros from ``lengths[b]`` on: what
     ``masked_attention_via_map`` takes, for a chunk of a prompt that attends to all before it.  In the cache's dtype, bfloat16 of a 4-bit
     cache, whose values that holds exactly (down to 2^-133).  Positions without a page read as zeros, and ``attention.device_status`` reports them.  Not differentiable."""
-    dev = _device(cache, "read_kv")
-    with nat.device_guard(dev):
-        return nat.host().read(*_pages(cache), lengths, int(max_length), nat.stream(dev))
+    return nat.host().read(cache.k, cache.v, cache.page_table, cache.k_scale, cache.v_scale, lengths, max_length)
 
 
 def paged_attention(q: torch.Tensor, cache: PagedCache, lengths: torch.Tensor, *, new_lengths: Optional[torch.Tensor] = None, scale: Optional[float] = None,
@@ -106,10 +90,8 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, lengths: torch.Tensor, *
     window or after its token, infinities and NaN included.  Positions without a page make the results invalid, and ``attention.device_status``
     reports them.  Repeated calls give the same bits; a sequence in another batch need not give those.  Not differentiable.
     """
-    dev = _device(cache, "paged_attention", q)
-    out_dtype = out_dtype or torch.float32
-    if out_dtype not in (torch.float32, torch.bfloat16):
+    if out_dtype is not None and out_dtype not in (torch.float32, torch.bfloat16):
         raise TypeError("out_dtype must be float32 or bfloat16")
-    with nat.device_guard(dev):
-        o, lse = nat.host().paged(*_pages(cache), q, lengths, new_lengths, scale, window, out_dtype == torch.bfloat16, return_lse, nat.stream(dev))
+    o, lse = nat.host().paged(cache.k, cache.v, cache.page_table, cache.k_scale, cache.v_scale, q, lengths, new_lengths, scale, window,
+                              out_dtype == torch.bfloat16, return_lse)
     return (o, lse) if return_lse else o

@@ -65,7 +65,7 @@ def test_rotate_heads_refuses_before_native_code(error, call):
 
 
 def rotate(q=heads(), k=heads(), positions=None, frequencies=F, layout=0, magnitude=1.0, q_weight=None, k_weight=None, eps=1e-6):
-    return nat.host().rotate(q, k, positions, frequencies, layout, magnitude, q_weight, k_weight, eps, 0)
+    return nat.host().rotate(q, k, positions, frequencies, layout, magnitude, q_weight, k_weight, eps)
 
 
 # What is wrong with the tensors is said before where they are (the native checks are reached with CPU tensors; none gets past them).
@@ -101,7 +101,7 @@ def cache(dtype=torch.float32, pages=5, page=4, H=2, d=32, B=2, width=3, **kw):
 def attend(c=None, q=None, lengths=torch.zeros(2, dtype=torch.int32), new_lengths=None, window=None):
     c = cache() if c is None else c
     q = heads(d=32) if q is None else q
-    return nat.host().paged(c.k, c.v, c.page_table, c.k_scale, c.v_scale, q, lengths, new_lengths, None, window, False, False, 0)
+    return nat.host().paged(c.k, c.v, c.page_table, c.k_scale, c.v_scale, q, lengths, new_lengths, None, window, False, False)
 
 
 @pytest.mark.parametrize("error,kwargs", [
@@ -151,7 +151,7 @@ def test_append_refuses(error, kwargs):
     a = dict(k=heads(H=2, d=32), v=heads(H=2, d=32), lengths=torch.zeros(2, dtype=torch.int32), new_lengths=None, q=None, frequencies=F, q_weight=None) | kwargs
     with pytest.raises(error):
         nat.host().append(c.k, c.v, c.page_table, c.k_scale, c.v_scale, a["k"], a["v"], a["lengths"], a["new_lengths"], a["q"], a["frequencies"], 0, 1.0, a["q_weight"],
-                          None, 1e-6, 0)
+                          None, 1e-6)
 
 
 def test_read_refuses():
@@ -159,7 +159,7 @@ def test_read_refuses():
     lengths = torch.zeros(2, dtype=torch.int32)
     for error, L in ((ValueError, 0), (RuntimeError, 4)):
         with pytest.raises(error):
-            nat.host().read(c.k, c.v, c.page_table, c.k_scale, c.v_scale, lengths, L, 0)
+            nat.host().read(c.k, c.v, c.page_table, c.k_scale, c.v_scale, lengths, L)
     with pytest.raises(RuntimeError, match="CUDA"):
         jm.read_kv(c, lengths, 4)
     with pytest.raises(RuntimeError, match="CUDA"):
