@@ -4,10 +4,11 @@
 // by memory.  What they have to do is to keep enough loads in flight, and to give every SM the same share of bytes whatever the
 // lengths are, which only the device knows.
 //
-// Work.  The walk over the keys of one (sequence, tile of rows, kv head) is an item, cut into units of kUnit keys.  All units of all items lie in
-// one sequence, which is cut into as many even runs as CTAs fit on the chip; a run ends in the middle of an item as a rule.  Each CTA finds its
-// run from the lengths.  An item that lies within one run is finished there; the parts of others go to the workspace, at most two from a
-// CTA, and paged_join_kernel puts them together in the order of the keys.
+// Work.  The walk over the keys of one (sequence, tile of rows, kv head) is an item, cut into units of a tile of keys for every warp.  All units of
+// all items lie on one line, each item's with a place before them, for what it takes to begin and finish an item (about a unit: without it a sequence of one
+// token, 8 items to finish, kept its CTA for 9 us after the others).  The line is cut into as many even runs as CTAs fit on the chip; a run ends in the
+// middle of an item as a rule.  Each CTA finds its run from the lengths.  An item that lies within one run is finished there; the parts of others go to the
+// workspace, at most two from a CTA, and paged_join_kernel puts them together in the order of the keys.
 //
 // Within a CTA the four warps take tiles of a unit in turn, each with its own ring of stages in shared memory that it fills by cp.async: no warp
 // waits for another before the end of an item, and the ring runs on into the next item.  Pages are looked up for every key (any page
@@ -117,13 +118,17 @@ __device__ __forceinline__ Entry entry_of(const PagedParams& p, int e) {
   return x;
 }
 
-// A place in the sequence of units.
+// A unit, and its place on the line.
+constexpr int kItem = 1;          // places before the units of an item
 template <int ROWS, int TILE>
 struct Cursor {
   Entry x;
   int e, h, unit;
+  int64_t at;
   __device__ __forceinline__ void next(const PagedParams& p) {
+    ++at;
     if (++unit < x.units) return;
+    at += kItem;
     unit = 0;
     if (++h < p.c.Hkv) return;
     h = 0;
@@ -910,11 +915,11 @@ __global__ void __launch_bounds__(kThreads, Core::kMinCtas) paged_kernel(const _
     }
     __syncthreads();
   };
-  auto units_of = [&](int e) { return e < p.entries ? entry_of<Core::kRows, Core::kTile>(p, e).units : 0; };
+  auto places_of = [&](int e) { return e < p.entries ? kItem + entry_of<Core::kRows, Core::kTile>(p, e).units : 0; };
   int64_t total = 0, before = 0, all = 0;
   int own = 0;
   for (int e0 = 0; e0 < p.entries; e0 += kThreads) {
-    own = units_of(e0 + threadIdx.x);
+    own = places_of(e0 + threadIdx.x);
     block_scan(own, before, all);
     total += all;
   }
@@ -926,7 +931,7 @@ __global__ void __launch_bounds__(kThreads, Core::kMinCtas) paged_kernel(const _
   int64_t gone = 0;
   for (int e0 = 0; e0 < p.entries; e0 += kThreads) {
     if (p.entries > kThreads) {
-      own = units_of(e0 + threadIdx.x);
+      own = places_of(e0 + threadIdx.x);
       block_scan(own, before, all);
     }
     const int64_t from = (gone + before) * p.c.Hkv;
@@ -941,34 +946,34 @@ __global__ void __launch_bounds__(kThreads, Core::kMinCtas) paged_kernel(const _
   next.e = (int)scan[kWarps + 1];
   const int64_t within = scan[kWarps + 2];
   next.x = entry_of<Core::kRows, Core::kTile>(p, next.e);
-  next.h = (int)(within / next.x.units);
-  next.unit = (int)(within - (int64_t)next.h * next.x.units);
+  next.h = (int)(within / (kItem + next.x.units));
+  const int inside = (int)(within - (int64_t)next.h * (kItem + next.x.units));      // of the item
+  next.unit = max(inside - kItem, 0);
+  next.at = begin - inside + kItem + next.unit;
   __syncthreads();              // (copies go there next)
 
   Core core;
   core.prepare(smem + kWarps * NS * Core::kStageBytes);
   Cur here = next;
-  const int n = (int)(end - begin);
+  if (here.at >= end) return;  // (a place before an item's units is all there is)
   core.look_up(p, next, warp, lane);
   int to = 0, from = 0;        // stages to fill and to read next
-  auto issue = [&](int i) {
-    if (i < n) {
+  auto issue = [&] {
+    if (next.at < end) {
       core.issue(p, next, ring + to * Core::kStageBytes, lane);
       to = to == NS - 1 ? 0 : to + 1;
-      if (i + 1 < n) {
-        next.next(p);
-        core.look_up(p, next, warp, lane);
-      }
+      next.next(p);
+      if (next.at < end) core.look_up(p, next, warp, lane);
     }
     copies_committed();
   };
-  for (int i = 0; i < NS - 1; ++i) issue(i);
+  for (int i = 0; i < NS - 1; ++i) issue();
   bool fresh = true;           // the first unit of an item in this run
   int first_unit = here.unit;
   bool first_item = true;
-  for (int i = 0; i < n; ++i) {
+  while (here.at < end) {
     core.settle();
-    issue(i + NS - 1);
+    issue();
     copies_awaited<NS - 1>();
     __syncwarp();
     if (fresh) {
@@ -980,11 +985,11 @@ __global__ void __launch_bounds__(kThreads, Core::kMinCtas) paged_kernel(const _
     if (k0 < here.x.hi) core.take(p, here, ring + from * Core::kStageBytes, k0, lane);
     __syncwarp();
     const bool last = here.unit + 1 == here.x.units;
-    if (last || i + 1 == n) {
+    if (last || here.at + 1 == end) {
       const bool whole = last && first_unit == 0;
       const int slot = 2 * blockIdx.x + (first_item ? 0 : 1);
       if (!whole && !last && first_unit == 0 && threadIdx.x == 0) {      // the first part of an item that goes on in other CTAs
-        const int64_t item_end = end + (here.x.units - here.unit - 1);   // (this run ends with unit here.unit of it)
+        const int64_t item_end = here.at + (here.x.units - here.unit);   // one past its last unit
         int cta = (int)((item_end - 1) * ctas / total);             // the CTA whose run holds its last unit
         while (run_begin(total, cta + 1, ctas) < item_end) ++cta;
         while (run_begin(total, cta, ctas) >= item_end) --cta;
