@@ -5,7 +5,7 @@
 // lengths are, which only the device knows.
 //
 // Work.  The walk over the keys of one (sequence, tile of rows, kv head) is an item, cut into units of a tile of keys for every warp.  All units of
-// all items lie on one line, each item's with a place before them, for what it takes to begin and finish an item (about a unit: without it a sequence of one
+// all items lie on one line, each item's with room before them for what it takes to begin and finish an item (half a unit, 1.5 in FMA arithmetic: without it a sequence of one
 // token, 8 items to finish, kept its CTA for 9 us after the others).  The line is cut into as many even runs as CTAs fit on the chip; a run ends in the
 // middle of an item as a rule.  Each CTA finds its run from the lengths.  An item that lies within one run is finished there; the parts of others go to the
 // workspace, at most two from a CTA, and paged_join_kernel puts them together in the order of the keys.
@@ -32,7 +32,8 @@ struct PagedParams {
   int positions;                       // what the page table covers
   int page_shift;                      // log2 of the page size, -1 where that is no power of two
   uint32_t page_units, slot_units, head_units;      // strides of the cache, in 16 bytes
-  int scale_words;                     // 4 bits: a head's four powers of two can be read at once
+  int scale_words;                     // 4 bits: a head's four powers of two can be read at once, at these strides in words
+  uint32_t scale_page, scale_slot, scale_head;
   float scale_log2;
   int* status;
   float* part_o;                       // [2 * CTAs][rows of a tile][DP]
@@ -119,16 +120,16 @@ __device__ __forceinline__ Entry entry_of(const PagedParams& p, int e) {
 }
 
 // A unit, and its place on the line.
-constexpr int kItem = 1;          // places before the units of an item
-template <int ROWS, int TILE>
+constexpr int kUnit = 2;          // places of a unit
+template <int ROWS, int TILE, int ITEM>      // ITEM: places before the units of an item
 struct Cursor {
   Entry x;
   int e, h, unit;
   int64_t at;
   __device__ __forceinline__ void next(const PagedParams& p) {
-    ++at;
+    at += kUnit;
     if (++unit < x.units) return;
-    at += kItem;
+    at += ITEM;
     unit = 0;
     if (++h < p.c.Hkv) return;
     h = 0;
@@ -231,6 +232,8 @@ __device__ __forceinline__ uint32_t seen_pair(const PagedParams& p, int at, int 
   if (key + 1 <= at && (p.a.window < 0 || key + 1 >= at - p.a.window)) m |= 0xffff0000u;
   return m;
 }
+// At the beginning of a branch that is rarely taken: without it the compiler runs both ways and selects, for every tile.
+__device__ __forceinline__ void rarely() { asm volatile("" ::: "memory"); }
 // An 8 x 8 matrix of 16-bit values, [keys, rows], turned
 __device__ __forceinline__ uint32_t turned(uint32_t x) {
   uint32_t y;
@@ -274,9 +277,9 @@ __device__ __forceinline__ void copy_rows(const PagedParams& p, uint32_t mine, i
 // tile, where rows as M would make 16 of one.  The weights go from the accumulators of the one to the operand of the other by movmatrix.
 template <int DP, int NT>
 struct CoreBf16 {
-  static constexpr int kDP = DP, kRows = NT * 8, kTile = 16, kStages = DP == 128 ? (NT == 1 ? 2 : 3) : 4, kMinCtas = NT == 1 ? 3 : 2;
+  static constexpr int kDP = DP, kRows = NT * 8, kTile = 16, kItem = 1, kStages = DP == 128 ? (NT == 1 ? 2 : 3) : 4, kMinCtas = NT == 1 ? 3 : 2;
   static constexpr int kRowBytes = DP * 2, kSide = kTile * kRowBytes, kStageBytes = 2 * kSide, kExtra = 0;
-  using Cur = Cursor<kRows, kTile>;
+  using Cur = Cursor<kRows, kTile, kItem>;
 
   uint32_t q[NT][DP / 16][2];
   float o[NT][DP / 16][4];
@@ -285,9 +288,9 @@ struct CoreBf16 {
 
   __device__ __forceinline__ void prepare(uint8_t*) {}
   __device__ __forceinline__ void look_up(const PagedParams& p, const Cur& c, int warp, int lane) { place.look_up(p, c.x, c.tile(warp) + (lane & 15)); }
-  __device__ __forceinline__ void settle() {}
-  __device__ __forceinline__ void issue(const PagedParams& p, const Cur& c, uint8_t* stage, int lane) {
-    copy_rows<kTile, DP / 8, kSide>(p, place.at(p, c.h), p.c.d / 8, smem_at(stage), lane, [](int r, int chunk) { return r * kRowBytes + ((chunk ^ (r & 7)) << 4); });
+  __device__ __forceinline__ void settle(uint8_t*) {}
+  __device__ __forceinline__ void issue(const PagedParams& p, const Cur& c, uint8_t* smem, int stage, int lane) {
+    copy_rows<kTile, DP / 8, kSide>(p, place.at(p, c.h), p.c.d / 8, smem_at(smem) + stage, lane, [](int r, int chunk) { return r * kRowBytes + ((chunk ^ (r & 7)) << 4); });
   }
   __device__ __forceinline__ void begin(const PagedParams& p, const Cur& c, int lane) {
     const int g = lane >> 2, t = lane & 3;
@@ -333,12 +336,15 @@ struct CoreBf16 {
     for (int i = 0; i < NT; ++i) {
       float top[2] = {rows.m[i][0], rows.m[i][1]};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float x = s[i][e] * p.scale_log2;
-        if (cut && !rows.sees(p, i, e & 1, k0 + (e >> 1) * 8 + g)) x = -INFINITY;
-        s[i][e] = x;
-        top[e & 1] = fmaxf(top[e & 1], x);
+      for (int e = 0; e < 4; ++e) s[i][e] *= p.scale_log2;
+      if (cut) {
+        rarely();
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (!rows.sees(p, i, e & 1, k0 + (e >> 1) * 8 + g)) s[i][e] = -INFINITY;
       }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top[e & 1] = fmaxf(top[e & 1], s[i][e]);
       rows.rescale(i, top, o[i]);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -411,12 +417,12 @@ struct CoreBf16 {
 // (turned: of two keys), and they are taken in the order in which they come.
 template <int DP, int NT>
 struct Core4bit {
-  static constexpr int kDP = DP, kRows = NT * 8, kTile = 32, kStages = 3, kMinCtas = NT == 1 ? 3 : 2;
+  static constexpr int kDP = DP, kRows = NT * 8, kTile = 32, kItem = 1, kStages = 3, kMinCtas = NT == 1 ? 3 : 2;
   static constexpr int kRowBytes = DP / 2, kSide = kTile * kRowBytes, kGroups = DP / 32;
   // after keys and values: powers of keys [32][4] (float32), of values [4][32] (float16, by key_of's rows), E and 2^-E of values [32][2]
   static constexpr int kKeyPowers = 2 * kSide, kValuePowers = kKeyPowers + 512, kTops = kValuePowers + 256, kStageBytes = kTops + 256, kExtra = 0;
   static constexpr float kWeightUp = 15.f;
-  using Cur = Cursor<kRows, kTile>;
+  using Cur = Cursor<kRows, kTile, kItem>;
 
   uint32_t q[NT][DP / 16][2];
   float o[NT][DP / 16][4];
@@ -424,23 +430,25 @@ struct Core4bit {
   Rows<NT> rows;
   Place place;
   uint32_t k_bytes, v_bytes;    // the powers of two of this lane's key of the last tile issued
-  uint8_t* pending;             // and its stage
+  int pending;                  // and where its stage lies, negative where there is none
 
-  __device__ __forceinline__ void prepare(uint8_t*) { pending = nullptr; }
+  __device__ __forceinline__ void prepare(uint8_t*) { pending = -1; }
   __device__ __forceinline__ void look_up(const PagedParams& p, const Cur& c, int warp, int lane) { place.look_up(p, c.x, c.tile(warp) + lane); }
   // 16-byte chunks of a row are permuted so that 8 rows of a chunk lie in different banks
   static __device__ __forceinline__ int chunk_at(int r, int chunk) { return r * kRowBytes + ((DP == 128 ? chunk ^ (r >> 1 & 3) : chunk ^ (r >> 2 & 1)) << 4); }
 
-  __device__ __forceinline__ void issue(const PagedParams& p, const Cur& c, uint8_t* stage, int lane) {
-    settle();
+  __device__ __forceinline__ void issue(const PagedParams& p, const Cur& c, uint8_t* smem, int stage, int lane) {
+    settle(smem);
     const uint32_t mine = place.at(p, c.h);
     k_bytes = v_bytes = 0;
     if (mine != kNowhere) {
-      const int64_t at = (int64_t)place.page * p.c.scale_stride_page + (int64_t)place.slot * p.c.scale_stride_slot + (int64_t)c.h * p.c.scale_stride_head;
       if (p.scale_words) {
-        k_bytes = __ldg(reinterpret_cast<const uint32_t*>(p.c.k_scale + at));
-        v_bytes = __ldg(reinterpret_cast<const uint32_t*>(p.c.v_scale + at));
+        const uint32_t word = place.page * p.scale_page + place.slot * p.scale_slot + c.h * p.scale_head;
+        k_bytes = __ldg(reinterpret_cast<const uint32_t*>(p.c.k_scale) + word);
+        v_bytes = __ldg(reinterpret_cast<const uint32_t*>(p.c.v_scale) + word);
       } else {
+        rarely();
+        const int64_t at = (int64_t)place.page * p.c.scale_stride_page + (int64_t)place.slot * p.c.scale_stride_slot + (int64_t)c.h * p.c.scale_stride_head;
         const int n = p.c.d / 32;
 #pragma unroll
         for (int i = 0; i < kGroups; ++i)
@@ -451,11 +459,12 @@ struct Core4bit {
       }
     }
     pending = stage;
-    copy_rows<kTile, DP / 32, kSide>(p, mine, p.c.d / 32, smem_at(stage), lane, [](int r, int chunk) { return chunk_at(r, chunk); });
+    copy_rows<kTile, DP / 32, kSide>(p, mine, p.c.d / 32, smem_at(smem) + stage, lane, [](int r, int chunk) { return chunk_at(r, chunk); });
   }
   // The powers of two that were asked for with the last tile, into its stage.
-  __device__ __forceinline__ void settle() {
-    if (!pending) return;
+  __device__ __forceinline__ void settle(uint8_t* smem) {
+    if (pending < 0) return;
+    uint8_t* to = smem + pending;
     const int lane = threadIdx.x & 31;
     int b[4] = {(int)(v_bytes & 255), (int)(v_bytes >> 8 & 255), (int)(v_bytes >> 16 & 255), (int)(v_bytes >> 24)};
     if (kGroups == 2) b[2] = b[3] = b[0];
@@ -471,6 +480,7 @@ struct Core4bit {
       kp[i] = __uint_as_float((i == 0 ? k_bytes << 23 : i == 1 ? k_bytes << 15 : i == 2 ? k_bytes << 7 : k_bytes >> 1) & 0x7f800000u);      // (2^-127 counts as 0)
     }
     if (__any_sync(0xffffffffu, rare || least < 127 - 65 - 14)) {        // bytes of 255, powers under 2^-14 of the head's largest
+      rarely();
       top = 127 - 65;
 #pragma unroll
       for (int i = 0; i < 4; ++i) top = b[i] == 255 ? top : max(top, b[i]);
@@ -481,12 +491,12 @@ struct Core4bit {
         if ((k_bytes >> (8 * i) & 255) == 255) kp[i] = __uint_as_float(0x7fffffffu);
       }
     }
-    uint16_t* vp = reinterpret_cast<uint16_t*>(pending + kValuePowers) + (lane & 16) + (lane & 6) + (lane >> 3 & 1) + (lane & 1) * 8;      // the row m of the key
+    uint16_t* vp = reinterpret_cast<uint16_t*>(to + kValuePowers) + (lane & 16) + (lane & 6) + (lane >> 3 & 1) + (lane & 1) * 8;      // the row m of the key
 #pragma unroll
     for (int i = 0; i < kGroups; ++i) vp[i * 32] = (uint16_t)f[i];
-    *reinterpret_cast<float4*>(pending + kKeyPowers + lane * 16) = make_float4(kp[0], kp[1], kp[2], kp[3]);
-    *reinterpret_cast<float2*>(pending + kTops + lane * 8) = make_float2((float)(top - 127), top == 254 ? __uint_as_float(0x00400000u) : __uint_as_float((uint32_t)(254 - top) << 23));
-    pending = nullptr;
+    *reinterpret_cast<float4*>(to + kKeyPowers + lane * 16) = make_float4(kp[0], kp[1], kp[2], kp[3]);
+    *reinterpret_cast<float2*>(to + kTops + lane * 8) = make_float2((float)(top - 127), top == 254 ? __uint_as_float(0x00400000u) : __uint_as_float((uint32_t)(254 - top) << 23));
+    pending = -1;
   }
   __device__ __forceinline__ void begin(const PagedParams& p, const Cur& c, int lane) {
     const int g = lane >> 2, t = lane & 3;
@@ -586,12 +596,19 @@ struct Core4bit {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float x = fmaf(s[h][i][e], scale[i][e & 1], tops[h][e >> 1].x);
-          if (cut && !rows.sees(p, i, e & 1, k0 + h * 16 + key_of((e >> 1) * 8 + g))) x = -INFINITY;
-          s[h][i][e] = x;
-          top[e & 1] = fmaxf(top[e & 1], x);
-        }
+        for (int e = 0; e < 4; ++e) s[h][i][e] = fmaf(s[h][i][e], scale[i][e & 1], tops[h][e >> 1].x);
+      if (cut) {
+        rarely();
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (!rows.sees(p, i, e & 1, k0 + h * 16 + key_of((e >> 1) * 8 + g))) s[h][i][e] = -INFINITY;
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top[e & 1] = fmaxf(top[e & 1], s[h][i][e]);
       rows.rescale(i, top, o[i], kWeightUp);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -683,12 +700,12 @@ struct Core4bit {
 // For the scores two lanes share a key, for the sums a lane has DP / 32 columns; the rows of Q are read from shared memory, by all lanes at once.
 template <int DP, int ROWS>
 struct CoreF32 {
-  static constexpr int kDP = DP, kRows = ROWS, kTile = 16, kStages = 2, kMinCtas = 1;
+  static constexpr int kDP = DP, kRows = ROWS, kTile = 16, kItem = 3, kStages = 2, kMinCtas = 1;
   static constexpr int kRowBytes = DP * 4, kSide = kTile * kRowBytes, kStageBytes = 2 * kSide;
   static constexpr int kQRow = DP + 4;         // floats: the second half of a row lies 4 further on, in other banks than the first
   static constexpr int kExtra = ROWS * kQRow * 4 + kWarps * kTile * ROWS * 4;
   static constexpr int kCols = DP / 32;
-  using Cur = Cursor<kRows, kTile>;
+  using Cur = Cursor<kRows, kTile, kItem>;
 
   float o[ROWS][kCols];
   float m[ROWS], l[ROWS];      // of all rows; l: this lane's key's share
@@ -700,9 +717,9 @@ struct CoreF32 {
     ps = qs + ROWS * kQRow + (threadIdx.x >> 5) * kTile * ROWS;
   }
   __device__ __forceinline__ void look_up(const PagedParams& p, const Cur& c, int warp, int lane) { place.look_up(p, c.x, c.tile(warp) + (lane & 15)); }
-  __device__ __forceinline__ void settle() {}
-  __device__ __forceinline__ void issue(const PagedParams& p, const Cur& c, uint8_t* stage, int lane) {
-    copy_rows<kTile, DP / 4, kSide>(p, place.at(p, c.h), p.c.d / 4, smem_at(stage), lane, [](int r, int chunk) { return r * kRowBytes + ((chunk ^ (r & 7)) << 4); });
+  __device__ __forceinline__ void settle(uint8_t*) {}
+  __device__ __forceinline__ void issue(const PagedParams& p, const Cur& c, uint8_t* smem, int stage, int lane) {
+    copy_rows<kTile, DP / 4, kSide>(p, place.at(p, c.h), p.c.d / 4, smem_at(smem) + stage, lane, [](int r, int chunk) { return r * kRowBytes + ((chunk ^ (r & 7)) << 4); });
   }
   __device__ __forceinline__ void begin(const PagedParams& p, const Cur& c, int lane) {
     const int n = min(ROWS, p.rows - c.x.row0);
@@ -744,6 +761,7 @@ struct CoreF32 {
       float x = (s[r] + __shfl_xor_sync(0xffffffffu, s[r], 16)) * p.scale_log2;
       bool seen = true;
       if (cut) {
+        rarely();
         const int row = c.x.row0 + r, t = row / p.G, at = row < p.rows && t < c.x.count ? c.x.first + t : -1, k = k0 + key;
         seen = k <= at && (p.a.window < 0 || k >= at - p.a.window);
         if (!seen) x = -INFINITY;
@@ -893,7 +911,6 @@ __global__ void __launch_bounds__(kThreads, Core::kMinCtas) paged_kernel(const _
   using Cur = typename Core::Cur;
   constexpr int NS = Core::kStages;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  uint8_t* ring = smem + warp * NS * Core::kStageBytes;
   asm volatile("griddepcontrol.launch_dependents;");
 
   // The run of this CTA: prefix sums of the entries' units, kThreads at a time.
@@ -915,7 +932,7 @@ __global__ void __launch_bounds__(kThreads, Core::kMinCtas) paged_kernel(const _
     }
     __syncthreads();
   };
-  auto places_of = [&](int e) { return e < p.entries ? kItem + entry_of<Core::kRows, Core::kTile>(p, e).units : 0; };
+  auto places_of = [&](int e) { return e < p.entries ? Core::kItem + kUnit * entry_of<Core::kRows, Core::kTile>(p, e).units : 0; };
   int64_t total = 0, before = 0, all = 0;
   int own = 0;
   for (int e0 = 0; e0 < p.entries; e0 += kThreads) {
@@ -925,7 +942,7 @@ __global__ void __launch_bounds__(kThreads, Core::kMinCtas) paged_kernel(const _
   }
   total *= p.c.Hkv;
   if (threadIdx.x == 0) p.meta[blockIdx.x] = make_int4(-1, 0, 0, 0);
-  const int ctas = (int)min((int64_t)gridDim.x, total);       // (no run is empty)
+  const int ctas = (int)min((int64_t)gridDim.x, max(total / kUnit, (int64_t)1));       // (within an item every run has a unit's beginning)
   if (blockIdx.x >= ctas) return;
   const int64_t begin = run_begin(total, blockIdx.x, ctas), end = run_begin(total, blockIdx.x + 1, ctas);
   int64_t gone = 0;
@@ -946,10 +963,16 @@ __global__ void __launch_bounds__(kThreads, Core::kMinCtas) paged_kernel(const _
   next.e = (int)scan[kWarps + 1];
   const int64_t within = scan[kWarps + 2];
   next.x = entry_of<Core::kRows, Core::kTile>(p, next.e);
-  next.h = (int)(within / (kItem + next.x.units));
-  const int inside = (int)(within - (int64_t)next.h * (kItem + next.x.units));      // of the item
-  next.unit = max(inside - kItem, 0);
-  next.at = begin - inside + kItem + next.unit;
+  const int places = Core::kItem + kUnit * next.x.units;
+  next.h = (int)(within / places);
+  const int inside = (int)(within - (int64_t)next.h * places);                      // of the item
+  next.unit = max(inside - Core::kItem + kUnit - 1, 0) / kUnit;                           // the first unit that begins in the run
+  next.at = begin - inside + Core::kItem + kUnit * next.unit;
+  if (next.unit >= next.x.units) {                                                  // (that is the next item's)
+    --next.unit;
+    next.at -= kUnit;
+    next.next(p);
+  }
   __syncthreads();              // (copies go there next)
 
   Core core;
@@ -960,7 +983,7 @@ __global__ void __launch_bounds__(kThreads, Core::kMinCtas) paged_kernel(const _
   int to = 0, from = 0;        // stages to fill and to read next
   auto issue = [&] {
     if (next.at < end) {
-      core.issue(p, next, ring + to * Core::kStageBytes, lane);
+      core.issue(p, next, smem, (warp * NS + to) * Core::kStageBytes, lane);
       to = to == NS - 1 ? 0 : to + 1;
       next.next(p);
       if (next.at < end) core.look_up(p, next, warp, lane);
@@ -972,7 +995,7 @@ __global__ void __launch_bounds__(kThreads, Core::kMinCtas) paged_kernel(const _
   int first_unit = here.unit;
   bool first_item = true;
   while (here.at < end) {
-    core.settle();
+    core.settle(smem);
     issue();
     copies_awaited<NS - 1>();
     __syncwarp();
@@ -982,14 +1005,14 @@ __global__ void __launch_bounds__(kThreads, Core::kMinCtas) paged_kernel(const _
       fresh = false;
     }
     const int k0 = here.tile(warp);
-    if (k0 < here.x.hi) core.take(p, here, ring + from * Core::kStageBytes, k0, lane);
+    if (k0 < here.x.hi) core.take(p, here, smem + (warp * NS + from) * Core::kStageBytes, k0, lane);
     __syncwarp();
     const bool last = here.unit + 1 == here.x.units;
-    if (last || here.at + 1 == end) {
+    if (last || here.at + kUnit >= end) {
       const bool whole = last && first_unit == 0;
       const int slot = 2 * blockIdx.x + (first_item ? 0 : 1);
       if (!whole && !last && first_unit == 0 && threadIdx.x == 0) {      // the first part of an item that goes on in other CTAs
-        const int64_t item_end = here.at + (here.x.units - here.unit);   // one past its last unit
+        const int64_t item_end = here.at + kUnit * (here.x.units - 1 - here.unit) + 1;   // one past where its last unit begins
         int cta = (int)((item_end - 1) * ctas / total);             // the CTA whose run holds its last unit
         while (run_begin(total, cta + 1, ctas) < item_end) ++cta;
         while (run_begin(total, cta, ctas) >= item_end) --cta;
@@ -1174,9 +1197,14 @@ int bma_paged_attn(const bma_paged_cache* cache, const bma_paged_attn_args* args
   p.page_shift = -1;
   for (int i = 0; i < 31; ++i)
     if (cache->page_size == 1 << i) p.page_shift = i;
-  p.scale_words = cache->dtype == BMA_DTYPE_MXFP4 && cache->d == 128 &&
+  const int64_t last_scale = (int64_t)(cache->pages - 1) * cache->scale_stride_page + (int64_t)(cache->page_size - 1) * cache->scale_stride_slot +
+                             (int64_t)(cache->Hkv - 1) * cache->scale_stride_head;
+  p.scale_words = cache->dtype == BMA_DTYPE_MXFP4 && cache->d == 128 && last_scale >= 0 && last_scale / 4 < (int64_t)kNowhere &&
                   ((reinterpret_cast<uintptr_t>(cache->k_scale) | reinterpret_cast<uintptr_t>(cache->v_scale) | (uintptr_t)cache->scale_stride_page |
                     (uintptr_t)cache->scale_stride_slot | (uintptr_t)cache->scale_stride_head) & 3) == 0;
+  p.scale_page = (uint32_t)(cache->scale_stride_page / 4);
+  p.scale_slot = (uint32_t)(cache->scale_stride_slot / 4);
+  p.scale_head = (uint32_t)(cache->scale_stride_head / 4);
   p.scale_log2 = args->scale * kLog2e;
   BMA_REQUIRE((p.status = device_status_ptr()) != nullptr, BMA_ERR_CUDA);
   p.part_o = static_cast<float*>(workspace);
