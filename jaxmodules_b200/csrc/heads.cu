@@ -965,51 +965,59 @@ __global__ void __launch_bounds__(1024) weight_sum_kernel(const float* partial, 
   }
 }
 
-// Pages back to dense rows: a thread moves 16 bytes of the output (8 values of a 4-bit cache) of keys and of values.
+// Pages back to dense rows: a thread moves 16 bytes of the output (8 values of a 4-bit cache) of keys and of values at a time.  A CTA takes kReadTokens
+// neighbouring tokens of a sequence, whose places it looks up at once, so that what then follows are loads that do not wait for one another.
+constexpr int kReadTokens = 16;
 template <int DTYPE>
 __global__ void __launch_bounds__(256) read_kv_kernel(const __grid_constant__ bma_paged_cache c, const int32_t* lengths, int L, const bma_tensor k, const bma_tensor v,
                                                       int* status) {
   using T = typename std::conditional<DTYPE == BMA_DTYPE_F32, float, __nv_bfloat16>::type;
   constexpr int VEC = Bits16<T>::n;
+  __shared__ int64_t held[kReadTokens], held_scale[kReadTokens];       // negative: nothing there
   const int per_head = c.d / VEC, per_token = c.Hkv * per_head;
-  const int64_t token = blockIdx.x * (int64_t)blockDim.y + threadIdx.y;
-  const int b = (int)(token / L), t = (int)(token - (int64_t)b * L);
-  if (b >= c.B) return;
-  int slot = 0, page = -1;
-  const bool there = t < __ldg(lengths + b);
-  if (there) {
-    page = page_of(c, b, t, slot);
-    if (page < 0 && threadIdx.x == 0) report_device_error(status, kStatusRead);
+  const int runs = (L + kReadTokens - 1) / kReadTokens, b = blockIdx.x / runs, t0 = (blockIdx.x - b * runs) * kReadTokens;
+  const int tid = threadIdx.y * blockDim.x + threadIdx.x, n = min(kReadTokens, L - t0);
+  if (tid < n) {
+    int slot = 0, page = -1;
+    if (t0 + tid < __ldg(lengths + b)) {
+      page = page_of(c, b, t0 + tid, slot);
+      if (page < 0) report_device_error(status, kStatusRead);
+    }
+    held[tid] = page < 0 ? -1 : (int64_t)page * c.stride_page + (int64_t)slot * c.stride_slot;
+    held_scale[tid] = page < 0 ? -1 : (int64_t)page * c.scale_stride_page + (int64_t)slot * c.scale_stride_slot;
   }
-  const int64_t held = page < 0 ? 0 : (int64_t)page * c.stride_page + (int64_t)slot * c.stride_slot;
-  const int64_t held_scale = page < 0 ? 0 : (int64_t)page * c.scale_stride_page + (int64_t)slot * c.scale_stride_slot;
+  __syncthreads();
   for (int i = threadIdx.x; i < per_token; i += blockDim.x) {
     const int h = i / per_head, at = (i - h * per_head) * VEC;
-    uint4 x[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-    if (page >= 0) {
+    T* to_k = static_cast<T*>(k.ptr) + b * k.stride_b + t0 * k.stride_l + h * k.stride_h + at;
+    T* to_v = static_cast<T*>(v.ptr) + b * v.stride_b + t0 * v.stride_l + h * v.stride_h + at;
+    const int64_t in_token = h * c.stride_head + (DTYPE == BMA_DTYPE_MXFP4 ? at / 2 : at), scale_in_token = h * c.scale_stride_head + at / 32;
+#pragma unroll 4
+    for (int t = threadIdx.y; t < n; t += blockDim.y) {
+      uint4 x[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+      const int64_t from = held[t];
+      if (from >= 0) {
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        if constexpr (DTYPE == BMA_DTYPE_MXFP4) {
-          const uint32_t codes = __ldg(reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(s ? c.v : c.k) + held + h * c.stride_head + at / 2));
-          const float f = e8m0_value(__ldg((s ? c.v_scale : c.k_scale) + held_scale + h * c.scale_stride_head + at / 32));
-          uint32_t pairs[4], w[4];
-          from_e2m1x8(codes, pairs);
+        for (int s = 0; s < 2; ++s) {
+          if constexpr (DTYPE == BMA_DTYPE_MXFP4) {
+            const uint32_t codes = __ldg(reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(s ? c.v : c.k) + from + in_token));
+            const float f = e8m0_value(__ldg((s ? c.v_scale : c.k_scale) + held_scale[t] + scale_in_token));
+            uint32_t pairs[4], w[4];
+            from_e2m1x8(codes, pairs);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&pairs[j]));
-            const __nv_bfloat162 r = __floats2bfloat162_rn(y.x * f, y.y * f);       // (exact: two significant bits)
-            w[j] = *reinterpret_cast<const uint32_t*>(&r);
+            for (int j = 0; j < 4; ++j) {
+              const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&pairs[j]));
+              const __nv_bfloat162 r = __floats2bfloat162_rn(y.x * f, y.y * f);       // (exact: two significant bits)
+              w[j] = *reinterpret_cast<const uint32_t*>(&r);
+            }
+            x[s] = make_uint4(w[0], w[1], w[2], w[3]);
+          } else {
+            x[s] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(s ? c.v : c.k) + from + in_token));
           }
-          x[s] = make_uint4(w[0], w[1], w[2], w[3]);
-        } else {
-          x[s] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(s ? c.v : c.k) + held + h * c.stride_head + at));
         }
       }
-    }
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const bma_tensor& o = s ? v : k;
-      *reinterpret_cast<uint4*>(static_cast<T*>(o.ptr) + b * o.stride_b + t * o.stride_l + h * o.stride_h + at) = x[s];
+      *reinterpret_cast<uint4*>(to_k + t * k.stride_l) = x[0];
+      *reinterpret_cast<uint4*>(to_v + t * v.stride_l) = x[1];
     }
   }
 }
@@ -1232,7 +1240,7 @@ int read_kv(const bma_paged_cache* c, const int32_t* lengths, int L, const bma_t
   BMA_REQUIRE(status != nullptr, BMA_ERR_CUDA);
   const int per_token = c->Hkv * c->d / vec;
   const int x = per_token >= 256 ? 256 : ((per_token + 31) & ~31), y = 256 / x;
-  const int64_t ctas = ((int64_t)c->B * L + y - 1) / y;
+  const int64_t ctas = (int64_t)c->B * ((L + kReadTokens - 1) / kReadTokens);
   BMA_REQUIRE(ctas < (1ll << 31), BMA_ERR_LIMIT);
   const dim3 block(x, y);
   if (c->dtype == BMA_DTYPE_F32) read_kv_kernel<BMA_DTYPE_F32><<<(unsigned)ctas, block, 0, st>>>(*c, lengths, L, *k, *v, status);

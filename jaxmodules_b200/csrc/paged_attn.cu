@@ -4,14 +4,16 @@
 // by memory.  What they have to do is to keep enough loads in flight, and to give every SM the same share of bytes whatever the
 // lengths are, which only the device knows.
 //
-// Work.  The walk over the keys of one (sequence, tile of rows, kv head) is an item, cut into units of a tile of keys for every warp.  All units of
-// all items lie on one line, each item's with room before them for what it takes to begin and finish an item (half a unit, 1.5 in FMA arithmetic: without it a sequence of one
+// Work.  The walk over the keys of one (sequence, tile of rows, group of kv heads) is an item.  The four warps of a CTA have a kv head each, so that they read
+// neighbouring bytes of the same tokens at about the same time (of a 4-bit cache, whose powers of two for 8 heads are one 32-byte sector, 1.8 times the bytes came
+// from memory when a CTA had one head), and no results to put together; with two or one head to a CTA, where their number allows no more or items are few, two
+// or four warps share one.  An item is cut into units, a tile of keys for every warp.  All units of all items lie on one line, each item's with room before them for what it takes to begin and finish an item (half a unit, 1.5 in FMA arithmetic: without it a sequence of one
 // token, 8 items to finish, kept its CTA for 9 us after the others).  The line is cut into as many even runs as CTAs fit on the chip; a run ends in the
 // middle of an item as a rule.  Each CTA finds its run from the lengths.  An item that lies within one run is finished there; the parts of others go to the
 // workspace, at most two from a CTA, and paged_join_kernel puts them together in the order of the keys.
 //
-// Within a CTA the four warps take tiles of a unit in turn, each with its own ring of stages in shared memory that it fills by cp.async: no warp
-// waits for another before the end of an item, and the ring runs on into the next item.  Pages are looked up for every key (any page
+// Each warp has its own ring of stages in shared memory that it fills by cp.async: no warp waits for another before the end of an item (nor there, with a
+// head of its own), and the ring runs on into the next item.  Pages are looked up for every key (any page
 // size), a tile ahead of the copy.
 //
 // Keys outside [lo, hi), which no row of the tile sees, are not read: zeros stand there.  Where the rows of a tile see different keys of a tile of
@@ -29,6 +31,7 @@ struct PagedParams {
   bma_paged_cache c;
   bma_paged_attn_args a;
   int G, rows, row_tiles, entries;     // query heads to a kv head, rows to a kv head, tiles of them, (sequence, tile) pairs
+  int heads, heads_log2, splits;       // kv heads to a CTA (1, 2, 4), warps to a head
   int positions;                       // what the page table covers
   int page_shift;                      // log2 of the page size, -1 where that is no power of two
   uint32_t page_units, slot_units, head_units;      // strides of the cache, in 16 bytes
@@ -36,9 +39,10 @@ struct PagedParams {
   uint32_t scale_page, scale_slot, scale_head;
   float scale_log2;
   int* status;
-  float* part_o;                       // [2 * CTAs][rows of a tile][DP]
-  float2* part_ml;                     // [2 * CTAs][rows of a tile]
-  int4* meta;                          // [CTAs]: item whose first part the CTA has (-1: none), slot of that part, CTA with the last part
+  float* part_o;                       // [2 * CTAs][heads][rows of a tile][DP]
+  float2* part_ml;                     // [2 * CTAs][heads][rows of a tile]
+  int by_item;                         // meta has a place for every item, else for every CTA, whichever are fewer:
+  int4* meta;                          // first CTA with a part of an item (-1: there are no parts to join), slot of its part, CTA with the last part, item
 };
 
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -115,7 +119,7 @@ __device__ __forceinline__ Entry entry_of(const PagedParams& p, int e) {
   x.all_to = x.first + x.t0;
   x.all_from = p.a.window < 0 ? x.lo : max(x.lo, (int)max((int64_t)x.first + x.t1 - p.a.window, (int64_t)0));
   x.base = x.lo & ~(TILE - 1);
-  x.units = max(1, (x.hi - x.base + kWarps * TILE - 1) / (kWarps * TILE));
+  x.units = max(1, (x.hi - x.base + p.splits * TILE - 1) / TILE >> (2 - p.heads_log2));      // (of splits * TILE keys)
   return x;
 }
 
@@ -124,18 +128,19 @@ constexpr int kUnit = 2;          // places of a unit
 template <int ROWS, int TILE, int ITEM>      // ITEM: places before the units of an item
 struct Cursor {
   Entry x;
-  int e, h, unit;
+  int e, h, unit;               // h: this warp's kv head
   int64_t at;
   __device__ __forceinline__ void next(const PagedParams& p) {
     at += kUnit;
     if (++unit < x.units) return;
     at += ITEM;
     unit = 0;
-    if (++h < p.c.Hkv) return;
-    h = 0;
+    h += p.heads;
+    if (h < p.c.Hkv) return;
+    h &= p.heads - 1;
     if (++e < p.entries) x = entry_of<ROWS, TILE>(p, e);
   }
-  __device__ __forceinline__ int tile(int warp) const { return x.base + (unit * kWarps + warp) * TILE; }
+  __device__ __forceinline__ int tile(const PagedParams& p, int warp) const { return x.base + (unit * p.splits + (warp >> p.heads_log2)) * TILE; }
 };
 
 // [begin, end) of CTA `cta`'s run
@@ -287,7 +292,7 @@ struct CoreBf16 {
   Place place;
 
   __device__ __forceinline__ void prepare(uint8_t*) {}
-  __device__ __forceinline__ void look_up(const PagedParams& p, const Cur& c, int warp, int lane) { place.look_up(p, c.x, c.tile(warp) + (lane & 15)); }
+  __device__ __forceinline__ void look_up(const PagedParams& p, const Cur& c, int warp, int lane) { place.look_up(p, c.x, c.tile(p, warp) + (lane & 15)); }
   __device__ __forceinline__ void settle(uint8_t*) {}
   __device__ __forceinline__ void issue(const PagedParams& p, const Cur& c, uint8_t* smem, int stage, int lane) {
     copy_rows<kTile, DP / 8, kSide>(p, place.at(p, c.h), p.c.d / 8, smem_at(smem) + stage, lane, [](int r, int chunk) { return r * kRowBytes + ((chunk ^ (r & 7)) << 4); });
@@ -433,7 +438,7 @@ struct Core4bit {
   int pending;                  // and where its stage lies, negative where there is none
 
   __device__ __forceinline__ void prepare(uint8_t*) { pending = -1; }
-  __device__ __forceinline__ void look_up(const PagedParams& p, const Cur& c, int warp, int lane) { place.look_up(p, c.x, c.tile(warp) + lane); }
+  __device__ __forceinline__ void look_up(const PagedParams& p, const Cur& c, int warp, int lane) { place.look_up(p, c.x, c.tile(p, warp) + lane); }
   // 16-byte chunks of a row are permuted so that 8 rows of a chunk lie in different banks
   static __device__ __forceinline__ int chunk_at(int r, int chunk) { return r * kRowBytes + ((DP == 128 ? chunk ^ (r >> 1 & 3) : chunk ^ (r >> 2 & 1)) << 4); }
 
@@ -703,7 +708,7 @@ struct CoreF32 {
   static constexpr int kDP = DP, kRows = ROWS, kTile = 16, kItem = 3, kStages = 2, kMinCtas = 1;
   static constexpr int kRowBytes = DP * 4, kSide = kTile * kRowBytes, kStageBytes = 2 * kSide;
   static constexpr int kQRow = DP + 4;         // floats: the second half of a row lies 4 further on, in other banks than the first
-  static constexpr int kExtra = ROWS * kQRow * 4 + kWarps * kTile * ROWS * 4;
+  static constexpr int kExtra = kWarps * (ROWS * kQRow + kTile * ROWS) * 4;
   static constexpr int kCols = DP / 32;
   using Cur = Cursor<kRows, kTile, kItem>;
 
@@ -713,25 +718,25 @@ struct CoreF32 {
   float *qs, *ps;
 
   __device__ __forceinline__ void prepare(uint8_t* extra) {
-    qs = reinterpret_cast<float*>(extra);
-    ps = qs + ROWS * kQRow + (threadIdx.x >> 5) * kTile * ROWS;
+    qs = reinterpret_cast<float*>(extra) + (threadIdx.x >> 5) * (ROWS * kQRow + kTile * ROWS);
+    ps = qs + ROWS * kQRow;
   }
-  __device__ __forceinline__ void look_up(const PagedParams& p, const Cur& c, int warp, int lane) { place.look_up(p, c.x, c.tile(warp) + (lane & 15)); }
+  __device__ __forceinline__ void look_up(const PagedParams& p, const Cur& c, int warp, int lane) { place.look_up(p, c.x, c.tile(p, warp) + (lane & 15)); }
   __device__ __forceinline__ void settle(uint8_t*) {}
   __device__ __forceinline__ void issue(const PagedParams& p, const Cur& c, uint8_t* smem, int stage, int lane) {
     copy_rows<kTile, DP / 4, kSide>(p, place.at(p, c.h), p.c.d / 4, smem_at(smem) + stage, lane, [](int r, int chunk) { return r * kRowBytes + ((chunk ^ (r & 7)) << 4); });
   }
   __device__ __forceinline__ void begin(const PagedParams& p, const Cur& c, int lane) {
     const int n = min(ROWS, p.rows - c.x.row0);
-    __syncthreads();             // (the last item's rows have been read)
-    for (int i = threadIdx.x; i < ROWS * DP; i += kThreads) {
+    __syncwarp();                // (the last item's rows have been read)
+    for (int i = lane; i < ROWS * DP; i += 32) {
       const int r = i / DP, d = i % DP, row = c.x.row0 + r;
       float x = 0.f;
       if (r < n && d < p.c.d)
         x = __ldg(static_cast<const float*>(p.a.q.ptr) + c.x.b * p.a.q.stride_b + (row / p.G) * p.a.q.stride_l + (c.h * p.G + row % p.G) * p.a.q.stride_h + d);
       qs[r * kQRow + d + (d >= DP / 2 ? 4 : 0)] = x;
     }
-    __syncthreads();
+    __syncwarp();
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
       m[r] = -INFINITY;
@@ -857,21 +862,24 @@ __device__ __forceinline__ void write_result(const PagedParams& p, int b, int h,
   if (col == 0 && p.a.lse) p.a.lse[((int64_t)b * p.a.Hq + head) * p.a.T + t] = any ? fmaf(top, kLn2, logf(sum)) : -INFINITY;
 }
 
-// The warps' parts of an item put together: written as the result where the CTA has all of it, else as a part.
+// A head's item, of one warp or put together from those that share the head: written as the result where the CTA has all of it, else as a part.
 template <class Core>
 __device__ __forceinline__ void finish(const PagedParams& p, Core& core, const typename Core::Cur& c, bool whole, int slot, const Buffer<Core::kDP>& buffer, int warp, int lane) {
   constexpr int DP = Core::kDP;
+  const auto meet = [&] {
+    if (p.splits == 1) __syncwarp();
+    else __syncthreads();
+  };
+  const int mine = warp & (p.heads - 1), of_head = (warp >> p.heads_log2) * 32 + lane;      // this warp's head of the CTA's; the thread among those of the head
   core.stats(buffer, warp, lane);
-  __syncthreads();
+  meet();
   const int n = min(Core::kRows, p.rows - c.x.row0);
   auto joined = [&](int row, float& top, float& sum) {      // over the warps; what their exponents are taken against
     top = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, buffer.stat(w, row).x);
+    for (int w = mine; w < kWarps; w += p.heads) top = fmaxf(top, buffer.stat(w, row).x);
     const float base = top == -INFINITY ? 0.f : top;
     sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = mine; w < kWarps; w += p.heads) {
       const float2 x = buffer.stat(w, row);
       sum = fmaf(x.y, exp2_approx(x.x - base), sum);
     }
@@ -883,25 +891,24 @@ __device__ __forceinline__ void finish(const PagedParams& p, Core& core, const t
       const float base = joined(row, top, sum);
       return exp2_approx(buffer.stat(warp, row).x - base);
     }, buffer.line(warp, 0), lane);
-    __syncthreads();
-    for (int i = threadIdx.x; i < 8 * (DP / 4); i += kThreads) {
+    meet();
+    for (int i = of_head; i < 8 * (DP / 4); i += p.splits * 32) {
       const int r = i / (DP / 4), col = i % (DP / 4) * 4, row = pass * 8 + r;
       if (row >= n) break;
-      float4 x = *reinterpret_cast<const float4*>(buffer.line(0, r) + col);
-#pragma unroll
-      for (int w = 1; w < kWarps; ++w) {
+      float4 x = *reinterpret_cast<const float4*>(buffer.line(mine, r) + col);
+      for (int w = mine + p.heads; w < kWarps; w += p.heads) {
         const float4 y = *reinterpret_cast<const float4*>(buffer.line(w, r) + col);
         x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
       }
       float top, sum;
       joined(row, top, sum);
       if (!whole) {
-        const int64_t at = (int64_t)slot * Core::kRows + row;
+        const int64_t at = ((int64_t)slot * p.heads + mine) * Core::kRows + row;
         *reinterpret_cast<float4*>(p.part_o + at * DP + col) = x;
         if (col == 0) p.part_ml[at] = make_float2(top, sum);
       } else write_result(p, c.x.b, c.h, c.x.row0 + row, (c.x.row0 + row) / p.G < c.x.count, col, x, top, sum);
     }
-    __syncthreads();
+    meet();
   }
 }
 
@@ -940,8 +947,9 @@ __global__ void __launch_bounds__(kThreads, Core::kMinCtas) paged_kernel(const _
     block_scan(own, before, all);
     total += all;
   }
-  total *= p.c.Hkv;
-  if (threadIdx.x == 0) p.meta[blockIdx.x] = make_int4(-1, 0, 0, 0);
+  const int groups = p.c.Hkv >> p.heads_log2;
+  total *= groups;
+  if (threadIdx.x == 0 && !p.by_item) p.meta[blockIdx.x] = make_int4(-1, 0, 0, 0);
   const int ctas = (int)min((int64_t)gridDim.x, max(total / kUnit, (int64_t)1));       // (within an item every run has a unit's beginning)
   if (blockIdx.x >= ctas) return;
   const int64_t begin = run_begin(total, blockIdx.x, ctas), end = run_begin(total, blockIdx.x + 1, ctas);
@@ -951,8 +959,8 @@ __global__ void __launch_bounds__(kThreads, Core::kMinCtas) paged_kernel(const _
       own = places_of(e0 + threadIdx.x);
       block_scan(own, before, all);
     }
-    const int64_t from = (gone + before) * p.c.Hkv;
-    if (begin >= from && begin < from + (int64_t)own * p.c.Hkv) {
+    const int64_t from = (gone + before) * groups;
+    if (begin >= from && begin < from + (int64_t)own * groups) {
       scan[kWarps + 1] = e0 + threadIdx.x;
       scan[kWarps + 2] = begin - from;
     }
@@ -964,8 +972,9 @@ __global__ void __launch_bounds__(kThreads, Core::kMinCtas) paged_kernel(const _
   const int64_t within = scan[kWarps + 2];
   next.x = entry_of<Core::kRows, Core::kTile>(p, next.e);
   const int places = Core::kItem + kUnit * next.x.units;
-  next.h = (int)(within / places);
-  const int inside = (int)(within - (int64_t)next.h * places);                      // of the item
+  const int group = (int)(within / places);
+  const int inside = (int)(within - (int64_t)group * places);                       // of the item
+  next.h = group * p.heads + (warp & (p.heads - 1));
   next.unit = max(inside - Core::kItem + kUnit - 1, 0) / kUnit;                           // the first unit that begins in the run
   next.at = begin - inside + Core::kItem + kUnit * next.unit;
   if (next.unit >= next.x.units) {                                                  // (that is the next item's)
@@ -1004,19 +1013,22 @@ __global__ void __launch_bounds__(kThreads, Core::kMinCtas) paged_kernel(const _
       first_unit = here.unit;
       fresh = false;
     }
-    const int k0 = here.tile(warp);
+    const int k0 = here.tile(p, warp);
     if (k0 < here.x.hi) core.take(p, here, smem + (warp * NS + from) * Core::kStageBytes, k0, lane);
     __syncwarp();
     const bool last = here.unit + 1 == here.x.units;
     if (last || here.at + kUnit >= end) {
       const bool whole = last && first_unit == 0;
       const int slot = 2 * blockIdx.x + (first_item ? 0 : 1);
-      if (!whole && !last && first_unit == 0 && threadIdx.x == 0) {      // the first part of an item that goes on in other CTAs
-        const int64_t item_end = here.at + kUnit * (here.x.units - 1 - here.unit) + 1;   // one past where its last unit begins
-        int cta = (int)((item_end - 1) * ctas / total);             // the CTA whose run holds its last unit
-        while (run_begin(total, cta + 1, ctas) < item_end) ++cta;
-        while (run_begin(total, cta, ctas) >= item_end) --cta;
-        p.meta[blockIdx.x] = make_int4(here.e, here.h, slot, cta);
+      if (first_unit == 0 && threadIdx.x == 0) {        // the first part of an item, or all of it
+        const int item = here.e * groups + (here.h >> p.heads_log2);
+        if (!whole) {
+          const int64_t item_end = here.at + kUnit * (here.x.units - 1 - here.unit) + 1;   // one past where its last unit begins
+          int cta = (int)((item_end - 1) * ctas / total);             // the CTA whose run holds that
+          while (run_begin(total, cta + 1, ctas) < item_end) ++cta;
+          while (run_begin(total, cta, ctas) >= item_end) --cta;
+          p.meta[p.by_item ? item : blockIdx.x] = make_int4(blockIdx.x, slot, cta, item);
+        } else if (p.by_item) p.meta[item] = make_int4(-1, 0, 0, 0);
       }
       const Buffer<Core::kDP> buffer{smem + from * Core::kStageBytes, NS * Core::kStageBytes};
       finish<Core>(p, core, here, whole, slot, buffer, warp, lane);
@@ -1029,18 +1041,19 @@ __global__ void __launch_bounds__(kThreads, Core::kMinCtas) paged_kernel(const _
   copies_awaited<0>();
 }
 
-// One CTA: a row of an item that several CTAs had parts of, its warps taking parts in turn.
+// One CTA: a row of a head of an item that several CTAs had parts of, its warps taking parts in turn.
 template <int DP, int ROWS>
 __global__ void __launch_bounds__(kThreads) paged_join_kernel(const __grid_constant__ PagedParams p) {
   __shared__ float4 sums[kWarps][DP / 4];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int4 m = p.meta[blockIdx.x];
   if (m.x < 0) return;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.y;
-  const int b = m.x / p.row_tiles, row0 = (m.x - b * p.row_tiles) * ROWS;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, mine = blockIdx.y & (p.heads - 1), row = blockIdx.y >> p.heads_log2;
+  const int groups = p.c.Hkv >> p.heads_log2, e = m.w / groups, head = (m.w - e * groups) * p.heads + mine;
+  const int b = e / p.row_tiles, row0 = (e - b * p.row_tiles) * ROWS;
   if (row >= min(ROWS, p.rows - row0)) return;
-  const int parts = m.w - blockIdx.x + 1;
-  auto slot = [&](int i) { return (int64_t)(i == 0 ? m.z : 2 * (blockIdx.x + i)) * ROWS + row; };
+  const int parts = m.z - m.x + 1;
+  auto slot = [&](int i) { return ((int64_t)(i == 0 ? m.y : 2 * (m.x + i)) * p.heads + mine) * ROWS + row; };
   float top = -INFINITY;
   for (int i = lane; i < parts; i += 32) top = fmaxf(top, p.part_ml[slot(i)].x);
 #pragma unroll
@@ -1076,7 +1089,7 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(const __grid_const
     x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
   }
   const bool real = (row0 + row) / p.G < new_tokens(p.a.lengths, p.a.new_lengths, b, p.a.T).count;
-  write_result(p, b, m.y, row0 + row, real, lane * 4, x, top, sum);
+  write_result(p, b, head, row0 + row, real, lane * 4, x, top, sum);
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------
@@ -1096,9 +1109,10 @@ int validate_paged(const bma_paged_cache* c, const bma_paged_attn_args* a) {
 }
 
 struct PagedLaunch {
-  int rows_of_tile, dp, tile, ctas_per_sm;
-  int ctas, entries, row_tiles;
-  size_t bytes() const { return (size_t)ctas * (2 * (size_t)rows_of_tile * (dp * 4 + 8) + 16); }
+  int rows_of_tile, dp, tile, ctas_per_sm, heads;
+  int ctas, entries, row_tiles, groups;
+  int metas() const { return (int)std::min<int64_t>(ctas, (int64_t)entries * groups); }
+  size_t bytes() const { return (size_t)ctas * 2 * heads * rows_of_tile * (dp * 4 + 8) + (size_t)metas() * 16; }
 };
 
 // The instance for a call: heads of up to 64 or 128 components; tiles of as many rows as the call has, up to 32 on the tensor core (more would not
@@ -1113,8 +1127,17 @@ bool plan_paged(const bma_paged_cache& c, const bma_paged_attn_args& a, PagedLau
   const int64_t entries = (int64_t)c.B * l.row_tiles;
   if (entries >= (1 << 30)) return false;
   l.entries = (int)entries;
-  const int64_t units = entries * c.Hkv * (((int64_t)c.width * c.page_size + kWarps * l.tile - 1) / (kWarps * l.tile) + 1);
-  l.ctas = (int)std::min<int64_t>((int64_t)device_sms(current_device()) * l.ctas_per_sm, units);
+  // Heads to a CTA: as many as there are warps, as long as the CTAs do not get more than 8 parts of an item.  (64 sequences of up to 8192 tokens, 8 kv heads of 128, 128
+  // items for 444 CTAs: 4 bits 119 us with four heads, 140 with one, bfloat16 225 and 224; one sequence of 131072, four tokens, 2 or 8 items for 296 CTAs: 92 and 81,
+  // for four times the parts.)
+  const int64_t at_once = (int64_t)device_sms(current_device()) * l.ctas_per_sm;
+  l.heads = c.Hkv % 4 == 0 ? 4 : c.Hkv % 2 == 0 ? 2 : 1;
+  if (entries * (c.Hkv / l.heads) * 8 < at_once) l.heads = 1;
+  const int64_t keys = kWarps / l.heads * l.tile;      // of a unit
+  l.groups = c.Hkv / l.heads;
+  if (entries * l.groups >= (1ll << 31)) return false;
+  const int64_t units = entries * l.groups * (((int64_t)c.width * c.page_size + keys - 1) / keys + 1);
+  l.ctas = (int)std::min<int64_t>(at_once, units);
   return true;
 }
 
@@ -1130,7 +1153,7 @@ int launch_paged(const PagedParams& p, const PagedLaunch& l, cudaStream_t st) {
   paged_kernel<Core><<<l.ctas, kThreads, smem, st>>>(p);
   BMA_CUDA_TRY(cudaGetLastError());
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(l.ctas, std::min(Core::kRows, p.rows));
+  cfg.gridDim = dim3(l.metas(), std::min(Core::kRows, p.rows) * p.heads);
   cfg.blockDim = dim3(kThreads);
   cfg.stream = st;
   cudaLaunchAttribute attr{};
@@ -1189,6 +1212,10 @@ int bma_paged_attn(const bma_paged_cache* cache, const bma_paged_attn_args* args
   p.rows = args->T * p.G;
   p.row_tiles = l.row_tiles;
   p.entries = l.entries;
+  p.by_item = (int64_t)l.entries * l.groups <= l.ctas;
+  p.heads = l.heads;
+  p.heads_log2 = l.heads / 2;
+  p.splits = kWarps / l.heads;
   p.positions = cache->width * cache->page_size;
   const int64_t bytes = cache->dtype == BMA_DTYPE_F32 ? 4 : cache->dtype == BMA_DTYPE_BF16 ? 2 : 1;      // (their products fit 32 bits: validate_paged)
   p.page_units = (uint32_t)(cache->stride_page * bytes / 16);
@@ -1208,8 +1235,8 @@ int bma_paged_attn(const bma_paged_cache* cache, const bma_paged_attn_args* args
   p.scale_log2 = args->scale * kLog2e;
   BMA_REQUIRE((p.status = device_status_ptr()) != nullptr, BMA_ERR_CUDA);
   p.part_o = static_cast<float*>(workspace);
-  p.part_ml = reinterpret_cast<float2*>(p.part_o + (size_t)2 * l.ctas * l.rows_of_tile * l.dp);
-  p.meta = reinterpret_cast<int4*>(p.part_ml + (size_t)2 * l.ctas * l.rows_of_tile);
+  p.part_ml = reinterpret_cast<float2*>(p.part_o + (size_t)2 * l.ctas * l.heads * l.rows_of_tile * l.dp);
+  p.meta = reinterpret_cast<int4*>(p.part_ml + (size_t)2 * l.ctas * l.heads * l.rows_of_tile);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return l.dp == 64 ? dispatch_paged<64>(p, l, st) : dispatch_paged<128>(p, l, st);
 }

@@ -105,6 +105,9 @@ ATTEND = [
     ([20000], 1, 16, 2, 128, 16),
     ([20000], 2, 4, 1, 64, 256),
     ([33], 33, 4, 1, 64, 16),                     # a whole prompt
+    (list(range(0, 480, 8)), 1, 8, 4, 128, 16),   # many sequences: four kv heads to a CTA
+    (list(range(1, 400, 6)), 3, 4, 2, 64, 16),    # two kv heads
+    (list(range(1, 300, 5)) + [9000], 2, 32, 8, 128, 16),      # a long one among them
 ]
 
 
