@@ -702,12 +702,13 @@ struct Core4bit {
 };
 
 // ---- float32: FMA arithmetic ----------------------------------------------------------------------------------------------
-// For the scores two lanes share a key, for the sums a lane has DP / 32 columns; the rows of Q are read from shared memory, by all lanes at once.
+// For the scores two or four lanes share a key, for the sums a lane has DP / 32 columns; the rows of Q are read from shared memory, by all lanes at once.
 template <int DP, int ROWS>
 struct CoreF32 {
-  static constexpr int kDP = DP, kRows = ROWS, kTile = 16, kItem = 3, kStages = 2, kMinCtas = 1;
+  static constexpr int kDP = DP, kRows = ROWS, kTile = DP == 128 ? 8 : 16, kItem = 3, kStages = DP == 128 ? 3 : 2, kMinCtas = DP == 64 && ROWS <= 4 ? 3 : 2;
   static constexpr int kRowBytes = DP * 4, kSide = kTile * kRowBytes, kStageBytes = 2 * kSide;
-  static constexpr int kQRow = DP + 4;         // floats: the second half of a row lies 4 further on, in other banks than the first
+  static constexpr int kParts = 32 / kTile, kChunks = DP / 4 / kParts;      // lanes to a key, 16-byte chunks to each of them
+  static constexpr int kQRow = DP + 4 * kParts;      // floats: each part of a row lies 4 further on than the one before would have it, in other banks
   static constexpr int kExtra = kWarps * (ROWS * kQRow + kTile * ROWS) * 4;
   static constexpr int kCols = DP / 32;
   using Cur = Cursor<kRows, kTile, kItem>;
@@ -721,7 +722,7 @@ struct CoreF32 {
     qs = reinterpret_cast<float*>(extra) + (threadIdx.x >> 5) * (ROWS * kQRow + kTile * ROWS);
     ps = qs + ROWS * kQRow;
   }
-  __device__ __forceinline__ void look_up(const PagedParams& p, const Cur& c, int warp, int lane) { place.look_up(p, c.x, c.tile(p, warp) + (lane & 15)); }
+  __device__ __forceinline__ void look_up(const PagedParams& p, const Cur& c, int warp, int lane) { place.look_up(p, c.x, c.tile(p, warp) + (lane & (kTile - 1))); }
   __device__ __forceinline__ void settle(uint8_t*) {}
   __device__ __forceinline__ void issue(const PagedParams& p, const Cur& c, uint8_t* smem, int stage, int lane) {
     copy_rows<kTile, DP / 4, kSide>(p, place.at(p, c.h), p.c.d / 4, smem_at(smem) + stage, lane, [](int r, int chunk) { return r * kRowBytes + ((chunk ^ (r & 7)) << 4); });
@@ -734,7 +735,7 @@ struct CoreF32 {
       float x = 0.f;
       if (r < n && d < p.c.d)
         x = __ldg(static_cast<const float*>(p.a.q.ptr) + c.x.b * p.a.q.stride_b + (row / p.G) * p.a.q.stride_l + (c.h * p.G + row % p.G) * p.a.q.stride_h + d);
-      qs[r * kQRow + d + (d >= DP / 2 ? 4 : 0)] = x;
+      qs[r * kQRow + d + d / (4 * kChunks) * 4] = x;
     }
     __syncwarp();
 #pragma unroll
@@ -746,24 +747,27 @@ struct CoreF32 {
     }
   }
   __device__ __forceinline__ void take(const PagedParams& p, const Cur& c, const uint8_t* stage, int k0, int lane) {
-    const int key = lane & 15, half = lane >> 4;
+    const int key = lane & (kTile - 1), part = lane / kTile;
     float s[ROWS];
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) s[r] = 0.f;
 #pragma unroll 4
-    for (int i = 0; i < DP / 8; ++i) {
-      const int chunk = half * (DP / 8) + i;
+    for (int i = 0; i < kChunks; ++i) {
+      const int chunk = part * kChunks + i;
       const float4 k = *reinterpret_cast<const float4*>(stage + key * kRowBytes + ((chunk ^ (key & 7)) << 4));
 #pragma unroll
       for (int r = 0; r < ROWS; ++r) {
-        const float4 x = *reinterpret_cast<const float4*>(qs + r * kQRow + chunk * 4 + half * 4);
+        const float4 x = *reinterpret_cast<const float4*>(qs + r * kQRow + chunk * 4 + part * 4);
         s[r] = fmaf(x.x, k.x, fmaf(x.y, k.y, fmaf(x.z, k.z, fmaf(x.w, k.w, s[r]))));
       }
     }
     const bool cut = c.x.cut(k0, kTile);
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
-      float x = (s[r] + __shfl_xor_sync(0xffffffffu, s[r], 16)) * p.scale_log2;
+      float x = s[r];
+#pragma unroll
+      for (int b = kTile; b < 32; b <<= 1) x += __shfl_xor_sync(0xffffffffu, x, b);
+      x *= p.scale_log2;
       bool seen = true;
       if (cut) {
         rarely();
@@ -773,7 +777,7 @@ struct CoreF32 {
       }
       float top = fmaxf(m[r], x);
 #pragma unroll
-      for (int b = 1; b < 16; b <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, b));
+      for (int b = 1; b < kTile; b <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, b));
       const float base = top == -INFINITY ? 0.f : top;
       if (top != m[r]) {
         const float f = exp2_approx(m[r] - base);
@@ -789,7 +793,7 @@ struct CoreF32 {
     const bool strict = cut && p.a.T > 1;      // some row sees what another does not
 #pragma unroll
     for (int r = 0; r < ROWS; ++r)
-      if (half == 0) ps[key * ROWS + r] = s[r] == -1.f && !strict ? 0.f : s[r];
+      if (part == 0) ps[key * ROWS + r] = s[r] == -1.f && !strict ? 0.f : s[r];
     __syncwarp();
 #pragma unroll 4
     for (int k = 0; k < kTile; ++k) {
@@ -802,12 +806,17 @@ struct CoreF32 {
         const float2 x = *reinterpret_cast<const float2*>(row + (((lane >> 1) ^ (k & 7)) << 4) + (lane & 1) * 8);
         v[0] = x.x; v[1] = x.y;
       }
+      constexpr int kAtOnce = ROWS < 4 ? ROWS : 4;
 #pragma unroll
-      for (int r4 = 0; r4 < ROWS; r4 += 4) {
-        const float4 w4 = *reinterpret_cast<const float4*>(ps + k * ROWS + r4);
-        const float w[4] = {w4.x, w4.y, w4.z, w4.w};
+      for (int r4 = 0; r4 < ROWS; r4 += kAtOnce) {
+        float w[4];
+        if constexpr (ROWS == 1) w[0] = ps[k];
+        else {
+          const float4 w4 = *reinterpret_cast<const float4*>(ps + k * ROWS + r4);
+          w[0] = w4.x; w[1] = w4.y; w[2] = w4.z; w[3] = w4.w;
+        }
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
+        for (int r = 0; r < kAtOnce; ++r)
 #pragma unroll
           for (int j = 0; j < kCols; ++j) {
             if (strict && w[r] == -1.f) continue;
@@ -822,7 +831,7 @@ struct CoreF32 {
     for (int r = 0; r < ROWS; ++r) {
       float x = l[r];
 #pragma unroll
-      for (int b = 1; b < 16; b <<= 1) x += __shfl_xor_sync(0xffffffffu, x, b);
+      for (int b = 1; b < kTile; b <<= 1) x += __shfl_xor_sync(0xffffffffu, x, b);
       if (lane == 0) buffer.stat(warp, r) = make_float2(m[r], x);
     }
   }
@@ -1120,9 +1129,9 @@ struct PagedLaunch {
 bool plan_paged(const bma_paged_cache& c, const bma_paged_attn_args& a, PagedLaunch& l) {
   const int rows = a.T * (a.Hq / c.Hkv);
   l.dp = c.d <= 64 ? 64 : 128;
-  l.tile = c.dtype == BMA_DTYPE_MXFP4 ? 32 : 16;
-  l.rows_of_tile = c.dtype == BMA_DTYPE_F32 && rows <= 4 ? 4 : rows <= 8 ? 8 : c.dtype == BMA_DTYPE_F32 || rows <= 16 ? 16 : 32;
-  l.ctas_per_sm = c.dtype == BMA_DTYPE_F32 ? (l.dp == 128 ? 1 : 2) : l.rows_of_tile == 8 ? 3 : 2;
+  l.tile = c.dtype == BMA_DTYPE_MXFP4 ? 32 : c.dtype == BMA_DTYPE_F32 && l.dp == 128 ? 8 : 16;
+  l.rows_of_tile = c.dtype == BMA_DTYPE_F32 && rows <= 4 ? (rows == 1 ? 1 : 4) : rows <= 8 ? 8 : c.dtype == BMA_DTYPE_F32 || rows <= 16 ? 16 : 32;
+  l.ctas_per_sm = (c.dtype == BMA_DTYPE_F32 ? l.dp == 64 && l.rows_of_tile <= 4 : l.rows_of_tile == 8) ? 3 : 2;
   l.row_tiles = ceil_div(rows, l.rows_of_tile);
   const int64_t entries = (int64_t)c.B * l.row_tiles;
   if (entries >= (1 << 30)) return false;
@@ -1170,6 +1179,7 @@ template <int DP>
 int dispatch_paged(const PagedParams& p, const PagedLaunch& l, cudaStream_t st) {
   switch (p.c.dtype) {
     case BMA_DTYPE_F32:
+      if (l.rows_of_tile == 1) return launch_paged<CoreF32<DP, 1>>(p, l, st);
       if (l.rows_of_tile == 4) return launch_paged<CoreF32<DP, 4>>(p, l, st);
       if (l.rows_of_tile == 8) return launch_paged<CoreF32<DP, 8>>(p, l, st);
       return launch_paged<CoreF32<DP, 16>>(p, l, st);
