@@ -282,7 +282,7 @@ __device__ __forceinline__ void copy_rows(const PagedParams& p, uint32_t mine, i
 // tile, where rows as M would make 16 of one.  The weights go from the accumulators of the one to the operand of the other by movmatrix.
 template <int DP, int NT>
 struct CoreBf16 {
-  static constexpr int kDP = DP, kRows = NT * 8, kTile = 16, kItem = 1, kStages = DP == 128 ? (NT == 1 ? 2 : 3) : 4, kMinCtas = NT == 1 ? 3 : 2;
+  static constexpr int kDP = DP, kRows = NT * 8, kTile = 16, kItem = 1, kStages = DP == 128 ? (NT == 1 ? 2 : 3) : 4, kMinCtas = NT == 1 ? 3 : 2;      // (two stages and three CTAs 220 us, three and two 238: 64 sequences of up to 8192)
   static constexpr int kRowBytes = DP * 2, kSide = kTile * kRowBytes, kStageBytes = 2 * kSide, kExtra = 0;
   using Cur = Cursor<kRows, kTile, kItem>;
 
@@ -422,7 +422,7 @@ struct CoreBf16 {
 // (turned: of two keys), and they are taken in the order in which they come.
 template <int DP, int NT>
 struct Core4bit {
-  static constexpr int kDP = DP, kRows = NT * 8, kTile = 32, kItem = 1, kStages = 3, kMinCtas = NT == 1 ? 3 : 2;
+  static constexpr int kDP = DP, kRows = NT * 8, kTile = 32, kItem = 1, kStages = 2, kMinCtas = NT > 1 ? 2 : DP == 64 ? 4 : 3;
   static constexpr int kRowBytes = DP / 2, kSide = kTile * kRowBytes, kGroups = DP / 32;
   // after keys and values: powers of keys [32][4] (float32), of values [4][32] (float16, by key_of's rows), E and 2^-E of values [32][2]
   static constexpr int kKeyPowers = 2 * kSide, kValuePowers = kKeyPowers + 512, kTops = kValuePowers + 256, kStageBytes = kTops + 256, kExtra = 0;
@@ -786,7 +786,7 @@ struct CoreF32 {
         for (int j = 0; j < kCols; ++j) o[r][j] *= f;
         m[r] = top;
       }
-      x = exp2f(x - base);
+      x = exp2_approx(x - base);
       l[r] += x;
       s[r] = seen ? x : -1.f;
     }
@@ -1124,14 +1124,17 @@ struct PagedLaunch {
   size_t bytes() const { return (size_t)ctas * 2 * heads * rows_of_tile * (dp * 4 + 8) + (size_t)metas() * 16; }
 };
 
-// The instance for a call: heads of up to 64 or 128 components; tiles of as many rows as the call has, up to 32 on the tensor core (more would not
-// leave room for the sums in registers) and 16 in FMA arithmetic.  As many CTAs as run at once, or as there can be units.
+// The instance for a call: heads of up to 64 or 128 components; tiles of as many rows as the call has, up to 16: more do not leave room for the sums in
+// registers (32 sequences of up to 8192 tokens with 28 rows to a kv head of 128, bfloat16, 353 us in one tile of 32, 257 in two of 16, the second of which finds
+// the keys in the L2).
+// As many CTAs as run at once, or as there can be units.
 bool plan_paged(const bma_paged_cache& c, const bma_paged_attn_args& a, PagedLaunch& l) {
   const int rows = a.T * (a.Hq / c.Hkv);
   l.dp = c.d <= 64 ? 64 : 128;
   l.tile = c.dtype == BMA_DTYPE_MXFP4 ? 32 : c.dtype == BMA_DTYPE_F32 && l.dp == 128 ? 8 : 16;
-  l.rows_of_tile = c.dtype == BMA_DTYPE_F32 && rows <= 4 ? (rows == 1 ? 1 : 4) : rows <= 8 ? 8 : c.dtype == BMA_DTYPE_F32 || rows <= 16 ? 16 : 32;
-  l.ctas_per_sm = (c.dtype == BMA_DTYPE_F32 ? l.dp == 64 && l.rows_of_tile <= 4 : l.rows_of_tile == 8) ? 3 : 2;
+  l.rows_of_tile = c.dtype == BMA_DTYPE_F32 && rows <= 4 ? (rows == 1 ? 1 : 4) : rows <= 8 ? 8 : 16;
+  // (what registers and shared memory allow; the kMinCtas of the instances)
+  l.ctas_per_sm = c.dtype == BMA_DTYPE_F32 ? (l.dp == 64 && l.rows_of_tile <= 4 ? 3 : 2) : l.rows_of_tile > 8 ? 2 : c.dtype == BMA_DTYPE_MXFP4 && l.dp == 64 ? 4 : 3;
   l.row_tiles = ceil_div(rows, l.rows_of_tile);
   const int64_t entries = (int64_t)c.B * l.row_tiles;
   if (entries >= (1 << 30)) return false;
@@ -1185,10 +1188,10 @@ int dispatch_paged(const PagedParams& p, const PagedLaunch& l, cudaStream_t st) 
       return launch_paged<CoreF32<DP, 16>>(p, l, st);
     case BMA_DTYPE_BF16:
       if (l.rows_of_tile == 8) return launch_paged<CoreBf16<DP, 1>>(p, l, st);
-      return l.rows_of_tile == 16 ? launch_paged<CoreBf16<DP, 2>>(p, l, st) : launch_paged<CoreBf16<DP, 4>>(p, l, st);
+      return launch_paged<CoreBf16<DP, 2>>(p, l, st);
     default:
       if (l.rows_of_tile == 8) return launch_paged<Core4bit<DP, 1>>(p, l, st);
-      return l.rows_of_tile == 16 ? launch_paged<Core4bit<DP, 2>>(p, l, st) : launch_paged<Core4bit<DP, 4>>(p, l, st);
+      return launch_paged<Core4bit<DP, 2>>(p, l, st);
   }
 }
 
