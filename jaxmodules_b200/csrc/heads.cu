@@ -151,8 +151,22 @@ struct Side {
   int before;            // heads of the sides before
 };
 
+// Division of numbers below 2^31 by one that a launch fixes: n * m >> 31 + s with m = ceil(2^(31 + s) / d), 2^s >= d, whose error n / 2^31 * d' / d < 1 / d is too
+// small to reach the next whole number.
+struct Divider {
+  uint32_t m, s, d;
+  __device__ __forceinline__ int operator()(int n) const { return d == 1 ? n : (int)(((uint64_t)(uint32_t)n * m) >> 31 >> s); }
+};
+inline Divider divider(int d) {
+  Divider r{0, 0, (uint32_t)d};
+  while ((1u << r.s) < r.d) ++r.s;
+  r.m = (uint32_t)((((uint64_t)1 << (31 + r.s)) + r.d - 1) / r.d);
+  return r;
+}
+
 struct HeadsParams {
   Side side[3];          // q, k, v
+  Divider by_length, by_slabs;
   int B, L, d, slabs, slab_heads;
   HeadMap map;
   const double* frequencies;
@@ -527,18 +541,21 @@ struct Unit {
 __device__ __forceinline__ float2 swapped(float2 v) { return make_float2(v.y, v.x); }
 __device__ __forceinline__ float2 twice(float x) { return make_float2(x, x); }
 
-// 64-bit steps of the pairs (a CTA makes them once), and a warp's cosines and sines of a token.
+// 64-bit steps of the pairs (a CTA makes them once), and a warp's cosines and sines of a token, a gap after every unit's, so that lanes read from different banks.
 constexpr int kPairs = 128;
+template <int VEC>
+constexpr int kTurns = kPairs / VEC * (VEC + 1);
 __device__ __forceinline__ void make_steps(unsigned long long* steps, const double* frequencies, int pairs) {
   for (int i = threadIdx.x; i < pairs; i += blockDim.x) steps[i] = step_of(__ldg(frequencies + i));
   __syncthreads();
 }
+template <int VEC>
 __device__ __forceinline__ void make_turns(float2* turns, const unsigned long long* steps, int pairs, long long position, float magnitude, int lane) {
   __syncwarp();            // (those of the last token have been read)
   for (int i = lane; i < pairs; i += 32) {
     float c, s;
     turn_of(steps[i], position, magnitude, c, s);
-    turns[i] = make_float2(c, s);
+    turns[i + i / VEC] = make_float2(c, s);
   }
   __syncwarp();
 }
@@ -575,9 +592,9 @@ struct RowsAhead {
   }
   __device__ __forceinline__ bool open(const HeadsParams& p) {
     if (item >= items) return false;
-    const int token = p.slabs == 1 ? item : item / p.slabs;
+    const int token = p.by_slabs(item);
     begin = (item - token * p.slabs) * p.slab_heads;
-    b = token / p.L;
+    b = p.by_length(token);
     t = token - b * p.L;
     real = KIND == kRotate || t < new_tokens(p.lengths, p.new_lengths, b, p.L).count;
     si = -1;
@@ -621,7 +638,7 @@ __global__ void __launch_bounds__(kHeadsThreads, 4) heads_wide_kernel(const __gr
   constexpr int VEC = Bits16<T>::n;
   constexpr bool HALF = LAYOUT == BMA_ROTARY_HALF;
   __shared__ unsigned long long steps[kPairs];
-  __shared__ float2 turns[kHeadsWarps][kPairs];
+  __shared__ float2 turns[kHeadsWarps][kTurns<VEC>];
   __shared__ uint4 rings[kHeadsWarps][kAhead][2][32];
   __shared__ __align__(16) float weights[2][2 * kPairs];
   __shared__ float rows[KIND == kAppend4 ? kHeadsWarps : 1][KIND == kAppend4 ? 8 : 1][KIND == kAppend4 ? kPagedHeadDim + 4 : 1];
@@ -649,15 +666,15 @@ __global__ void __launch_bounds__(kHeadsThreads, 4) heads_wide_kernel(const __gr
   int from = 0;
 #pragma unroll 1
   for (int item = first_item; item < items; item += stride) {
-    const int token = p.slabs == 1 ? item : item / p.slabs;
+    const int token = p.by_slabs(item);
     const int slab_begin = (item - token * p.slabs) * p.slab_heads, slab_end = slab_begin + p.slab_heads;
-    const int b = token / p.L, t = token - b * p.L;
+    const int b = p.by_length(token), t = token - b * p.L;
     long long position = t;
     bool real = true;
     int64_t held = 0, held_scale = 0;      // offsets of the token in the cache
     if constexpr (KIND == kRotate) position = position_of(p, b, t);
     else real = token_place(p, b, t, lane, position, held, held_scale);
-    if (pairs && real) make_turns(turns[warp], steps, pairs, position, p.back ? -p.magnitude : p.magnitude, lane);
+    if (pairs && real) make_turns<VEC>(turns[warp], steps, pairs, position, p.back ? -p.magnitude : p.magnitude, lane);
 #pragma unroll 1
     for (int si = 0; si < (KIND == kRotate ? 2 : 3); ++si) {
       const Side& side = p.side[si];
@@ -696,7 +713,7 @@ __global__ void __launch_bounds__(kHeadsThreads, 4) heads_wide_kernel(const __gr
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
           cs[j] = make_float2(1.f, 0.f);
-          if (side.turned && (FULL || live >> j & 1) && u * VEC + j < pairs) cs[j] = turns[warp][u * VEC + j];
+          if (side.turned && (FULL || live >> j & 1) && u * VEC + j < pairs) cs[j] = turns[warp][u * (VEC + 1) + j];
           if (p.back) cs[j].x = (FULL || live >> j & 1) ? -cs[j].x : cs[j].x;      // (-magnitude gave -cos and -sin)
         }
         if constexpr (HALF) {
@@ -777,7 +794,7 @@ __global__ void __launch_bounds__(kHeadsThreads, 4) rotate_back_wide_kernel(cons
   constexpr bool HALF = LAYOUT == BMA_ROTARY_HALF;
   constexpr int CS = HALF ? VEC / 2 : VEC;
   __shared__ unsigned long long steps[kPairs];
-  __shared__ float2 turns[kHeadsWarps][kPairs];
+  __shared__ float2 turns[kHeadsWarps][kTurns<VEC>];
   __shared__ uint4 rings[kHeadsWarps][kAhead][4][32];       // (the sums of the warps lie there at the end)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int tpr = p.map.tpr, group = lane / tpr, u = lane & (tpr - 1), groups = 32 / tpr, chunks = p.map.chunks;
@@ -855,10 +872,10 @@ __global__ void __launch_bounds__(kHeadsThreads, 4) rotate_back_wide_kernel(cons
     // cosines and sines of the unit's values: HALF, of pairs 2i and 2i + 1 and the sines with the other sign, too; else of both values of pair i, the sine
     // with its sign
     float2 c[CS], s[CS], ns[CS];
-    if (pairs) make_turns(turns[warp], steps, pairs, position_of(p, b, t), p.magnitude, lane);
+    if (pairs) make_turns<VEC>(turns[warp], steps, pairs, position_of(p, b, t), p.magnitude, lane);
 #pragma unroll
     for (int i = 0; i < CS; ++i) {
-      const auto at = [&](int j) { return (FULL || live >> j & 1) && u * VEC + j < pairs ? turns[warp][u * VEC + j] : make_float2(1.f, 0.f); };
+      const auto at = [&](int j) { return (FULL || live >> j & 1) && u * VEC + j < pairs ? turns[warp][u * (VEC + 1) + j] : make_float2(1.f, 0.f); };
       if constexpr (HALF) {
         const float2 x = at(2 * i), y = at(2 * i + 1);
         c[i] = make_float2(x.x, y.x);
@@ -1068,6 +1085,8 @@ int launch_heads(HeadsParams& p, const bma_rotary& r, bool wide, cudaStream_t st
   p.side[1].before = p.side[0].heads;
   p.side[2].before = p.side[0].heads + p.side[1].heads;
   BMA_REQUIRE(tokens * p.slabs < (1ll << 30), BMA_ERR_LIMIT);
+  p.by_length = divider(p.L);
+  p.by_slabs = divider(p.slabs);
   int64_t ctas = (tokens * p.slabs + kHeadsWarps - 1) / kHeadsWarps;
   if (wide) {
     ctas = std::min<int64_t>(ctas, (int64_t)device_sms(current_device()) * kHeadsCtas);
