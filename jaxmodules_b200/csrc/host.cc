@@ -461,6 +461,7 @@ struct RotateNode : torch::autograd::Function<RotateNode> {
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "rotate_heads has no second derivatives: do not ask for create_graph");
     const variable_list saved = ctx->get_saved_variables();
     const auto optional = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
     const Rotation r{optional(saved[2]), optional(saved[3]), (int)ctx->saved_data["layout"].toInt(), ctx->saved_data["magnitude"].toDouble(), optional(saved[4]),

@@ -6,7 +6,8 @@ The reference has no counterpart: its attention takes dense keys and values of t
     q = append_kv(cache, k, v, lengths, q=q, frequencies=f)      # [B, 1, H, d]
     o = paged_attention(q, cache, lengths)
 
-and both calls, like ``read_kv``, can be captured into a CUDA graph: everything that changes between steps lies on the device.
+and both calls, like ``read_kv``, can be captured into a CUDA graph (after a first call outside of one): everything that changes between steps lies
+on the device.
 """
 from __future__ import annotations
 

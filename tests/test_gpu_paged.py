@@ -108,6 +108,8 @@ ATTEND = [
     (list(range(0, 480, 8)), 1, 8, 4, 128, 16),   # many sequences: four kv heads to a CTA
     (list(range(1, 400, 6)), 3, 4, 2, 64, 16),    # two kv heads
     (list(range(1, 300, 5)) + [9000], 2, 32, 8, 128, 16),      # a long one among them
+    ([i * 7 % 50 for i in range(300)], 1, 4, 2, 64, 16),       # more sequences than a CTA has threads
+    ([i * 13 % 90 for i in range(700)] + [3000], 1, 6, 3, 64, 16),
 ]
 
 
@@ -119,6 +121,29 @@ def test_attention(case, kind):
     new = [T if n else 0 for n in lengths]
     c = make(kind, lengths, Hkv, d, page, seed=len(lengths) + T)
     check(queries(len(lengths), T, Hq, d, kind), c, lengths, new)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("d", [8, 40, 72, 120])
+def test_head_dimensions(d, kind):
+    lengths = [77, 300]
+    check(queries(2, 2, 6, d, kind), make(kind, lengths, 3, d, 16, seed=d), lengths)
+
+
+def test_4bit_powers_far_apart():
+    """Powers of two from 2^-30 to 2^20 in one head, and a head of zeros: codes under 2^-24 of the head's largest may be dropped, 6 * 2^-25 of the largest power at
+    most, of weights that sum to one."""
+    lengths = [200, 64]
+    c = make("4bit", lengths, 2, 128, 16, seed=5)
+    for s in (c.k_scale, c.v_scale):
+        s.copy_(torch.randint(97, 148, s.shape, device="cuda", generator=gen(3), dtype=torch.uint8))
+    c.k_scale.clamp_(max=124)
+    c.v[0], c.v_scale[0] = 0, 0
+    q = queries(2, 2, 4, 128, "4bit")
+    o, lse = jm.paged_attention(q, c, ints(lengths), return_lse=True)
+    want, want_lse, size = po.attend(q.double(), *contexts(c, lengths), lengths, [2, 2])
+    assert ((o.double() - want).abs() <= (2.0 ** -8 + 2.0 ** -17) * size + 6 * 2.0 ** (20 - 25) + 6 * 200 * 2.0 ** (20 - 40)).all()
+    assert (lse.double() - want_lse).abs().max() <= 128 * 8 * 2.0 ** -24 * 4
 
 
 @pytest.mark.parametrize("kind", KINDS)

@@ -176,6 +176,53 @@ def test_no_keys_one_norm_and_float32_weights():
     assert torch.equal(only, dx)
 
 
+def test_broadcast_inputs_and_shared_tensors():
+    """One head expanded over several, and one tensor as queries and keys: gradients add up."""
+    q, k, qw, kw, gq, gk = inputs(4, 2, 5, 4, 4, 64, F32)
+    f = jm.rotary_frequencies(64)
+    one = q[:, :, :1].contiguous().requires_grad_(True)
+    y, _ = jm.rotate_heads(one.expand(2, 5, 4, 64), None, None, f, q_weight=qw)
+    (got,) = torch.autograd.grad(y, [one], gq)
+    whole = q[:, :, :1].expand(2, 5, 4, 64).contiguous().requires_grad_(True)
+    z, _ = jm.rotate_heads(whole, None, None, f, q_weight=qw)
+    (each,) = torch.autograd.grad(z, [whole], gq)
+    assert torch.equal(y, z) and torch.allclose(got, each.sum(2, keepdim=True), rtol=1e-5, atol=1e-5)
+    x = q.clone().requires_grad_(True)
+    a, b = jm.rotate_heads(x, x, None, f, q_weight=qw, k_weight=kw)
+    (both,) = torch.autograd.grad([a, b], [x], [gq, gk])
+    x1, x2 = (q.clone().requires_grad_(True) for _ in range(2))
+    d1, d2 = torch.autograd.grad(jm.rotate_heads(x1, x2, None, f, q_weight=qw, k_weight=kw), [x1, x2], [gq, gk])
+    assert torch.equal(both, d1 + d2)
+
+
+def test_second_derivatives_are_refused():
+    q, k, qw, *_ = inputs(4, 1, 5, 2, 2, 64, F32)
+    q.requires_grad_(True)
+    y, _ = jm.rotate_heads(q, None, None, jm.rotary_frequencies(64), q_weight=qw)
+    with pytest.raises(RuntimeError, match="second"):
+        torch.autograd.grad(y.square().sum(), [q], create_graph=True)
+
+
+def test_a_training_step_with_attention():
+    """Norm, rotation and causal attention, and back: every gradient against float64."""
+    B, L, Hq, Hkv, d = 2, 70, 4, 2, 64
+    q, k, qw, kw, gq, gk = inputs(6, B, L, Hq, Hkv, d, F32)
+    v = torch.randn_like(k)
+    f = jm.rotary_frequencies(d)
+    leaves = [t.requires_grad_(True) for t in (q, k, v, qw, kw)]
+    o = jm.masked_attention_via_map(*jm.rotate_heads(q, k, None, f, q_weight=qw, k_weight=kw), v, is_causal=True)
+    grads = torch.autograd.grad(o, leaves, gq)
+    e = [t.detach().double().requires_grad_(True) for t in leaves]
+    at = torch.arange(L, device="cuda")[None, :, None]
+    rq, rk = po.rotate(e[0], at, f, weight=e[3]), po.rotate(e[1], at, f, weight=e[4])
+    logits = torch.einsum("bqhd,bkhd->bhqk", rq, rk.repeat_interleave(Hq // Hkv, 2)) / d ** 0.5
+    logits = logits.masked_fill(torch.ones(L, L, device="cuda").triu(1).bool(), -torch.inf)
+    want = torch.einsum("bhqk,bkhd->bqhd", logits.softmax(-1), e[2].repeat_interleave(Hq // Hkv, 2))
+    assert (o.double() - want).norm() <= 3e-6 * want.norm()
+    for got, w in zip(grads, torch.autograd.grad(want, e, gq.double())):        # (2e-6 of attention, and of rotation the same)
+        assert (got.double() - w).norm() <= 5e-6 * w.norm()
+
+
 def test_components_that_are_not_rotated_keep_infinities():
     q = torch.ones((1, 2, 1, 64), device="cuda")
     q[..., 40], q[..., 41] = torch.inf, torch.nan
