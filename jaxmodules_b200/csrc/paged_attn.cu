@@ -705,7 +705,7 @@ struct Core4bit {
 // For the scores two or four lanes share a key, for the sums a lane has DP / 32 columns; the rows of Q are read from shared memory, by all lanes at once.
 template <int DP, int ROWS>
 struct CoreF32 {
-  static constexpr int kDP = DP, kRows = ROWS, kTile = DP == 128 ? 8 : 16, kItem = 3, kStages = DP == 128 ? 3 : 2, kMinCtas = DP == 64 && ROWS <= 4 ? 3 : 2;
+  static constexpr int kDP = DP, kRows = ROWS, kTile = DP == 128 ? 8 : 16, kItem = 3, kStages = 2, kMinCtas = ROWS <= 4 ? 3 : 2;
   static constexpr int kRowBytes = DP * 4, kSide = kTile * kRowBytes, kStageBytes = 2 * kSide;
   static constexpr int kParts = 32 / kTile, kChunks = DP / 4 / kParts;      // lanes to a key, 16-byte chunks to each of them
   static constexpr int kQRow = DP + 4 * kParts;      // floats: each part of a row lies 4 further on than the one before would have it, in other banks
@@ -713,8 +713,11 @@ struct CoreF32 {
   static constexpr int kCols = DP / 32;
   using Cur = Cursor<kRows, kTile, kItem>;
 
+  static constexpr int kOwn = ROWS >= kParts ? ROWS / kParts : ROWS;      // rows whose softmax a lane takes: a key's lanes share them out, where there are enough
+
   float o[ROWS][kCols];
-  float m[ROWS], l[ROWS];      // of all rows; l: this lane's key's share
+  float m[kOwn], l[kOwn];      // of the lane's rows; l: its key's share
+  int own;                     // the first of them
   Place place;
   float *qs, *ps;
 
@@ -738,13 +741,21 @@ struct CoreF32 {
       qs[r * kQRow + d + d / (4 * kChunks) * 4] = x;
     }
     __syncwarp();
+    own = 0;
+    if (ROWS >= kParts) {        // halves of the rows, then quarters: as they are handed out in `take`
+      int n = ROWS;
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r) {
+      for (int b = 16; b >= kTile; b >>= 1) own += lane & b ? (n >>= 1) : (n >>= 1, 0);
+    }
+#pragma unroll
+    for (int r = 0; r < kOwn; ++r) {
       m[r] = -INFINITY;
       l[r] = 0.f;
+    }
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
 #pragma unroll
       for (int j = 0; j < kCols; ++j) o[r][j] = 0.f;
-    }
   }
   __device__ __forceinline__ void take(const PagedParams& p, const Cur& c, const uint8_t* stage, int k0, int lane) {
     const int key = lane & (kTile - 1), part = lane / kTile;
@@ -761,17 +772,36 @@ struct CoreF32 {
         s[r] = fmaf(x.x, k.x, fmaf(x.y, k.y, fmaf(x.z, k.z, fmaf(x.w, k.w, s[r]))));
       }
     }
-    const bool cut = c.x.cut(k0, kTile);
+    // The lanes of a key add up their parts of its products; each ends with its own rows.
+    if constexpr (ROWS >= kParts) {
+      int n = ROWS;
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r) {
-      float x = s[r];
+      for (int b = 16; b >= kTile; b >>= 1) {
+        n >>= 1;
+        const bool upper = lane & b;
 #pragma unroll
-      for (int b = kTile; b < 32; b <<= 1) x += __shfl_xor_sync(0xffffffffu, x, b);
-      x *= p.scale_log2;
+        for (int r = 0; r < ROWS / 2; ++r)
+          if (r < n) {
+            const float give = upper ? s[r] : s[r + n], keep = upper ? s[r + n] : s[r];
+            s[r] = keep + __shfl_xor_sync(0xffffffffu, give, b);
+          }
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+        for (int b = kTile; b < 32; b <<= 1) s[r] += __shfl_xor_sync(0xffffffffu, s[r], b);
+    }
+    const bool cut = c.x.cut(k0, kTile), strict = cut && p.a.T > 1;      // strict: some row sees what another does not
+    float f[kOwn];
+    bool moved = false;
+#pragma unroll
+    for (int r = 0; r < kOwn; ++r) {
+      float x = s[r] * p.scale_log2;
       bool seen = true;
       if (cut) {
         rarely();
-        const int row = c.x.row0 + r, t = row / p.G, at = row < p.rows && t < c.x.count ? c.x.first + t : -1, k = k0 + key;
+        const int row = c.x.row0 + own + r, t = row / p.G, at = row < p.rows && t < c.x.count ? c.x.first + t : -1, k = k0 + key;
         seen = k <= at && (p.a.window < 0 || k >= at - p.a.window);
         if (!seen) x = -INFINITY;
       }
@@ -779,21 +809,31 @@ struct CoreF32 {
 #pragma unroll
       for (int b = 1; b < kTile; b <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, b));
       const float base = top == -INFINITY ? 0.f : top;
-      if (top != m[r]) {
-        const float f = exp2_approx(m[r] - base);
-        l[r] *= f;
-#pragma unroll
-        for (int j = 0; j < kCols; ++j) o[r][j] *= f;
-        m[r] = top;
-      }
+      f[r] = top == m[r] ? 1.f : exp2_approx(m[r] - base);
+      moved |= top != m[r];
+      m[r] = top;
       x = exp2_approx(x - base);
-      l[r] += x;
-      s[r] = seen ? x : -1.f;
+      l[r] = fmaf(l[r], f[r], x);
+      if (ROWS >= kParts || part == 0) ps[key * ROWS + own + r] = seen ? x : strict ? -1.f : 0.f;
     }
-    const bool strict = cut && p.a.T > 1;      // some row sees what another does not
+    if (__any_sync(0xffffffffu, moved)) {
+      // what has been added up, to the new maxima; row r is that of the lanes of key 0 that own it
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r)
-      if (part == 0) ps[key * ROWS + r] = s[r] == -1.f && !strict ? 0.f : s[r];
+      for (int r = 0; r < ROWS; ++r) {
+        float g = f[r % kOwn];
+        if (ROWS >= kParts) {
+          int from = 0, n = ROWS, q = r;
+#pragma unroll
+          for (int b = 16; b >= kTile; b >>= 1) {
+            n >>= 1;
+            if (q >= n) { from |= b; q -= n; }
+          }
+          g = __shfl_sync(0xffffffffu, f[q], from);
+        }
+#pragma unroll
+        for (int j = 0; j < kCols; ++j) o[r][j] *= g;
+      }
+    }
     __syncwarp();
 #pragma unroll 4
     for (int k = 0; k < kTile; ++k) {
@@ -828,11 +868,11 @@ struct CoreF32 {
   }
   __device__ __forceinline__ void stats(const Buffer<DP>& buffer, int warp, int lane) const {
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r) {
+    for (int r = 0; r < kOwn; ++r) {
       float x = l[r];
 #pragma unroll
       for (int b = 1; b < kTile; b <<= 1) x += __shfl_xor_sync(0xffffffffu, x, b);
-      if (lane == 0) buffer.stat(warp, r) = make_float2(m[r], x);
+      if (ROWS >= kParts ? (lane & (kTile - 1)) == 0 : lane == 0) buffer.stat(warp, own + r) = make_float2(m[r], x);
     }
   }
   template <typename F>
@@ -851,7 +891,9 @@ struct CoreF32 {
 template <class Core>
 constexpr int paged_smem() {
   static_assert(Core::kStageBytes >= Buffer<Core::kDP>::kBytes && Core::kStageBytes % 16 == 0, "a warp's rows fit into a stage");
-  return kWarps * Core::kStages * Core::kStageBytes + Core::kExtra;
+  constexpr int bytes = kWarps * Core::kStages * Core::kStageBytes + Core::kExtra;
+  static_assert(Core::kMinCtas * (bytes + 1024) <= 228 * 1024, "the CTAs that plan_paged counts on fit an SM's shared memory");
+  return bytes;
 }
 
 // A finished row's value: four components and (at the first) the log-sum-exp; zeros for a token that is not real.
@@ -1134,7 +1176,7 @@ bool plan_paged(const bma_paged_cache& c, const bma_paged_attn_args& a, PagedLau
   l.tile = c.dtype == BMA_DTYPE_MXFP4 ? 32 : c.dtype == BMA_DTYPE_F32 && l.dp == 128 ? 8 : 16;
   l.rows_of_tile = c.dtype == BMA_DTYPE_F32 && rows <= 4 ? (rows == 1 ? 1 : 4) : rows <= 8 ? 8 : 16;
   // (what registers and shared memory allow; the kMinCtas of the instances)
-  l.ctas_per_sm = c.dtype == BMA_DTYPE_F32 ? (l.dp == 64 && l.rows_of_tile <= 4 ? 3 : 2) : l.rows_of_tile > 8 ? 2 : c.dtype == BMA_DTYPE_MXFP4 && l.dp == 64 ? 4 : 3;
+  l.ctas_per_sm = c.dtype == BMA_DTYPE_F32 ? (l.rows_of_tile <= 4 ? 3 : 2) : l.rows_of_tile > 8 ? 2 : c.dtype == BMA_DTYPE_MXFP4 && l.dp == 64 ? 4 : 3;
   l.row_tiles = ceil_div(rows, l.rows_of_tile);
   const int64_t entries = (int64_t)c.B * l.row_tiles;
   if (entries >= (1 << 30)) return false;
