@@ -310,7 +310,8 @@ Tensor heads_of(const Tensor& t, const char* name) {
   TORCH_CHECK_VALUE(t.dim() == 4, name, " must be [batch, length, heads, components]");
   TORCH_CHECK_VALUE(t.size(0) > 0 && t.size(1) > 0 && t.size(2) > 0 && t.size(3) > 0, name, " is empty");
   TORCH_CHECK_VALUE(t.size(0) <= INT32_MAX && t.size(1) <= INT32_MAX && t.size(2) <= 65535, name, " is too large");
-  return t.stride(3) == 1 || t.size(3) == 1 ? t : t.contiguous();
+  if (t.stride(3) == 1) return t;
+  return t.size(3) == 1 ? t.as_strided(t.sizes(), {t.stride(0), t.stride(1), t.stride(2), 1}) : t.contiguous();
 }
 
 bma_rotary rotary_of(Devices& on, int64_t d, const OptTensor& frequencies, int layout, double magnitude, const OptTensor& q_weight, const OptTensor& k_weight,

@@ -262,6 +262,24 @@ def test_repeated_streams_and_capture():
         assert all(torch.equal(a, b) for a, b in zip(out, want))
 
 
+def test_captured_backward():
+    q, k, qw, kw, gq, gk = inputs(8, 2, 33, 4, 2, 64, F32)
+    f = jm.rotary_frequencies(64)
+    leaves = [t.requires_grad_(True) for t in (q, k, qw, kw)]
+    step = lambda: torch.autograd.grad(jm.rotate_heads(q, k, None, f, q_weight=qw, k_weight=kw), leaves, [gq, gk])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    gq.mul_(-0.5)
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(got, step()))
+
+
 def test_many_tokens():
     """More (token, head) rows than 2^31 / 256: offsets in 64 bits."""
     B, L, H, d = 1, 70000, 128, 256
