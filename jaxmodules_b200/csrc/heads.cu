@@ -1,6 +1,8 @@
 // Norm and rotation of query and key heads, and what moves whole heads into and out of the pages of a cache.
 //
-// All of these read every value once and write every result once: they are bound by memory, or for a few tokens by the launch.
+// All of these read every value once and write every result once: they are bound by memory, for heads of few rows to a token by instructions, for a few tokens by the
+// launch.  Measured: forward and backward of 4 x 4096 tokens of 64 heads of 128 bfloat16 values 248 us, 82 % of the copy rate; prompts of 8 sequences of up to 2500
+// tokens, 8 heads, appended in 30 us (2.8 TB/s); contexts of 16 sequences of up to 5001 tokens read back in 85 us, 94 %.
 //
 // Rotation.  Component pairs are (i, i + dim/2) or (2i, 2i + 1).  A lane holds two 16-byte chunks of a head that hold both halves of its pairs
 // (chunks u and u + dim/2 of a head, or chunks 2u and 2u + 1), so that no value crosses lanes; only the sum of squares does.  A head of 128
