@@ -10,6 +10,8 @@
 #include <torch/csrc/utils/pybind.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <ATen/ATen.h>
+#include <ATen/EmptyTensor.h>
+#include <c10/core/Allocator.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
 
@@ -297,6 +299,11 @@ struct Place {
   explicit Place(const Tensor& t) : guard(t.device()), stream(c10::impl::VirtualGuardImpl(at::kCUDA).getStream(t.device()).native_handle()) {}
 };
 
+// at::empty on the current CUDA device (which Place has made the call's), without the dispatcher: 0.5 us less.
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType dtype) {
+  return at::detail::empty_generic(sizes, c10::GetAllocator(at::kCUDA), c10::DispatchKeySet(c10::DispatchKey::CUDA), dtype, std::nullopt);
+}
+
 bool wants_gradient(std::initializer_list<const Tensor*> tensors) {
   if (!at::GradMode::is_enabled()) return false;
   for (const Tensor* t : tensors)
@@ -389,11 +396,10 @@ std::tuple<Tensor, OptTensor> rotate_forward(const Tensor& q_in, const OptTensor
   bma_rotate_args a = rotate_args(on, q, k, r.positions, r.frequencies, r.layout, r.magnitude, r.q_weight, r.k_weight, r.eps);
   on.check();
   const Place place(q);
-  const at::TensorOptions like = q.options().requires_grad(false);
-  Tensor q_out = at::empty(q.sizes(), like);
+  Tensor q_out = fresh(q.sizes(), q.scalar_type());
   a.q = describe(q); a.q_out = describe(q_out);
   if (k) {
-    k_out = at::empty(k->sizes(), like);
+    k_out = fresh(k->sizes(), k->scalar_type());
     a.k = describe(*k); a.k_out = describe(*k_out);
   }
   int rc;
@@ -421,18 +427,17 @@ std::tuple<Tensor, OptTensor, OptTensor, OptTensor> rotate_backward(const Tensor
   if (k) on.add(*g_k, "the cotangent of k");
   on.check();
   const Place place(q);
-  const at::TensorOptions like = q.options().requires_grad(false);
-  Tensor dq = at::empty(q.sizes(), like);
+  Tensor dq = fresh(q.sizes(), q.scalar_type());
   a.q = describe(q); a.q_out = describe(g_q); a.dq = describe(dq);
   if (k) {
-    dk = at::empty(k->sizes(), like);
+    dk = fresh(k->sizes(), k->scalar_type());
     a.k = describe(*k); a.k_out = describe(*g_k); a.dk = describe(*dk);
   }
-  if (r.q_weight) a.dq_weight = (dqw = at::empty(r.q_weight->sizes(), r.q_weight->options().requires_grad(false)))->data_ptr();
-  if (r.k_weight) a.dk_weight = (dkw = at::empty(r.k_weight->sizes(), r.k_weight->options().requires_grad(false)))->data_ptr();
+  if (r.q_weight) a.dq_weight = (dqw = fresh(r.q_weight->sizes(), r.q_weight->scalar_type()))->data_ptr();
+  if (r.k_weight) a.dk_weight = (dkw = fresh(r.k_weight->sizes(), r.k_weight->scalar_type()))->data_ptr();
   const size_t ws_bytes = lib.bma_rotate_bwd_workspace_bytes(&a);
   Tensor ws;
-  if (ws_bytes) ws = bytes_on(q, ws_bytes);
+  if (ws_bytes) ws = fresh({(int64_t)ws_bytes}, at::kByte);
   nvtxRangePushA("bma.rotate_bwd");
   const int rc = lib.bma_rotate_bwd(&a, ws_bytes ? ws.data_ptr() : nullptr, ws_bytes, place.stream);
   nvtxRangePop();
@@ -576,7 +581,7 @@ OptTensor append(const Tensor& pages_k, const Tensor& pages_v, const Tensor& tab
   const Place place(pages_k);
   a.k = describe(k); a.v = describe(v);
   if (q) {
-    q_out = at::empty(q->sizes(), q->options().requires_grad(false));
+    q_out = fresh(q->sizes(), q->scalar_type());
     a.Hq = (int32_t)q->size(2);
     a.q = describe(*q); a.q_out = describe(*q_out);
   }
@@ -598,8 +603,8 @@ std::tuple<Tensor, Tensor> read_pages(const Tensor& pages_k, const Tensor& pages
   const int32_t* at_lengths = counts_of(on, lengths, c, "lengths");
   on.check();
   const Place place(pages_k);
-  const at::TensorOptions like = pages_k.options().dtype(c.dtype == BMA_DTYPE_F32 ? at::kFloat : at::kBFloat16).requires_grad(false);
-  Tensor k = at::empty({c.B, L, c.Hkv, c.d}, like), v = at::empty({c.B, L, c.Hkv, c.d}, like);
+  const at::ScalarType dtype = c.dtype == BMA_DTYPE_F32 ? at::kFloat : at::kBFloat16;
+  Tensor k = fresh({c.B, L, c.Hkv, c.d}, dtype), v = fresh({c.B, L, c.Hkv, c.d}, dtype);
   const bma_tensor dk = describe(k), dv = describe(v);
   int rc;
   {
@@ -631,15 +636,14 @@ std::tuple<Tensor, OptTensor> paged(const Tensor& pages_k, const Tensor& pages_v
   a.window = window ? (int32_t)*window : -1;
   on.check();
   const Place place(pages_k);
-  const at::TensorOptions f32 = q.options().dtype(at::kFloat).requires_grad(false);
-  Tensor o = at::empty(q.sizes(), bf16_out ? f32.dtype(at::kBFloat16) : f32);
+  Tensor o = fresh(q.sizes(), bf16_out ? at::kBFloat16 : at::kFloat);
   OptTensor lse;
-  if (with_lse) lse = at::empty({c.B, a.Hq, a.T}, f32);
+  if (with_lse) lse = fresh({c.B, a.Hq, a.T}, at::kFloat);
   a.q = describe(q); a.o = describe(o);
   a.lse = lse ? lse->data_ptr<float>() : nullptr;
   const size_t ws_bytes = lib.bma_paged_attn_workspace_bytes(&c, &a);
   Tensor ws;
-  if (ws_bytes) ws = bytes_on(q, ws_bytes);
+  if (ws_bytes) ws = fresh({(int64_t)ws_bytes}, at::kByte);
   int rc;
   {
     Group group("bma.paged_attn");
