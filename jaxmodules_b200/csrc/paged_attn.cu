@@ -1058,13 +1058,13 @@ __global__ void __launch_bounds__(kThreads, Core::kMinCtas) paged_kernel(const _
   while (here.at < end) {
     core.settle(smem);
     issue();
-    copies_awaited<NS - 1>();
-    __syncwarp();
-    if (fresh) {
+    if (fresh) {                 // (its queries come while the keys do)
       core.begin(p, here, lane);
       first_unit = here.unit;
       fresh = false;
     }
+    copies_awaited<NS - 1>();
+    __syncwarp();
     const int k0 = here.tile(p, warp);
     if (k0 < here.x.hi) core.take(p, here, smem + (warp * NS + from) * Core::kStageBytes, k0, lane);
     __syncwarp();
@@ -1104,6 +1104,7 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(const __grid_const
   const int groups = p.c.Hkv >> p.heads_log2, e = m.w / groups, head = (m.w - e * groups) * p.heads + mine;
   const int b = e / p.row_tiles, row0 = (e - b * p.row_tiles) * ROWS;
   if (row >= min(ROWS, p.rows - row0)) return;
+  const bool real = (row0 + row) / p.G < new_tokens(p.a.lengths, p.a.new_lengths, b, p.a.T).count;
   const int parts = m.z - m.x + 1;
   auto slot = [&](int i) { return ((int64_t)(i == 0 ? m.y : 2 * (m.x + i)) * p.heads + mine) * ROWS + row; };
   float top = -INFINITY;
@@ -1140,7 +1141,6 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(const __grid_const
     const float4 y = sums[w][lane];
     x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
   }
-  const bool real = (row0 + row) / p.G < new_tokens(p.a.lengths, p.a.new_lengths, b, p.a.T).count;
   write_result(p, b, head, row0 + row, real, lane * 4, x, top, sum);
 }
 
