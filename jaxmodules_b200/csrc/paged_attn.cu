@@ -1107,28 +1107,29 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(const __grid_const
   const bool real = (row0 + row) / p.G < new_tokens(p.a.lengths, p.a.new_lengths, b, p.a.T).count;
   const int parts = m.z - m.x + 1;
   auto slot = [&](int i) { return ((int64_t)(i == 0 ? m.y : 2 * (m.x + i)) * p.heads + mine) * ROWS + row; };
-  float top = -INFINITY;
-  for (int i = lane; i < parts; i += 32) top = fmaxf(top, p.part_ml[slot(i)].x);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  const float base = top == -INFINITY ? 0.f : top;
+  // Parts 32 at a time, all that is read of them at once: their statistics by every warp, a part to a lane, their sums by the warps in turn.
+  float top = -INFINITY, sum = 0.f;
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-  float sum = 0.f;
   for (int i0 = 0; i0 < parts; i0 += 32) {
-    float f = 0.f;                       // of part i0 + lane
-    if (i0 + lane < parts) {
-      const float2 ml = p.part_ml[slot(i0 + lane)];
-      f = exp2_approx(ml.x - base);
-      sum = fmaf(ml.y, f, sum);
-    }
+    const float2 ml = i0 + lane < parts ? p.part_ml[slot(i0 + lane)] : make_float2(-INFINITY, 0.f);
+    float4 y[32 / kWarps];
 #pragma unroll
-    for (int k = 0; k < 32; k += kWarps) {
-      const int i = i0 + k + warp;
-      const float fi = __shfl_sync(0xffffffffu, f, k + warp);
-      if (i < parts && lane * 4 < DP) {
-        const float4 y = *reinterpret_cast<const float4*>(p.part_o + slot(i) * DP + lane * 4);
-        x.x = fmaf(y.x, fi, x.x); x.y = fmaf(y.y, fi, x.y); x.z = fmaf(y.z, fi, x.z); x.w = fmaf(y.w, fi, x.w);
-      }
+    for (int k = 0; k < 32 / kWarps; ++k) {
+      const int i = i0 + k * kWarps + warp;
+      y[k] = i < parts && lane * 4 < DP ? *reinterpret_cast<const float4*>(p.part_o + slot(i) * DP + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    float t = ml.x;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
+    t = fmaxf(t, top);
+    const float base = t == -INFINITY ? 0.f : t, f = exp2_approx(ml.x - base), g = top == t ? 1.f : exp2_approx(top - base);
+    top = t;
+    sum = fmaf(sum, g, ml.y * f);
+    x.x *= g; x.y *= g; x.z *= g; x.w *= g;
+#pragma unroll
+    for (int k = 0; k < 32 / kWarps; ++k) {
+      const float fi = __shfl_sync(0xffffffffu, f, k * kWarps + warp);
+      x.x = fmaf(y[k].x, fi, x.x); x.y = fmaf(y[k].y, fi, x.y); x.z = fmaf(y[k].z, fi, x.z); x.w = fmaf(y[k].w, fi, x.w);
     }
   }
 #pragma unroll
