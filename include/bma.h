@@ -185,7 +185,7 @@ typedef struct bma_rotate_args {
 enum { BMA_DTYPE_MXFP4 = 2 };
 
 typedef struct bma_paged_cache {
-  void *k, *v;                      /* [pages, page_size, Hkv, d] (MXFP4: d / 2 bytes), the same strides for both */
+  void *k, *v;                      /* [pages, page_size, Hkv, d] (MXFP4: d / 2 bytes), the same strides for both, none negative */
   int64_t stride_page, stride_slot, stride_head;                    /* in elements (MXFP4: bytes) */
   uint8_t *k_scale, *v_scale;       /* MXFP4: [pages, page_size, Hkv, d / 32]                 */
   int64_t scale_stride_page, scale_stride_slot, scale_stride_head;

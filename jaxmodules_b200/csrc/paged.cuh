@@ -59,7 +59,9 @@ inline int validate_cache(const bma_paged_cache* c) {
   const int64_t unit = c->dtype == BMA_DTYPE_F32 ? 4 : c->dtype == BMA_DTYPE_BF16 ? 8 : 16;   // rows start on 16 bytes: copies are that wide
   BMA_REQUIRE(((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15) == 0, BMA_ERR_UNSUPPORTED);
   BMA_REQUIRE(c->stride_page % unit == 0 && c->stride_slot % unit == 0 && c->stride_head % unit == 0, BMA_ERR_UNSUPPORTED);
+  BMA_REQUIRE(c->stride_page >= 0 && c->stride_slot >= 0 && c->stride_head >= 0, BMA_ERR_ARG);      // (negative offsets stand for no place)
   BMA_REQUIRE(c->dtype != BMA_DTYPE_MXFP4 || (c->k_scale && c->v_scale), BMA_ERR_ARG);
+  BMA_REQUIRE(c->dtype != BMA_DTYPE_MXFP4 || (c->scale_stride_page >= 0 && c->scale_stride_slot >= 0 && c->scale_stride_head >= 0), BMA_ERR_ARG);
   return BMA_OK;
 }
 

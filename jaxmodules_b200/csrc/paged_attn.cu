@@ -76,7 +76,7 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 // Where a CTA puts the parts of its warps together, in the stages that they have just read: eight rows of a warp at a time, lines of DP + 8 floats; the last
-// 8 floats of a line hold maximum and sum of four rows, r, r + 8, r + 16 and r + 24.
+// 8 floats of a line keep the lines in different banks; they hold maximum and sum of rows r and r + 8.
 template <int DP>
 struct Buffer {
   static constexpr int kLine = DP + 8, kBytes = 8 * kLine * 4;
@@ -1157,7 +1157,7 @@ int validate_paged(const bma_paged_cache* c, const bma_paged_attn_args* a) {
   // the kernels count in 16 bytes
   const int64_t bytes = c->dtype == BMA_DTYPE_F32 ? 4 : c->dtype == BMA_DTYPE_BF16 ? 2 : 1;
   const int64_t last = ((int64_t)(c->pages - 1) * c->stride_page + (int64_t)(c->page_size - 1) * c->stride_slot + (int64_t)(c->Hkv - 1) * c->stride_head) * bytes / 16;
-  BMA_REQUIRE(c->stride_page >= 0 && c->stride_slot >= 0 && c->stride_head >= 0 && last < (int64_t)kNowhere, BMA_ERR_LIMIT);
+  BMA_REQUIRE(last < (int64_t)kNowhere, BMA_ERR_LIMIT);
   return BMA_OK;
 }
 
@@ -1283,7 +1283,7 @@ int bma_paged_attn(const bma_paged_cache* cache, const bma_paged_attn_args* args
     if (cache->page_size == 1 << i) p.page_shift = i;
   const int64_t last_scale = (int64_t)(cache->pages - 1) * cache->scale_stride_page + (int64_t)(cache->page_size - 1) * cache->scale_stride_slot +
                              (int64_t)(cache->Hkv - 1) * cache->scale_stride_head;
-  p.scale_words = cache->dtype == BMA_DTYPE_MXFP4 && cache->d == 128 && last_scale >= 0 && last_scale / 4 < (int64_t)kNowhere &&
+  p.scale_words = cache->dtype == BMA_DTYPE_MXFP4 && cache->d == 128 && last_scale / 4 < (int64_t)kNowhere &&
                   ((reinterpret_cast<uintptr_t>(cache->k_scale) | reinterpret_cast<uintptr_t>(cache->v_scale) | (uintptr_t)cache->scale_stride_page |
                     (uintptr_t)cache->scale_stride_slot | (uintptr_t)cache->scale_stride_head) & 3) == 0;
   p.scale_page = (uint32_t)(cache->scale_stride_page / 4);

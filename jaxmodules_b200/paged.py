@@ -26,7 +26,7 @@ class PagedCache:
 
     ``k``, ``v``: ``[pages, page_size, Hkv, d]``, float32 or bfloat16, d a multiple of 8 and at most 128; the strides of both alike, every head on 16 bytes.
     ``page_table``: int32 ``[B, width]``: ``page_table[b, i]`` is the page of positions ``i * page_size`` and up of sequence b; entries that no position
-    reaches may be anything.  Sequences may share pages that are not written any more.
+    reaches may be anything.  Sequences may share pages that are not written any more.  ``paged_attention`` takes up to 64 GiB of keys and as much of values.
 
     4 bits: ``k``, ``v`` are uint8 ``[pages, page_size, Hkv, d / 2]``, d 32, 64, 96 or 128: e2m1 codes, two to a byte, the earlier component in the lower
     half; ``k_scale``, ``v_scale`` uint8 ``[pages, page_size, Hkv, d / 32]``: every 32 components share the power of two ``2 ** (byte - 127)``, 255 is NaN.

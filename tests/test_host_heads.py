@@ -194,6 +194,22 @@ def test_entry_points_refuse_without_a_device():
     assert lib.bma_paged_attn(C.byref(c), C.byref(p), None, 0, None) == nat.BMA_ERR_LIMIT
 
 
+def test_negative_strides_of_a_cache_are_refused():
+    lib = nat.lib()
+    lengths = 16
+    p = nat.PagedAttnArgs(T=1, Hq=2, lengths=lengths)
+    p.q.dtype = nat.BMA_DTYPE_BF16
+    for dtype, field in [(nat.BMA_DTYPE_BF16, "stride_page"), (nat.BMA_DTYPE_BF16, "stride_slot"), (nat.BMA_DTYPE_BF16, "stride_head"),
+                         (nat.BMA_DTYPE_MXFP4, "scale_stride_page"), (nat.BMA_DTYPE_MXFP4, "scale_stride_slot"), (nat.BMA_DTYPE_MXFP4, "scale_stride_head")]:
+        c = nat.PagedCacheArgs(k=16, v=16, k_scale=16, v_scale=16, page_table=16, pages=1, page_size=1, Hkv=2, d=128, B=1, width=1, dtype=dtype)
+        setattr(c, field, -64)
+        k = nat.Tensor(ptr=16, dtype=nat.BMA_DTYPE_BF16)
+        assert lib.bma_paged_attn(C.byref(c), C.byref(p), None, 0, None) == nat.BMA_ERR_ARG, field
+        assert lib.bma_read_kv(C.byref(c), C.c_void_p(lengths), 1, C.byref(k), C.byref(k), None) == nat.BMA_ERR_ARG, field
+        a = nat.AppendArgs(T=1, lengths=lengths, k=k, v=k)
+        assert lib.bma_append_kv(C.byref(c), C.byref(a), None) == nat.BMA_ERR_ARG, field
+
+
 def test_4bit_oracle():
     """Known answers of the format: exact values stay, ties go to the even code, the power of two is the smallest that fits."""
     exact = torch.tensor([0, 0.5, 1, 1.5, 2, 3, 4, 6], dtype=torch.float64)
