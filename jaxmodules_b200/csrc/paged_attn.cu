@@ -732,15 +732,23 @@ struct CoreF32 {
     copy_rows<kTile, DP / 4, kSide>(p, place.at(p, c.h), p.c.d / 4, smem_at(smem) + stage, lane, [](int r, int chunk) { return r * kRowBytes + ((chunk ^ (r & 7)) << 4); });
   }
   __device__ __forceinline__ void begin(const PagedParams& p, const Cur& c, int lane) {
-    const int n = min(ROWS, p.rows - c.x.row0);
-    __syncwarp();                // (the last item's rows have been read)
-    for (int i = lane; i < ROWS * DP; i += 32) {
-      const int r = i / DP, d = i % DP, row = c.x.row0 + r;
-      float x = 0.f;
+    // All of the rows are asked for before one is put down: CTAs with many short items are the last to end.  (A value at a time, and `finish` with the statistics
+    // of a row for every value: 16 sequences of up to 4096 tokens, 4 kv heads of 128, 16 rows to each 231 us, so 76; 8 kv heads, 4 rows 125 and 58.)
+    constexpr int kLanes = DP / 4, kAtOnce = 32 / kLanes;       // lanes to a row, rows at a time
+    const int n = min(ROWS, p.rows - c.x.row0), d = lane % kLanes * 4;
+    float4 x[(ROWS + kAtOnce - 1) / kAtOnce];
+#pragma unroll
+    for (int r0 = 0; r0 < ROWS; r0 += kAtOnce) {
+      const int r = r0 + lane / kLanes, row = c.x.row0 + r, t = row / p.G;
+      x[r0 / kAtOnce] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (r < n && d < p.c.d)
-        x = __ldg(static_cast<const float*>(p.a.q.ptr) + c.x.b * p.a.q.stride_b + (row / p.G) * p.a.q.stride_l + (c.h * p.G + row % p.G) * p.a.q.stride_h + d);
-      qs[r * kQRow + d + d / (4 * kChunks) * 4] = x;
+        x[r0 / kAtOnce] = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p.a.q.ptr) + c.x.b * p.a.q.stride_b + t * p.a.q.stride_l +
+                                                                (c.h * p.G + row - t * p.G) * p.a.q.stride_h + d));
     }
+    __syncwarp();                // (the last item's rows have been read)
+#pragma unroll
+    for (int r0 = 0; r0 < ROWS; r0 += kAtOnce)
+      if (r0 + lane / kLanes < ROWS) *reinterpret_cast<float4*>(qs + (r0 + lane / kLanes) * kQRow + d + d / (4 * kChunks) * 4) = x[r0 / kAtOnce];
     __syncwarp();
     own = 0;
     if (ROWS >= kParts) {        // halves of the rows, then quarters: as they are handed out in `take`
@@ -926,39 +934,32 @@ __device__ __forceinline__ void finish(const PagedParams& p, Core& core, const t
   core.stats(buffer, warp, lane);
   meet();
   const int n = min(Core::kRows, p.rows - c.x.row0);
-  auto joined = [&](int row, float& top, float& sum) {      // over the warps; what their exponents are taken against
-    top = -INFINITY;
-    for (int w = mine; w < kWarps; w += p.heads) top = fmaxf(top, buffer.stat(w, row).x);
-    const float base = top == -INFINITY ? 0.f : top;
-    sum = 0.f;
+  for (int pass = 0; pass * 8 < n; ++pass) {
+    // statistics of the warps that share the head, a row to a lane (and again in every 8 lanes)
+    const int of_lane = pass * 8 + (lane & 7);
+    float top = -INFINITY, sum = 0.f;
+    for (int w = mine; w < kWarps; w += p.heads) top = fmaxf(top, buffer.stat(w, of_lane).x);
+    const float base = top == -INFINITY ? 0.f : top, factor = exp2_approx(buffer.stat(warp, of_lane).x - base);
     for (int w = mine; w < kWarps; w += p.heads) {
-      const float2 x = buffer.stat(w, row);
+      const float2 x = buffer.stat(w, of_lane);
       sum = fmaf(x.y, exp2_approx(x.x - base), sum);
     }
-    return base;
-  };
-  for (int pass = 0; pass * 8 < n; ++pass) {
-    core.put(pass, [&](int row) {
-      float top, sum;
-      const float base = joined(row, top, sum);
-      return exp2_approx(buffer.stat(warp, row).x - base);
-    }, buffer.line(warp, 0), lane);
+    core.put(pass, [&](int row) { return __shfl_sync(0xffffffffu, factor, row & 7); }, buffer.line(warp, 0), lane);
     meet();
     for (int i = of_head; i < 8 * (DP / 4); i += p.splits * 32) {
       const int r = i / (DP / 4), col = i % (DP / 4) * 4, row = pass * 8 + r;
-      if (row >= n) break;
+      const float row_top = __shfl_sync(0xffffffffu, top, r), row_sum = __shfl_sync(0xffffffffu, sum, r);
+      if (row >= n) continue;
       float4 x = *reinterpret_cast<const float4*>(buffer.line(mine, r) + col);
       for (int w = mine + p.heads; w < kWarps; w += p.heads) {
         const float4 y = *reinterpret_cast<const float4*>(buffer.line(w, r) + col);
         x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
       }
-      float top, sum;
-      joined(row, top, sum);
       if (!whole) {
         const int64_t at = ((int64_t)slot * p.heads + mine) * Core::kRows + row;
         *reinterpret_cast<float4*>(p.part_o + at * DP + col) = x;
-        if (col == 0) p.part_ml[at] = make_float2(top, sum);
-      } else write_result(p, c.x.b, c.h, c.x.row0 + row, (c.x.row0 + row) / p.G < c.x.count, col, x, top, sum);
+        if (col == 0) p.part_ml[at] = make_float2(row_top, row_sum);
+      } else write_result(p, c.x.b, c.h, c.x.row0 + row, (c.x.row0 + row) / p.G < c.x.count, col, x, row_top, row_sum);
     }
     meet();
   }
