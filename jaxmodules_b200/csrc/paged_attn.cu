@@ -20,6 +20,8 @@
 // Keys outside [lo, hi), which no row of the tile sees, are not read: zeros stand there.  Where the rows of a tile see different keys of a tile of
 // keys (several new tokens), each token's rows are multiplied by values that are zero where the token does not see them, so that an infinity or
 // a NaN reaches only the rows that see it.
+#include <type_traits>
+
 #include "paged.cuh"
 
 namespace bma {
@@ -1146,6 +1148,51 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(const __grid_const
   write_result(p, b, head, row0 + row, real, lane * 4, x, top, sum);
 }
 
+// The same where most items have few parts: a warp to a row.
+template <int DP, int ROWS>
+__global__ void __launch_bounds__(kThreads) paged_join_few_kernel(const __grid_constant__ PagedParams p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int4 m = p.meta[blockIdx.x];
+  if (m.x < 0) return;
+  const int lane = threadIdx.x & 31, of_item = blockIdx.y * kWarps + (threadIdx.x >> 5), mine = of_item & (p.heads - 1), row = of_item >> p.heads_log2;
+  const int groups = p.c.Hkv >> p.heads_log2, e = m.w / groups, head = (m.w - e * groups) * p.heads + mine;
+  const int b = e / p.row_tiles, row0 = (e - b * p.row_tiles) * ROWS;
+  if (row >= min(ROWS, p.rows - row0)) return;
+  const bool real = (row0 + row) / p.G < new_tokens(p.a.lengths, p.a.new_lengths, b, p.a.T).count;
+  const int parts = m.z - m.x + 1;
+  auto slot = [&](int i) { return ((int64_t)(i == 0 ? m.y : 2 * (m.x + i)) * p.heads + mine) * ROWS + row; };
+  float top = -INFINITY, sum = 0.f;
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto take = [&](int i0, auto at_once) {       // parts i0 and up, all that is read of them at once
+    constexpr int N = decltype(at_once)::value;
+    float2 ml[N];
+    float4 y[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const bool in = i0 + k < parts;
+      ml[k] = in ? p.part_ml[slot(i0 + k)] : make_float2(-INFINITY, 0.f);
+      y[k] = in && lane * 4 < DP ? *reinterpret_cast<const float4*>(p.part_o + slot(i0 + k) * DP + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    float t = top;
+#pragma unroll
+    for (int k = 0; k < N; ++k) t = fmaxf(t, ml[k].x);
+    const float base = t == -INFINITY ? 0.f : t, g = top == t ? 1.f : exp2_approx(top - base);
+    top = t;
+    sum *= g;
+    x.x *= g; x.y *= g; x.z *= g; x.w *= g;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const float f = exp2_approx(ml[k].x - base);
+      sum = fmaf(ml[k].y, f, sum);
+      x.x = fmaf(y[k].x, f, x.x); x.y = fmaf(y[k].y, f, x.y); x.z = fmaf(y[k].z, f, x.z); x.w = fmaf(y[k].w, f, x.w);
+    }
+  };
+  if (parts <= 4) take(0, std::integral_constant<int, 4>());
+  else
+    for (int i0 = 0; i0 < parts; i0 += 16) take(i0, std::integral_constant<int, 16>());      // a long sequence among many short ones
+  if (lane * 4 < DP) write_result(p, b, head, row0 + row, real, lane * 4, x, top, sum);
+}
+
 // ---- host ---------------------------------------------------------------------------------------------------------------
 int validate_paged(const bma_paged_cache* c, const bma_paged_attn_args* a) {
   int rc = validate_cache(c);
@@ -1209,8 +1256,13 @@ int launch_paged(const PagedParams& p, const PagedLaunch& l, cudaStream_t st) {
   }
   paged_kernel<Core><<<l.ctas, kThreads, smem, st>>>(p);
   BMA_CUDA_TRY(cudaGetLastError());
+  // Where the average item has fewer than four parts a row to a warp, else to a CTA.  (8 kv heads of 128, bfloat16: 128 sequences of up to 256 tokens, 256 items for 444
+  // CTAs, 27 us and 33; 256 of up to 512 71 and 78; 32 of up to 8192 with 28 rows, 128 items for 296 CTAs, 240 and 248, with 16 rows, 64 items, 145 and 142.  One long
+  // sequence among many short ones has many parts, and pays for that: 32768 tokens among 299 of 100 75 and 68.)
+  const int rows = std::min(Core::kRows, p.rows) * p.heads;
+  const bool few = (int64_t)l.entries * l.groups * 3 > l.ctas;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(l.metas(), std::min(Core::kRows, p.rows) * p.heads);
+  cfg.gridDim = dim3(l.metas(), few ? ceil_div(rows, kWarps) : rows);
   cfg.blockDim = dim3(kThreads);
   cfg.stream = st;
   cudaLaunchAttribute attr{};
@@ -1218,7 +1270,8 @@ int launch_paged(const PagedParams& p, const PagedLaunch& l, cudaStream_t st) {
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  BMA_CUDA_TRY(cudaLaunchKernelEx(&cfg, paged_join_kernel<Core::kDP, Core::kRows>, p));
+  if (few) BMA_CUDA_TRY(cudaLaunchKernelEx(&cfg, paged_join_few_kernel<Core::kDP, Core::kRows>, p));
+  else BMA_CUDA_TRY(cudaLaunchKernelEx(&cfg, paged_join_kernel<Core::kDP, Core::kRows>, p));
   count_launches(2);
   return BMA_OK;
 }
