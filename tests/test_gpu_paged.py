@@ -123,6 +123,16 @@ def test_attention(case, kind):
     check(queries(len(lengths), T, Hq, d, kind), c, lengths, new)
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("T,Hq,Hkv,d", [(1, 4, 2, 64), (2, 6, 1, 128)])
+@pytest.mark.parametrize("long", [400, 3000, 20000])
+def test_a_long_sequence_among_many_short_ones(long, T, Hq, Hkv, d, kind):
+    """Its walk is cut into 2 to several hundred parts, those of the others into one or two."""
+    lengths = [T + i * 5 % 40 for i in range(230)]
+    lengths[101] = long
+    check(queries(len(lengths), T, Hq, d, kind), make(kind, lengths, Hkv, d, 16, seed=long), lengths)
+
+
 @pytest.mark.parametrize("kind", ["bf16", "f32"])
 @pytest.mark.parametrize("d", [8, 40, 72, 120])
 def test_head_dimensions(d, kind):
