@@ -127,7 +127,7 @@ def test_attention(case, kind):
 @pytest.mark.parametrize("T,Hq,Hkv,d", [(1, 4, 2, 64), (2, 6, 1, 128)])
 @pytest.mark.parametrize("long", [400, 3000, 20000])
 def test_a_long_sequence_among_many_short_ones(long, T, Hq, Hkv, d, kind):
-    """Its walk is cut into 2 to several hundred parts, those of the others into one or two."""
+    """Its walk is cut into 7 to 280 parts, those of the others into one or two."""
     lengths = [T + i * 5 % 40 for i in range(230)]
     lengths[101] = long
     check(queries(len(lengths), T, Hq, d, kind), make(kind, lengths, Hkv, d, 16, seed=long), lengths)
