@@ -3,15 +3,18 @@
 // Every key and value in reach is read once and meets the few rows (tokens x query heads of its kv head) of one sequence: the kernels are bound
 // by memory.  What they have to do is to keep enough loads in flight, and to give every SM the same share of bytes whatever the
 // lengths are, which only the device knows.  Measured, 64 sequences of up to 8192 tokens, 8 kv heads of 128, 4 query heads to each: bfloat16 216 - 226 us, 94 - 99 %
-// of the copy rate; 4 bits 115 us, where instructions count (49 %); float32, 8 sequences, 16 heads of 64, window of 2048, 27.2 us (57 %).
+// of the copy rate; 4 bits 113 us, where instructions count (50 %); float32, 8 sequences, 16 heads of 64, window of 2048, 27.2 us (57 %).
 //
-// Work.  The walk over the keys of one (sequence, tile of rows, group of kv heads) is an item.  The four warps of a CTA have a kv head each, so that they read
-// neighbouring bytes of the same tokens at about the same time (of a 4-bit cache, whose powers of two for 8 heads are one 32-byte sector, 1.8 times the bytes came
-// from memory when a CTA had one head), and no results to put together; with two or one head to a CTA, where their number allows no more or items are few, two
-// or four warps share one.  An item is cut into units, a tile of keys for every warp.  All units of all items lie on one line, each item's with room before them for what it takes to begin and finish an item (half a unit, 1.5 in FMA arithmetic: without it a sequence of one
-// token, 8 items to finish, kept its CTA for 9 us after the others).  The line is cut into as many even runs as CTAs fit on the chip; a run ends in the
-// middle of an item as a rule.  Each CTA finds its run from the lengths.  An item that lies within one run is finished there; the parts of others go to the
-// workspace, at most two from a CTA, and paged_join_kernel puts them together in the order of the keys.
+// Work.  The walk over the keys of one (sequence, tile of rows, group of kv heads) is an item.  The four warps of a CTA have a kv head each, so that they
+// read neighbouring bytes of the same tokens at about the same time (of a 4-bit cache, whose powers of two for 8 heads are one 32-byte sector, 1.8 times the
+// bytes came from memory when a CTA had one head), and no results to put together; with two or one head to a CTA, where their number allows no more or items
+// are few, two or four warps share one.  An item is cut into units, a tile of keys for every warp.  All units of all items lie on one line, each item's with
+// room before them for what it takes to begin and finish an item: 1.5 units with eight rows to a tile, 3 with sixteen, 2 in FMA arithmetic.  (Without it a
+// sequence of one token, 8 items to finish, kept its CTA for 9 us after the others.  With 0.5 units in place of these: 128 sequences of up to 256 tokens 27
+// us and 23, 32 of up to 8192 with 28 rows 240 and 227, of 4 bits 204 and 182.  3 units for eight rows take 23 and 68 in place of 70 for 256 of up to 512,
+// and 12.3 in place of 11 for one sequence of 1500.) The line is cut into as many even runs as CTAs fit on the chip; a run ends in the middle of an item as a
+// rule.  Each CTA finds its run from the lengths.  An item that lies within one run is finished there; the parts of others go to the workspace, at most two
+// from a CTA, and paged_join_kernel puts them together in the order of the keys.
 //
 // Each warp has its own ring of stages in shared memory that it fills by cp.async: no warp waits for another before the end of an item (nor there, with a
 // head of its own), and the ring runs on into the next item.  Pages are looked up for every key (any page
@@ -285,7 +288,7 @@ __device__ __forceinline__ void copy_rows(const PagedParams& p, uint32_t mine, i
 // tile, where rows as M would make 16 of one.  The weights go from the accumulators of the one to the operand of the other by movmatrix.
 template <int DP, int NT>
 struct CoreBf16 {
-  static constexpr int kDP = DP, kRows = NT * 8, kTile = 16, kItem = 1, kStages = DP == 128 ? (NT == 1 ? 2 : 3) : 4, kMinCtas = NT == 1 ? 3 : 2;      // (two stages and three CTAs 220 us, three and two 238: 64 sequences of up to 8192)
+  static constexpr int kDP = DP, kRows = NT * 8, kTile = 16, kItem = NT == 1 ? 3 : 6, kStages = DP == 128 ? (NT == 1 ? 2 : 3) : 4, kMinCtas = NT == 1 ? 3 : 2;      // (two stages and three CTAs 220 us, three and two 238: 64 sequences of up to 8192)
   static constexpr int kRowBytes = DP * 2, kSide = kTile * kRowBytes, kStageBytes = 2 * kSide, kExtra = 0;
   using Cur = Cursor<kRows, kTile, kItem>;
 
@@ -425,7 +428,7 @@ struct CoreBf16 {
 // (turned: of two keys), and they are taken in the order in which they come.
 template <int DP, int NT>
 struct Core4bit {
-  static constexpr int kDP = DP, kRows = NT * 8, kTile = 32, kItem = 1, kStages = 2, kMinCtas = NT > 1 ? 2 : DP == 64 ? 4 : 3;
+  static constexpr int kDP = DP, kRows = NT * 8, kTile = 32, kItem = NT == 1 ? 3 : 6, kStages = 2, kMinCtas = NT > 1 ? 2 : DP == 64 ? 4 : 3;
   static constexpr int kRowBytes = DP / 2, kSide = kTile * kRowBytes, kGroups = DP / 32;
   // after keys and values: powers of keys [32][4] (float32), of values [4][32] (float16, by key_of's rows), E and 2^-E of values [32][2]
   static constexpr int kKeyPowers = 2 * kSide, kValuePowers = kKeyPowers + 512, kTops = kValuePowers + 256, kStageBytes = kTops + 256, kExtra = 0;
@@ -708,7 +711,7 @@ struct Core4bit {
 // For the scores two or four lanes share a key, for the sums a lane has DP / 32 columns; the rows of Q are read from shared memory, by all lanes at once.
 template <int DP, int ROWS>
 struct CoreF32 {
-  static constexpr int kDP = DP, kRows = ROWS, kTile = DP == 128 ? 8 : 16, kItem = 3, kStages = 2, kMinCtas = ROWS <= 4 ? 3 : 2;
+  static constexpr int kDP = DP, kRows = ROWS, kTile = DP == 128 ? 8 : 16, kItem = 4, kStages = 2, kMinCtas = ROWS <= 4 ? 3 : 2;
   static constexpr int kRowBytes = DP * 4, kSide = kTile * kRowBytes, kStageBytes = 2 * kSide;
   static constexpr int kParts = 32 / kTile, kChunks = DP / 4 / kParts;      // lanes to a key, 16-byte chunks to each of them
   static constexpr int kQRow = DP + 4 * kParts;      // floats: each part of a row lies 4 further on than the one before would have it, in other banks
@@ -735,7 +738,7 @@ struct CoreF32 {
   }
   __device__ __forceinline__ void begin(const PagedParams& p, const Cur& c, int lane) {
     // All of the rows are asked for before one is put down: CTAs with many short items are the last to end.  (A value at a time, and `finish` with the statistics
-    // of a row for every value: 16 sequences of up to 4096 tokens, 4 kv heads of 128, 16 rows to each 231 us, so 76; 8 kv heads, 4 rows 125 and 58.)
+    // of a row for every value: 16 sequences of up to 4096 tokens, 4 kv heads of 128, 16 rows to each 231 us, so 73; 8 kv heads, 4 rows 125 and 58.)
     constexpr int kLanes = DP / 4, kAtOnce = 32 / kLanes;       // lanes to a row, rows at a time
     const int n = min(ROWS, p.rows - c.x.row0), d = lane % kLanes * 4;
     float4 x[(ROWS + kAtOnce - 1) / kAtOnce];
@@ -1257,8 +1260,8 @@ int launch_paged(const PagedParams& p, const PagedLaunch& l, cudaStream_t st) {
   paged_kernel<Core><<<l.ctas, kThreads, smem, st>>>(p);
   BMA_CUDA_TRY(cudaGetLastError());
   // Where the average item has fewer than four parts a row to a warp, else to a CTA.  (8 kv heads of 128, bfloat16: 128 sequences of up to 256 tokens, 256 items for 444
-  // CTAs, 27 us and 33; 256 of up to 512 71 and 78; 32 of up to 8192 with 28 rows, 128 items for 296 CTAs, 240 and 248, with 16 rows, 64 items, 145 and 142.  One long
-  // sequence among many short ones has many parts, and pays for that: 32768 tokens among 299 of 100 75 and 68.)
+  // CTAs, 6 us less; 256 of up to 512 7 less; 32 of up to 8192 with 28 rows, 128 items for 296 CTAs, 8 less, with 16 rows, 64 items, 3 more.  One long
+  // sequence among many short ones has many parts, and pays for that: 32768 tokens among 299 of 100 7 more.)
   const int rows = std::min(Core::kRows, p.rows) * p.heads;
   const bool few = (int64_t)l.entries * l.groups * 3 > l.ctas;
   cudaLaunchConfig_t cfg{};
