@@ -11,8 +11,8 @@
 // are few, two or four warps share one.  An item is cut into units, a tile of keys for every warp.  All units of all items lie on one line, each item's with
 // room before them for what it takes to begin and finish an item: 1.5 units with eight rows to a tile, 3 with sixteen, 2 in FMA arithmetic.  (Without it a
 // sequence of one token, 8 items to finish, kept its CTA for 9 us after the others.  With 0.5 units in place of these: 128 sequences of up to 256 tokens 27
-// us and 23, 32 of up to 8192 with 28 rows 240 and 227, of 4 bits 204 and 182.  3 units for eight rows take 23 and 68 in place of 70 for 256 of up to 512,
-// and 12.3 in place of 11 for one sequence of 1500.) The line is cut into as many even runs as CTAs fit on the chip; a run ends in the middle of an item as a
+// us and 23, 32 of up to 8192 with 28 rows 240 and 227, of 4 bits 204 and 182.  With 3 units for eight rows, too,
+// 256 sequences of up to 512 take 68 in place of 70, one of 1500 12.3 in place of 11.)  The line is cut into as many even runs as CTAs fit on the chip; a run ends in the middle of an item as a
 // rule.  Each CTA finds its run from the lengths.  An item that lies within one run is finished there; the parts of others go to the workspace, at most two
 // from a CTA, and paged_join_kernel puts them together in the order of the keys.
 //
