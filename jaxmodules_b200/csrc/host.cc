@@ -310,6 +310,10 @@ bool wants_gradient(std::initializer_list<const Tensor*> tensors) {
     if (t && t->requires_grad()) return true;
   return false;
 }
+// Forward mode hands its tangents along beside the values, and a result without one counts as a constant there: none is dropped in silence.
+void no_tangents(std::initializer_list<const Tensor*> tensors, const char* name) {
+  for (const Tensor* t : tensors) TORCH_CHECK_VALUE(!t || !t->defined() || !t->_fw_grad(/*level=*/0).defined(), name, " has no derivatives in forward mode");
+}
 const Tensor* pointer(const OptTensor& t) { return t ? &*t : nullptr; }
 
 // [B, L, H, d] heads; copied only where the components of a head do not lie side by side
@@ -468,6 +472,7 @@ struct RotateNode : torch::autograd::Function<RotateNode> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     TORCH_CHECK(!at::GradMode::is_enabled(), "rotate_heads has no second derivatives: do not ask for create_graph");
+    for (const Tensor& g : grads) no_tangents({&g}, "the backward pass of rotate_heads");
     const variable_list saved = ctx->get_saved_variables();
     const auto optional = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
     const Rotation r{optional(saved[2]), optional(saved[3]), (int)ctx->saved_data["layout"].toInt(), ctx->saved_data["magnitude"].toDouble(), optional(saved[4]),
@@ -486,6 +491,8 @@ struct RotateNode : torch::autograd::Function<RotateNode> {
 
 std::tuple<Tensor, OptTensor> rotate(const Tensor& q, const OptTensor& k, const OptTensor& positions, const OptTensor& frequencies, int layout, double magnitude,
                                      const OptTensor& q_weight, const OptTensor& k_weight, double eps) {
+  no_tangents({&q, pointer(k), pointer(q_weight), pointer(k_weight), pointer(frequencies)}, "rotate_heads");
+  TORCH_CHECK_VALUE(!wants_gradient({pointer(frequencies)}), "rotate_heads is not differentiable in frequencies: detach them");
   if (!wants_gradient({&q, pointer(k), pointer(q_weight), pointer(k_weight)})) return rotate_forward(q, k, {positions, frequencies, layout, magnitude, q_weight, k_weight, eps}, true);
   const variable_list out = RotateNode::apply(q, k, positions, frequencies, (int64_t)layout, magnitude, q_weight, k_weight, eps);
   return {out[0], out.size() > 1 ? OptTensor(out[1]) : OptTensor()};
@@ -558,7 +565,8 @@ void fits_cache(Devices& on, const Tensor& t, const bma_paged_cache& c, int64_t 
 OptTensor append(const Tensor& pages_k, const Tensor& pages_v, const Tensor& table, const OptTensor& k_scale, const OptTensor& v_scale, const Tensor& k_in,
                  const Tensor& v_in, const Tensor& lengths, const OptTensor& new_lengths, const OptTensor& q_in, const OptTensor& frequencies, int layout, double magnitude,
                  const OptTensor& q_weight, const OptTensor& k_weight, double eps) {
-  TORCH_CHECK_VALUE(!wants_gradient({&k_in, &v_in, pointer(q_in), pointer(q_weight), pointer(k_weight), &pages_k, &pages_v}),
+  no_tangents({&k_in, &v_in, pointer(q_in), pointer(q_weight), pointer(k_weight), pointer(frequencies), &pages_k, &pages_v}, "append_kv");
+  TORCH_CHECK_VALUE(!wants_gradient({&k_in, &v_in, pointer(q_in), pointer(q_weight), pointer(k_weight), pointer(frequencies), &pages_k, &pages_v}),
                     "append_kv is not differentiable: call it under torch.no_grad()");
   Devices on;
   const bma_paged_cache c = cache_of(on, pages_k, pages_v, table, k_scale, v_scale);
@@ -598,6 +606,7 @@ std::tuple<Tensor, Tensor> read_pages(const Tensor& pages_k, const Tensor& pages
                                 const Tensor& lengths, int64_t L) {
   Devices on;
   const bma_paged_cache c = cache_of(on, pages_k, pages_v, table, k_scale, v_scale);
+  no_tangents({&pages_k, &pages_v}, "read_kv");
   TORCH_CHECK_VALUE(!wants_gradient({&pages_k, &pages_v}), "read_kv is not differentiable: call it under torch.no_grad()");
   TORCH_CHECK_VALUE(L > 0 && L <= INT32_MAX, "max_length must be positive");
   const int32_t* at_lengths = counts_of(on, lengths, c, "lengths");
@@ -618,6 +627,7 @@ std::tuple<Tensor, Tensor> read_pages(const Tensor& pages_k, const Tensor& pages
 std::tuple<Tensor, OptTensor> paged(const Tensor& pages_k, const Tensor& pages_v, const Tensor& table, const OptTensor& k_scale, const OptTensor& v_scale,
                                     const Tensor& q_in, const Tensor& lengths, const OptTensor& new_lengths, std::optional<double> scale,
                                     std::optional<int64_t> window, bool bf16_out, bool with_lse) {
+  no_tangents({&q_in, &pages_k, &pages_v}, "paged_attention");
   TORCH_CHECK_VALUE(!wants_gradient({&q_in, &pages_k, &pages_v}), "paged_attention is not differentiable: call it under torch.no_grad()");
   Devices on;
   const bma_paged_cache c = cache_of(on, pages_k, pages_v, table, k_scale, v_scale);

@@ -67,7 +67,8 @@ def rotate_heads(q: torch.Tensor, k: Optional[torch.Tensor], positions: Optional
     None: no rotation.  ``positions``: int32 or int64, ``[L]`` or ``[B, L]``, None for 0 .. L-1; the angles are as exact at position 2^30 as at 1.
 
     Repeated calls give the same bits, gradients included.  The gradients of the weights are sums over all tokens and heads in an order that
-    the sizes of the call fix.  There are no second derivatives: a backward pass with ``create_graph`` is refused.  A forward and backward
+    the sizes of the call fix.  There are no second derivatives, none in forward mode and none in the frequencies: a backward pass with
+    ``create_graph``, a dual tensor and ``frequencies`` that require a gradient are refused.  A forward and backward
     pass can be captured into a CUDA graph as long as no eager results that depend on the same leaves are held: torch's engine, for any operator, ends
     a capture that reaches a leaf which an eager graph holds.
     """

@@ -7,7 +7,7 @@ The reference has no counterpart: its attention takes dense keys and values of t
     o = paged_attention(q, cache, lengths)
 
 and both calls, like ``read_kv``, can be captured into a CUDA graph (after a first call outside of one): everything that changes between steps lies
-on the device.
+on the device.  None of the three is differentiable: tensors that require a gradient, and dual tensors of forward mode, are refused.
 """
 from __future__ import annotations
 
