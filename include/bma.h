@@ -181,7 +181,8 @@ typedef struct bma_rotate_args {
 } bma_rotate_args;
 
 /* dtype of a cache: BMA_DTYPE_F32, BMA_DTYPE_BF16 or this, every 32 components of a head as e2m1 codes (two to a byte, the earlier in the lower half)
- * and one power of two (a byte, biased by 127; 255: NaN).  Appending takes the smallest power with which the largest of the 32 is at most 6. */
+ * and one power of two (a byte, biased by 127; 255: NaN).  Appending takes the smallest power with which the largest of the 32 is at most 6.
+ * Reading is exact (in bfloat16); attention may take values below 2^-100 as zeros, and a component of a query counts to 2^-40 of the largest of its row. */
 enum { BMA_DTYPE_MXFP4 = 2 };
 
 typedef struct bma_paged_cache {

@@ -419,10 +419,16 @@ struct CoreBf16 {
 // ---- 4 bits: the same products in float16 -----------------------------------------------------------------------------
 // Codes become float16 as they are, and products of codes are exact; the powers of two join elsewhere.  Keys: a k-step of the instruction lies within 32
 // components, whose sum is multiplied by their power in float32.  Values: of a head's powers the largest, 2^E, is taken out and joins the exponent of the weight;
-// what remains, 2^(e - E) <= 1, multiplies the weights of each 32 components.  The running maximum is over score + E, so that the weights that go through
-// float16 are at most 1, and the sum of weights takes 2^-E back out.  Rows of Q are brought to at most 2 by a power of two.  Weights are held times
-// 2^15, as large as float16 allows: they are good to 2^-12 of themselves down to 2^-29 of the row's largest, and to 2^-40 of that below.  (E
-// counts as at least -65, so that no sum of weights overflows.)
+// what remains, 2^(e - E) from 2^-14 to 1, multiplies the weights of each 32 components.  The running maximum is over score + E, so that the weights that go through
+// float16 are at most 1, and the sum of weights takes 2^-E back out.  Rows of Q are brought to at most 2^15 by a power of two (what float16 holds: their components
+// count to 2^-40 of the row's largest).  Weights are held times 2^15, too: they are good to 2^-11 of themselves
+// down to 2^-29 of the row's largest, and to 2^-40 of that below, where their products with 2^(e - E) are rounded once more.
+//
+// That holds as long as E is between -40 and 40 (with one maximum for both, a weight 2^-126 below it is lost to the sum of weights, whose key may be the only one
+// of ordinary values) and no power of a head lies 2^14 below its largest.  Powers of 2^-103 and less count as zeros: they are what heads of zeros have.  From a tile of keys on
+// that breaks this (`far`), a warp takes its item as take_wide does: maximum and sum of weights as without powers, the products of every 32
+// components with maxima of their own.  There a component is as good as if its group of 32 stood alone, for any powers.  (All tiles taken so: 64 sequences of up to 8192 tokens,
+// 8 kv heads of 128, 187 us in place of 114, one of 131072, four tokens, 138 in place of 78.)
 //
 // Where components lie among those of a k-step, or of a tile of the sums, is free as long as both operands agree: ldmatrix hands each lane four codes of 32 components
 // (turned: of two keys), and they are taken in the order in which they come.
@@ -430,9 +436,12 @@ template <int DP, int NT>
 struct Core4bit {
   static constexpr int kDP = DP, kRows = NT * 8, kTile = 32, kItem = NT == 1 ? 3 : 6, kStages = 2, kMinCtas = NT > 1 ? 2 : DP == 64 ? 4 : 3;
   static constexpr int kRowBytes = DP / 2, kSide = kTile * kRowBytes, kGroups = DP / 32;
-  // after keys and values: powers of keys [32][4] (float32), of values [4][32] (float16, by key_of's rows), E and 2^-E of values [32][2]
-  static constexpr int kKeyPowers = 2 * kSide, kValuePowers = kKeyPowers + 512, kTops = kValuePowers + 256, kStageBytes = kTops + 256, kExtra = 0;
+  // after keys and values: powers of keys [32][4] (float32), of values [4][32] (float16, by key_of's rows), E and 2^-E of values [32][2], bytes of their powers [32] (take_wide's)
+  static constexpr int kKeyPowers = 2 * kSide, kValuePowers = kKeyPowers + 512, kTops = kValuePowers + 256, kBytes = kTops + 256, kStageBytes = kBytes + 128, kExtra = 0;
+  static_assert(kStages == 2, "`far` is that of the tile taken next");
   static constexpr float kWeightUp = 15.f;
+  static constexpr float kWideUp = -24.f;      // take_wide: sums of weights times values of 2^127 overflow from 2^24 keys on
+  static constexpr int kLeastTop = 127 - 40, kMostTop = 127 + 40, kSpread = 14, kZero = 127 - 103, kMostKey = 127 + 100;
   using Cur = Cursor<kRows, kTile, kItem>;
 
   uint32_t q[NT][DP / 16][2];
@@ -442,8 +451,9 @@ struct Core4bit {
   Place place;
   uint32_t k_bytes, v_bytes;    // the powers of two of this lane's key of the last tile issued
   int pending;                  // and where its stage lies, negative where there is none
+  bool far, wide;               // the last tile settled, and this item from some tile on, are take_wide's
 
-  __device__ __forceinline__ void prepare(uint8_t*) { pending = -1; }
+  __device__ __forceinline__ void prepare(uint8_t*) { pending = -1; wide = false; }
   __device__ __forceinline__ void look_up(const PagedParams& p, const Cur& c, int warp, int lane) { place.look_up(p, c.x, c.tile(p, warp) + lane); }
   // 16-byte chunks of a row are permuted so that 8 rows of a chunk lie in different banks
   static __device__ __forceinline__ int chunk_at(int r, int chunk) { return r * kRowBytes + ((DP == 128 ? chunk ^ (r >> 1 & 3) : chunk ^ (r >> 2 & 1)) << 4); }
@@ -451,7 +461,7 @@ struct Core4bit {
   __device__ __forceinline__ void issue(const PagedParams& p, const Cur& c, uint8_t* smem, int stage, int lane) {
     settle(smem);
     const uint32_t mine = place.at(p, c.h);
-    k_bytes = v_bytes = 0;
+    k_bytes = v_bytes = 0;       // (of a key that is not read: zeros)
     if (mine != kNowhere) {
       if (p.scale_words) {
         const uint32_t word = place.page * p.scale_page + place.slot * p.scale_slot + c.h * p.scale_head;
@@ -462,11 +472,14 @@ struct Core4bit {
         const int64_t at = (int64_t)place.page * p.c.scale_stride_page + (int64_t)place.slot * p.c.scale_stride_slot + (int64_t)c.h * p.c.scale_stride_head;
         const int n = p.c.d / 32;
 #pragma unroll
-        for (int i = 0; i < kGroups; ++i)
-          if (i < n) {
+        for (int i = 0; i < 4; ++i)
+          if (i < kGroups && i < n) {
             k_bytes |= (uint32_t)__ldg(p.c.k_scale + at + i) << (8 * i);
             v_bytes |= (uint32_t)__ldg(p.c.v_scale + at + i) << (8 * i);
-          } else v_bytes |= (v_bytes & 255) << (8 * i);      // (no components there)
+          } else {                                           // (no components there)
+            k_bytes |= (k_bytes & 255) << (8 * i);
+            v_bytes |= (v_bytes & 255) << (8 * i);
+          }
       }
     }
     pending = stage;
@@ -477,40 +490,49 @@ struct Core4bit {
     if (pending < 0) return;
     uint8_t* to = smem + pending;
     const int lane = threadIdx.x & 31;
-    int b[4] = {(int)(v_bytes & 255), (int)(v_bytes >> 8 & 255), (int)(v_bytes >> 16 & 255), (int)(v_bytes >> 24)};
-    if (kGroups == 2) b[2] = b[3] = b[0];
+    const int b[4] = {(int)(v_bytes & 255), (int)(v_bytes >> 8 & 255), (int)(v_bytes >> 16 & 255), (int)(v_bytes >> 24)};
     int top = max(max(b[0], b[1]), max(b[2], b[3]));
     const int least = min(min(b[0], b[1]), min(b[2], b[3]));
-    const bool rare = top == 255 || least < top - 14 || (k_bytes & ((k_bytes & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u);
-    top = max(top, 127 - 65);
+    // a byte of a key that is 0 or above kMostKey (top bits: it borrows, or it carries)
+    const uint32_t odd_key = (((k_bytes - 0x01010101u) & ~k_bytes) | (((k_bytes & 0x7f7f7f7fu) + (255 - kMostKey) * 0x01010101u) & k_bytes)) & 0x80808080u;
+    const bool rare = top > kMostTop || least < max(top, kLeastTop) - kSpread || odd_key;
+    top = max(top, kLeastTop);
     uint32_t f[4];      // 2^(e - E) as float16
     float kp[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       f[i] = b[i] * 1024 + (15 - top) * 1024;
-      kp[i] = __uint_as_float((i == 0 ? k_bytes << 23 : i == 1 ? k_bytes << 15 : i == 2 ? k_bytes << 7 : k_bytes >> 1) & 0x7f800000u);      // (2^-127 counts as 0)
+      kp[i] = __uint_as_float((i == 0 ? k_bytes << 23 : i == 1 ? k_bytes << 15 : i == 2 ? k_bytes << 7 : k_bytes >> 1) & 0x7f800000u);
     }
-    if (__any_sync(0xffffffffu, rare || least < 127 - 65 - 14)) {        // bytes of 255, powers under 2^-14 of the head's largest
+    far = false;
+    if (__any_sync(0xffffffffu, rare)) {
       rarely();
-      top = 127 - 65;
+      top = kLeastTop;
 #pragma unroll
       for (int i = 0; i < 4; ++i) top = b[i] == 255 ? top : max(top, b[i]);
+      bool mine = top > kMostTop;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int x = b[i] - top + 15;
-        f[i] = b[i] == 255 ? 0x7fff : x > 0 ? x << 10 : 0x400 >> min(1 - x, 31);
-        if ((k_bytes >> (8 * i) & 255) == 255) kp[i] = __uint_as_float(0x7fffffffu);
+        mine |= b[i] > kZero && x < 15 - kSpread;
+        f[i] = b[i] == 255 ? 0x7fff : x >= 15 - kSpread ? x << 10 : 0;
+        const int key = k_bytes >> (8 * i) & 255;
+        mine |= key > kMostKey && key != 255;
+        kp[i] = e8m0_value(key);
       }
+      far = __any_sync(0xffffffffu, mine);
     }
+    if (far || wide) *reinterpret_cast<uint32_t*>(to + kBytes + lane * 4) = v_bytes;
     uint16_t* vp = reinterpret_cast<uint16_t*>(to + kValuePowers) + (lane & 16) + (lane & 6) + (lane >> 3 & 1) + (lane & 1) * 8;      // the row m of the key
 #pragma unroll
     for (int i = 0; i < kGroups; ++i) vp[i * 32] = (uint16_t)f[i];
     *reinterpret_cast<float4*>(to + kKeyPowers + lane * 16) = make_float4(kp[0], kp[1], kp[2], kp[3]);
-    *reinterpret_cast<float2*>(to + kTops + lane * 8) = make_float2((float)(top - 127), top == 254 ? __uint_as_float(0x00400000u) : __uint_as_float((uint32_t)(254 - top) << 23));
+    *reinterpret_cast<float2*>(to + kTops + lane * 8) = make_float2((float)(top - 127), __uint_as_float((uint32_t)(254 - top) << 23));
     pending = -1;
   }
   __device__ __forceinline__ void begin(const PagedParams& p, const Cur& c, int lane) {
     const int g = lane >> 2, t = lane & 3;
+    wide = false;
     rows.start(p, c.x, lane);
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
@@ -531,8 +553,8 @@ struct Core4bit {
       }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const int e = min(max((int)(__float_as_uint(top) >> 23), 1), 253);      // top < 2^(e - 126)
-      const float down = __uint_as_float((uint32_t)(254 - e) << 23), up = p.scale_log2 * __uint_as_float((uint32_t)e << 23);
+      const int e = min(max((int)(__float_as_uint(top) >> 23), 15), 254);      // top < 2^(e - 126)
+      const float down = __uint_as_float((uint32_t)(268 - e) << 23), up = p.scale_log2 * __uint_as_float((uint32_t)(e - 14) << 23);
       scale[i][0] = __shfl_sync(0xffffffffu, up, t * 8);                      // (row 2t is that of lanes 8t to 8t + 3)
       scale[i][1] = __shfl_sync(0xffffffffu, up, t * 8 + 4);
 #pragma unroll
@@ -555,7 +577,9 @@ struct Core4bit {
   }
   // The key of row m of a tile of 16: so that the values' codes of keys m = 2t and 2t + 8, which the sums want in one register, lie in neighbouring keys.
   static __device__ __forceinline__ int key_of(int m) { return (m & 1) * 8 + (m & 6) + (m >> 3); }
-  // Scores of keys 16 h and up: s[i][e] for key key_of((e >> 1) * 8 + g), row 2t + (e & 1)
+  // Scores of keys 16 h and up: s[i][e] for key key_of((e >> 1) * 8 + g), row 2t + (e & 1).  SCALED: with the row's scale (which comes first there: powers of keys may
+  // be as large as a float32 is)
+  template <bool SCALED>
   __device__ __forceinline__ void scores(const uint8_t* stage, int h, int lane, float (&s)[NT][4]) const {
     const int g = lane >> 2;
     uint32_t w[2][kGroups];      // codes of keys g and g + 8
@@ -585,16 +609,24 @@ struct Core4bit {
         mma_f16_first(z, a[0], q[i][2 * k][0], q[i][2 * k][1]);
         mma_f16(z, a[1], q[i][2 * k + 1][0], q[i][2 * k + 1][1]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[i][e] = k ? fmaf(z[e], f[e >> 1][k], s[i][e]) : z[e] * f[e >> 1][k];
+        for (int e = 0; e < 4; ++e) {
+          if (SCALED) z[e] *= scale[i][e & 1];
+          s[i][e] = k ? fmaf(z[e], f[e >> 1][k], s[i][e]) : z[e] * f[e >> 1][k];
+        }
       }
     }
   }
   __device__ __forceinline__ void take(const PagedParams& p, const Cur& c, const uint8_t* stage, int k0, int lane) {
+    if (far || wide) {
+      rarely();
+      take_wide(p, c, stage, k0, lane);
+      return;
+    }
     const int g = lane >> 2;
     const bool cut = c.x.cut(k0, kTile);
     float s[2][NT][4];
-    scores(stage, 0, lane, s[0]);
-    scores(stage, 1, lane, s[1]);
+    scores<false>(stage, 0, lane, s[0]);
+    scores<false>(stage, 1, lane, s[1]);
     float2 tops[2][2];
 #pragma unroll
     for (int h = 0; h < 2; ++h)
@@ -644,18 +676,102 @@ struct Core4bit {
         values<true>(p, stage, k0, 1, lane, w[1], c.x.first + tok);
       }
   }
+  // The codes of keys 16 h and up, of components 32 k to 32 k + 63: four of keys 2t and 2t + 1 (rows m = 2t and 2t + 8 of the tile), and of keys 8 further on (m = 2t + 1 and 2t + 9)
+  static __device__ __forceinline__ void codes(const uint8_t* stage, int h, int k, int lane, uint32_t (&x)[2][2]) {
+    uint32_t y[4];
+    matrices_turned(y, smem_at(stage) + kSide + chunk_at(h * 16 + (lane >> 3 & 1) * 8 + (lane & 7), k + (lane >> 4)));
+    x[0][0] = y[0]; x[0][1] = y[1]; x[1][0] = y[2]; x[1][1] = y[3];
+  }
+  // and as operands: a byte for each pair of keys and component
+  static __device__ __forceinline__ void operands(const uint32_t (&x)[2], uint32_t (&a)[2][4]) {
+    uint32_t even[4], odd[4];
+    from_e2m1x8((x[0] & 0x0f0f0f0fu) | ((x[1] * 16u) & 0xf0f0f0f0u), even);                      // components 0 and 2 of four, of rows m = 2t; of 2t + 8
+    from_e2m1x8((__umulhi(x[0], 1u << 28) & 0x0f0f0f0fu) | (x[1] & 0xf0f0f0f0u), odd);           // (a shift by the multiplier, which has time)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) { a[j][0] = even[j]; a[j][1] = odd[j]; a[j][2] = even[j + 2]; a[j][3] = odd[j + 2]; }
+  }
+  // The same tile whatever its powers: o += V^T (weight times power), for every 32 components against the tile's own maximum of that.  From here on o and l are in
+  // units of 2^(m - kWideUp), m the maximum of the scores.
+  __device__ __forceinline__ void take_wide(const PagedParams& p, const Cur& c, const uint8_t* stage, int k0, int lane) {
+    const int g = lane >> 2;
+    if (!wide) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int z = 0; z < 2; ++z) rows.m[i][z] += kWideUp - kWeightUp;      // (the same units: m need not be the maximum, only near it)
+      wide = true;
+    }
+    float s[2][NT][4];
+    scores<true>(stage, 0, lane, s[0]);
+    scores<true>(stage, 1, lane, s[1]);
+    uint32_t bytes[2][2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) bytes[h][u] = *reinterpret_cast<const uint32_t*>(stage + kBytes + (h * 16 + key_of(u * 8 + g)) * 4);
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      float top[2] = {rows.m[i][0], rows.m[i][1]};
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (!rows.sees(p, i, e & 1, k0 + h * 16 + key_of((e >> 1) * 8 + g))) s[h][i][e] = -INFINITY;
+          top[e & 1] = fmaxf(top[e & 1], s[h][i][e]);
+        }
+      rows.rescale(i, top, o[i], kWideUp);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) rows.l[i][e & 1] += exp2_approx(s[h][i][e] - top[e & 1]);
+#pragma unroll
+      for (int k = 0; k < kGroups; ++k) {
+        float x[2][4], most[2] = {-INFINITY, -INFINITY}, f[2], acc[2][4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int b = bytes[h][e >> 1] >> (8 * k) & 255;
+            x[h][e] = s[h][i][e] == -INFINITY ? -INFINITY : s[h][i][e] + (b == 255 ? __uint_as_float(0x7fffffffu) : (float)(b - 127));
+            most[e & 1] = fmaxf(most[e & 1], x[h][e]);
+          }
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+#pragma unroll
+          for (int lanes = 4; lanes < 32; lanes <<= 1) most[z] = fmaxf(most[z], __shfl_xor_sync(0xffffffffu, most[z], lanes));
+          most[z] = most[z] == -INFINITY ? 0.f : most[z] - kWeightUp;
+          f[z] = exp2_approx(0.5f * (most[z] - top[z]));          // (twice: the product may be below 2^-126)
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t b[2], y[2][2], a[2][4];
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const __half2 w = __floats2half2_rn(exp2_approx(x[h][2 * u] - most[0]), exp2_approx(x[h][2 * u + 1] - most[1]));
+            b[u] = turned(*reinterpret_cast<const uint32_t*>(&w));
+          }
+          codes(stage, h, k & ~1, lane, y);
+          operands(y[k & 1], a);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            if (h == 0) mma_f16_first(acc[j], a[j], b[0], b[1]);
+            else mma_f16(acc[j], a[j], b[0], b[1]);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[i][2 * k + j][e] = fmaf(acc[j][e] * f[e & 1], f[e & 1], o[i][2 * k + j][e]);
+      }
+    }
+  }
   // o += V^T w over keys 16 h and up.  ONE: only the rows of the token at `at`, of the keys that it sees.
   template <bool ONE>
   __device__ __forceinline__ void values(const PagedParams& p, const uint8_t* stage, int k0, int h, int lane, const uint32_t (&w)[NT][2], int at) {
     const int t = lane & 3;
-    // four codes of keys 2t and 2t + 1 (rows m = 2t and 2t + 8 of the tile), and of keys 8 further on (m = 2t + 1 and 2t + 9)
-    uint32_t x[kGroups][2];
+    uint32_t x[kGroups / 2][2][2];
 #pragma unroll
-    for (int k = 0; k < kGroups; k += 2) {
-      uint32_t y[4];
-      matrices_turned(y, smem_at(stage) + kSide + chunk_at(h * 16 + (lane >> 3 & 1) * 8 + (lane & 7), k + (lane >> 4)));
-      x[k][0] = y[0]; x[k][1] = y[1]; x[k + 1][0] = y[2]; x[k + 1][1] = y[3];
-    }
+    for (int k = 0; k < kGroups; k += 2) codes(stage, h, k, lane, x[k / 2]);
     uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
     if (ONE) {
       const uint32_t a = seen_pair(p, at, k0 + h * 16 + 2 * t), b = seen_pair(p, at, k0 + h * 16 + 8 + 2 * t);
@@ -666,11 +782,8 @@ struct Core4bit {
     for (int k = 0; k < kGroups; ++k) {
       const uint32_t f0 = *reinterpret_cast<const uint32_t*>(stage + kValuePowers + (k * 32 + h * 16 + 2 * t) * 2);
       const uint32_t f1 = *reinterpret_cast<const uint32_t*>(stage + kValuePowers + (k * 32 + h * 16 + 8 + 2 * t) * 2);
-      // a byte for each pair of keys and component
-      uint32_t even[4], odd[4];
-      from_e2m1x8((x[k][0] & 0x0f0f0f0fu) | ((x[k][1] * 16u) & 0xf0f0f0f0u), even);                      // components 0 and 2 of four, of rows m = 2t; of 2t + 8
-      from_e2m1x8((__umulhi(x[k][0], 1u << 28) & 0x0f0f0f0fu) | (x[k][1] & 0xf0f0f0f0u), odd);           // (a shift by the multiplier, which has time)
-      const uint32_t a[2][4] = {{even[0], odd[0], even[2], odd[2]}, {even[1], odd[1], even[3], odd[3]}};
+      uint32_t a[2][4];
+      operands(x[k / 2][k & 1], a);
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
         uint32_t b0 = times(w[i][0], f0), b1 = times(w[i][1], f1);
@@ -689,7 +802,7 @@ struct Core4bit {
       }
     }
   }
-  __device__ __forceinline__ void stats(const Buffer<DP>& buffer, int warp, int lane) const { rows.stats(buffer, warp, lane, kWeightUp); }
+  __device__ __forceinline__ void stats(const Buffer<DP>& buffer, int warp, int lane) const { rows.stats(buffer, warp, lane, wide ? kWideUp : kWeightUp); }
   template <typename F>
   __device__ __forceinline__ void put(int pass, F factor, float* out, int lane) const {
     const int g = lane >> 2, t = lane & 3;
