@@ -599,6 +599,9 @@ OptTensor append(const Tensor& pages_k, const Tensor& pages_v, const Tensor& tab
     rc = lib.bma_append_kv(&c, &a, place.stream);
   }
   check(rc, "bma_append_kv");
+  // a graph that has saved pages has to notice (tensors made in inference mode have no version, and no graph)
+  for (const Tensor* t : {&pages_k, &pages_v, pointer(k_scale), pointer(v_scale)})
+    if (t && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
   return q_out;
 }
 
