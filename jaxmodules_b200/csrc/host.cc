@@ -392,7 +392,8 @@ struct Rotation {
   double eps;
 };
 
-std::tuple<Tensor, OptTensor> rotate_forward(const Tensor& q_in, const OptTensor& k_in, const Rotation& r, bool from_python) {
+// (both ways here come from Python and hold its lock)
+std::tuple<Tensor, OptTensor> rotate_forward(const Tensor& q_in, const OptTensor& k_in, const Rotation& r) {
   const Tensor q = heads_of(q_in, "q");
   OptTensor k, k_out;
   if (k_in) k = heads_of(*k_in, "k");
@@ -407,11 +408,11 @@ std::tuple<Tensor, OptTensor> rotate_forward(const Tensor& q_in, const OptTensor
     a.k = describe(*k); a.k_out = describe(*k_out);
   }
   int rc;
-  if (from_python) {
+  {
     Group group("bma.rotate");
     rc = lib.bma_rotate(&a, place.stream);
-  } else rc = lib.bma_rotate(&a, place.stream);
-  TORCH_CHECK(rc == BMA_OK, "bma_rotate: status ", std::to_string(rc), ": ", lib.bma_error_string(rc));
+  }
+  check(rc, "bma_rotate");
   return {q_out, k_out};
 }
 
@@ -456,7 +457,7 @@ struct RotateNode : torch::autograd::Function<RotateNode> {
                                double magnitude, const OptTensor& q_weight, const OptTensor& k_weight, double eps) {
     at::AutoDispatchBelowADInplaceOrView below;
     const auto or_none = [](const OptTensor& t) { return t ? *t : Tensor(); };
-    auto [q_out, k_out] = rotate_forward(q, k, {positions, frequencies, (int)layout, magnitude, q_weight, k_weight, eps}, true);
+    auto [q_out, k_out] = rotate_forward(q, k, {positions, frequencies, (int)layout, magnitude, q_weight, k_weight, eps});
     // a rotation alone is undone without its input: only the shape, the dtype and the device are kept
     ctx->save_for_backward({q_weight ? q : Tensor(), k && k_weight ? *k : Tensor(), or_none(positions), or_none(frequencies), or_none(q_weight), or_none(k_weight)});
     ctx->saved_data["layout"] = layout;
@@ -493,7 +494,7 @@ std::tuple<Tensor, OptTensor> rotate(const Tensor& q, const OptTensor& k, const 
                                      const OptTensor& q_weight, const OptTensor& k_weight, double eps) {
   no_tangents({&q, pointer(k), pointer(q_weight), pointer(k_weight), pointer(frequencies)}, "rotate_heads");
   TORCH_CHECK_VALUE(!wants_gradient({pointer(frequencies)}), "rotate_heads is not differentiable in frequencies: detach them");
-  if (!wants_gradient({&q, pointer(k), pointer(q_weight), pointer(k_weight)})) return rotate_forward(q, k, {positions, frequencies, layout, magnitude, q_weight, k_weight, eps}, true);
+  if (!wants_gradient({&q, pointer(k), pointer(q_weight), pointer(k_weight)})) return rotate_forward(q, k, {positions, frequencies, layout, magnitude, q_weight, k_weight, eps});
   const variable_list out = RotateNode::apply(q, k, positions, frequencies, (int64_t)layout, magnitude, q_weight, k_weight, eps);
   return {out[0], out.size() > 1 ? OptTensor(out[1]) : OptTensor()};
 }
