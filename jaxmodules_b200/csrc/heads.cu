@@ -1254,6 +1254,7 @@ int read_kv(const bma_paged_cache* c, const int32_t* lengths, int L, const bma_t
   int rc = validate_cache(c);
   if (rc != BMA_OK) return rc;
   BMA_REQUIRE(lengths && L > 0 && k && v, BMA_ERR_ARG);
+  BMA_REQUIRE(L < (1ll << 31) - 4096, BMA_ERR_LIMIT);      // (as many as a table may cover; rounded up to kReadTokens it fits an int)
   const int dtype = c->dtype == BMA_DTYPE_F32 ? BMA_DTYPE_F32 : BMA_DTYPE_BF16, vec = dtype == BMA_DTYPE_F32 ? 4 : 8;
   if ((rc = validate_heads(*k, dtype)) || (rc = validate_heads(*v, dtype))) return rc;
   BMA_REQUIRE(wide_tensor(*k, vec) && wide_tensor(*v, vec), BMA_ERR_UNSUPPORTED);

@@ -612,7 +612,7 @@ std::tuple<Tensor, Tensor> read_pages(const Tensor& pages_k, const Tensor& pages
   const bma_paged_cache c = cache_of(on, pages_k, pages_v, table, k_scale, v_scale);
   no_tangents({&pages_k, &pages_v}, "read_kv");
   TORCH_CHECK_VALUE(!wants_gradient({&pages_k, &pages_v}), "read_kv is not differentiable: call it under torch.no_grad()");
-  TORCH_CHECK_VALUE(L > 0 && L <= INT32_MAX, "max_length must be positive");
+  TORCH_CHECK_VALUE(L > 0 && L < (1ll << 31) - 4096, "max_length must be positive, and below 2^31 - 4096");
   const int32_t* at_lengths = counts_of(on, lengths, c, "lengths");
   on.check();
   const Place place(pages_k);
