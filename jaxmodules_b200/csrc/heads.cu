@@ -28,41 +28,6 @@ template <typename T> struct Bits16;   // values of a 16-byte chunk
 template <> struct Bits16<float> { static constexpr int n = 4; };
 template <> struct Bits16<__nv_bfloat16> { static constexpr int n = 8; };
 
-// VEC values: one, where the tensors allow no wider access
-template <typename T, int VEC>
-struct Chunk {
-  uint4 raw;
-  __device__ __forceinline__ void load(const T* p) {
-    if constexpr (VEC == 1) raw.x = sizeof(T) == 4 ? __float_as_uint(to_float(*p)) : (uint32_t)*reinterpret_cast<const unsigned short*>(p);
-    else raw = *reinterpret_cast<const uint4*>(p);
-  }
-  __device__ __forceinline__ void zero() { raw = make_uint4(0, 0, 0, 0); }
-  __device__ __forceinline__ void get(float (&x)[VEC]) const {
-    if constexpr (VEC == 1) x[0] = sizeof(T) == 4 ? __uint_as_float(raw.x) : __uint_as_float(raw.x << 16);
-    else if constexpr (VEC == 4) {
-      x[0] = __uint_as_float(raw.x); x[1] = __uint_as_float(raw.y); x[2] = __uint_as_float(raw.z); x[3] = __uint_as_float(raw.w);
-    } else {
-      const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
-    }
-  }
-};
-template <typename T, int VEC>
-__device__ __forceinline__ void store_chunk(T* p, const float (&x)[VEC]) {
-  if constexpr (VEC == 1) *p = from_float<T>(x[0]);
-  else if constexpr (VEC == 4) *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
-  else {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-      w[i] = *reinterpret_cast<const uint32_t*>(&h);
-    }
-    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-  }
-}
-
 // frequency / 2 pi as a multiple of 2^-64, modulo 1
 __device__ __forceinline__ unsigned long long step_of(double frequency) {
   double turns = frequency * 0.15915494309189533577;
@@ -77,71 +42,63 @@ __device__ __forceinline__ void turn_of(unsigned long long step, long long posit
   s *= magnitude;
 }
 
-// How the lanes of a warp lie on heads: `tpr` lanes (a power of two) to a head, each with UPT units of two chunks.
+// How the lanes of a warp lie on heads: `tpr` lanes (a power of two) to a head, each with a unit of two chunks (the narrow form: four units, a value to a chunk).
 struct HeadMap {
   int tpr, chunks, half_chunks, dim, layout;   // half_chunks: dim / 2 in chunks (HALF layout)
 };
 
-template <int VEC>
 __device__ __forceinline__ void unit_chunks(const HeadMap& m, int u, int& ca, int& cb) {
   if (m.layout == BMA_ROTARY_INTERLEAVED) { ca = 2 * u; cb = 2 * u + 1; }
   else if (u < m.half_chunks) { ca = u; cb = u + m.half_chunks; }
   else { ca = 2 * u; cb = 2 * u + 1; }   // (what is not rotated: chunks from 2 * half_chunks on)
 }
 
-// The pairs of one unit: pair j is rotated where bit j of `live` is set.
-template <int VEC>
-struct Turns {
-  float c[VEC], s[VEC];
-  uint32_t live;
+// The narrow form's unit: one pair, and how it is turned.
+constexpr int kUnits = 4;      // to a lane: 32 lanes hold 256 components
+struct Turn {
+  float c, s;
+  bool live;             // the pair is rotated
   __device__ __forceinline__ void make(const HeadMap& m, const double* frequencies, int u, long long position, float magnitude) {
-    live = 0;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      const int i = u * VEC + j;
-      c[j] = 1.f; s[j] = 0.f;
-      if (2 * i < m.dim) {
-        live |= 1u << j;
-        turn_of(step_of(__ldg(frequencies + i)), position, magnitude, c[j], s[j]);
-      }
-    }
+    c = 1.f;
+    s = 0.f;
+    live = 2 * u < m.dim;
+    if (live) turn_of(step_of(__ldg(frequencies + u)), position, magnitude, c, s);
   }
   // BACK: by the negative angle
   template <bool BACK>
-  __device__ __forceinline__ void apply(int layout, float (&a)[VEC], float (&b)[VEC]) const {
-    if (VEC > 1 && layout == BMA_ROTARY_INTERLEAVED) {
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        float& x = 2 * j < VEC ? a[(2 * j) % VEC] : b[(2 * j) % VEC];
-        float& y = 2 * j < VEC ? a[(2 * j + 1) % VEC] : b[(2 * j + 1) % VEC];
-        one<BACK>(j, x, y);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) one<BACK>(j, a[j], b[j]);
-    }
-  }
-  template <bool BACK>
-  __device__ __forceinline__ void one(int j, float& x, float& y) const {
-    const float sn = BACK ? -s[j] : s[j];
-    const float p = x * c[j] - y * sn, q = y * c[j] + x * sn;
-    if (live >> j & 1) { x = p; y = q; }
+  __device__ __forceinline__ void apply(float& x, float& y) const {
+    const float sn = BACK ? -s : s;
+    const float p = x * c - y * sn, q = y * c + x * sn;
+    if (live) { x = p; y = q; }
   }
 };
+
+// A lane's values of a head, all of them asked for at once; zeros where there are none.
+template <typename T>
+__device__ __forceinline__ void load_units(const T* head, bool there, const int (&ca)[kUnits], const int (&cb)[kUnits], int d, float (&a)[kUnits], float (&b)[kUnits]) {
+  T x[kUnits], y[kUnits];
+#pragma unroll
+  for (int i = 0; i < kUnits; ++i) {
+    x[i] = y[i] = from_float<T>(0.f);
+    if (there) {
+      if (ca[i] < d) x[i] = head[ca[i]];
+      if (cb[i] < d) y[i] = head[cb[i]];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kUnits; ++i) {
+    a[i] = to_float(x[i]);
+    b[i] = to_float(y[i]);
+  }
+}
 
 __device__ __forceinline__ float group_sum(float x, int tpr) {
   for (int o = tpr >> 1; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
   return x;
 }
 
-template <int VEC>
-__device__ __forceinline__ void load_weight(const void* w, int dtype, int chunk, int chunks, float (&x)[VEC]) {
-#pragma unroll
-  for (int j = 0; j < VEC; ++j) {
-    x[j] = 0.f;
-    if (chunk < chunks) x[j] = dtype == BMA_DTYPE_F32 ? __ldg(static_cast<const float*>(w) + chunk * VEC + j)
-                                                      : __bfloat162float(static_cast<const __nv_bfloat16*>(w)[chunk * VEC + j]);
-  }
+__device__ __forceinline__ float weight_at(const void* w, int dtype, int i) {
+  return dtype == BMA_DTYPE_F32 ? __ldg(static_cast<const float*>(w) + i) : __bfloat162float(static_cast<const __nv_bfloat16*>(w)[i]);
 }
 
 // One side (q, k or v) of a launch: where its heads come from and go to.
@@ -243,8 +200,8 @@ __device__ __forceinline__ void store_4bit(const float* row, bool there, int d, 
   }
 }
 
-// A warp takes one token and a slab of its heads (all sides counted through), `tpr` lanes to a head, NR heads at a time.
-template <typename T, int VEC, int UPT, int NR, int KIND>
+// The narrow form.  A warp takes one token and a slab of its heads (all sides counted through), `tpr` lanes to a head, a value at a time.
+template <typename T, int KIND>
 __global__ void __launch_bounds__(kHeadsThreads) heads_kernel(const __grid_constant__ HeadsParams p) {
   __shared__ float rows[KIND == kAppend4 ? kHeadsWarps : 1][KIND == kAppend4 ? 8 : 1][KIND == kAppend4 ? kPagedHeadDim + 4 : 1];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -261,23 +218,21 @@ __global__ void __launch_bounds__(kHeadsThreads) heads_kernel(const __grid_const
   if constexpr (KIND == kRotate) position = position_of(p, b, t);
   else real = token_place(p, b, t, lane, position, held, held_scale);
 
-  Turns<VEC> turns[UPT];
-  int ca[UPT], cb[UPT];
+  Turn turns[kUnits];
+  int ca[kUnits], cb[kUnits];
   const bool turned = p.map.dim > 0;
 #pragma unroll
-  for (int i = 0; i < UPT; ++i) {
-    unit_chunks<VEC>(p.map, u0 + i * tpr, ca[i], cb[i]);
+  for (int i = 0; i < kUnits; ++i) {
+    unit_chunks(p.map, u0 + i * tpr, ca[i], cb[i]);
     if (turned) turns[i].make(p.map, p.frequencies, u0 + i * tpr, position, p.magnitude);
   }
   const int slab_begin = slab * p.slab_heads, slab_end = slab_begin + p.slab_heads;
   const float inv_d = 1.f / (float)p.d;
 
-  int first = 0;      // heads of the sides before
 #pragma unroll 1
   for (int si = 0; si < (KIND == kRotate ? 2 : 3); ++si) {
     const Side& side = p.side[si];
-    const int lo = max(slab_begin - first, 0), hi = min(slab_end - first, side.heads);
-    first += side.heads;
+    const int lo = max(slab_begin - side.before, 0), hi = min(slab_end - side.before, side.heads);
     if (lo >= hi) continue;
     const bool cached = KIND != kRotate && si > 0;
     if (cached && (!real || held < 0)) continue;
@@ -288,85 +243,49 @@ __global__ void __launch_bounds__(kHeadsThreads) heads_kernel(const __grid_const
       out = static_cast<T*>(si == 1 ? p.cache.k : p.cache.v) + held;      // (a 4-bit cache is not written through this)
       out_head = p.cache.stride_head;
     }
-    float wa[UPT][VEC], wb[UPT][VEC];
     const bool normed = side.weight != nullptr;
-    if (normed) {
+    float wa[kUnits], wb[kUnits];
 #pragma unroll
-      for (int i = 0; i < UPT; ++i) {
-        load_weight<VEC>(side.weight, p.weight_dtype, ca[i], p.map.chunks, wa[i]);
-        load_weight<VEC>(side.weight, p.weight_dtype, cb[i], p.map.chunks, wb[i]);
-      }
+    for (int i = 0; i < kUnits; ++i) {
+      wa[i] = normed && ca[i] < p.map.chunks ? weight_at(side.weight, p.weight_dtype, ca[i]) : 0.f;
+      wb[i] = normed && cb[i] < p.map.chunks ? weight_at(side.weight, p.weight_dtype, cb[i]) : 0.f;
     }
 #pragma unroll 1
-    for (int h0 = lo; h0 < hi; h0 += groups * NR) {
-      Chunk<T, VEC> a[NR][UPT], c[NR][UPT];
+    for (int h = lo + group; h - group < hi; h += groups) {
+      float xa[kUnits], xb[kUnits];
+      float sum = 0.f;
+      load_units(in + h * side.in.stride_h, h < hi && real, ca, cb, p.map.chunks, xa, xb);
+      if (normed) {
 #pragma unroll
-      for (int r = 0; r < NR; ++r) {
-        const int h = h0 + r * groups + group;
+        for (int i = 0; i < kUnits; ++i) sum = fmaf(xa[i], xa[i], fmaf(xb[i], xb[i], sum));
+        const float inv = rsqrtf(group_sum(sum, tpr) * inv_d + p.eps);
 #pragma unroll
-        for (int i = 0; i < UPT; ++i) {
-          a[r][i].zero();
-          c[r][i].zero();
-          if (h < hi && real) {
-            if (ca[i] < p.map.chunks) a[r][i].load(in + h * side.in.stride_h + ca[i] * VEC);
-            if (cb[i] < p.map.chunks) c[r][i].load(in + h * side.in.stride_h + cb[i] * VEC);
-          }
+        for (int i = 0; i < kUnits; ++i) { xa[i] *= inv * wa[i]; xb[i] *= inv * wb[i]; }
+      }
+      if (turned && side.turned) {
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) {
+          if (p.back) turns[i].template apply<true>(xa[i], xb[i]);
+          else turns[i].template apply<false>(xa[i], xb[i]);
         }
       }
+      if (KIND == kAppend4 && cached) {
+        float* row = rows[warp][group];
+        __syncwarp();
 #pragma unroll
-      for (int r = 0; r < NR; ++r) {
-        const int h = h0 + r * groups + group;
-        float xa[UPT][VEC], xb[UPT][VEC];
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < UPT; ++i) {
-          a[r][i].get(xa[i]);
-          c[r][i].get(xb[i]);
+        for (int i = 0; i < kUnits; ++i) {
+          if (ca[i] < p.map.chunks) row[ca[i]] = xa[i];
+          if (cb[i] < p.map.chunks) row[cb[i]] = xb[i];
         }
-        if (normed) {
+        __syncwarp();
+        uint8_t* codes = static_cast<uint8_t*>(si == 1 ? p.cache.k : p.cache.v) + held + h * p.cache.stride_head;
+        uint8_t* scales = (si == 1 ? p.cache.k_scale : p.cache.v_scale) + held_scale + h * p.cache.scale_stride_head;
+        store_4bit(row, h < hi, p.d, tpr, u0, codes, scales);
+      } else if (h < hi) {
 #pragma unroll
-          for (int i = 0; i < UPT; ++i)
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) sum = fmaf(xa[i][j], xa[i][j], fmaf(xb[i][j], xb[i][j], sum));
-          const float inv = rsqrtf(group_sum(sum, tpr) * inv_d + p.eps);
-#pragma unroll
-          for (int i = 0; i < UPT; ++i)
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) { xa[i][j] *= inv * wa[i][j]; xb[i][j] *= inv * wb[i][j]; }
-        }
-        if (turned && side.turned) {
-#pragma unroll
-          for (int i = 0; i < UPT; ++i) {
-            if (p.back) turns[i].template apply<true>(p.map.layout, xa[i], xb[i]);
-            else turns[i].template apply<false>(p.map.layout, xa[i], xb[i]);
-          }
-        }
-        if (KIND == kAppend4 && cached) {
-          float* row = rows[warp][group];
-          __syncwarp();
-#pragma unroll
-          for (int i = 0; i < UPT; ++i)
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-              if (ca[i] < p.map.chunks) row[ca[i] * VEC + j] = xa[i][j];
-              if (cb[i] < p.map.chunks) row[cb[i] * VEC + j] = xb[i][j];
-            }
-          __syncwarp();
-          uint8_t* codes = static_cast<uint8_t*>(si == 1 ? p.cache.k : p.cache.v) + held + h * p.cache.stride_head;
-          uint8_t* scales = (si == 1 ? p.cache.k_scale : p.cache.v_scale) + held_scale + h * p.cache.scale_stride_head;
-          store_4bit(row, h < hi, p.d, tpr, u0, codes, scales);
-        } else if (h < hi) {
-          if (!real) {
-#pragma unroll
-            for (int i = 0; i < UPT; ++i)
-#pragma unroll
-              for (int j = 0; j < VEC; ++j) xa[i][j] = xb[i][j] = 0.f;
-          }
-#pragma unroll
-          for (int i = 0; i < UPT; ++i) {
-            if (ca[i] < p.map.chunks) store_chunk<T, VEC>(out + h * out_head + ca[i] * VEC, xa[i]);
-            if (cb[i] < p.map.chunks) store_chunk<T, VEC>(out + h * out_head + cb[i] * VEC, xb[i]);
-          }
+        for (int i = 0; i < kUnits; ++i) {      // (zeros for a token that is not real)
+          if (ca[i] < p.map.chunks) out[h * out_head + ca[i]] = from_float<T>(real ? xa[i] : 0.f);
+          if (cb[i] < p.map.chunks) out[h * out_head + cb[i]] = from_float<T>(real ? xb[i] : 0.f);
         }
       }
     }
@@ -391,7 +310,7 @@ struct BackParams {
   float* partial;
 };
 
-template <typename T, int VEC, int UPT>
+template <typename T>
 __global__ void __launch_bounds__(kHeadsThreads, 4) rotate_back_kernel(const __grid_constant__ BackParams p) {
   __shared__ float sums[kHeadsWarps][256];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -401,96 +320,70 @@ __global__ void __launch_bounds__(kHeadsThreads, 4) rotate_back_kernel(const __g
   const Side& side = p.side[si];
   const bma_tensor& g = p.g[si];
   const float inv_d = 1.f / (float)p.d;
-  int ca[UPT], cb[UPT];
-  float wa[UPT][VEC], wb[UPT][VEC], da[UPT][VEC], db[UPT][VEC];
+  int ca[kUnits], cb[kUnits];
+  float wa[kUnits], wb[kUnits], da[kUnits], db[kUnits];
 #pragma unroll
-  for (int i = 0; i < UPT; ++i) {
-    unit_chunks<VEC>(p.map, u0 + i * tpr, ca[i], cb[i]);
-    load_weight<VEC>(side.weight, p.weight_dtype, ca[i], p.map.chunks, wa[i]);
-    load_weight<VEC>(side.weight, p.weight_dtype, cb[i], p.map.chunks, wb[i]);
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) da[i][j] = db[i][j] = 0.f;
+  for (int i = 0; i < kUnits; ++i) {
+    unit_chunks(p.map, u0 + i * tpr, ca[i], cb[i]);
+    wa[i] = ca[i] < p.map.chunks ? weight_at(side.weight, p.weight_dtype, ca[i]) : 0.f;
+    wb[i] = cb[i] < p.map.chunks ? weight_at(side.weight, p.weight_dtype, cb[i]) : 0.f;
+    da[i] = db[i] = 0.f;
   }
   const int64_t tokens = (int64_t)p.B * p.L;
 #pragma unroll 1
   for (int64_t token = (int64_t)cta * kHeadsWarps + warp; token < tokens; token += (int64_t)ctas * kHeadsWarps) {
     const int b = (int)(token / p.L), t = (int)(token - (int64_t)b * p.L);
     const long long position = position_of(p, b, t);
-    Turns<VEC> turns[UPT];
+    Turn turns[kUnits];
     const bool turned = p.map.dim > 0;
     if (turned) {
 #pragma unroll
-      for (int i = 0; i < UPT; ++i) turns[i].make(p.map, p.frequencies, u0 + i * tpr, position, p.magnitude);
+      for (int i = 0; i < kUnits; ++i) turns[i].make(p.map, p.frequencies, u0 + i * tpr, position, p.magnitude);
     }
     const T* in = static_cast<const T*>(side.in.ptr) + b * side.in.stride_b + t * side.in.stride_l;
     const T* gin = static_cast<const T*>(g.ptr) + b * g.stride_b + t * g.stride_l;
     T* out = static_cast<T*>(side.out.ptr) + b * side.out.stride_b + t * side.out.stride_l;
 #pragma unroll 1
-    for (int h0 = 0; h0 < side.heads; h0 += groups) {
-      const int h = h0 + group;
-      Chunk<T, VEC> xa[UPT], xb[UPT], ga[UPT], gb[UPT];
-#pragma unroll
-      for (int i = 0; i < UPT; ++i) {
-        xa[i].zero(); xb[i].zero(); ga[i].zero(); gb[i].zero();
-        if (h < side.heads && ca[i] < p.map.chunks) {
-          xa[i].load(in + h * side.in.stride_h + ca[i] * VEC);
-          ga[i].load(gin + h * g.stride_h + ca[i] * VEC);
-        }
-        if (h < side.heads && cb[i] < p.map.chunks) {
-          xb[i].load(in + h * side.in.stride_h + cb[i] * VEC);
-          gb[i].load(gin + h * g.stride_h + cb[i] * VEC);
-        }
-      }
-      float fa[UPT][VEC], fb[UPT][VEC], ea[UPT][VEC], eb[UPT][VEC];
+    for (int h = group; h - group < side.heads; h += groups) {
+      const bool there = h < side.heads;
+      float fa[kUnits], fb[kUnits], ea[kUnits], eb[kUnits];
       float sum = 0.f, dot = 0.f;
+      load_units(in + h * side.in.stride_h, there, ca, cb, p.map.chunks, fa, fb);
+      load_units(gin + h * g.stride_h, there, ca, cb, p.map.chunks, ea, eb);
 #pragma unroll
-      for (int i = 0; i < UPT; ++i) {
-        xa[i].get(fa[i]); xb[i].get(fb[i]); ga[i].get(ea[i]); gb[i].get(eb[i]);
-        if (turned) turns[i].template apply<true>(p.map.layout, ea[i], eb[i]);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          sum = fmaf(fa[i][j], fa[i][j], fmaf(fb[i][j], fb[i][j], sum));
-          dot = fmaf(ea[i][j] * wa[i][j], fa[i][j], fmaf(eb[i][j] * wb[i][j], fb[i][j], dot));
-        }
+      for (int i = 0; i < kUnits; ++i) {
+        if (turned) turns[i].template apply<true>(ea[i], eb[i]);
+        sum = fmaf(fa[i], fa[i], fmaf(fb[i], fb[i], sum));
+        dot = fmaf(ea[i] * wa[i], fa[i], fmaf(eb[i] * wb[i], fb[i], dot));
       }
       for (int o = tpr >> 1; o; o >>= 1) {
         sum += __shfl_xor_sync(0xffffffffu, sum, o);
         dot += __shfl_xor_sync(0xffffffffu, dot, o);
       }
       const float inv = rsqrtf(sum * inv_d + p.eps), m = dot * inv * inv_d;     // m = mean(g' w x^)
+      if (!there) continue;
 #pragma unroll
-      for (int i = 0; i < UPT; ++i) {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float ha = fa[i][j] * inv, hb = fb[i][j] * inv;
-          if (h < side.heads) {
-            da[i][j] = fmaf(ea[i][j], ha, da[i][j]);
-            db[i][j] = fmaf(eb[i][j], hb, db[i][j]);
-          }
-          ea[i][j] = inv * (ea[i][j] * wa[i][j] - ha * m);
-          eb[i][j] = inv * (eb[i][j] * wb[i][j] - hb * m);
-        }
-        if (h < side.heads) {
-          if (ca[i] < p.map.chunks) store_chunk<T, VEC>(out + h * side.out.stride_h + ca[i] * VEC, ea[i]);
-          if (cb[i] < p.map.chunks) store_chunk<T, VEC>(out + h * side.out.stride_h + cb[i] * VEC, eb[i]);
-        }
+      for (int i = 0; i < kUnits; ++i) {
+        const float ha = fa[i] * inv, hb = fb[i] * inv;
+        da[i] = fmaf(ea[i], ha, da[i]);
+        db[i] = fmaf(eb[i], hb, db[i]);
+        if (ca[i] < p.map.chunks) out[h * side.out.stride_h + ca[i]] = from_float<T>(inv * (ea[i] * wa[i] - ha * m));
+        if (cb[i] < p.map.chunks) out[h * side.out.stride_h + cb[i]] = from_float<T>(inv * (eb[i] * wb[i] - hb * m));
       }
     }
   }
   // the groups of a warp, the warps of the CTA
 #pragma unroll
-  for (int i = 0; i < UPT; ++i)
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      for (int o = tpr; o < 32; o <<= 1) {
-        da[i][j] += __shfl_xor_sync(0xffffffffu, da[i][j], o);
-        db[i][j] += __shfl_xor_sync(0xffffffffu, db[i][j], o);
-      }
-      if (group == 0) {
-        if (ca[i] < p.map.chunks) sums[warp][ca[i] * VEC + j] = da[i][j];
-        if (cb[i] < p.map.chunks) sums[warp][cb[i] * VEC + j] = db[i][j];
-      }
+  for (int i = 0; i < kUnits; ++i) {
+    for (int o = tpr; o < 32; o <<= 1) {
+      da[i] += __shfl_xor_sync(0xffffffffu, da[i], o);
+      db[i] += __shfl_xor_sync(0xffffffffu, db[i], o);
     }
+    if (group == 0) {
+      if (ca[i] < p.map.chunks) sums[warp][ca[i]] = da[i];
+      if (cb[i] < p.map.chunks) sums[warp][cb[i]] = db[i];
+    }
+  }
   __syncthreads();
   for (int c = threadIdx.x; c < p.d; c += kHeadsThreads) {
     float s = 0.f;
@@ -648,7 +541,7 @@ __global__ void __launch_bounds__(kHeadsThreads, 4) heads_wide_kernel(const __gr
   const int tpr = p.map.tpr, group = lane / tpr, u = lane & (tpr - 1), groups = 32 / tpr, chunks = p.map.chunks;
   const int pairs = p.map.dim / 2;
   int ca, cb;
-  unit_chunks<VEC>(p.map, u, ca, cb);
+  unit_chunks(p.map, u, ca, cb);
   const uint32_t live = live_pairs<VEC>(u, pairs);
   const float inv_d = 1.f / (float)p.d;
   const bool A = ca < chunks, B = cb < chunks;
@@ -662,7 +555,7 @@ __global__ void __launch_bounds__(kHeadsThreads, 4) heads_wide_kernel(const __gr
   for (int i = threadIdx.x; i < 2 * p.d; i += kHeadsThreads) {
     const int si = i >= p.d, k = i - si * p.d;
     const void* w = p.side[si].weight;
-    weights[si][k] = !w ? 1.f : p.weight_dtype == BMA_DTYPE_F32 ? __ldg(static_cast<const float*>(w) + k) : __bfloat162float(static_cast<const __nv_bfloat16*>(w)[k]);
+    weights[si][k] = w ? weight_at(w, p.weight_dtype, k) : 1.f;
   }
   make_steps(steps, p.frequencies, pairs);
   int from = 0;
@@ -789,7 +682,7 @@ __global__ void __launch_bounds__(kHeadsThreads, 4) heads_wide_kernel(const __gr
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-// The same work as rotate_back_kernel's.
+// The same work as rotate_back_kernel's.  (Four CTAs to an SM: 128 registers, for which bfloat16 spills 8 to 40 bytes.)
 template <typename T, int LAYOUT, bool FULL>
 __global__ void __launch_bounds__(kHeadsThreads, 4) rotate_back_wide_kernel(const __grid_constant__ BackParams p) {
   constexpr int VEC = Bits16<T>::n;
@@ -807,7 +700,7 @@ __global__ void __launch_bounds__(kHeadsThreads, 4) rotate_back_wide_kernel(cons
   const float inv_d = 1.f / (float)p.d;
   const int pairs = p.map.dim / 2, heads = side.heads;
   int ca, cb;
-  unit_chunks<VEC>(p.map, u, ca, cb);
+  unit_chunks(p.map, u, ca, cb);
   const bool A = ca < chunks, B = cb < chunks;
   const uint32_t live = live_pairs<VEC>(u, pairs);
   const int tokens = p.B * p.L, stride = ctas * kHeadsWarps;       // (below 2^30: rotate_backward)
@@ -856,13 +749,11 @@ __global__ void __launch_bounds__(kHeadsThreads, 4) rotate_back_wide_kernel(cons
 
   float2 w[VEC], dw[VEC];
   {
-    float wa[VEC], wb[VEC];
-    load_weight<VEC>(side.weight, p.weight_dtype, ca, chunks, wa);
-    load_weight<VEC>(side.weight, p.weight_dtype, cb, chunks, wb);
+    const auto at = [&](int chunk, int j) { return chunk < chunks ? weight_at(side.weight, p.weight_dtype, chunk * VEC + j) : 0.f; };
 #pragma unroll
     for (int i = 0; i < VEC / 2; ++i) {
-      w[i] = make_float2(wa[2 * i], wa[2 * i + 1]);
-      w[VEC / 2 + i] = make_float2(wb[2 * i], wb[2 * i + 1]);
+      w[i] = make_float2(at(ca, 2 * i), at(ca, 2 * i + 1));
+      w[VEC / 2 + i] = make_float2(at(cb, 2 * i), at(cb, 2 * i + 1));
     }
 #pragma unroll
     for (int i = 0; i < VEC; ++i) dw[i] = make_float2(0.f, 0.f);
@@ -1097,7 +988,7 @@ int launch_heads(HeadsParams& p, const bma_rotary& r, bool wide, cudaStream_t st
     if (r.layout == BMA_ROTARY_HALF) { if (full) BMA_WIDE(BMA_ROTARY_HALF, true); else BMA_WIDE(BMA_ROTARY_HALF, false); }
     else { if (full) BMA_WIDE(BMA_ROTARY_INTERLEAVED, true); else BMA_WIDE(BMA_ROTARY_INTERLEAVED, false); }
 #undef BMA_WIDE
-  } else heads_kernel<T, 1, 4, 1, KIND><<<(unsigned)ctas, kHeadsThreads, 0, st>>>(p);
+  } else heads_kernel<T, KIND><<<(unsigned)ctas, kHeadsThreads, 0, st>>>(p);
   count_launches(1);
   BMA_CUDA_TRY(cudaGetLastError());
   return BMA_OK;
@@ -1198,7 +1089,7 @@ int rotate_backward(const bma_rotate_args* a, void* workspace, size_t bytes, cud
     const bool full = a->rotary.dim == a->d, half = a->rotary.layout == BMA_ROTARY_HALF;
 #define BMA_BACK(T)                                                                                                       \
   do {                                                                                                                    \
-    if (!wide) rotate_back_kernel<T, 1, 4><<<ctas, kHeadsThreads, 0, st>>>(p);                                            \
+    if (!wide) rotate_back_kernel<T><<<ctas, kHeadsThreads, 0, st>>>(p);                                            \
     else if (half && full) rotate_back_wide_kernel<T, BMA_ROTARY_HALF, true><<<ctas, kHeadsThreads, 0, st>>>(p);          \
     else if (half) rotate_back_wide_kernel<T, BMA_ROTARY_HALF, false><<<ctas, kHeadsThreads, 0, st>>>(p);                 \
     else if (full) rotate_back_wide_kernel<T, BMA_ROTARY_INTERLEAVED, true><<<ctas, kHeadsThreads, 0, st>>>(p);           \
