@@ -196,7 +196,7 @@ typedef struct bma_paged_cache {
   int32_t dtype, reserved_;
 } bma_paged_cache;
 
-/* Of the T tokens that are given of sequence b the first new_lengths[b] (null: all T) are real; they are its newest, at positions
+/* Of the T tokens that are given of sequence b the first new_lengths[b] (taken as at least 0 and at most T; null: all T) are real; they are its newest, at positions
  * lengths[b] - new_lengths[b] and up: `lengths` counts them.  A position that the table does not cover, and a page that is not one of the
  * cache's, is neither read nor written; the status word (bma_device_status) says so, and the results of that call are invalid. */
 typedef struct bma_append_args {

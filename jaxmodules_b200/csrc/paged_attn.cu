@@ -2,8 +2,8 @@
 //
 // Every key and value in reach is read once and meets the few rows (tokens x query heads of its kv head) of one sequence: the kernels are bound
 // by memory.  What they have to do is to keep enough loads in flight, and to give every SM the same share of bytes whatever the
-// lengths are, which only the device knows.  Measured, 64 sequences of up to 8192 tokens, 8 kv heads of 128, 4 query heads to each: bfloat16 216 - 226 us, 94 - 99 %
-// of the copy rate; 4 bits 113 us, where instructions count (50 %); float32, 8 sequences, 16 heads of 64, window of 2048, 27.2 us (57 %).
+// lengths are, which only the device knows.  Measured, 64 sequences of up to 8192 tokens, 8 kv heads of 128, 4 query heads to each: bfloat16 222 - 225 us, 95 %
+// of the copy rate; 4 bits 114 us, where the chain of a tile counts (50 %; a warp waits for its own instruction before, with three to a scheduler); float32, 8 sequences, 16 heads of 64, window of 2048, 27.2 us (57 %).
 //
 // Work.  The walk over the keys of one (sequence, tile of rows, group of kv heads) is an item.  The four warps of a CTA have a kv head each, so that they
 // read neighbouring bytes of the same tokens at about the same time (of a 4-bit cache, whose powers of two for 8 heads are one 32-byte sector, 1.8 times the

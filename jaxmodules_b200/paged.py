@@ -58,7 +58,7 @@ def append_kv(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, lengths: torc
     """Writes the keys and values of new tokens into their pages, and returns the queries ready for ``paged_attention`` (None without ``q``).
 
     ``k``, ``v``: ``[B, T, Hkv, d]``, ``q``: ``[B, T, Hq, d]``, of the cache's dtype (float32 or bfloat16 for a 4-bit cache).  ``lengths``: int32 ``[B]``, the tokens
-    of each sequence with the new ones; of the T given the first ``new_lengths[b]`` (int32, None: all) are real and lie at positions
+    of each sequence with the new ones; of the T given the first ``new_lengths[b]`` (int32, taken as at least 0 and at most T; None: all) are real and lie at positions
     ``lengths[b] - new_lengths[b]`` and up.  The others are not written, and their queries come back as zeros.
 
     Queries and keys are normed and rotated on the way as by ``rotate_heads``, at the positions they lie at; values are not changed.  A 4-bit
