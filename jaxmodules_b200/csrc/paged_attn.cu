@@ -1221,30 +1221,50 @@ __global__ void __launch_bounds__(kThreads, Core::kMinCtas) paged_kernel(const _
   copies_awaited<0>();
 }
 
-// One CTA: a row of a head of an item that several CTAs had parts of, its warps taking parts in turn.
+// A row of a head of an item that several CTAs had parts of.
+template <int ROWS>
+struct Joined {
+  int4 m;                        // (of PagedParams::meta)
+  int b, head, mine, row, of_sequence, parts, heads;
+  bool real;
+  // Row and head `of_item` of the item of this CTA; false: there are no parts, or no such row.
+  __device__ __forceinline__ bool open(const PagedParams& p, int of_item) {
+    m = p.meta[blockIdx.x];
+    if (m.x < 0) return false;
+    heads = p.heads;
+    mine = of_item & (p.heads - 1);
+    row = of_item >> p.heads_log2;
+    const int groups = p.c.Hkv >> p.heads_log2, e = m.w / groups;
+    head = (m.w - e * groups) * p.heads + mine;
+    b = e / p.row_tiles;
+    const int row0 = (e - b * p.row_tiles) * ROWS;
+    of_sequence = row0 + row;
+    if (row >= min(ROWS, p.rows - row0)) return false;
+    real = of_sequence / p.G < new_tokens(p.a.lengths, p.a.new_lengths, b, p.a.T).count;
+    parts = m.z - m.x + 1;
+    return true;
+  }
+  __device__ __forceinline__ int64_t slot(int i) const { return ((int64_t)(i == 0 ? m.y : 2 * (m.x + i)) * heads + mine) * ROWS + row; }      // of part i
+};
+
+// One CTA: a row, its warps taking parts in turn.
 template <int DP, int ROWS>
 __global__ void __launch_bounds__(kThreads) paged_join_kernel(const __grid_constant__ PagedParams p) {
   __shared__ float4 sums[kWarps][DP / 4];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int4 m = p.meta[blockIdx.x];
-  if (m.x < 0) return;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, mine = blockIdx.y & (p.heads - 1), row = blockIdx.y >> p.heads_log2;
-  const int groups = p.c.Hkv >> p.heads_log2, e = m.w / groups, head = (m.w - e * groups) * p.heads + mine;
-  const int b = e / p.row_tiles, row0 = (e - b * p.row_tiles) * ROWS;
-  if (row >= min(ROWS, p.rows - row0)) return;
-  const bool real = (row0 + row) / p.G < new_tokens(p.a.lengths, p.a.new_lengths, b, p.a.T).count;
-  const int parts = m.z - m.x + 1;
-  auto slot = [&](int i) { return ((int64_t)(i == 0 ? m.y : 2 * (m.x + i)) * p.heads + mine) * ROWS + row; };
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  Joined<ROWS> of;
+  if (!of.open(p, blockIdx.y)) return;
   // Parts 32 at a time, all that is read of them at once: their statistics by every warp, a part to a lane, their sums by the warps in turn.
   float top = -INFINITY, sum = 0.f;
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i0 = 0; i0 < parts; i0 += 32) {
-    const float2 ml = i0 + lane < parts ? p.part_ml[slot(i0 + lane)] : make_float2(-INFINITY, 0.f);
+  for (int i0 = 0; i0 < of.parts; i0 += 32) {
+    const float2 ml = i0 + lane < of.parts ? p.part_ml[of.slot(i0 + lane)] : make_float2(-INFINITY, 0.f);
     float4 y[32 / kWarps];
 #pragma unroll
     for (int k = 0; k < 32 / kWarps; ++k) {
       const int i = i0 + k * kWarps + warp;
-      y[k] = i < parts && lane * 4 < DP ? *reinterpret_cast<const float4*>(p.part_o + slot(i) * DP + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+      y[k] = i < of.parts && lane * 4 < DP ? *reinterpret_cast<const float4*>(p.part_o + of.slot(i) * DP + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
     float t = ml.x;
 #pragma unroll
@@ -1270,22 +1290,16 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(const __grid_const
     const float4 y = sums[w][lane];
     x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
   }
-  write_result(p, b, head, row0 + row, real, lane * 4, x, top, sum);
+  write_result(p, of.b, of.head, of.of_sequence, of.real, lane * 4, x, top, sum);
 }
 
 // The same where most items have few parts: a warp to a row.
 template <int DP, int ROWS>
 __global__ void __launch_bounds__(kThreads) paged_join_few_kernel(const __grid_constant__ PagedParams p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int4 m = p.meta[blockIdx.x];
-  if (m.x < 0) return;
-  const int lane = threadIdx.x & 31, of_item = blockIdx.y * kWarps + (threadIdx.x >> 5), mine = of_item & (p.heads - 1), row = of_item >> p.heads_log2;
-  const int groups = p.c.Hkv >> p.heads_log2, e = m.w / groups, head = (m.w - e * groups) * p.heads + mine;
-  const int b = e / p.row_tiles, row0 = (e - b * p.row_tiles) * ROWS;
-  if (row >= min(ROWS, p.rows - row0)) return;
-  const bool real = (row0 + row) / p.G < new_tokens(p.a.lengths, p.a.new_lengths, b, p.a.T).count;
-  const int parts = m.z - m.x + 1;
-  auto slot = [&](int i) { return ((int64_t)(i == 0 ? m.y : 2 * (m.x + i)) * p.heads + mine) * ROWS + row; };
+  const int lane = threadIdx.x & 31;
+  Joined<ROWS> of;
+  if (!of.open(p, blockIdx.y * kWarps + (threadIdx.x >> 5))) return;
   float top = -INFINITY, sum = 0.f;
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
   auto take = [&](int i0, auto at_once) {       // parts i0 and up, all that is read of them at once
@@ -1294,9 +1308,9 @@ __global__ void __launch_bounds__(kThreads) paged_join_few_kernel(const __grid_c
     float4 y[N];
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-      const bool in = i0 + k < parts;
-      ml[k] = in ? p.part_ml[slot(i0 + k)] : make_float2(-INFINITY, 0.f);
-      y[k] = in && lane * 4 < DP ? *reinterpret_cast<const float4*>(p.part_o + slot(i0 + k) * DP + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+      const bool in = i0 + k < of.parts;
+      ml[k] = in ? p.part_ml[of.slot(i0 + k)] : make_float2(-INFINITY, 0.f);
+      y[k] = in && lane * 4 < DP ? *reinterpret_cast<const float4*>(p.part_o + of.slot(i0 + k) * DP + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
     float t = top;
 #pragma unroll
@@ -1312,10 +1326,10 @@ __global__ void __launch_bounds__(kThreads) paged_join_few_kernel(const __grid_c
       x.x = fmaf(y[k].x, f, x.x); x.y = fmaf(y[k].y, f, x.y); x.z = fmaf(y[k].z, f, x.z); x.w = fmaf(y[k].w, f, x.w);
     }
   };
-  if (parts <= 4) take(0, std::integral_constant<int, 4>());
+  if (of.parts <= 4) take(0, std::integral_constant<int, 4>());
   else
-    for (int i0 = 0; i0 < parts; i0 += 16) take(i0, std::integral_constant<int, 16>());      // a long sequence among many short ones
-  if (lane * 4 < DP) write_result(p, b, head, row0 + row, real, lane * 4, x, top, sum);
+    for (int i0 = 0; i0 < of.parts; i0 += 16) take(i0, std::integral_constant<int, 16>());      // a long sequence among many short ones
+  if (lane * 4 < DP) write_result(p, of.b, of.head, of.of_sequence, of.real, lane * 4, x, top, sum);
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------
