@@ -748,8 +748,9 @@ struct Core4bit {
         for (int z = 0; z < 2; ++z) {
 #pragma unroll
           for (int lanes = 4; lanes < 32; lanes <<= 1) most[z] = fmaxf(most[z], __shfl_xor_sync(0xffffffffu, most[z], lanes));
-          most[z] = most[z] == -INFINITY ? 0.f : most[z] - kWeightUp;
-          f[z] = exp2_approx(0.5f * (most[z] - top[z]));          // (twice: the product may be below 2^-126)
+          const bool none = most[z] == -INFINITY;                 // (there `top` says nothing of what the factor may be)
+          most[z] = none ? 0.f : most[z] - kWeightUp;
+          f[z] = none ? 0.f : exp2_approx(0.5f * (most[z] - top[z]));          // (twice: the product may be below 2^-126)
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {

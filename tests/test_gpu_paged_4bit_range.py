@@ -156,6 +156,27 @@ def test_small_components_of_a_query(down):
     check(q, c, lengths, False)
 
 
+@pytest.mark.parametrize("size", [1, 40, 200])
+def test_rows_that_see_nothing_of_a_tile(size):
+    """Far below zero as the logits of all that such a row has seen may be.  (So many sequences that a warp has all tiles of some of them.)"""
+    B, T = 500, 3
+    lengths = [33 + i % 3 for i in range(B)]
+    c = cache(lengths, 4, 64)
+    c.k[:] = 0x22                                    # ones
+    c.k_scale[:] = 127
+    c.v_scale[..., 1] = 90
+    q = torch.full((B, T, 8, 64), -float(size), device="cuda").bfloat16()
+    o, lse = jm.paged_attention(q, c, torch.tensor(lengths, dtype=torch.int32, device="cuda"), return_lse=True)
+    # logits are -8 size, exactly, so that all weights of a row are the same
+    values = po.held_values(c.v, c.v_scale).repeat_interleave(2, 2)
+    for b, length in enumerate(lengths):
+        v = values[at(c, b, list(range(length)))]
+        for t in range(T):
+            end = length - T + t + 1
+            assert ((o[b, t].double() - v[:end].mean(0)).abs() <= (2.0 ** -11 + 2.0 ** -17) * v[:end].abs().mean(0)).all()
+            assert ((lse[b, :, t].double() + 8 * size - math.log(end)).abs() <= 2.0 ** -22 * 8 * size + 2.0 ** -17).all()
+
+
 def test_an_appended_infinity():
     """It is kept as 6 * 2^126: where its weight is small enough the result is finite."""
     n = 64
