@@ -86,7 +86,7 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, lengths: torch.Tensor, *
     ``q``: ``[B, T, Hq, d]``, of the cache's dtype (bfloat16 for a 4-bit cache); the heads of the cache divide Hq.  ``lengths`` and ``new_lengths`` as for
     ``append_kv``.  Token i sees the keys at its own position and before; with ``window`` only those at most ``window`` positions before.
     ``scale`` replaces ``1 / sqrt(d)``.  Rows that see no key, and tokens that are not real, are zeros, with a log-sum-exp of -inf.
-    Products are summed in float32, with weights that are good to 2^-16 (bfloat16 cache) or 2^-11 (4 bits) of themselves.
+    Products are summed in float32, with weights that are good to 2^-15 (bfloat16 cache) or 2^-11 (4 bits) of themselves.
     ``out_dtype`` is float32 as for ``masked_attention_via_map``, or bfloat16; ``return_lse``: also the log-sum-exp ``[B, Hq, T]``.
 
     Made for few new tokens: the time is that of reading the keys and values once.  For the many tokens of a prompt, ``read_kv`` and

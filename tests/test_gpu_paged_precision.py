@@ -1,7 +1,7 @@
 """How near paged_attention over a bfloat16 cache comes to float64: as near as float32 arithmetic, not as near as bfloat16 weights would.
 
-Tolerances, per component, in units of sum p |v|: weights go through the product as two bfloat16 numbers, the second of which is what the first left (2^-8 of the weight) and is rounded by
-2^-8 of itself: 2^-16.  Sums and exponentials in float32 2^-17, as for float32 caches.  A logit is a sum of d products: d 2^-24 of the sum of their sizes at worst, which
+Tolerances, per component, in units of sum p |v|: weights go through the product as two bfloat16 numbers, the first cut off after 8 bits, the second what is left (less than 2^-7 of
+the weight) and rounded by 2^-8 of itself: 2^-15, with 2^-20 that is added to keep both above zero.  Sums and exponentials in float32 2^-17, as for float32 caches.  A logit is a sum of d products: d 2^-24 of the sum of their sizes at worst, which
 counts twice (in its weight, and in the sum of all)."""
 import math
 
@@ -37,8 +37,25 @@ def test_bfloat16(lengths, T, Hq, H, d, window):
     most = max((q[b].double().abs().reshape(T, H, -1, d).transpose(1, 2).reshape(-1, H, d).unsqueeze(1) * ks[b].abs()).sum(-1).max() for b in range(B))
     off = float(most) * d * 2.0 ** -24 / math.sqrt(d)
     assert off < 2.0 ** -12
-    bound = (2.0 ** -16 + 2.0 ** -17 + 2 * off) * size
+    bound = (2.0 ** -15 + 2.0 ** -20 + 2.0 ** -17 + 2 * off) * size
     assert ((o.double() - want).abs() <= bound + 1e-30).all(), ((o.double() - want).abs() / (bound + 1e-30)).max()
     assert ((half.double() - want).abs() <= 2.0 ** -8 * want.abs() + bound * (1 + 2.0 ** -8) + 1e-30).all()
     seen = want_lse > -torch.inf
     assert ((lse.double() - want_lse).abs()[seen] <= off + 2.0 ** -17).all()
+
+
+@pytest.mark.parametrize("T", [1, 3])
+@pytest.mark.parametrize("where", [0, 17, 99])
+def test_infinite_values(where, T):
+    """A weight makes an infinity of an infinity, whatever its bits, in every row that sees it."""
+    n, H, d = 100, 2, 64
+    g = torch.Generator(device="cuda").manual_seed(where)
+    pages = [torch.randn((7, 16, H, d), device="cuda", generator=g).bfloat16() for _ in range(2)]
+    pages[1][where // 16, where % 16, :, 5], pages[1][where // 16, where % 16, :, 6] = torch.inf, -torch.inf
+    c = jm.PagedCache(*pages, torch.arange(7, dtype=torch.int32, device="cuda")[None])
+    q = torch.randn((1, T, 8, d), device="cuda", generator=g).bfloat16()
+    q[:, :, ::2] = 0                                 # weights of 1
+    o = jm.paged_attention(q, c, torch.tensor([n], dtype=torch.int32, device="cuda"))
+    sees = torch.arange(n - T, n, device="cuda") >= where
+    assert (o[0, sees][..., 5] == torch.inf).all() and (o[0, sees][..., 6] == -torch.inf).all()
+    assert o[0, ~sees].isfinite().all() and o[..., :5].isfinite().all() and o[..., 7:].isfinite().all()
